@@ -40,7 +40,9 @@ typedef enum {
     NB200_ERR_CUDA = 7          /* a CUDA runtime call or launch failed                          */
 } nb200_status;
 
-typedef enum { NB200_F32 = 0, NB200_F64 = 1 } nb200_dtype;
+/* The sparse operators take NB200_F32 and NB200_F64; the dense operators of the graph layers (at the end of
+ * this file) take all four. */
+typedef enum { NB200_F32 = 0, NB200_F64 = 1, NB200_BF16 = 2, NB200_F16 = 3 } nb200_dtype;
 typedef enum { NB200_I32 = 0, NB200_I64 = 1 } nb200_itype;
 
 typedef void* nb200_stream; /* a cudaStream_t */
@@ -595,6 +597,62 @@ NB200_API int nb200_ipc_alloc(size_t bytes, void** ptr, void* handle64);
 NB200_API int nb200_ipc_open(const void* handle64, void** ptr);
 NB200_API int nb200_ipc_close(void* ptr);
 NB200_API int nb200_ipc_free(void* ptr);
+
+/* ---------------------------------------------------------------------------------------------
+ * Dense operators of the graph layers.  Node features are channels-last rows; `dtype` is any
+ * nb200_dtype; sums, statistics and activations are held in 32 bits (64 for NB200_F64) and results
+ * are rounded once.  `activation` is an nb200_activation.
+ * ------------------------------------------------------------------------------------------- */
+typedef enum {
+    NB200_ACT_NONE = 0,
+    NB200_ACT_RELU = 1,
+    NB200_ACT_SILU = 2,   /* z / (1 + exp(-z))              */
+    NB200_ACT_GELU = 3,   /* z (1 + erf(z / sqrt 2)) / 2    */
+    NB200_ACT_TANH = 4
+} nb200_activation;
+
+/* y = act(x w + bias) + residual.   x [m, k], w [k, n], residual [m, n] with row strides ldx, ldw, ldr in
+ * elements (rows themselves contiguous); bias [n] and residual may be NULL; y [m, n] contiguous.  z (may be NULL)
+ * receives x w + bias, [m, n] contiguous, which the backward pass reads when there is an activation.
+ *
+ * Backward, dz = dy act'(z):  dx = dz w^T [m, k],  dw = x^T dz [k, n],  dbias = column sums of dz [n], each
+ * contiguous and each skipped when NULL; the residual's gradient is dy itself.  z may be NULL for NB200_ACT_NONE.
+ * No alignment is required of any array but `work` (16 bytes).  Results do not depend on the run: sums are cut at
+ * places that depend on the sizes alone and joined in order. */
+NB200_API int nb200_linear_forward(int64_t m, int64_t k, int64_t n, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                                   const void* bias, const void* residual, int64_t ldr, int activation, void* z, void* y,
+                                   int dtype, nb200_stream stream);
+NB200_API size_t nb200_linear_backward_workspace_bytes(int64_t m, int64_t k, int64_t n, int activation, int dtype);
+NB200_API int nb200_linear_backward(int64_t m, int64_t k, int64_t n, const void* dy, int64_t lddy, const void* x, int64_t ldx,
+                                    const void* w, int64_t ldw, const void* z, int activation, void* dx, void* dw, void* dbias,
+                                    void* work, size_t work_bytes, int dtype, nb200_stream stream);
+
+/* Group norm with an activation, y = act((x - mean) rstd weight + bias), over contiguous rows [rows, channels].
+ * Mean and biased variance are taken over the rows of a segment and the channels / groups neighbouring channels of
+ * a group; rstd = (variance + eps)^(-1/2).  Segment s is rows ptr[s] .. ptr[s+1] (ptr: segments + 1 ascending row
+ * numbers on the device) or, with ptr NULL, the s-th of `segments` runs of rows / segments rows.  Rows outside every
+ * segment get y = 0 and dx = 0.  Row numbers out of order or out of range give unspecified values but touch nothing
+ * outside the arrays.  weight and bias [channels] may be NULL (1 and 0).  mean and rstd [segments, groups] are
+ * float (double for NB200_F64), written by the forward pass and read by the backward pass; 0 for empty segments.
+ * dx, dweight and dbias are skipped when NULL.  x, y, dy, dx and work 16-byte aligned. */
+NB200_API size_t nb200_group_norm_workspace_bytes(int64_t rows, int64_t channels, int64_t groups, int64_t segments, int dtype);
+NB200_API int nb200_group_norm_forward(int64_t rows, int64_t channels, int64_t groups, int64_t segments, const int64_t* ptr,
+                                       const void* x, const void* weight, const void* bias, double eps, int activation,
+                                       void* y, void* mean, void* rstd, void* work, size_t work_bytes, int dtype,
+                                       nb200_stream stream);
+NB200_API int nb200_group_norm_backward(int64_t rows, int64_t channels, int64_t groups, int64_t segments, const int64_t* ptr,
+                                        const void* dy, const void* x, const void* weight, const void* bias, const void* mean,
+                                        const void* rstd, int activation, void* dx, void* dweight, void* dbias, void* work,
+                                        size_t work_bytes, int dtype, nb200_stream stream);
+
+/* Dropout, y[i] = (u[i] >= round(p 2^32) ? x[i] / (1 - p) : 0) + residual[i] over n contiguous elements; u[i] is a
+ * 32-bit number that depends on (seed, offset, i) alone, so the same call on the gradient is the backward pass.
+ * Generator: Philox4x32 with ten rounds, key = seed, counter = (i / 8, offset [63 bits], one stream bit); the high
+ * half of u[i] is half-word i % 8 of stream 0's output, the low half the same half-word of stream 1's.  0 <= p <= 1;
+ * p = 1 gives zeros.  `state` (may be NULL): two int64 words on the device that are read in the place of seed and
+ * offset.  residual may be NULL.  x, y and residual 16-byte aligned. */
+NB200_API int nb200_dropout(int64_t n, const void* x, const void* residual, void* y, double p, uint64_t seed, uint64_t offset,
+                            const int64_t* state, int dtype, nb200_stream stream);
 
 #ifdef __cplusplus
 }

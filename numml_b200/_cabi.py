@@ -10,8 +10,9 @@ from . import build as _build
 
 _c = ctypes
 _i64, _int, _vp, _sz = _c.c_int64, _c.c_int, _c.c_void_p, _c.c_size_t
+_u64, _f64 = _c.c_uint64, _c.c_double
 
-F32, F64 = 0, 1
+F32, F64, BF16, F16 = 0, 1, 2, 3
 I32, I64 = 0, 1
 
 # name -> (restype, argtypes); mirrors include/numml_b200.h one to one
@@ -84,6 +85,14 @@ SIGNATURES = {
     "nb200_ipc_open": (_int, [_vp, _c.POINTER(_vp)]),
     "nb200_ipc_close": (_int, [_vp]),
     "nb200_ipc_free": (_int, [_vp]),
+    "nb200_linear_forward": (_int, [_i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _int, _vp, _vp, _int, _vp]),
+    "nb200_linear_backward_workspace_bytes": (_sz, [_i64, _i64, _i64, _int, _int]),
+    "nb200_linear_backward": (_int, [_i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _int, _vp, _vp, _vp, _vp, _sz, _int, _vp]),
+    "nb200_group_norm_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _int]),
+    "nb200_group_norm_forward": (_int, [_i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _f64, _int, _vp, _vp, _vp, _vp, _sz, _int, _vp]),
+    "nb200_group_norm_backward": (_int, [_i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _sz,
+                                         _int, _vp]),
+    "nb200_dropout": (_int, [_i64, _vp, _vp, _vp, _f64, _u64, _u64, _vp, _int, _vp]),
     "nb200_spdmm_backward_grad_A": (_int, [_i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _vp]),
 }
 

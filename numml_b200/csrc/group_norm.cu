@@ -1,0 +1,563 @@
+// Group norm with an activation over channels-last rows [rows, channels]:
+//   y = act(xhat * gamma + beta),   xhat = (x - mean) * rstd,   rstd = (var + eps)^(-1/2)
+// where mean and (biased) variance are taken over the rows of a segment (one graph of a batch) and the
+// channels / groups neighbouring channels of a group.  Backward, with dz = dy act'(z) and h = dz gamma:
+//   dx = rstd (h - mean(h) - xhat mean(h xhat)),  dgamma = sum dz xhat,  dbeta = sum dz.
+//
+// Segments may be of any length, so rows are cut into equal chunks, one per block, and not by segment:
+// the work is balanced however ragged the batch is.  A chunk holds pieces of several segments and a
+// segment pieces of several chunks; piece (block b, segment s) has workspace slot b + s, which is unique
+// because b and s never decrease from one piece to the next.  A pass writes per-channel partial results
+// of its pieces, a small kernel joins them per (segment, group) in a fixed order (no atomics: two runs
+// give the same bits), and a second pass over the rows applies them.
+//
+// Variances come from differences: a thread sums (x - k) and (x - k)^2 with k the first value it meets
+// of its channel in the piece, and partial results are joined as (count, mean, sum of squared
+// deviations), the join over pieces in 64 bits.  E[x^2] - E[x]^2 never appears.
+#include "dense_common.cuh"
+
+namespace nb200 {
+namespace {
+
+constexpr int kThreads = 256;
+
+// Everything that the kernels of a call share.
+struct Shape {
+    int64_t rows, chunk;          // rows of the array; rows per block
+    int channels, groups, lanes;  // lanes = vectors of a row that a block covers (blockIdx.y selects which)
+    int64_t segments;
+    const int64_t* ptr;           // segments + 1 row pointers, or NULL: segments of `equal` rows
+    int64_t equal;
+};
+
+__device__ __forceinline__ int64_t clamp_row(int64_t r, int64_t rows) { return r < 0 ? 0 : (r > rows ? rows : r); }
+__device__ __forceinline__ int64_t segment_begin(const Shape& sh, int64_t s) {
+    return sh.ptr ? clamp_row(sh.ptr[s], sh.rows) : s * sh.equal;
+}
+
+// The segment that holds `row` (-1: before the first, `segments`: behind the last) and where the run of
+// rows with that answer ends.  Row pointers out of order or out of range give some in-range answer that
+// still advances, so a broken pointer array cannot make a kernel leave its arrays or loop for ever.
+__device__ __forceinline__ int64_t find_segment(const Shape& sh, int64_t row, int64_t limit, int64_t& end) {
+    if (!sh.ptr) {
+        const int64_t s = row / sh.equal;
+        end = min(limit, (s + 1) * sh.equal);
+        return s;
+    }
+    int64_t lo = 0, hi = sh.segments + 1;          // first index whose pointer is > row
+    while (lo < hi) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (sh.ptr[mid] > row) hi = mid; else lo = mid + 1;
+    }
+    end = lo <= sh.segments ? min(limit, max(sh.ptr[lo], row + 1)) : limit;
+    return lo - 1;
+}
+
+// Join (n, mean, m2) with (nb, mean_b, m2_b).
+template <typename A>
+__device__ __forceinline__ void join(A& n, A& mean, A& m2, A nb, A mean_b, A m2_b) {
+    if (nb == A(0)) return;
+    if (n == A(0)) {
+        n = nb;
+        mean = mean_b;
+        m2 = m2_b;
+        return;
+    }
+    const A total = n + nb;
+    const A d = mean_b - mean, f = nb / total;
+    mean += d * f;
+    m2 += m2_b + d * d * n * f;
+    n = total;
+}
+
+// ---- forward, first pass: per channel (mean, m2) of every piece ---------------------------------------
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) stats_kernel(Shape sh, const T* __restrict__ x, acc_t<T>* __restrict__ part) {
+    using A = acc_t<T>;
+    __shared__ A sm_mean[kThreads * V], sm_m2[kThreads * V], sm_n[kThreads];
+    const int lane = threadIdx.x % sh.lanes, row_lane = threadIdx.x / sh.lanes, row_lanes = kThreads / sh.lanes;
+    const int c = (blockIdx.y * sh.lanes + lane) * V;
+    const bool live = row_lane < row_lanes && c < sh.channels;
+    const int64_t limit = min(sh.rows, (blockIdx.x + 1) * sh.chunk);
+    for (int64_t row = blockIdx.x * sh.chunk, end; row < limit; row = end) {
+        const int64_t s = find_segment(sh, row, limit, end);
+        if (s < 0 || s >= sh.segments) continue;
+        A k[V] = {}, sum[V] = {}, sq[V] = {}, n = 0;
+        if (live) {
+            int64_t r = row + row_lane;
+            if (r < end) load_acc<T, V>(x + r * sh.channels + c, k);
+#pragma unroll 4
+            for (; r < end; r += row_lanes) {
+                A v[V];
+                load_acc<T, V>(x + r * sh.channels + c, v);
+#pragma unroll
+                for (int q = 0; q < V; ++q) {
+                    const A d = v[q] - k[q];
+                    sum[q] += d;
+                    sq[q] += d * d;
+                }
+                n += A(1);
+            }
+        }
+        A mean[V], m2[V];
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+            const A d = n > A(0) ? sum[q] / n : A(0);
+            mean[q] = k[q] + d;
+            m2[q] = max(sq[q] - d * sum[q], A(0));
+            if (sq[q] != sq[q]) m2[q] = sq[q];      // NaN must not end as zero
+            sm_mean[threadIdx.x * V + q] = mean[q];
+            sm_m2[threadIdx.x * V + q] = m2[q];
+        }
+        sm_n[threadIdx.x] = n;
+        __syncthreads();
+        int width = 1;
+        while (width < row_lanes) width <<= 1;
+        for (int off = width >> 1; off > 0; off >>= 1) {
+            const int other = threadIdx.x + off * sh.lanes;
+            if (live && row_lane < off && row_lane + off < row_lanes) {
+                const A nb = sm_n[other];
+                A n_new = n;
+#pragma unroll
+                for (int q = 0; q < V; ++q) {
+                    n_new = n;
+                    join(n_new, mean[q], m2[q], nb, sm_mean[other * V + q], sm_m2[other * V + q]);
+                    sm_mean[threadIdx.x * V + q] = mean[q];
+                    sm_m2[threadIdx.x * V + q] = m2[q];
+                }
+                n = n_new;
+                sm_n[threadIdx.x] = n;
+            }
+            __syncthreads();
+        }
+        if (live && row_lane == 0) {
+            A* out = part + (blockIdx.x + s) * 2 * sh.channels + c;
+#pragma unroll
+            for (int q = 0; q < V; ++q) {
+                out[q] = mean[q];
+                out[sh.channels + q] = m2[q];
+            }
+        }
+    }
+}
+
+// Rows of segment s that lie in chunk b.
+__device__ __forceinline__ int64_t piece_rows(int64_t begin, int64_t end, int64_t b, int64_t chunk) {
+    return min(end, (b + 1) * chunk) - max(begin, b * chunk);
+}
+
+// One team of TEAM threads per (segment, group).
+template <typename A, int TEAM>
+__global__ void __launch_bounds__(kThreads) stats_join_kernel(Shape sh, const A* __restrict__ part, double eps,
+                                                              A* __restrict__ mean_out, A* __restrict__ rstd_out) {
+    __shared__ double sm[3][kThreads];
+    const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM;
+    const int64_t item = blockIdx.x * int64_t(kThreads / TEAM) + team;
+    const bool live = item < sh.segments * sh.groups;
+    const int64_t s = live ? item / sh.groups : 0;
+    const int g = static_cast<int>(live ? item % sh.groups : 0), width = sh.channels / sh.groups;
+    const int64_t begin = segment_begin(sh, s), end = max(begin, segment_begin(sh, s + 1));
+    double n = 0, mean = 0, m2 = 0;
+    if (live && end > begin) {
+        const int64_t first = begin / sh.chunk, last = (end - 1) / sh.chunk, work = (last - first + 1) * width;
+        for (int64_t e = t; e < work; e += TEAM) {
+            const int64_t b = first + e / width;
+            const A* p = part + (b + s) * 2 * sh.channels + g * width + e % width;
+            join(n, mean, m2, static_cast<double>(piece_rows(begin, end, b, sh.chunk)), static_cast<double>(p[0]),
+                 static_cast<double>(p[sh.channels]));
+        }
+    }
+    sm[0][threadIdx.x] = n;
+    sm[1][threadIdx.x] = mean;
+    sm[2][threadIdx.x] = m2;
+    __syncthreads();
+    for (int off = TEAM / 2; off > 0; off >>= 1) {
+        if (t < off) {
+            join(n, mean, m2, sm[0][threadIdx.x + off], sm[1][threadIdx.x + off], sm[2][threadIdx.x + off]);
+            sm[0][threadIdx.x] = n;
+            sm[1][threadIdx.x] = mean;
+            sm[2][threadIdx.x] = m2;
+        }
+        __syncthreads();
+    }
+    if (live && t == 0) {
+        mean_out[item] = static_cast<A>(mean);
+        rstd_out[item] = n > 0 ? static_cast<A>(1.0 / sqrt(m2 / n + eps)) : A(0);
+    }
+}
+
+// ---- what a thread knows of its V channels ------------------------------------------------------------
+template <typename T, int V>
+struct ChannelParams {
+    acc_t<T> gamma[V], beta[V];
+    int group[V];
+    __device__ __forceinline__ void load(const Shape& sh, int c, const T* w, const T* b) {
+        const int width = sh.channels / sh.groups;
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+            gamma[q] = w ? to_acc(w[c + q]) : acc_t<T>(1);
+            beta[q] = b ? to_acc(b[c + q]) : acc_t<T>(0);
+            group[q] = (c + q) / width;
+        }
+    }
+};
+
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads) apply_kernel(Shape sh, const T* __restrict__ x, const T* __restrict__ w,
+                                                         const T* __restrict__ bias, const acc_t<T>* __restrict__ mean,
+                                                         const acc_t<T>* __restrict__ rstd, T* __restrict__ y) {
+    using A = acc_t<T>;
+    const int lane = threadIdx.x % sh.lanes, row_lane = threadIdx.x / sh.lanes, row_lanes = kThreads / sh.lanes;
+    const int c = (blockIdx.y * sh.lanes + lane) * V;
+    if (row_lane >= row_lanes || c >= sh.channels) return;
+    ChannelParams<T, V> cp;
+    cp.load(sh, c, w, bias);
+    const int64_t limit = min(sh.rows, (blockIdx.x + 1) * sh.chunk);
+    for (int64_t row = blockIdx.x * sh.chunk, end; row < limit; row = end) {
+        const int64_t s = find_segment(sh, row, limit, end);
+        if (s < 0 || s >= sh.segments) {
+            const A zero[V] = {};
+            for (int64_t r = row + row_lane; r < end; r += row_lanes) store_acc<T, V>(y + r * sh.channels + c, zero);
+            continue;
+        }
+        A m[V], a[V];
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+            m[q] = mean[s * sh.groups + cp.group[q]];
+            a[q] = rstd[s * sh.groups + cp.group[q]] * cp.gamma[q];
+        }
+#pragma unroll 4
+        for (int64_t r = row + row_lane; r < end; r += row_lanes) {
+            A v[V];
+            load_acc<T, V>(x + r * sh.channels + c, v);
+#pragma unroll
+            for (int q = 0; q < V; ++q) v[q] = activate<ACT>((v[q] - m[q]) * a[q] + cp.beta[q]);
+            store_acc<T, V>(y + r * sh.channels + c, v);
+        }
+    }
+}
+
+// ---- backward, first pass: per channel (sum dz, sum dz xhat) of every piece and of every block ---------
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads) grad_sums_kernel(Shape sh, const T* __restrict__ x, const T* __restrict__ dy,
+                                                             const T* __restrict__ w, const T* __restrict__ bias,
+                                                             const acc_t<T>* __restrict__ mean, const acc_t<T>* __restrict__ rstd,
+                                                             acc_t<T>* __restrict__ part, acc_t<T>* __restrict__ block_sums) {
+    using A = acc_t<T>;
+    __shared__ A sm[2][kThreads * V];
+    const int lane = threadIdx.x % sh.lanes, row_lane = threadIdx.x / sh.lanes, row_lanes = kThreads / sh.lanes;
+    const int c = (blockIdx.y * sh.lanes + lane) * V;
+    const bool live = row_lane < row_lanes && c < sh.channels;
+    ChannelParams<T, V> cp;
+    if (live) cp.load(sh, c, w, bias);
+    A total1[V] = {}, total2[V] = {};
+    const int64_t limit = min(sh.rows, (blockIdx.x + 1) * sh.chunk);
+    for (int64_t row = blockIdx.x * sh.chunk, end; row < limit; row = end) {
+        const int64_t s = find_segment(sh, row, limit, end);
+        if (s < 0 || s >= sh.segments) continue;
+        A s1[V] = {}, s2[V] = {};
+        if (live) {
+            A m[V], rs[V];
+#pragma unroll
+            for (int q = 0; q < V; ++q) {
+                m[q] = mean[s * sh.groups + cp.group[q]];
+                rs[q] = rstd[s * sh.groups + cp.group[q]];
+            }
+#pragma unroll 2
+            for (int64_t r = row + row_lane; r < end; r += row_lanes) {
+                A v[V], g[V];
+                load_acc<T, V>(x + r * sh.channels + c, v);
+                load_acc<T, V>(dy + r * sh.channels + c, g);
+#pragma unroll
+                for (int q = 0; q < V; ++q) {
+                    const A xhat = (v[q] - m[q]) * rs[q];
+                    const A dz = g[q] * activate_slope<ACT>(xhat * cp.gamma[q] + cp.beta[q]);
+                    s1[q] += dz;
+                    s2[q] += dz * xhat;
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+            sm[0][threadIdx.x * V + q] = s1[q];
+            sm[1][threadIdx.x * V + q] = s2[q];
+        }
+        __syncthreads();
+        int width = 1;
+        while (width < row_lanes) width <<= 1;
+        for (int off = width >> 1; off > 0; off >>= 1) {
+            const int other = threadIdx.x + off * sh.lanes;
+            if (live && row_lane < off && row_lane + off < row_lanes) {
+#pragma unroll
+                for (int q = 0; q < V; ++q) {
+                    sm[0][threadIdx.x * V + q] = s1[q] += sm[0][other * V + q];
+                    sm[1][threadIdx.x * V + q] = s2[q] += sm[1][other * V + q];
+                }
+            }
+            __syncthreads();
+        }
+        if (live && row_lane == 0) {
+            A* out = part + (blockIdx.x + s) * 2 * sh.channels + c;
+#pragma unroll
+            for (int q = 0; q < V; ++q) {
+                out[q] = s1[q];
+                out[sh.channels + q] = s2[q];
+                total1[q] += s1[q];
+                total2[q] += s2[q];
+            }
+        }
+    }
+    if (live && row_lane == 0) {
+        A* out = block_sums + blockIdx.x * int64_t(2) * sh.channels + c;
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+            out[q] = total1[q];
+            out[sh.channels + q] = total2[q];
+        }
+    }
+}
+
+// mean(h) and mean(h xhat) of every (segment, group), from the per-channel sums of its pieces.
+template <typename T, int TEAM>
+__global__ void __launch_bounds__(kThreads) grad_join_kernel(Shape sh, const acc_t<T>* __restrict__ part, const T* __restrict__ w,
+                                                             acc_t<T>* __restrict__ coef) {
+    __shared__ double sm[2][kThreads];
+    const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM;
+    const int64_t item = blockIdx.x * int64_t(kThreads / TEAM) + team;
+    const bool live = item < sh.segments * sh.groups;
+    const int64_t s = live ? item / sh.groups : 0;
+    const int g = static_cast<int>(live ? item % sh.groups : 0), width = sh.channels / sh.groups;
+    const int64_t begin = segment_begin(sh, s), end = max(begin, segment_begin(sh, s + 1));
+    double a = 0, b = 0;
+    if (live && end > begin) {
+        const int64_t first = begin / sh.chunk, last = (end - 1) / sh.chunk, work = (last - first + 1) * width;
+        for (int64_t e = t; e < work; e += TEAM) {
+            const int c = g * width + static_cast<int>(e % width);
+            const acc_t<T>* p = part + (first + e / width + s) * 2 * sh.channels + c;
+            const double gamma = w ? static_cast<double>(to_acc(w[c])) : 1.0;
+            a += gamma * static_cast<double>(p[0]);
+            b += gamma * static_cast<double>(p[sh.channels]);
+        }
+    }
+    sm[0][threadIdx.x] = a;
+    sm[1][threadIdx.x] = b;
+    __syncthreads();
+    for (int off = TEAM / 2; off > 0; off >>= 1) {
+        if (t < off) {
+            sm[0][threadIdx.x] = a += sm[0][threadIdx.x + off];
+            sm[1][threadIdx.x] = b += sm[1][threadIdx.x + off];
+        }
+        __syncthreads();
+    }
+    if (live && t == 0) {
+        const double n = static_cast<double>(end - begin) * width;
+        coef[2 * item] = static_cast<acc_t<T>>(n > 0 ? a / n : 0.0);
+        coef[2 * item + 1] = static_cast<acc_t<T>>(n > 0 ? b / n : 0.0);
+    }
+}
+
+// dbeta and dgamma: columns of block_sums [blocks][2][channels] added up; 32 columns x 8 rows of threads.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) column_sums_kernel(int64_t blocks, int channels, const acc_t<T>* __restrict__ block_sums,
+                                                               T* __restrict__ dbeta, T* __restrict__ dgamma) {
+    __shared__ double sm[8][33];
+    const int col = blockIdx.x * 32 + threadIdx.x % 32, part = threadIdx.x / 32;
+    double a = 0;
+    if (col < 2 * channels)
+        for (int64_t b = part; b < blocks; b += 8) a += static_cast<double>(block_sums[b * 2 * channels + col]);
+    sm[part][threadIdx.x % 32] = a;
+    __syncthreads();
+    if (part == 0 && col < 2 * channels) {
+        for (int q = 1; q < 8; ++q) a += sm[q][threadIdx.x % 32];
+        T* out = col < channels ? dbeta : dgamma;
+        if (out) out[col % channels] = from_acc<T>(static_cast<acc_t<T>>(a));
+    }
+}
+
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads) grad_apply_kernel(Shape sh, const T* __restrict__ x, const T* __restrict__ dy,
+                                                              const T* __restrict__ w, const T* __restrict__ bias,
+                                                              const acc_t<T>* __restrict__ mean, const acc_t<T>* __restrict__ rstd,
+                                                              const acc_t<T>* __restrict__ coef, T* __restrict__ dx) {
+    using A = acc_t<T>;
+    const int lane = threadIdx.x % sh.lanes, row_lane = threadIdx.x / sh.lanes, row_lanes = kThreads / sh.lanes;
+    const int c = (blockIdx.y * sh.lanes + lane) * V;
+    if (row_lane >= row_lanes || c >= sh.channels) return;
+    ChannelParams<T, V> cp;
+    cp.load(sh, c, w, bias);
+    const int64_t limit = min(sh.rows, (blockIdx.x + 1) * sh.chunk);
+    for (int64_t row = blockIdx.x * sh.chunk, end; row < limit; row = end) {
+        const int64_t s = find_segment(sh, row, limit, end);
+        if (s < 0 || s >= sh.segments) {
+            const A zero[V] = {};
+            for (int64_t r = row + row_lane; r < end; r += row_lanes) store_acc<T, V>(dx + r * sh.channels + c, zero);
+            continue;
+        }
+        A m[V], rs[V], c1[V], c2[V];
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+            const int64_t item = s * sh.groups + cp.group[q];
+            m[q] = mean[item];
+            rs[q] = rstd[item];
+            c1[q] = coef[2 * item];
+            c2[q] = coef[2 * item + 1];
+        }
+#pragma unroll 2
+        for (int64_t r = row + row_lane; r < end; r += row_lanes) {
+            A v[V], g[V];
+            load_acc<T, V>(x + r * sh.channels + c, v);
+            load_acc<T, V>(dy + r * sh.channels + c, g);
+#pragma unroll
+            for (int q = 0; q < V; ++q) {
+                const A xhat = (v[q] - m[q]) * rs[q];
+                const A h = g[q] * activate_slope<ACT>(xhat * cp.gamma[q] + cp.beta[q]) * cp.gamma[q];
+                v[q] = rs[q] * (h - c1[q] - xhat * c2[q]);
+            }
+            store_acc<T, V>(dx + r * sh.channels + c, v);
+        }
+    }
+}
+
+// ---- host side ------------------------------------------------------------------------------------------
+int64_t block_count(int64_t rows) {
+    const int64_t wanted = ceil_div(rows, 32);
+    return wanted < kSMs * 8 ? (wanted < 1 ? 1 : wanted) : kSMs * 8;
+}
+
+// Partial results of the pieces, of the blocks, and the two coefficients per (segment, group).
+size_t part_elements(int64_t rows, int channels, int64_t segments) { return size_t(block_count(rows) + segments) * 2 * channels; }
+
+bool bad_shape(int64_t rows, int64_t channels, int64_t groups, int64_t segments, const int64_t* ptr) {
+    return rows < 0 || channels < 1 || channels > (1 << 20) || groups < 1 || channels % groups != 0 || segments < 0 ||
+           segments > INT32_MAX || (!ptr && (segments < 1 ? rows != 0 : rows % segments != 0));
+}
+
+struct Launch {
+    Shape sh;
+    dim3 grid;
+    bool vector;
+};
+
+template <typename T>
+Launch make_launch(int64_t rows, int64_t channels, int64_t groups, int64_t segments, const int64_t* ptr) {
+    Launch l;
+    constexpr int V = 16 / sizeof(T);
+    l.vector = channels % V == 0;
+    const int vectors = static_cast<int>(l.vector ? channels / V : channels);
+    const int64_t blocks = block_count(rows), chunk = ceil_div(rows, blocks);
+    const int lanes = vectors < kThreads ? vectors : kThreads;
+    l.sh = {rows, chunk, static_cast<int>(channels), static_cast<int>(groups), lanes, segments, ptr,
+            segments > 0 ? rows / segments : rows};
+    l.grid = dim3(static_cast<unsigned>(ceil_div(rows, chunk)), static_cast<unsigned>(ceil_div(vectors, lanes)));
+    return l;
+}
+
+template <typename T, int V>
+int forward(const Launch& l, const T* x, const T* w, const T* b, double eps, int act, T* y, acc_t<T>* mean, acc_t<T>* rstd,
+            acc_t<T>* part, cudaStream_t stream) {
+    using A = acc_t<T>;
+    stats_kernel<T, V><<<l.grid, kThreads, 0, stream>>>(l.sh, x, part);
+    const int64_t items = l.sh.segments * l.sh.groups;
+    if (items > 0) {
+        if (items > kSMs * 8)
+            stats_join_kernel<A, 32><<<static_cast<unsigned>(ceil_div(items, kThreads / 32)), kThreads, 0, stream>>>(l.sh, part, eps, mean, rstd);
+        else
+            stats_join_kernel<A, kThreads><<<static_cast<unsigned>(items), kThreads, 0, stream>>>(l.sh, part, eps, mean, rstd);
+    }
+    return NB200_DISPATCH_ACT(act, (apply_kernel<T, V, ACT><<<l.grid, kThreads, 0, stream>>>(l.sh, x, w, b, mean, rstd, y), launch_status()));
+}
+
+template <typename T, int V>
+int backward(const Launch& l, const T* dy, const T* x, const T* w, const T* b, const acc_t<T>* mean, const acc_t<T>* rstd, int act,
+             T* dx, T* dw, T* db, acc_t<T>* part, cudaStream_t stream) {
+    using A = acc_t<T>;
+    A* block_sums = part + part_elements(l.sh.rows, l.sh.channels, l.sh.segments);
+    A* coef = block_sums + size_t(block_count(l.sh.rows)) * 2 * l.sh.channels;
+    int rc = NB200_DISPATCH_ACT(act, (grad_sums_kernel<T, V, ACT><<<l.grid, kThreads, 0, stream>>>(l.sh, x, dy, w, b, mean, rstd, part,
+                                                                                                 block_sums), launch_status()));
+    if (rc != NB200_OK) return rc;
+    if (dw || db)
+        column_sums_kernel<T><<<static_cast<unsigned>(ceil_div(2 * l.sh.channels, 32)), kThreads, 0, stream>>>(
+            l.grid.x, l.sh.channels, block_sums, db, dw);
+    if (!dx) return launch_status();
+    const int64_t items = l.sh.segments * l.sh.groups;
+    if (items > 0) {
+        if (items > kSMs * 8)
+            grad_join_kernel<T, 32><<<static_cast<unsigned>(ceil_div(items, kThreads / 32)), kThreads, 0, stream>>>(l.sh, part, w, coef);
+        else
+            grad_join_kernel<T, kThreads><<<static_cast<unsigned>(items), kThreads, 0, stream>>>(l.sh, part, w, coef);
+    }
+    return NB200_DISPATCH_ACT(act, (grad_apply_kernel<T, V, ACT><<<l.grid, kThreads, 0, stream>>>(l.sh, x, dy, w, b, mean, rstd, coef, dx),
+                                    launch_status()));
+}
+
+}  // namespace
+}  // namespace nb200
+
+using namespace nb200;
+
+extern "C" size_t nb200_group_norm_workspace_bytes(int64_t rows, int64_t channels, int64_t groups, int64_t segments, int dtype) {
+    if (rows < 0 || channels < 1 || groups < 1 || segments < 0) return 0;
+    const size_t a = dtype == NB200_F64 ? 8 : 4;
+    return a * (part_elements(rows, static_cast<int>(channels), segments) + size_t(block_count(rows)) * 2 * channels +
+                size_t(segments) * groups * 2);
+}
+
+extern "C" int nb200_group_norm_forward(int64_t rows, int64_t channels, int64_t groups, int64_t segments, const int64_t* ptr,
+                                        const void* x, const void* weight, const void* bias, double eps, int activation, void* y,
+                                        void* mean, void* rstd, void* work, size_t work_bytes, int dtype, nb200_stream stream) {
+    if (bad_shape(rows, channels, groups, segments, ptr) || !known_dense_dtype(dtype) || !known_activation(activation) || !(eps >= 0.0))
+        return NB200_ERR_BAD_ARG;
+    if (rows == 0 && segments == 0) return NB200_OK;
+    if ((segments > 0 && (!mean || !rstd)) || !work || (rows > 0 && (!x || !y))) return NB200_ERR_BAD_ARG;
+    if (work_bytes < nb200_group_norm_workspace_bytes(rows, channels, groups, segments, dtype)) return NB200_ERR_WORKSPACE;
+    if (!aligned16(x) || !aligned16(y) || !aligned16(work)) return NB200_ERR_ALIGN;
+    if (rows == 0) {
+        const size_t bytes = size_t(segments) * groups * (dtype == NB200_F64 ? 8 : 4);
+        if (cudaMemsetAsync(mean, 0, bytes, as_stream(stream)) != cudaSuccess ||
+            cudaMemsetAsync(rstd, 0, bytes, as_stream(stream)) != cudaSuccess)
+            return NB200_ERR_CUDA;
+        return NB200_OK;
+    }
+    return NB200_DISPATCH_DENSE(dtype, ([&]() -> int {
+        using A = acc_t<T>;
+        const Launch l = make_launch<T>(rows, channels, groups, segments, ptr);
+        const T *xt = static_cast<const T*>(x), *wt = static_cast<const T*>(weight), *bt = static_cast<const T*>(bias);
+        A *m = static_cast<A*>(mean), *rs = static_cast<A*>(rstd), *part = static_cast<A*>(work);
+        T* yt = static_cast<T*>(y);
+        constexpr int V = 16 / sizeof(T);
+        return l.vector ? forward<T, V>(l, xt, wt, bt, eps, activation, yt, m, rs, part, as_stream(stream))
+                        : forward<T, 1>(l, xt, wt, bt, eps, activation, yt, m, rs, part, as_stream(stream));
+    }()));
+}
+
+extern "C" int nb200_group_norm_backward(int64_t rows, int64_t channels, int64_t groups, int64_t segments, const int64_t* ptr,
+                                         const void* dy, const void* x, const void* weight, const void* bias, const void* mean,
+                                         const void* rstd, int activation, void* dx, void* dweight, void* dbias, void* work,
+                                         size_t work_bytes, int dtype, nb200_stream stream) {
+    if (bad_shape(rows, channels, groups, segments, ptr) || !known_dense_dtype(dtype) || !known_activation(activation))
+        return NB200_ERR_BAD_ARG;
+    if (rows == 0) {
+        const size_t bytes = size_t(channels) * dense_dtype_size(dtype);
+        if ((dweight && cudaMemsetAsync(dweight, 0, bytes, as_stream(stream)) != cudaSuccess) ||
+            (dbias && cudaMemsetAsync(dbias, 0, bytes, as_stream(stream)) != cudaSuccess))
+            return NB200_ERR_CUDA;
+        return NB200_OK;
+    }
+    if (!x || !dy || (segments > 0 && (!mean || !rstd)) || !work) return NB200_ERR_BAD_ARG;
+    if (work_bytes < nb200_group_norm_workspace_bytes(rows, channels, groups, segments, dtype)) return NB200_ERR_WORKSPACE;
+    if (!aligned16(x) || !aligned16(dy) || !aligned16(work) || (dx && !aligned16(dx))) return NB200_ERR_ALIGN;
+    return NB200_DISPATCH_DENSE(dtype, ([&]() -> int {
+        using A = acc_t<T>;
+        const Launch l = make_launch<T>(rows, channels, groups, segments, ptr);
+        const T *xt = static_cast<const T*>(x), *gt = static_cast<const T*>(dy), *wt = static_cast<const T*>(weight),
+                *bt = static_cast<const T*>(bias);
+        const A *m = static_cast<const A*>(mean), *rs = static_cast<const A*>(rstd);
+        A* part = static_cast<A*>(work);
+        T *dxt = static_cast<T*>(dx), *dwt = static_cast<T*>(dweight), *dbt = static_cast<T*>(dbias);
+        constexpr int V = 16 / sizeof(T);
+        return l.vector ? backward<T, V>(l, gt, xt, wt, bt, m, rs, activation, dxt, dwt, dbt, part, as_stream(stream))
+                        : backward<T, 1>(l, gt, xt, wt, bt, m, rs, activation, dxt, dwt, dbt, part, as_stream(stream));
+    }()));
+}

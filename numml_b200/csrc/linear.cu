@@ -1,0 +1,257 @@
+// Dense product of the graph layers with its epilogue,  y = act(x w + bias) + residual,  and its gradients:
+//   dz = dy act'(z),  dx = dz w^T,  dw = x^T dz,  dbias = column sums of dz
+// with z = x w + bias as the forward pass left it.  x [m, k], w [k, n], y [m, n].
+//
+// This file holds the entry points and the kernels that take any type, size and stride on the CUDA cores.
+#include "dense_common.cuh"
+
+namespace nb200 {
+namespace {
+
+constexpr int kTile = 64, kDepth = 16, kThreads = 256;
+
+// What the epilogue of a product needs; absent parts are NULL.
+template <typename T>
+struct Epilogue {
+    const T* bias;
+    const T* residual;
+    int64_t ldr;
+    T* z;                 // [rows, cols] contiguous
+    T* y;                 // [rows, cols] contiguous
+    acc_t<T>* partial;    // instead of all of the above: [splits, rows, cols]
+};
+
+// z as the backward pass will read it.  Rounding to 16 bits keeps the sign, which is all that relu's slope
+// needs, except that a positive z below half the smallest fp16 number would become zero.
+template <typename T, int ACT>
+__device__ __forceinline__ T rounded_z(acc_t<T> v) {
+    T r = from_acc<T>(v);
+    if constexpr (ACT == NB200_ACT_RELU && sizeof(T) == 2)
+        if (v > 0.f && to_acc(r) == 0.f) r = from_acc<T>(5.9604644775390625e-8f);   // 2^-24, representable in both types
+    return r;
+}
+
+// C[i, j] = sum_k A(i, k) B(k, j), one 64 x 64 tile per block, blockIdx.z cuts the sum.  A(i, k) is
+// a[i * as + k] with A_K (k contiguous) or a[i + k * as]; B(k, j) is b[k + j * bs] with B_K or b[k * bs + j].
+template <typename T, bool A_K, bool B_K, int ACT>
+__global__ void __launch_bounds__(kThreads) tile_kernel(int64_t rows, int64_t cols, int64_t depth, int64_t depth_per_split,
+                                                        const T* __restrict__ a, int64_t as, const T* __restrict__ b, int64_t bs,
+                                                        Epilogue<T> ep) {
+    using A = acc_t<T>;
+    __shared__ A sa[kDepth][kTile + 1], sb[kDepth][kTile + 1];
+    const int64_t i0 = blockIdx.x * int64_t(kTile), j0 = blockIdx.y * int64_t(kTile);
+    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    const int64_t k_begin = blockIdx.z * depth_per_split, k_end = min(depth, k_begin + depth_per_split);
+    A acc[4][4] = {};
+    for (int64_t k0 = k_begin; k0 < k_end; k0 += kDepth) {
+#pragma unroll
+        for (int e = threadIdx.x; e < kTile * kDepth; e += kThreads) {
+            const int ai = A_K ? e / kDepth : e % kTile, ak = A_K ? e % kDepth : e / kTile;
+            const int64_t i = i0 + ai, k = k0 + ak;
+            sa[ak][ai] = i < rows && k < k_end ? to_acc(A_K ? a[i * as + k] : a[i + k * as]) : A(0);
+            const int bj = B_K ? e / kDepth : e % kTile, bk = B_K ? e % kDepth : e / kTile;
+            const int64_t j = j0 + bj, kb = k0 + bk;
+            sb[bk][bj] = j < cols && kb < k_end ? to_acc(B_K ? b[kb + j * bs] : b[kb * bs + j]) : A(0);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kDepth; ++k) {
+            A av[4], bv[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                av[q] = sa[k][ty + 16 * q];
+                bv[q] = sb[k][tx + 16 * q];
+            }
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) acc[p][q] += av[p] * bv[q];
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        const int64_t i = i0 + ty + 16 * p;
+        if (i >= rows) continue;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int64_t j = j0 + tx + 16 * q;
+            if (j >= cols) continue;
+            A v = acc[p][q];
+            if (ep.partial) {
+                ep.partial[(blockIdx.z * rows + i) * cols + j] = v;
+                continue;
+            }
+            if (ep.bias) v += to_acc(ep.bias[j]);
+            if (ep.z) ep.z[i * cols + j] = rounded_z<T, ACT>(v);
+            v = activate<ACT>(v);
+            if (ep.residual) v += to_acc(ep.residual[i * ep.ldr + j]);
+            ep.y[i * cols + j] = from_acc<T>(v);
+        }
+    }
+}
+
+// Sum of the splits, in order.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) join_splits_kernel(int64_t size, int splits, const acc_t<T>* __restrict__ partial,
+                                                               T* __restrict__ out) {
+    for (int64_t e = blockIdx.x * int64_t(kThreads) + threadIdx.x; e < size; e += int64_t(gridDim.x) * kThreads) {
+        acc_t<T> v = 0;
+        for (int s = 0; s < splits; ++s) v += partial[s * size + e];
+        out[e] = from_acc<T>(v);
+    }
+}
+
+// dz = dy act'(z) (not stored when dz is NULL: then dy is dz) and the column sums of dz over a band of rows;
+// a block covers 32 columns x its band, 8 rows of threads.
+template <typename T, int ACT>
+__global__ void __launch_bounds__(kThreads) slope_kernel(int64_t rows, int64_t cols, int64_t band, const T* __restrict__ dy, int64_t ldd,
+                                                         const T* __restrict__ z, T* __restrict__ dz, acc_t<T>* __restrict__ sums) {
+    using A = acc_t<T>;
+    __shared__ A sm[8][33];
+    const int64_t j = blockIdx.y * int64_t(32) + threadIdx.x % 32;
+    const int lane = threadIdx.x / 32;
+    const int64_t limit = min(rows, (blockIdx.x + 1) * band);
+    A sum = 0;
+    if (j < cols)
+        for (int64_t i = blockIdx.x * band + lane; i < limit; i += 8) {
+            A v = to_acc(dy[i * ldd + j]);
+            if (ACT != NB200_ACT_NONE) {
+                v *= activate_slope<ACT>(to_acc(z[i * cols + j]));
+                dz[i * cols + j] = from_acc<T>(v);
+            }
+            sum += v;
+        }
+    sm[lane][threadIdx.x % 32] = sum;
+    __syncthreads();
+    if (lane == 0 && j < cols && sums) {
+        for (int q = 1; q < 8; ++q) sum += sm[q][threadIdx.x];
+        sums[blockIdx.x * cols + j] = sum;
+    }
+}
+
+constexpr int64_t kMaxBands = 512;
+int64_t band_rows(int64_t rows) { return rows <= 64 * kMaxBands ? 64 : ceil_div(rows, kMaxBands); }
+int64_t band_count(int64_t rows) { return ceil_div(rows, band_rows(rows)); }
+
+int64_t split_count(int64_t rows, int64_t cols, int64_t depth) {
+    if (rows == 0 || cols == 0) return 1;
+    const int64_t tiles = ceil_div(rows, kTile) * ceil_div(cols, kTile), wanted = ceil_div(kSMs * 4, tiles);
+    const int64_t most = ceil_div(depth, 8 * kDepth);
+    const int64_t s = wanted < most ? wanted : most;
+    return s < 1 ? 1 : s;
+}
+
+size_t round16(size_t bytes) { return (bytes + 15) / 16 * 16; }
+
+struct BackwardLayout {
+    size_t dz, sums, partial, total;
+};
+BackwardLayout backward_layout(int64_t m, int64_t k, int64_t n, int act, int dtype) {
+    const size_t s = dense_dtype_size(dtype), a = dtype == NB200_F64 ? 8 : 4;
+    BackwardLayout l;
+    l.dz = 0;
+    l.sums = l.dz + (act == NB200_ACT_NONE ? 0 : round16(s * m * n));
+    l.partial = l.sums + round16(a * band_count(m) * n);
+    l.total = l.partial + round16(a * split_count(k, n, m) * k * n);
+    return l;
+}
+
+template <typename T, bool A_K, bool B_K, int ACT>
+int launch_tiles(int64_t rows, int64_t cols, int64_t depth, int64_t splits, const T* a, int64_t as, const T* b, int64_t bs,
+                 const Epilogue<T>& ep, cudaStream_t stream) {
+    const int64_t gx = ceil_div(rows, kTile), gy = ceil_div(cols, kTile);
+    if (gx > INT32_MAX || gy > 65535) return NB200_ERR_TOO_LARGE;
+    const int64_t per = ceil_div(ceil_div(depth, splits), kDepth) * kDepth;
+    tile_kernel<T, A_K, B_K, ACT><<<dim3(gx, gy, splits), kThreads, 0, stream>>>(rows, cols, depth, per > 0 ? per : 1, a, as, b, bs, ep);
+    return launch_status();
+}
+
+template <typename T>
+int backward(int64_t m, int64_t k, int64_t n, const T* dy, int64_t ldd, const T* x, int64_t ldx, const T* w, int64_t ldw, const T* z,
+             int act, T* dx, T* dw, T* db, char* work, const BackwardLayout& lay, cudaStream_t stream) {
+    using A = acc_t<T>;
+    T* dz = act == NB200_ACT_NONE ? nullptr : reinterpret_cast<T*>(work + lay.dz);
+    A* sums = reinterpret_cast<A*>(work + lay.sums);
+    A* partial = reinterpret_cast<A*>(work + lay.partial);
+    int rc = NB200_OK;
+    if (dz || db) {
+        const int64_t bands = band_count(m), gy = ceil_div(n, 32);
+        if (gy > 65535) return NB200_ERR_TOO_LARGE;
+        rc = NB200_DISPATCH_ACT(act, (slope_kernel<T, ACT><<<dim3(bands, gy), kThreads, 0, stream>>>(m, n, band_rows(m), dy, ldd, z, dz,
+                                                                                                db ? sums : nullptr), launch_status()));
+        if (rc == NB200_OK && db) {
+            join_splits_kernel<T><<<static_cast<unsigned>(ceil_div(n, kThreads)), kThreads, 0, stream>>>(n, static_cast<int>(bands), sums, db);
+            rc = launch_status();
+        }
+        if (rc != NB200_OK) return rc;
+    }
+    const T* g = dz ? dz : dy;
+    const int64_t ldg = dz ? n : ldd;
+    if (dx) {
+        rc = launch_tiles<T, true, true, NB200_ACT_NONE>(m, k, n, 1, g, ldg, w, ldw, {nullptr, nullptr, 0, nullptr, dx, nullptr}, stream);
+        if (rc != NB200_OK) return rc;
+    }
+    if (dw) {
+        const int64_t splits = split_count(k, n, m);
+        rc = launch_tiles<T, false, false, NB200_ACT_NONE>(k, n, m, splits, x, ldx, g, ldg, {nullptr, nullptr, 0, nullptr, nullptr, partial}, stream);
+        if (rc != NB200_OK) return rc;
+        const int64_t blocks = ceil_div(k * n, kThreads);
+        join_splits_kernel<T><<<static_cast<unsigned>(blocks < kSMs * 8 ? blocks : kSMs * 8), kThreads, 0, stream>>>(
+            k * n, static_cast<int>(splits), partial, dw);
+        rc = launch_status();
+    }
+    return rc;
+}
+
+bool bad_sizes(int64_t m, int64_t k, int64_t n) {
+    constexpr int64_t most = int64_t(1) << 31;
+    return m < 0 || k < 0 || n < 0 || m >= (int64_t(1) << 37) || k >= most || n >= most;
+}
+
+}  // namespace
+}  // namespace nb200
+
+using namespace nb200;
+
+extern "C" int nb200_linear_forward(int64_t m, int64_t k, int64_t n, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                                    const void* bias, const void* residual, int64_t ldr, int activation, void* z, void* y, int dtype,
+                                    nb200_stream stream) {
+    if (bad_sizes(m, k, n) || !known_dense_dtype(dtype) || !known_activation(activation)) return NB200_ERR_BAD_ARG;
+    if (m == 0 || n == 0) return NB200_OK;
+    if ((k > 0 && (!x || !w)) || !y || ldx < k || ldw < n || (residual && ldr < n)) return NB200_ERR_BAD_ARG;
+    return NB200_DISPATCH_DENSE(dtype, ([&]() -> int {
+        const Epilogue<T> ep{static_cast<const T*>(bias), static_cast<const T*>(residual), ldr, static_cast<T*>(z), static_cast<T*>(y), nullptr};
+        return NB200_DISPATCH_ACT(activation, (launch_tiles<T, true, false, ACT>(m, n, k, 1, static_cast<const T*>(x), ldx,
+                                                                                static_cast<const T*>(w), ldw, ep, as_stream(stream))));
+    }()));
+}
+
+extern "C" size_t nb200_linear_backward_workspace_bytes(int64_t m, int64_t k, int64_t n, int activation, int dtype) {
+    if (bad_sizes(m, k, n) || !known_dense_dtype(dtype) || !known_activation(activation)) return 0;
+    return backward_layout(m, k, n, activation, dtype).total;
+}
+
+extern "C" int nb200_linear_backward(int64_t m, int64_t k, int64_t n, const void* dy, int64_t lddy, const void* x, int64_t ldx,
+                                     const void* w, int64_t ldw, const void* z, int activation, void* dx, void* dw, void* dbias,
+                                     void* work, size_t work_bytes, int dtype, nb200_stream stream) {
+    if (bad_sizes(m, k, n) || !known_dense_dtype(dtype) || !known_activation(activation)) return NB200_ERR_BAD_ARG;
+    const size_t s = dense_dtype_size(dtype);
+    const cudaStream_t st = as_stream(stream);
+    if (m == 0 || n == 0) {                      // empty sums
+        if ((dx && m * k > 0 && cudaMemsetAsync(dx, 0, s * m * k, st) != cudaSuccess) ||
+            (dw && k * n > 0 && cudaMemsetAsync(dw, 0, s * k * n, st) != cudaSuccess) ||
+            (dbias && n > 0 && cudaMemsetAsync(dbias, 0, s * n, st) != cudaSuccess))
+            return NB200_ERR_CUDA;
+        return NB200_OK;
+    }
+    if (!dy || lddy < n || ldx < k || ldw < n || (activation != NB200_ACT_NONE && !z)) return NB200_ERR_BAD_ARG;
+    if (k > 0 && ((dx && !w) || (dw && !x))) return NB200_ERR_BAD_ARG;
+    const BackwardLayout lay = backward_layout(m, k, n, activation, dtype);
+    if (lay.total > 0 && (!work || work_bytes < lay.total)) return NB200_ERR_WORKSPACE;
+    if (!aligned16(work)) return NB200_ERR_ALIGN;
+    return NB200_DISPATCH_DENSE(dtype, (backward<T>(m, k, n, static_cast<const T*>(dy), lddy, static_cast<const T*>(x), ldx,
+                                                    static_cast<const T*>(w), ldw, static_cast<const T*>(z), activation,
+                                                    k > 0 ? static_cast<T*>(dx) : nullptr, k > 0 ? static_cast<T*>(dw) : nullptr,
+                                                    static_cast<T*>(dbias), static_cast<char*>(work), lay, st)));
+}

@@ -6,8 +6,14 @@ helpers ``:171-234``): same class names, constructor arguments, parameter names 
 is the SpMM ``A @ X`` (``SparseCSRTensor.__matmul__`` -> ``spdmm``) and, when the layer normalises,
 the row sums of A (``SparseCSRTensor.row_sum`` -> ``sprowsum``); both run on this package's CUDA
 kernels and are differentiable with respect to the stored values of A as well as X.
+
+Beside them, for the dense half of a network and with the same calling convention ``layer(A, X)``:
+``Linear`` (product, bias, activation and residual in one kernel), ``GroupNorm`` (with an activation, per
+graph of a batch) and ``Dropout`` (mask recomputed from a counter), on :mod:`numml_b200.functional`.
 """
 import torch
+
+from . import functional as F
 
 
 def _as_feature_matrix(X):
@@ -21,10 +27,13 @@ def _inv_sqrt_degree(row_sums):
 
 
 class _GraphConv(torch.nn.Module):
-    """What the two layers share: channel counts, the normalisation switch, the bias."""
+    """What the two layers share: channel counts, the normalisation switch, the bias, and how the dense
+    products X W run: by ``torch.matmul``, or with ``fused=True`` by ``functional.linear`` (which needs CUDA
+    tensors, adds a bias or the sum so far in its epilogue and takes float32 products to the tensor cores)."""
 
-    def __init__(self, in_channels, out_channels, normalize, weight_shape):
+    def __init__(self, in_channels, out_channels, normalize, weight_shape, fused=False):
         super().__init__()
+        self.fused = fused
         # registration order (weights, then bias) fixes the layout of model_to_vector
         self.weights = torch.nn.Parameter(torch.randn(*weight_shape))
         self.bias = torch.nn.Parameter(torch.randn(out_channels))
@@ -38,11 +47,12 @@ class GCNConv(_GraphConv):
     ``Y = D~^(-1/2) (A + I) D~^(-1/2) X W + b`` (``normalize=True``) or ``Y = A X W + b``.
     Reference ``numml/nn.py:6-101``."""
 
-    def __init__(self, in_channels, out_channels, normalize=True):
-        super().__init__(in_channels, out_channels, normalize, (in_channels, out_channels))
+    def __init__(self, in_channels, out_channels, normalize=True, fused=False):
+        super().__init__(in_channels, out_channels, normalize, (in_channels, out_channels), fused)
 
-    def _convolve(self, matmul, row_sums, X):
-        Z = _as_feature_matrix(X) @ self.weights
+    def _convolve(self, matmul, row_sums, X, fused=False):
+        X = _as_feature_matrix(X)
+        Z = F.linear(X, self.weights) if fused else X @ self.weights
         if self.normalize:
             d = _inv_sqrt_degree(row_sums())
             Z = d * Z
@@ -53,7 +63,7 @@ class GCNConv(_GraphConv):
 
     def forward(self, A, X):
         """A: ``SparseCSRTensor`` or ``LinearOperator``; X: [nodes, in_channels] or [nodes]."""
-        return self._convolve(lambda Z: A @ Z, A.row_sum, X)
+        return self._convolve(lambda Z: A @ Z, A.row_sum, X, self.fused)
 
     def forward_dense(self, A, X):
         """The same layer evaluated on ``A.to_dense()`` (a check, and the only form that runs on CPU)."""
@@ -66,8 +76,8 @@ class TAGConv(_GraphConv):
     ``P(X) = A X`` or, normalised, ``P(X) = d * (A (d * X + X))`` with ``d = (rowsum(A) + 1)^(-1/2)``
     (the reference's update, ``numml/nn.py:104-168``, kept as it is written there)."""
 
-    def __init__(self, in_channels, out_channels, k=2, normalize=True):
-        super().__init__(in_channels, out_channels, normalize, (k, in_channels, out_channels))
+    def __init__(self, in_channels, out_channels, k=2, normalize=True, fused=False):
+        super().__init__(in_channels, out_channels, normalize, (k, in_channels, out_channels), fused)
         self.k = k
 
     def forward(self, A, X):
@@ -76,11 +86,85 @@ class TAGConv(_GraphConv):
         H = None
         for j in range(self.k):
             Xc = d * (A @ (d * Xc + Xc)) if self.normalize else A @ Xc
+            if self.fused:                             # bias with the first hop, each further hop on top of the sum
+                H = F.linear(Xc, self.weights[j], bias=self.bias if H is None else None, residual=H)
+                continue
             term = Xc @ self.weights[j]
             H = term if H is None else H + term
         if H is None:                                  # k = 0: only the bias
             H = torch.zeros(Xc.shape[0], self.out_channels, dtype=Xc.dtype, device=Xc.device)
+        elif self.fused:
+            return H
         return H + self.bias
+
+
+class Linear(torch.nn.Module):
+    """``act(X W + b) + residual`` on the node features (the graph argument is not used)."""
+
+    def __init__(self, in_channels, out_channels, bias=True, activation=None):
+        super().__init__()
+        F._activation_code(activation)
+        self.weights = torch.nn.Parameter(torch.randn(in_channels, out_channels) * in_channels ** -0.5 if in_channels else
+                                          torch.zeros(in_channels, out_channels))
+        self.bias = torch.nn.Parameter(torch.zeros(out_channels)) if bias else None
+        self.in_channels, self.out_channels, self.activation = in_channels, out_channels, activation
+
+    def forward(self, A, X, residual=None):
+        """X: [nodes, in_channels] or [nodes]; residual: [nodes, out_channels] or None."""
+        return F.linear(_as_feature_matrix(X), self.weights, self.bias, self.activation, residual)
+
+
+class GroupNorm(torch.nn.Module):
+    """Group norm over the nodes of each graph with an activation (the matrix argument is not used).
+    Call with ``ptr`` for a batch of graphs, see :func:`numml_b200.functional.group_norm`."""
+
+    def __init__(self, groups, channels, eps=1e-5, affine=True, activation=None):
+        super().__init__()
+        F._activation_code(activation)
+        if groups < 1 or channels % groups != 0:
+            raise RuntimeError(f"{channels} channels cannot be split into {groups} groups")
+        self.groups, self.channels, self.eps, self.activation = groups, channels, eps, activation
+        self.weight = torch.nn.Parameter(torch.ones(channels)) if affine else None
+        self.bias = torch.nn.Parameter(torch.zeros(channels)) if affine else None
+
+    def forward(self, A, X, ptr=None):
+        return F.group_norm(_as_feature_matrix(X), self.groups, self.weight, self.bias, self.eps, self.activation, ptr)
+
+
+class Dropout(torch.nn.Module):
+    """Dropout of the node features in training mode, the identity in evaluation mode.
+
+    ``seed`` (drawn from torch's generator when None) and a counter of the calls made so far name the mask.
+    They live on the host, where a captured CUDA graph would freeze them, so a call under capture raises
+    unless the layer was made with ``capturable=True``: then they are a buffer on the device that every
+    call advances, and a replayed graph takes new masks."""
+
+    def __init__(self, p=0.5, seed=None, capturable=False):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise RuntimeError(f"dropout probability must be in [0, 1], got {p}")
+        self.p = p
+        self.seed = int(torch.randint(0, 1 << 62, (1,))) if seed is None else int(seed)
+        self.calls = 0
+        if capturable:
+            # the words are int64: a seed of 2**63 and above is stored as the negative number of the same bits
+            word = self.seed - (1 << 64) if self.seed >= 1 << 63 else self.seed
+            self.register_buffer("state", torch.tensor([word, 0], dtype=torch.int64), persistent=False)
+        else:
+            self.state = None
+
+    def forward(self, A, X):
+        if not self.training:
+            return X
+        if self.state is None:
+            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("Dropout under CUDA graph capture needs capturable=True: "
+                                   "the captured graph would repeat one mask for ever")
+            self.calls += 1
+            return F.dropout(X, self.p, self.seed, self.calls - 1)
+        now = self.state.clone()
+        self.state[1] += 1
+        return F.dropout(X, self.p, now)
 
 
 class SeqWrapper(torch.nn.Module):
