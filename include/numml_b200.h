@@ -617,15 +617,16 @@ typedef enum {
  *
  * Backward, dz = dy act'(z):  dx = dz w^T [m, k],  dw = x^T dz [k, n],  dbias = column sums of dz [n], each
  * contiguous and each skipped when NULL; the residual's gradient is dy itself.  z may be NULL for NB200_ACT_NONE.
- * No alignment is required of any array but `work` (16 bytes).  Results do not depend on the run: sums are cut at
+ * `status` (device word, may be NULL) receives NB200_ERR_WAIT_BUDGET if a bounded wait of a kernel ever runs out.
+ * No alignment is required of any array but `work` (16 bytes); aligned rows are read faster.  Results do not depend on the run: sums are cut at
  * places that depend on the sizes alone and joined in order. */
 NB200_API int nb200_linear_forward(int64_t m, int64_t k, int64_t n, const void* x, int64_t ldx, const void* w, int64_t ldw,
                                    const void* bias, const void* residual, int64_t ldr, int activation, void* z, void* y,
-                                   int dtype, nb200_stream stream);
+                                   int32_t* status, int dtype, nb200_stream stream);
 NB200_API size_t nb200_linear_backward_workspace_bytes(int64_t m, int64_t k, int64_t n, int activation, int dtype);
 NB200_API int nb200_linear_backward(int64_t m, int64_t k, int64_t n, const void* dy, int64_t lddy, const void* x, int64_t ldx,
                                     const void* w, int64_t ldw, const void* z, int activation, void* dx, void* dw, void* dbias,
-                                    void* work, size_t work_bytes, int dtype, nb200_stream stream);
+                                    void* work, size_t work_bytes, int32_t* status, int dtype, nb200_stream stream);
 
 /* Group norm with an activation, y = act((x - mean) rstd weight + bias), over contiguous rows [rows, channels].
  * Mean and biased variance are taken over the rows of a segment and the channels / groups neighbouring channels of

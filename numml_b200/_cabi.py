@@ -85,9 +85,10 @@ SIGNATURES = {
     "nb200_ipc_open": (_int, [_vp, _c.POINTER(_vp)]),
     "nb200_ipc_close": (_int, [_vp]),
     "nb200_ipc_free": (_int, [_vp]),
-    "nb200_linear_forward": (_int, [_i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _int, _vp, _vp, _int, _vp]),
+    "nb200_linear_forward": (_int, [_i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _int, _vp, _vp, _vp, _int, _vp]),
     "nb200_linear_backward_workspace_bytes": (_sz, [_i64, _i64, _i64, _int, _int]),
-    "nb200_linear_backward": (_int, [_i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _int, _vp, _vp, _vp, _vp, _sz, _int, _vp]),
+    "nb200_linear_backward": (_int, [_i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _int, _vp, _vp, _vp, _vp, _sz, _vp, _int,
+                                     _vp]),
     "nb200_group_norm_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _int]),
     "nb200_group_norm_forward": (_int, [_i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _f64, _int, _vp, _vp, _vp, _vp, _sz, _int, _vp]),
     "nb200_group_norm_backward": (_int, [_i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _sz,

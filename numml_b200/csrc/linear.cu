@@ -2,34 +2,17 @@
 //   dz = dy act'(z),  dx = dz w^T,  dw = x^T dz,  dbias = column sums of dz
 // with z = x w + bias as the forward pass left it.  x [m, k], w [k, n], y [m, n].
 //
-// This file holds the entry points and the kernels that take any type, size and stride on the CUDA cores.
-#include "dense_common.cuh"
+// This file holds the entry points, the products that run on the CUDA cores (double, for which the tensor
+// cores of this GPU are no faster, and empty sums) and the passes around the products; linear_mma.cu holds
+// the products on the tensor cores.
+#include <type_traits>
+
+#include "linear_mma.cuh"
 
 namespace nb200 {
 namespace {
 
 constexpr int kTile = 64, kDepth = 16, kThreads = 256;
-
-// What the epilogue of a product needs; absent parts are NULL.
-template <typename T>
-struct Epilogue {
-    const T* bias;
-    const T* residual;
-    int64_t ldr;
-    T* z;                 // [rows, cols] contiguous
-    T* y;                 // [rows, cols] contiguous
-    acc_t<T>* partial;    // instead of all of the above: [splits, rows, cols]
-};
-
-// z as the backward pass will read it.  Rounding to 16 bits keeps the sign, which is all that relu's slope
-// needs, except that a positive z below half the smallest fp16 number would become zero.
-template <typename T, int ACT>
-__device__ __forceinline__ T rounded_z(acc_t<T> v) {
-    T r = from_acc<T>(v);
-    if constexpr (ACT == NB200_ACT_RELU && sizeof(T) == 2)
-        if (v > 0.f && to_acc(r) == 0.f) r = from_acc<T>(5.9604644775390625e-8f);   // 2^-24, representable in both types
-    return r;
-}
 
 // C[i, j] = sum_k A(i, k) B(k, j), one 64 x 64 tile per block, blockIdx.z cuts the sum.  A(i, k) is
 // a[i * as + k] with A_K (k contiguous) or a[i + k * as]; B(k, j) is b[k + j * bs] with B_K or b[k * bs + j].
@@ -134,12 +117,27 @@ constexpr int64_t kMaxBands = 512;
 int64_t band_rows(int64_t rows) { return rows <= 64 * kMaxBands ? 64 : ceil_div(rows, kMaxBands); }
 int64_t band_count(int64_t rows) { return ceil_div(rows, band_rows(rows)); }
 
-int64_t split_count(int64_t rows, int64_t cols, int64_t depth) {
-    if (rows == 0 || cols == 0) return 1;
+// Whether a product runs on the tensor cores.
+template <typename T>
+constexpr bool on_tensor_cores(int64_t depth) { return !std::is_same<T, double>::value && depth > 0; }
+
+// Into how many parts the sum over the rows is cut for dw, so that there is work for every SM, and how long one is.
+struct Split {
+    int64_t parts, per;
+};
+Split split_sum(int64_t rows, int64_t cols, int64_t depth, int dtype) {
+    if (rows == 0 || cols == 0 || depth == 0) return {1, kMmaChunk};
+    if (dtype != NB200_F64) {
+        const int64_t tiles = ceil_div(rows, kMmaTile) * ceil_div(cols, kMmaTile);
+        const int64_t wanted = tiles < kSMs ? kSMs / tiles : 1;
+        const int64_t per = ceil_div(ceil_div(depth, wanted), kMmaChunk) * kMmaChunk;
+        return {ceil_div(depth, per), per};
+    }
     const int64_t tiles = ceil_div(rows, kTile) * ceil_div(cols, kTile), wanted = ceil_div(kSMs * 4, tiles);
     const int64_t most = ceil_div(depth, 8 * kDepth);
-    const int64_t s = wanted < most ? wanted : most;
-    return s < 1 ? 1 : s;
+    const int64_t parts = wanted < most ? wanted : (most < 1 ? 1 : most);
+    const int64_t per = ceil_div(ceil_div(depth, parts), kDepth) * kDepth;
+    return {ceil_div(depth, per), per};
 }
 
 size_t round16(size_t bytes) { return (bytes + 15) / 16 * 16; }
@@ -153,23 +151,27 @@ BackwardLayout backward_layout(int64_t m, int64_t k, int64_t n, int act, int dty
     l.dz = 0;
     l.sums = l.dz + (act == NB200_ACT_NONE ? 0 : round16(s * m * n));
     l.partial = l.sums + round16(a * band_count(m) * n);
-    l.total = l.partial + round16(a * split_count(k, n, m) * k * n);
+    l.total = l.partial + round16(a * split_sum(k, n, m, dtype).parts * k * n);
     return l;
 }
 
 template <typename T, bool A_K, bool B_K, int ACT>
-int launch_tiles(int64_t rows, int64_t cols, int64_t depth, int64_t splits, const T* a, int64_t as, const T* b, int64_t bs,
-                 const Epilogue<T>& ep, cudaStream_t stream) {
+int product(int64_t rows, int64_t cols, int64_t depth, Split split, const T* a, int64_t as, const T* b, int64_t bs,
+            const Epilogue<T>& ep, int32_t* status, cudaStream_t stream) {
+    if constexpr (!std::is_same<T, double>::value)
+        if (on_tensor_cores<T>(depth))
+            return mma_product<T, A_K, B_K, ACT>(rows, cols, depth, split.parts, split.per, a, as, b, bs, ep, status, stream);
     const int64_t gx = ceil_div(rows, kTile), gy = ceil_div(cols, kTile);
     if (gx > INT32_MAX || gy > 65535) return NB200_ERR_TOO_LARGE;
-    const int64_t per = ceil_div(ceil_div(depth, splits), kDepth) * kDepth;
-    tile_kernel<T, A_K, B_K, ACT><<<dim3(gx, gy, splits), kThreads, 0, stream>>>(rows, cols, depth, per > 0 ? per : 1, a, as, b, bs, ep);
+    tile_kernel<T, A_K, B_K, ACT><<<dim3(gx, gy, split.parts), kThreads, 0, stream>>>(rows, cols, depth, split.per, a, as, b, bs, ep);
     return launch_status();
 }
 
+Split whole(int64_t depth) { return {1, depth > 0 ? ceil_div(depth, kMmaChunk) * kMmaChunk : kMmaChunk}; }
+
 template <typename T>
 int backward(int64_t m, int64_t k, int64_t n, const T* dy, int64_t ldd, const T* x, int64_t ldx, const T* w, int64_t ldw, const T* z,
-             int act, T* dx, T* dw, T* db, char* work, const BackwardLayout& lay, cudaStream_t stream) {
+             int act, T* dx, T* dw, T* db, char* work, const BackwardLayout& lay, int dtype, int32_t* status, cudaStream_t stream) {
     using A = acc_t<T>;
     T* dz = act == NB200_ACT_NONE ? nullptr : reinterpret_cast<T*>(work + lay.dz);
     A* sums = reinterpret_cast<A*>(work + lay.sums);
@@ -189,16 +191,18 @@ int backward(int64_t m, int64_t k, int64_t n, const T* dy, int64_t ldd, const T*
     const T* g = dz ? dz : dy;
     const int64_t ldg = dz ? n : ldd;
     if (dx) {
-        rc = launch_tiles<T, true, true, NB200_ACT_NONE>(m, k, n, 1, g, ldg, w, ldw, {nullptr, nullptr, 0, nullptr, dx, nullptr}, stream);
+        rc = product<T, true, true, NB200_ACT_NONE>(m, k, n, whole(n), g, ldg, w, ldw, {nullptr, nullptr, 0, nullptr, dx, nullptr}, status,
+                                                    stream);
         if (rc != NB200_OK) return rc;
     }
     if (dw) {
-        const int64_t splits = split_count(k, n, m);
-        rc = launch_tiles<T, false, false, NB200_ACT_NONE>(k, n, m, splits, x, ldx, g, ldg, {nullptr, nullptr, 0, nullptr, nullptr, partial}, stream);
+        const Split split = split_sum(k, n, m, dtype);
+        rc = product<T, false, false, NB200_ACT_NONE>(k, n, m, split, x, ldx, g, ldg, {nullptr, nullptr, 0, nullptr, nullptr, partial}, status,
+                                                      stream);
         if (rc != NB200_OK) return rc;
         const int64_t blocks = ceil_div(k * n, kThreads);
         join_splits_kernel<T><<<static_cast<unsigned>(blocks < kSMs * 8 ? blocks : kSMs * 8), kThreads, 0, stream>>>(
-            k * n, static_cast<int>(splits), partial, dw);
+            k * n, static_cast<int>(split.parts), partial, dw);
         rc = launch_status();
     }
     return rc;
@@ -215,15 +219,15 @@ bool bad_sizes(int64_t m, int64_t k, int64_t n) {
 using namespace nb200;
 
 extern "C" int nb200_linear_forward(int64_t m, int64_t k, int64_t n, const void* x, int64_t ldx, const void* w, int64_t ldw,
-                                    const void* bias, const void* residual, int64_t ldr, int activation, void* z, void* y, int dtype,
-                                    nb200_stream stream) {
+                                    const void* bias, const void* residual, int64_t ldr, int activation, void* z, void* y,
+                                    int32_t* status, int dtype, nb200_stream stream) {
     if (bad_sizes(m, k, n) || !known_dense_dtype(dtype) || !known_activation(activation)) return NB200_ERR_BAD_ARG;
     if (m == 0 || n == 0) return NB200_OK;
     if ((k > 0 && (!x || !w)) || !y || ldx < k || ldw < n || (residual && ldr < n)) return NB200_ERR_BAD_ARG;
     return NB200_DISPATCH_DENSE(dtype, ([&]() -> int {
         const Epilogue<T> ep{static_cast<const T*>(bias), static_cast<const T*>(residual), ldr, static_cast<T*>(z), static_cast<T*>(y), nullptr};
-        return NB200_DISPATCH_ACT(activation, (launch_tiles<T, true, false, ACT>(m, n, k, 1, static_cast<const T*>(x), ldx,
-                                                                                static_cast<const T*>(w), ldw, ep, as_stream(stream))));
+        return NB200_DISPATCH_ACT(activation, (product<T, true, false, ACT>(m, n, k, whole(k), static_cast<const T*>(x), ldx,
+                                                                           static_cast<const T*>(w), ldw, ep, status, as_stream(stream))));
     }()));
 }
 
@@ -234,7 +238,7 @@ extern "C" size_t nb200_linear_backward_workspace_bytes(int64_t m, int64_t k, in
 
 extern "C" int nb200_linear_backward(int64_t m, int64_t k, int64_t n, const void* dy, int64_t lddy, const void* x, int64_t ldx,
                                      const void* w, int64_t ldw, const void* z, int activation, void* dx, void* dw, void* dbias,
-                                     void* work, size_t work_bytes, int dtype, nb200_stream stream) {
+                                     void* work, size_t work_bytes, int32_t* status, int dtype, nb200_stream stream) {
     if (bad_sizes(m, k, n) || !known_dense_dtype(dtype) || !known_activation(activation)) return NB200_ERR_BAD_ARG;
     const size_t s = dense_dtype_size(dtype);
     const cudaStream_t st = as_stream(stream);
@@ -253,5 +257,5 @@ extern "C" int nb200_linear_backward(int64_t m, int64_t k, int64_t n, const void
     return NB200_DISPATCH_DENSE(dtype, (backward<T>(m, k, n, static_cast<const T*>(dy), lddy, static_cast<const T*>(x), ldx,
                                                     static_cast<const T*>(w), ldw, static_cast<const T*>(z), activation,
                                                     k > 0 ? static_cast<T*>(dx) : nullptr, k > 0 ? static_cast<T*>(dw) : nullptr,
-                                                    static_cast<T*>(dbias), static_cast<char*>(work), lay, st)));
+                                                    static_cast<T*>(dbias), static_cast<char*>(work), lay, dtype, status, st)));
 }

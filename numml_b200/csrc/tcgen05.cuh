@@ -1,0 +1,100 @@
+// The few PTX instructions of the 5th-generation tensor cores that this library uses: tensor memory
+// allocation, matrix products from shared-memory descriptors, commits to mbarriers, loads of accumulators.
+#pragma once
+#include "common.cuh"
+
+namespace nb200 {
+namespace tc {
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+// ---- mbarriers; every wait is bounded -----------------------------------------------------------------
+constexpr long long kWaitCycles = 4000000000LL;      // about two seconds: a wait that long means a mistake, not load
+
+__device__ __forceinline__ void mbar_init(uint64_t* bar, unsigned count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(smem_u32(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" :: "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t addr, unsigned parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(addr), "r"(parity) : "memory");
+    return ok != 0;
+}
+// False when the wait ran out, or when another warp's has (`gave_up`): the caller leaves its loop.
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, unsigned parity, volatile int* gave_up) {
+    const uint32_t addr = smem_u32(bar);
+    if (mbar_try(addr, parity)) return true;
+    const long long t0 = clock64();
+    while (!mbar_try(addr, parity))
+        if (*gave_up || clock64() - t0 > kWaitCycles) {
+            *gave_up = 1;
+            return false;
+        }
+    return true;
+}
+
+// ---- tensor memory ------------------------------------------------------------------------------------
+// Whole warp; `columns` a power of two, 32..512.
+__device__ __forceinline__ void tmem_alloc(uint32_t* where, uint32_t columns) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(where)), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_dealloc(uint32_t base, uint32_t columns) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(base), "r"(columns));
+}
+// 32 consecutive columns of the warp's 32 lanes: thread l receives lane l's.
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+                   "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+                   "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int q = 0; q < 32; ++q) v[q] = __uint_as_float(r[q]);
+}
+__device__ __forceinline__ void fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// Shared memory written by this thread becomes visible to the tensor cores and bulk copies.
+__device__ __forceinline__ void fence_smem_for_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// ---- operands in shared memory ------------------------------------------------------------------------
+// Both layouts are made of 1024-byte atoms of eight 128-byte lines, 16-byte unit u of line l stored at unit u ^ l.
+// K-major: a line is one row's 64 values along the sum; atoms follow one another every eight rows, 1024 bytes.
+// MN-major: a line is one sum index's 64 rows; the next eight sum indices are 1024 bytes further, the next 64
+// rows `block` bytes further.
+__device__ __forceinline__ uint64_t smem_descriptor(uint32_t addr, uint32_t leading_bytes, uint32_t stride_bytes) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | static_cast<uint64_t>((leading_bytes >> 4) & 0x3FFF) << 16 |
+           static_cast<uint64_t>((stride_bytes >> 4) & 0x3FFF) << 32 | uint64_t(1) << 46 /* version */ |
+           uint64_t(2) << 61 /* 128-byte swizzle */;
+}
+// kind::f16 with float accumulators, M = 128.
+__host__ __device__ constexpr uint32_t instruction_descriptor(bool bf16, bool a_mn_major, bool b_mn_major, int n) {
+    return 1u << 4 | (bf16 ? 1u : 0u) << 7 | (bf16 ? 1u : 0u) << 10 | (a_mn_major ? 1u : 0u) << 15 | (b_mn_major ? 1u : 0u) << 16 |
+           static_cast<uint32_t>(n / 8) << 17 | (128u / 16) << 24;
+}
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u) : "memory");
+}
+// Arrives on `bar` when all products issued so far by this thread are done.
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(smem_u32(bar)) : "memory");
+}
+
+// ---- asynchronous 16-byte copies, the bytes beyond `valid` filled with zeros -----------------------------
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(valid) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+
+}  // namespace tc
+}  // namespace nb200

@@ -17,7 +17,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _cabi
-from .numml_torch_cpp import _on, _ptr, _require_cuda, _stream
+from .numml_torch_cpp import _on, _ptr, _require_cuda, _status_word, _stream
 
 _DTYPES = {torch.float32: _cabi.F32, torch.float64: _cabi.F64, torch.bfloat16: _cabi.BF16, torch.float16: _cabi.F16}
 _ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "tanh": 4}
@@ -80,7 +80,7 @@ def _linear_forward(X, weights, bias, residual, act, keep_z):
         y = torch.empty(X.shape[:-1] + (N,), dtype=X.dtype, device=X.device)
         z = torch.empty((M, N), dtype=X.dtype, device=X.device) if keep_z and act else None
         _cabi.call("nb200_linear_forward", M, K, N, _ptr(x), ldx, _ptr(w), ldw, _ptr(b), _ptr(r), ldr, act, _ptr(z), _ptr(y),
-                   _DTYPES[X.dtype], _stream())
+                   _ptr(_status_word(X.device)), _DTYPES[X.dtype], _stream())
     return y, z
 
 
@@ -97,7 +97,7 @@ def _linear_backward(dY, X, weights, z, act, want_x, want_w, want_b):
         db = torch.empty((N,), dtype=X.dtype, device=X.device) if want_b else None
         work = torch.empty(_cabi.lib().nb200_linear_backward_workspace_bytes(M, K, N, act, code), dtype=torch.uint8, device=X.device)
         _cabi.call("nb200_linear_backward", M, K, N, _ptr(g), ldg, _ptr(x), ldx, _ptr(w), ldw, _ptr(z), act, _ptr(dx), _ptr(dw),
-                   _ptr(db), _ptr(work), work.numel(), code, _stream())
+                   _ptr(db), _ptr(work), work.numel(), _ptr(_status_word(X.device)), code, _stream())
     return dx, dw, db
 
 
