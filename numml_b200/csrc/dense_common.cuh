@@ -51,13 +51,18 @@ __device__ __forceinline__ double erf_acc(double v) { return erf(v); }
 __device__ __forceinline__ float tanh_acc(float v) { return tanhf(v); }
 __device__ __forceinline__ double tanh_acc(double v) { return tanh(v); }
 
+// 1 / (1 + exp(-z)).  In 32 bits with the short exponential and division, whose errors of a few units relative to
+// exp(-z) are multiplied by exp(-z) / (1 + exp(-z)): they fade where they grow.  exp(-z) = infinity gives 0.
+__device__ __forceinline__ float logistic(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+__device__ __forceinline__ double logistic(double z) { return 1.0 / (1.0 + exp(-z)); }
+
 constexpr double kRootHalf = 0.70710678118654752440;     // 1 / sqrt(2)
 constexpr double kInvRoot2Pi = 0.39894228040143267794;   // 1 / sqrt(2 pi)
 
 template <int ACT, typename A>
 __device__ __forceinline__ A activate(A z) {
     if constexpr (ACT == NB200_ACT_RELU) return z > A(0) ? z : (z != z ? z : A(0));
-    if constexpr (ACT == NB200_ACT_SILU) return z / (A(1) + exp_acc(-z));
+    if constexpr (ACT == NB200_ACT_SILU) return z * logistic(z);
     if constexpr (ACT == NB200_ACT_GELU) return A(0.5) * z * (A(1) + erf_acc(z * A(kRootHalf)));
     if constexpr (ACT == NB200_ACT_TANH) return tanh_acc(z);
     return z;
@@ -68,7 +73,7 @@ template <int ACT, typename A>
 __device__ __forceinline__ A activate_slope(A z) {
     if constexpr (ACT == NB200_ACT_RELU) return z > A(0) ? A(1) : (z != z ? z : A(0));
     if constexpr (ACT == NB200_ACT_SILU) {
-        const A s = A(1) / (A(1) + exp_acc(-z));
+        const A s = logistic(z);
         return s * (A(1) + z * (A(1) - s));
     }
     if constexpr (ACT == NB200_ACT_GELU)

@@ -7,9 +7,9 @@
 // term, under the rounding of one float multiply-add.  bfloat16 and half go in as they are.
 //
 // One persistent block per SM, warps specialised: eight loader warps bring chunks of 64 terms of both
-// operands into shared memory (float: through registers, split on the way; 16-bit types: asynchronous
-// copies), one thread issues the products, eight epilogue warps take finished accumulators out of tensor
-// memory, turn them so that a row is written in whole 128-byte lines, and apply bias, activation, residual
+// operands into shared memory (float: through registers, split on the way; 16-bit types: one thread issues
+// tiled bulk copies, or, where rows do not start on 16-byte boundaries, all gather them), one thread issues
+// the products, eight epilogue warps take finished accumulators out of tensor memory, turn them so that a row is written in whole 128-byte lines, and apply bias, activation, residual
 // and rounding.  Accumulators are double-buffered, so the products of a tile run under the epilogue of the
 // one before.  When a tile's second operand fits beside the ring of the first (the weights of a layer with
 // few channels), it is loaded and split once per block and the rows stream past it.
@@ -18,6 +18,9 @@
 // therefore have an accumulator of their own, into which one addition goes per 16 terms (the five smaller ones
 // go to a second, where a truncation weighs 2^-8 as much), and both are taken out every kDrainChunks chunks
 // and added up in registers with rounding to nearest.
+#include <cuda.h>
+
+#include <atomic>
 #include <type_traits>
 
 #include "linear_mma.cuh"
@@ -27,7 +30,11 @@ namespace nb200 {
 namespace {
 
 constexpr int kEpilogueWarps = 8, kLoaderWarps = 8, kLoaders = kLoaderWarps * 32;
-constexpr int kThreads = (kEpilogueWarps + kLoaderWarps + 1) * 32;
+constexpr int kThreads = (kEpilogueWarps + kLoaderWarps + 4) * 32;   // whole warpgroups; three warps of the last are idle
+// Registers per thread at launch (float; checked on the host) and after the warpgroups have shared them out anew.
+constexpr int kLaunchRegisters = 96, kEpilogueRegisters = 104, kLoaderRegisters = 112, kProductRegisters = 48;
+static_assert(kEpilogueWarps * kEpilogueRegisters + kLoaderWarps * kLoaderRegisters + 4 * kProductRegisters <=
+              (kEpilogueWarps + kLoaderWarps + 4) * kLaunchRegisters, "registers beyond the block's own would be waited for for ever");
 constexpr int kPieceBytes = kMmaTile * kMmaChunk * 2;              // one piece of one operand's chunk: 16 KB
 constexpr int kUnits = kMmaTile * kMmaChunk / 8 / kLoaders;        // units of eight values per loader thread
 constexpr int kDrainChunks = 2;
@@ -66,10 +73,10 @@ struct Operand {
 template <typename T>
 struct Args {
     Operand<T> a, b;
-    int64_t rows, cols, depth, per;
-    int64_t row_tiles, col_tiles, items;
-    int chunks;               // chunks of the longest part of the sum
-    bool resident, vector_out;
+    int64_t rows, cols, depth;
+    int row_tiles, col_tiles, items;
+    int chunks;               // chunks of a part of the sum (the last part may have fewer)
+    bool resident, vector_out, tiled;
     Epilogue<T> ep;
     int32_t* status;
 };
@@ -132,26 +139,21 @@ __device__ __forceinline__ void split_store(uint32_t addr, const float (&v)[8]) 
 }
 
 template <typename T, bool K_MAJOR>
-__device__ __forceinline__ void copy_units(const Operand<T>& o, uint32_t slot, int t, int64_t m0, int64_t k0, int64_t k_end) {
+__device__ __forceinline__ void gather_units(const Operand<T>& o, uint32_t slot, int t, int64_t m0, int64_t k0, int64_t k_end) {
     using U = UnitPlace<T, K_MAJOR>;
 #pragma unroll
     for (int q = 0; q < kUnits; ++q) {
         const int64_t m = m0 + U::mn(t, q), k = k0 + U::k(t, q);
         const int valid = U::valid(m, k, o.extent, k_end);
-        const T* p = valid > 0 ? U::address(o, m, k) : o.p;
-        const uint32_t dst = slot + U::offset(t, q);
-        if (o.vector) {
-            tc::copy16(dst, p, valid * 2);
-        } else {
-            uint32_t w[4];
+        const unsigned short* p = reinterpret_cast<const unsigned short*>(U::address(o, m, k));
+        uint32_t w[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t lo = 2 * e < valid ? __ldg(reinterpret_cast<const unsigned short*>(p) + 2 * e) : 0u;
-                const uint32_t hi = 2 * e + 1 < valid ? __ldg(reinterpret_cast<const unsigned short*>(p) + 2 * e + 1) : 0u;
-                w[e] = lo | hi << 16;
-            }
-            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" :: "r"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t lo = 2 * e < valid ? __ldg(p + 2 * e) : 0u, hi = 2 * e + 1 < valid ? __ldg(p + 2 * e + 1) : 0u;
+            w[e] = lo | hi << 16;
         }
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" :: "r"(slot + U::offset(t, q)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                     : "memory");
     }
 }
 
@@ -159,21 +161,21 @@ __device__ __forceinline__ void copy_units(const Operand<T>& o, uint32_t slot, i
 template <typename T>
 struct Walk {
     const Args<T>& g;
-    int64_t item;
-    int64_t i0, j0, k_begin, k_end, split;
-    int chunks, chunk;
+    int item, row_tile, col_tile, split, chunks, chunk;
     __device__ __forceinline__ explicit Walk(const Args<T>& args) : g(args), item(blockIdx.x), chunk(0) { place(); }
     __device__ __forceinline__ bool live() const { return item < g.items; }
+    __device__ __forceinline__ int64_t i0() const { return int64_t(row_tile) * kMmaTile; }
+    __device__ __forceinline__ int64_t j0() const { return int64_t(col_tile) * kMmaTile; }
+    __device__ __forceinline__ int64_t k_begin() const { return int64_t(split) * g.chunks * kMmaChunk; }
+    __device__ __forceinline__ int64_t k0() const { return k_begin() + chunk * kMmaChunk; }
+    __device__ __forceinline__ int64_t k_end() const { return min(g.depth, k_begin() + int64_t(g.chunks) * kMmaChunk); }
     __device__ __forceinline__ void place() {
         if (!live()) return;
-        const int64_t tile = item % (g.row_tiles * g.col_tiles);
-        split = item / (g.row_tiles * g.col_tiles);
-        j0 = tile % g.col_tiles * kMmaTile;
-        i0 = tile / g.col_tiles * kMmaTile;
-        k_begin = split * g.per;
-        k_end = min(g.depth, k_begin + g.per);
-        chunks = static_cast<int>((k_end - k_begin + kMmaChunk - 1) / kMmaChunk);
-        if (chunks < 1) chunks = 1;                     // an empty sum is a chunk of zeros
+        col_tile = item % g.col_tiles;
+        row_tile = item / g.col_tiles % g.row_tiles;
+        split = item / g.col_tiles / g.row_tiles;
+        const int64_t left = (g.depth + kMmaChunk - 1) / kMmaChunk - int64_t(split) * g.chunks;
+        chunks = static_cast<int>(min(int64_t(g.chunks), left));
     }
     __device__ __forceinline__ void next_item() {
         item += gridDim.x;
@@ -185,91 +187,107 @@ struct Walk {
     }
 };
 
+// Slot of a ring and the parity of its use; steps through the ring.
+template <int SLOTS>
+struct Ring {
+    int slot = 0;
+    unsigned parity = 0;
+    bool wrapped = false;
+    __device__ __forceinline__ void next() {
+        if (++slot == SLOTS) {
+            slot = 0;
+            parity ^= 1;
+            wrapped = true;
+        }
+    }
+};
+
 template <typename T, bool A_K, bool B_K>
-__device__ void load_role(const Args<T>& g, uint32_t a_ring, uint32_t b_ring, Control* ctl) {
-    using Tr = Traits<T>;
-    constexpr int S = Tr::a_slots;
+__device__ __forceinline__ void load_split(const Args<T>& g, uint32_t a_ring, uint32_t b_ring, Control* ctl) {
+    // registers hold the units of the next chunk; a unit is refilled right after it has been stored
     const int t = threadIdx.x - kEpilogueWarps * 32;
-    Walk<T> w(g);
-    bool first = true;                                   // the block's first item loads the resident operand
-    if constexpr (Tr::pieces == 3) {
-        // registers hold the units of the next chunk; a unit is refilled right after it has been stored
-        float ra[kUnits][8], rb[kUnits][8];
-        Walk<T> ahead(g);
-        bool ahead_b = true;
-        auto fetch_a = [&](int q) {
-            fetch<A_K>(g.a, ahead.i0 + UnitPlace<T, A_K>::mn(t, q),
-                       ahead.k_begin + ahead.chunk * kMmaChunk + UnitPlace<T, A_K>::k(t, q), ahead.k_end, ra[q]);
-        };
-        auto fetch_b = [&](int q) {
-            fetch<B_K>(g.b, ahead.j0 + UnitPlace<T, B_K>::mn(t, q),
-                       ahead.k_begin + ahead.chunk * kMmaChunk + UnitPlace<T, B_K>::k(t, q), ahead.k_end, rb[q]);
-        };
-        if (ahead.live()) {
+    float ra[kUnits][8], rb[kUnits][8];
+    Walk<T> w(g), ahead(g);
+    bool with_b = true, ahead_b = true;                  // a resident operand is loaded with the block's first item
+    auto fetch_a = [&](int q) {
+        fetch<A_K>(g.a, ahead.i0() + UnitPlace<T, A_K>::mn(t, q), ahead.k0() + UnitPlace<T, A_K>::k(t, q), ahead.k_end(), ra[q]);
+    };
+    auto fetch_b = [&](int q) {
+        fetch<B_K>(g.b, ahead.j0() + UnitPlace<T, B_K>::mn(t, q), ahead.k0() + UnitPlace<T, B_K>::k(t, q), ahead.k_end(), rb[q]);
+    };
+    if (!w.live()) return;
+#pragma unroll
+    for (int q = 0; q < kUnits; ++q) {
+        fetch_a(q);
+        fetch_b(q);
+    }
+    for (Ring<Traits<T>::a_slots> ring; w.live(); ring.next()) {
+        if (ring.wrapped && !tc::mbar_wait(&ctl->empty[ring.slot], ring.parity ^ 1, &ctl->gave_up)) return;
+        ahead.next_chunk();
+        if (g.resident && ahead.chunk == 0) ahead_b = false;
+        const bool more = ahead.live();
+        const uint32_t a_slot = a_ring + ring.slot * slot_bytes<T>(), b_slot = b_ring + (g.resident ? w.chunk : ring.slot) * slot_bytes<T>();
+#pragma unroll
+        for (int q = 0; q < kUnits; ++q) {
+            split_store(a_slot + UnitPlace<T, A_K>::offset(t, q), ra[q]);
+            if (more) fetch_a(q);
+        }
+        if (with_b) {
 #pragma unroll
             for (int q = 0; q < kUnits; ++q) {
-                fetch_a(q);
-                fetch_b(q);
+                split_store(b_slot + UnitPlace<T, B_K>::offset(t, q), rb[q]);
+                if (more && ahead_b) fetch_b(q);
             }
         }
-        for (int64_t step = 0; w.live(); ++step) {
-            const int slot = static_cast<int>(step % S);
-            if (step >= S && !tc::mbar_wait(&ctl->empty[slot], static_cast<unsigned>((step / S - 1) & 1), &ctl->gave_up)) return;
-            const int64_t item_now = ahead.item;
-            ahead.next_chunk();
-            if (ahead.item != item_now && g.resident) ahead_b = false;
-            const bool with_b = !g.resident || first;
-            const uint32_t b_slot = b_ring + (g.resident ? w.chunk : slot) * slot_bytes<T>();
-#pragma unroll
-            for (int q = 0; q < kUnits; ++q) {
-                split_store(a_ring + slot * slot_bytes<T>() + UnitPlace<T, A_K>::offset(t, q), ra[q]);
-                if (ahead.live()) fetch_a(q);
-            }
-            if (with_b) {
-#pragma unroll
-                for (int q = 0; q < kUnits; ++q) {
-                    split_store(b_slot + UnitPlace<T, B_K>::offset(t, q), rb[q]);
-                    if (ahead.live() && ahead_b) fetch_b(q);
-                }
-            }
-            tc::fence_smem_for_async();
-            __syncwarp();
-            if (threadIdx.x % 32 == 0) tc::mbar_arrive(&ctl->full[slot]);
-            const int64_t item = w.item;
-            w.next_chunk();
-            if (w.item != item) first = false;
-        }
-    } else {
-        // copies of chunk n are announced S - 1 chunks later, when they have landed
-        constexpr int LAG = S - 1;
-        int64_t step = 0;
-        bool ok = true;
-        for (; w.live(); ++step) {
-            const int slot = static_cast<int>(step % S);
-            if (step >= S && !tc::mbar_wait(&ctl->empty[slot], static_cast<unsigned>((step / S - 1) & 1), &ctl->gave_up)) {
-                ok = false;
-                break;
-            }
-            const int64_t k0 = w.k_begin + w.chunk * kMmaChunk;
-            copy_units<T, A_K>(g.a, a_ring + slot * slot_bytes<T>(), t, w.i0, k0, w.k_end);
-            if (!g.resident || first)
-                copy_units<T, B_K>(g.b, b_ring + (g.resident ? w.chunk : slot) * slot_bytes<T>(), t, w.j0, k0, w.k_end);
-            tc::copy_commit();
-            if (step >= LAG) {
-                tc::copy_wait<LAG>();
-                tc::fence_smem_for_async();
-                __syncwarp();
-                if (threadIdx.x % 32 == 0) tc::mbar_arrive(&ctl->full[(step - LAG) % S]);
-            }
-            const int64_t item = w.item;
-            w.next_chunk();
-            if (w.item != item) first = false;
-        }
-        tc::copy_wait<0>();
         tc::fence_smem_for_async();
         __syncwarp();
-        if (ok && threadIdx.x % 32 == 0)
-            for (int64_t s = step > LAG ? step - LAG : 0; s < step; ++s) tc::mbar_arrive(&ctl->full[s % S]);
+        if (threadIdx.x % 32 == 0) tc::mbar_arrive(&ctl->full[ring.slot]);
+        w.next_chunk();
+        if (g.resident && w.chunk == 0) with_b = false;
+    }
+}
+
+// 16-bit operands whose rows do not start on 16-byte boundaries.
+template <typename T, bool A_K, bool B_K>
+__device__ __forceinline__ void load_gathered(const Args<T>& g, uint32_t a_ring, uint32_t b_ring, Control* ctl) {
+    const int t = threadIdx.x - kEpilogueWarps * 32;
+    Walk<T> w(g);
+    bool with_b = true;
+    for (Ring<Traits<T>::a_slots> ring; w.live(); ring.next()) {
+        if (ring.wrapped && !tc::mbar_wait(&ctl->empty[ring.slot], ring.parity ^ 1, &ctl->gave_up)) return;
+        gather_units<T, A_K>(g.a, a_ring + ring.slot * slot_bytes<T>(), t, w.i0(), w.k0(), w.k_end());
+        if (with_b) gather_units<T, B_K>(g.b, b_ring + (g.resident ? w.chunk : ring.slot) * slot_bytes<T>(), t, w.j0(), w.k0(), w.k_end());
+        tc::fence_smem_for_async();
+        __syncwarp();
+        if (threadIdx.x % 32 == 0) tc::mbar_arrive(&ctl->full[ring.slot]);
+        w.next_chunk();
+        if (g.resident && w.chunk == 0) with_b = false;
+    }
+}
+
+// A chunk of an operand as one box of 128 rows (sum index contiguous) or two of 64 sum indices.
+template <bool K_MAJOR>
+__device__ __forceinline__ void load_boxes(uint32_t slot, const void* map, int64_t mn, int64_t k, uint64_t* bar) {
+    if (K_MAJOR) {
+        tc::tile_load(slot, map, static_cast<int>(k), static_cast<int>(mn), bar);
+    } else {
+        tc::tile_load(slot, map, static_cast<int>(mn), static_cast<int>(k), bar);
+        tc::tile_load(slot + kPieceBytes / 2, map, static_cast<int>(mn) + 64, static_cast<int>(k), bar);
+    }
+}
+
+template <typename T, bool A_K, bool B_K>
+__device__ __forceinline__ void load_tiled(const Args<T>& g, const void* map_a, const void* map_b, uint32_t a_ring, uint32_t b_ring, Control* ctl) {
+    Walk<T> w(g);
+    bool with_b = true;
+    for (Ring<Traits<T>::a_slots> ring; w.live(); ring.next()) {
+        if (ring.wrapped && !tc::mbar_wait(&ctl->empty[ring.slot], ring.parity ^ 1, &ctl->gave_up)) return;
+        uint64_t* bar = &ctl->full[ring.slot];
+        tc::mbar_expect(bar, with_b ? 2 * kPieceBytes : kPieceBytes);
+        load_boxes<A_K>(a_ring + ring.slot * slot_bytes<T>(), map_a, w.i0(), w.k0(), bar);
+        if (with_b) load_boxes<B_K>(b_ring + (g.resident ? w.chunk : ring.slot) * slot_bytes<T>(), map_b, w.j0(), w.k0(), bar);
+        w.next_chunk();
+        if (g.resident && w.chunk == 0) with_b = false;
     }
 }
 
@@ -279,20 +297,19 @@ __device__ void product_role(const Args<T>& g, uint32_t a_ring, uint32_t b_ring,
     constexpr int S = Tr::a_slots;
     constexpr uint32_t idesc = tc::instruction_descriptor(!std::is_same<T, __half>::value, !A_K, !B_K, kMmaTile);
     constexpr uint32_t a_step = A_K ? 32 : 2048, b_step = B_K ? 32 : 2048;       // bytes from one 16-term step to the next
-    int64_t groups = 0;                                                         // accumulators handed over so far
-    int64_t step = 0;
+    Ring<S> ring;
+    Ring<2> buffers;
     bool ok = true;
     for (Walk<T> w(g); ok && w.live(); w.next_item()) {
-        for (int c = 0; ok && c < w.chunks; ++c, ++step) {
-            const int slot = static_cast<int>(step % S), buffer = static_cast<int>(groups & 1);
+        for (int c = 0; ok && c < w.chunks; ++c, ring.next()) {
             const bool fresh = Tr::drains ? c % kDrainChunks == 0 : c == 0;
             const bool last = c + 1 == w.chunks || (Tr::drains && (c + 1) % kDrainChunks == 0);
-            if (fresh && groups >= 2) ok = tc::mbar_wait(&ctl->acc_empty[buffer], static_cast<unsigned>((groups / 2 - 1) & 1), &ctl->gave_up);
-            ok = ok && tc::mbar_wait(&ctl->full[slot], static_cast<unsigned>((step / S) & 1), &ctl->gave_up);
+            if (fresh && buffers.wrapped) ok = tc::mbar_wait(&ctl->acc_empty[buffers.slot], buffers.parity ^ 1, &ctl->gave_up);
+            ok = ok && tc::mbar_wait(&ctl->full[ring.slot], ring.parity, &ctl->gave_up);
             if (!ok) break;
             tc::fence_after_sync();
-            const uint32_t a = a_ring + slot * slot_bytes<T>(), b = b_ring + (g.resident ? c : slot) * slot_bytes<T>();
-            const uint32_t d = tmem + buffer * Tr::accumulators * kMmaTile;
+            const uint32_t a = a_ring + ring.slot * slot_bytes<T>(), b = b_ring + (g.resident ? c : ring.slot) * slot_bytes<T>();
+            const uint32_t d = tmem + buffers.slot * Tr::accumulators * kMmaTile;
             bool accumulate[2] = {!fresh, !fresh};
 #pragma unroll
             for (int k = 0; k < kMmaChunk / 16; ++k) {
@@ -314,10 +331,10 @@ __device__ void product_role(const Args<T>& g, uint32_t a_ring, uint32_t b_ring,
                 }
                 product(0, 0);
             }
-            tc::commit(&ctl->empty[slot]);
+            tc::commit(&ctl->empty[ring.slot]);
             if (last) {
-                tc::commit(&ctl->acc_full[buffer]);
-                ++groups;
+                tc::commit(&ctl->acc_full[buffers.slot]);
+                buffers.next();
             }
         }
     }
@@ -328,139 +345,177 @@ __device__ void product_role(const Args<T>& g, uint32_t a_ring, uint32_t b_ring,
     while (!tc::mbar_try(addr, 0) && clock64() - t0 < tc::kWaitCycles) {}
 }
 
-// An element in plain 32-bit arithmetic: taken when the pieces of an infinity, or of a value that rounds to
-// one in 16 bits, have made a NaN of it.
+// The elements of a staged 32 x 32 block that are not finite, again in plain 32-bit arithmetic: the pieces of an
+// infinity, or of a value that rounds to one in 16 bits, make a NaN where the product may be neither.
 template <typename T, bool A_K, bool B_K>
-__device__ __noinline__ float plain_element(const Args<T>& g, int64_t i, int64_t j, int64_t k_begin, int64_t k_end) {
-    float v = 0.f;
-    for (int64_t k = k_begin; k < k_end; ++k)
-        v = fmaf(to_acc(A_K ? g.a.p[i * g.a.ld + k] : g.a.p[k * g.a.ld + i]), to_acc(B_K ? g.b.p[j * g.b.ld + k] : g.b.p[k * g.b.ld + j]), v);
-    return v;
+__device__ __noinline__ void repair(const Args<T>& g, uint32_t stage, int64_t row0, int64_t col0, int64_t k_begin, int64_t k_end) {
+    const int lane = threadIdx.x % 32;
+    const int64_t i = row0 + lane;
+    for (int q = 0; q < 32; ++q) {
+        const int64_t j = col0 + q;
+        const uint32_t addr = stage + lane * 128 + (((q / 4) ^ (lane % 8)) * 16) + (q % 4) * 4;
+        float v;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+        if (isfinite(v) || i >= g.rows || j >= g.cols) continue;
+        v = 0.f;
+        for (int64_t k = k_begin; k < k_end; ++k)
+            v = fmaf(to_acc(A_K ? g.a.p[i * g.a.ld + k] : g.a.p[k * g.a.ld + i]), to_acc(B_K ? g.b.p[j * g.b.ld + k] : g.b.p[k * g.b.ld + j]), v);
+        asm volatile("st.shared.f32 [%0], %1;" :: "r"(addr), "f"(v) : "memory");
+    }
 }
 
-template <typename T, bool A_K, bool B_K, int ACT>
-__device__ __forceinline__ void write_rows(const Args<T>& g, const Walk<T>& w, uint32_t stage, int64_t row0, int64_t col0) {
-    const int lane = threadIdx.x % 32;
-    const int64_t j = col0 + (lane % 8) * 4;
+// A staged 32 x 32 block to memory: eight lanes cover a row's 32 columns, a warp four rows at a time.
+template <typename T, int ACT>
+__device__ __forceinline__ void write_block(const Args<T>& g, int split, uint32_t stage, int64_t row0, int64_t col0) {
+    const int lane = threadIdx.x % 32, first = lane / 8, unit = lane % 8;
+    const int64_t j = col0 + unit * 4, i0 = row0 + first;
     const Epilogue<T>& ep = g.ep;
     if (j >= g.cols) return;
     const int width = g.cols - j < 4 ? static_cast<int>(g.cols - j) : 4;
+    const int count = static_cast<int>(min(int64_t(8), (g.rows - i0 + 3) / 4));       // rows of this lane
+    auto staged = [&](int e, float (&v)[4]) {
+        const int r = first + 4 * e;
+        asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+                     : "r"(stage + r * 128 + ((unit ^ (r % 8)) * 16)));
+    };
+    if (ep.partial) {
+        float* out = reinterpret_cast<float*>(ep.partial) + (split * g.rows + i0) * g.cols + j;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float v[4];
+            staged(e, v);
+            if (e >= count) continue;
+            float* p = out + e * 4 * g.cols;
+            if (g.vector_out) {
+                *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (q < width) p[q] = v[q];
+            }
+        }
+        return;
+    }
     float bias[4] = {};
     if (ep.bias)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
             if (q < width) bias[q] = to_acc(ep.bias[j + q]);
+    const int64_t out = i0 * g.cols + j;
+    const T* res = ep.residual ? ep.residual + i0 * ep.ldr + j : nullptr;
+    if (g.vector_out) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int r = lane / 8 + 4 * e;
-        const int64_t i = row0 + r;
-        if (i >= g.rows) break;
-        float v[4];
-        asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
-                     : "r"(stage + r * 128 + (((lane % 8) ^ (r % 8)) * 16)));
-        if (Traits<T>::pieces == 3) {
+        for (int half = 0; half < 2; ++half) {
+            Pack<T, 4> r[4];
+            if (res)
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (!isfinite(v[q]) && q < width) v[q] = plain_element<T, A_K, B_K>(g, i, j + q, w.k_begin, w.k_end);
-        }
-        if (ep.partial) {
-            float* out = reinterpret_cast<float*>(ep.partial) + (w.split * g.rows + i) * g.cols + j;
-            if (g.vector_out) {
-                *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
-            } else {
+                for (int e = 0; e < 4; ++e)
+                    if (half * 4 + e < count) r[e] = *reinterpret_cast<const Pack<T, 4>*>(res + (half * 4 + e) * 4 * ep.ldr);
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (q < width) out[q] = v[q];
-            }
-            continue;
-        }
-        float res[4] = {};
-        if (ep.residual) {
-            const T* p = ep.residual + i * ep.ldr + j;
-            if (g.vector_out) {
-                load_acc<T, 4>(p, res);
-            } else {
+            for (int e = 0; e < 4; ++e) {
+                const int row = half * 4 + e;
+                float v[4];
+                staged(row, v);
+                Pack<T, 4> z, y;
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (q < width) res[q] = to_acc(p[q]);
-            }
-        }
-        Pack<T, 4> z, y;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const float s = v[q] + bias[q];
-            z.v[q] = rounded_z<T, ACT>(s);
-            float t = activate<ACT>(s);
-            if (ep.residual) t += res[q];
-            y.v[q] = from_acc<T>(t);
-        }
-        if (g.vector_out) {
-            if (ep.z) *reinterpret_cast<Pack<T, 4>*>(ep.z + i * g.cols + j) = z;
-            *reinterpret_cast<Pack<T, 4>*>(ep.y + i * g.cols + j) = y;
-        } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (q < width) {
-                    if (ep.z) ep.z[i * g.cols + j + q] = z.v[q];
-                    ep.y[i * g.cols + j + q] = y.v[q];
+                for (int q = 0; q < 4; ++q) {
+                    const float s = v[q] + bias[q];
+                    z.v[q] = rounded_z<T, ACT>(s);
+                    const float t = activate<ACT>(s);
+                    y.v[q] = from_acc<T>(res ? t + to_acc(r[e].v[q]) : t);
                 }
+                if (row >= count) continue;
+                if (ep.z) *reinterpret_cast<Pack<T, 4>*>(ep.z + out + row * 4 * g.cols) = z;
+                *reinterpret_cast<Pack<T, 4>*>(ep.y + out + row * 4 * g.cols) = y;
+            }
+        }
+    } else {
+        for (int e = 0; e < count; ++e) {
+            float v[4];
+            staged(e, v);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (q >= width) break;
+                const float s = v[q] + bias[q];
+                if (ep.z) ep.z[out + e * 4 * g.cols + q] = rounded_z<T, ACT>(s);
+                float t = activate<ACT>(s);
+                if (res) t += to_acc(res[e * 4 * ep.ldr + q]);
+                ep.y[out + e * 4 * g.cols + q] = from_acc<T>(t);
+            }
         }
     }
 }
 
 template <typename T, bool A_K, bool B_K, int ACT>
-__device__ void epilogue_role(const Args<T>& g, uint32_t staging, uint32_t tmem, Control* ctl) {
+__device__ __forceinline__ void epilogue_role(const Args<T>& g, uint32_t staging, uint32_t tmem, Control* ctl) {
     using Tr = Traits<T>;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int quarter = warp % 4, half = warp / 4;                 // tensor memory lanes and columns of this warp
     const uint32_t stage = staging + warp * 4096;
-    int64_t groups = 0;
+    Ring<2> buffers;
     for (Walk<T> w(g); w.live(); w.next_item()) {
-        float acc[Tr::drains ? 64 : 1];
+        float acc[4][16];                                          // sums of the parts that were taken out (float only)
         const int parts = Tr::drains ? (w.chunks + kDrainChunks - 1) / kDrainChunks : 1;
-        for (int part = 0; part < parts; ++part, ++groups) {
-            const int buffer = static_cast<int>(groups & 1);
-            if (!tc::mbar_wait(&ctl->acc_full[buffer], static_cast<unsigned>((groups / 2) & 1), &ctl->gave_up)) return;
+        for (int part = 0; part < parts; ++part, buffers.next()) {
+            const bool final = part + 1 == parts;
+            if (!tc::mbar_wait(&ctl->acc_full[buffers.slot], buffers.parity, &ctl->gave_up)) return;
             tc::fence_after_sync();
 #pragma unroll
-            for (int block = 0; block < 2; ++block) {
-                float v[32];
-                const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buffer * Tr::accumulators * kMmaTile + half * 64 + block * 32;
-                tc::tmem_load32(from, v);
-                if constexpr (Tr::drains) {
-                    float small[32];
-                    tc::tmem_load32(from + kMmaTile, small);
+            for (int block = 0; block < 4; ++block) {
+                const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buffers.slot * Tr::accumulators * kMmaTile +
+                                      half * 64 + block * 16;
+                float v[16];
+                tc::tmem_load16(from, v);
+                tc::tmem_wait(v);
+                if constexpr (Tr::accumulators == 2) {
 #pragma unroll
-                    for (int q = 0; q < 32; ++q) v[q] += small[q];
+                    for (int q = 0; q < 16; ++q) acc[block][q] = part == 0 ? v[q] : acc[block][q] + v[q];
+                    tc::tmem_load16(from + kMmaTile, v);
+                    tc::tmem_wait(v);
 #pragma unroll
-                    for (int q = 0; q < 32; ++q) acc[block * 32 + q] = part == 0 ? v[q] : acc[block * 32 + q] + v[q];
-                    if (part + 1 < parts) continue;
-#pragma unroll
-                    for (int q = 0; q < 32; ++q) v[q] = acc[block * 32 + q];
+                    for (int q = 0; q < 16; ++q) v[q] = acc[block][q] += v[q];
+                    if (!final) continue;
                 }
-                __syncwarp();                                        // the block before has been read out of the stage
+                bool finite = true;
+                if constexpr (Tr::pieces == 3) {
+                    float t = 0.f;                                 // NaN if any of the values is not finite
 #pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" :: "r"(stage + lane * 128 + ((q ^ (lane % 8)) * 16)), "f"(v[4 * q]),
-                                 "f"(v[4 * q + 1]), "f"(v[4 * q + 2]), "f"(v[4 * q + 3]) : "memory");
-                __syncwarp();
-                if (block == 1) {                                    // everything has left tensor memory
+                    for (int q = 0; q < 16; ++q) t = fmaf(v[q], 0.f, t);
+                    finite = t == t;
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" :: "r"(stage + lane * 128 + (((block % 2 * 4 + q) ^ (lane % 8)) * 16)),
+                                 "f"(v[4 * q]), "f"(v[4 * q + 1]), "f"(v[4 * q + 2]), "f"(v[4 * q + 3]) : "memory");
+                if (block == 3) {                                  // everything has left tensor memory
                     tc::fence_before_sync();
-                    if (lane == 0) tc::mbar_arrive(&ctl->acc_empty[buffer]);
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&ctl->acc_empty[buffers.slot]);
                 }
-                write_rows<T, A_K, B_K, ACT>(g, w, stage, w.i0 + quarter * 32, w.j0 + half * 64 + block * 32);
+                const int64_t row0 = w.i0() + quarter * 32, col0 = w.j0() + half * 64 + block / 2 * 32;
+                if (Tr::pieces == 3 && __any_sync(0xFFFFFFFFu, !finite)) {
+                    __syncwarp();
+                    repair<T, A_K, B_K>(g, stage, row0, col0, w.k_begin(), w.k_end());
+                }
+                if (block % 2 == 1) {
+                    __syncwarp();
+                    write_block<T, ACT>(g, w.split, stage, row0, col0);
+                    __syncwarp();
+                }
             }
-            if (Tr::drains && part + 1 < parts) {
+            if (!final) {
                 tc::fence_before_sync();
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&ctl->acc_empty[buffer]);
+                if (lane == 0) tc::mbar_arrive(&ctl->acc_empty[buffers.slot]);
             }
         }
     }
 }
 
 template <typename T, bool A_K, bool B_K, int ACT>
-__global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant__ Args<T> g) {
+__global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant__ Args<T> g,
+                                                          const __grid_constant__ CUtensorMap map_a,
+                                                          const __grid_constant__ CUtensorMap map_b) {
     using Tr = Traits<T>;
     extern __shared__ char raw[];
     __shared__ Control ctl;
@@ -469,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
     const int warp = threadIdx.x / 32;
     if (threadIdx.x == 0) {
         for (int s = 0; s < Tr::a_slots; ++s) {
-            tc::mbar_init(&ctl.full[s], kLoaderWarps);
+            tc::mbar_init(&ctl.full[s], g.tiled ? 1 : kLoaderWarps);
             tc::mbar_init(&ctl.empty[s], 1);
         }
         for (int s = 0; s < 2; ++s) {
@@ -485,12 +540,23 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = ctl.tmem;
+    // Float: the loaders hold a chunk of both operands and the epilogue the sums of 64 columns, so registers move to
+    // them from the products' warpgroup.
     if (warp < kEpilogueWarps) {
+        if constexpr (Tr::pieces == 3) tc::registers_up<kEpilogueRegisters>();
         epilogue_role<T, A_K, B_K, ACT>(g, staging, tmem, &ctl);
     } else if (warp < kEpilogueWarps + kLoaderWarps) {
-        load_role<T, A_K, B_K>(g, a_ring, b_ring, &ctl);
-    } else if (threadIdx.x % 32 == 0) {
-        product_role<T, A_K, B_K>(g, a_ring, b_ring, tmem, &ctl);
+        if constexpr (Tr::pieces == 3) {
+            tc::registers_up<kLoaderRegisters>();
+            load_split<T, A_K, B_K>(g, a_ring, b_ring, &ctl);
+        } else if (!g.tiled) {
+            load_gathered<T, A_K, B_K>(g, a_ring, b_ring, &ctl);
+        } else if (threadIdx.x == kEpilogueWarps * 32) {
+            load_tiled<T, A_K, B_K>(g, &map_a, &map_b, a_ring, b_ring, &ctl);
+        }
+    } else {
+        if constexpr (Tr::pieces == 3) tc::registers_down<kProductRegisters>();
+        if (threadIdx.x == (kEpilogueWarps + kLoaderWarps) * 32) product_role<T, A_K, B_K>(g, a_ring, b_ring, tmem, &ctl);
     }
     __syncwarp();
     tc::fence_before_sync();
@@ -501,27 +567,66 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
 
 bool multiple16(const void* p, int64_t ld, size_t size) { return aligned16(p) && (ld * size) % 16 == 0; }
 
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return fn;
+}
+
+// Boxes of 64 contiguous values by `lines` rows of a [outer, inner] array with row stride ld.
+template <typename T>
+bool make_map(CUtensorMap* map, const T* p, int64_t inner, int64_t outer, int64_t ld, int lines) {
+    const EncodeTiled encode = encode_tiled();
+    if (!encode || inner > INT32_MAX || outer > INT32_MAX || ld * int64_t(sizeof(T)) >= (int64_t(1) << 40)) return false;
+    const cuuint64_t size[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
+    const cuuint64_t stride[1] = {static_cast<cuuint64_t>(ld) * sizeof(T)};
+    const cuuint32_t box[2] = {kMmaChunk, static_cast<cuuint32_t>(lines)}, step[2] = {1, 1};
+    return encode(map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                  const_cast<T*>(p), size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace
 
 template <typename T, bool A_K, bool B_K, int ACT>
 int mma_product(int64_t rows, int64_t cols, int64_t depth, int64_t splits, int64_t per, const T* a, int64_t as, const T* b, int64_t bs,
                 const Epilogue<T>& ep, int32_t* status, cudaStream_t stream) {
+    const int64_t row_tiles = ceil_div(rows, kMmaTile), col_tiles = ceil_div(cols, kMmaTile);
+    if (row_tiles > INT32_MAX || col_tiles > INT32_MAX || row_tiles * col_tiles > INT32_MAX / 2 ||
+        row_tiles * col_tiles * splits > INT32_MAX / 2)
+        return NB200_ERR_TOO_LARGE;
     Args<T> g;
     g.a = {a, as, rows, multiple16(a, as, sizeof(T))};
     g.b = {b, bs, cols, multiple16(b, bs, sizeof(T))};
     g.rows = rows;
     g.cols = cols;
     g.depth = depth;
-    g.per = per;
-    g.row_tiles = ceil_div(rows, kMmaTile);
-    g.col_tiles = ceil_div(cols, kMmaTile);
-    g.items = g.row_tiles * g.col_tiles * splits;
+    g.row_tiles = static_cast<int>(row_tiles);
+    g.col_tiles = static_cast<int>(col_tiles);
+    g.items = static_cast<int>(row_tiles * col_tiles * splits);
     g.chunks = static_cast<int>(ceil_div(per < depth ? per : depth, kMmaChunk));
     g.ep = ep;
     g.status = status;
-    const size_t wide = 4 * sizeof(T);
+    const size_t wide = 4 * sizeof(T) < 16 ? 4 * sizeof(T) : 16;
     auto fits = [&](const void* p) { return !p || reinterpret_cast<uintptr_t>(p) % wide == 0; };
     g.vector_out = cols % 4 == 0 && fits(ep.z) && fits(ep.y) && fits(ep.residual) && (!ep.residual || ep.ldr % 4 == 0);
+    CUtensorMap map_a{}, map_b{};
+    g.tiled = false;
+    if constexpr (!std::is_same<T, float>::value) {
+        g.tiled = g.a.vector && g.b.vector &&
+                  (A_K ? make_map(&map_a, a, depth, rows, as, kMmaTile) : make_map(&map_a, a, rows, depth, as, kMmaChunk)) &&
+                  (B_K ? make_map(&map_b, b, depth, cols, bs, kMmaTile) : make_map(&map_b, b, cols, depth, bs, kMmaChunk));
+    }
     // a block keeps to one column of tiles when the grid is a multiple of their number
     int64_t grid = g.items < kSMs ? g.items : kSMs;
     g.resident = false;
@@ -532,8 +637,19 @@ int mma_product(int64_t rows, int64_t cols, int64_t depth, int64_t splits, int64
     }
     constexpr int smem = smem_bytes<T>();
     static_assert(smem + sizeof(Control) <= 227 * 1024, "shared memory of the product kernel");
-    if (cudaFuncSetAttribute(mma_kernel<T, A_K, B_K, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return NB200_ERR_CUDA;
-    mma_kernel<T, A_K, B_K, ACT><<<static_cast<unsigned>(grid), kThreads, smem, stream>>>(g);
+    // once per kernel and device
+    static std::atomic<uint64_t> prepared{0};
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return NB200_ERR_CUDA;
+    if (device >= 64 || !(prepared.load(std::memory_order_acquire) >> device & 1)) {
+        cudaFuncAttributes attr;
+        if (cudaFuncSetAttribute(mma_kernel<T, A_K, B_K, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+            cudaFuncGetAttributes(&attr, mma_kernel<T, A_K, B_K, ACT>) != cudaSuccess)
+            return NB200_ERR_CUDA;
+        if (Traits<T>::pieces == 3 && attr.numRegs != kLaunchRegisters) return NB200_ERR_PRECONDITION;
+        if (device < 64) prepared.fetch_or(uint64_t(1) << device, std::memory_order_release);
+    }
+    mma_kernel<T, A_K, B_K, ACT><<<static_cast<unsigned>(grid), kThreads, smem, stream>>>(g, map_a, map_b);
     return launch_status();
 }
 
