@@ -74,48 +74,99 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(int64_t rows, int64_t co
     }
 }
 
-// Sum of the splits, in order.
+// Sums over the leading index of partial [parts][size]: 32 columns x 8 lanes per block, lane l adds parts l, l + 8,
+// ..., then the lanes are added in order.  The order depends on the sizes alone.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) join_splits_kernel(int64_t size, int splits, const acc_t<T>* __restrict__ partial,
-                                                               T* __restrict__ out) {
-    for (int64_t e = blockIdx.x * int64_t(kThreads) + threadIdx.x; e < size; e += int64_t(gridDim.x) * kThreads) {
-        acc_t<T> v = 0;
-        for (int s = 0; s < splits; ++s) v += partial[s * size + e];
+__global__ void __launch_bounds__(kThreads) join_parts_kernel(int64_t size, int parts, const acc_t<T>* __restrict__ partial,
+                                                              T* __restrict__ out) {
+    using A = acc_t<T>;
+    __shared__ A sm[8][33];
+    const int64_t e = blockIdx.x * int64_t(32) + threadIdx.x % 32;
+    const int lane = threadIdx.x / 32;
+    A v = 0;
+    if (e < size)
+#pragma unroll 8
+        for (int s = lane; s < parts; s += 8) v += partial[s * size + e];
+    sm[lane][threadIdx.x % 32] = v;
+    __syncthreads();
+    if (lane == 0 && e < size) {
+#pragma unroll
+        for (int q = 1; q < 8; ++q) v += sm[q][threadIdx.x];
         out[e] = from_acc<T>(v);
     }
 }
 
-// dz = dy act'(z) (not stored when dz is NULL: then dy is dz) and the column sums of dz over a band of rows;
-// a block covers 32 columns x its band, 8 rows of threads.
-template <typename T, int ACT>
-__global__ void __launch_bounds__(kThreads) slope_kernel(int64_t rows, int64_t cols, int64_t band, const T* __restrict__ dy, int64_t ldd,
-                                                         const T* __restrict__ z, T* __restrict__ dz, acc_t<T>* __restrict__ sums) {
+// dz = dy act'(z) (not stored when dz is NULL: then dy is dz) and the column sums of dz over a band of rows.
+// A thread owns V neighbouring columns of every row_lanes-th row; blockIdx.y selects the columns.  Moves
+// 3 values per element (1 without an activation) and is bound by that.
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads) slope_kernel(int64_t rows, int64_t cols, int lanes, int64_t band, const T* __restrict__ dy,
+                                                         int64_t ldd, const T* __restrict__ z, T* __restrict__ dz,
+                                                         acc_t<T>* __restrict__ sums) {
     using A = acc_t<T>;
-    __shared__ A sm[8][33];
-    const int64_t j = blockIdx.y * int64_t(32) + threadIdx.x % 32;
-    const int lane = threadIdx.x / 32;
+    __shared__ A sm[kThreads * V];
+    const int lane = threadIdx.x % lanes, row_lane = threadIdx.x / lanes, row_lanes = kThreads / lanes;
+    const int64_t j = (blockIdx.y * int64_t(lanes) + lane) * V;
+    const bool live = row_lane < row_lanes && j < cols;
     const int64_t limit = min(rows, (blockIdx.x + 1) * band);
-    A sum = 0;
-    if (j < cols)
-        for (int64_t i = blockIdx.x * band + lane; i < limit; i += 8) {
-            A v = to_acc(dy[i * ldd + j]);
+    A sum[V] = {};
+    if (live) {
+#pragma unroll 4
+        for (int64_t i = blockIdx.x * band + row_lane; i < limit; i += row_lanes) {
+            A v[V];
+            load_acc<T, V>(dy + i * ldd + j, v);
             if (ACT != NB200_ACT_NONE) {
-                v *= activate_slope<ACT>(to_acc(z[i * cols + j]));
-                dz[i * cols + j] = from_acc<T>(v);
+                A s[V];
+                load_acc<T, V>(z + i * cols + j, s);
+#pragma unroll
+                for (int q = 0; q < V; ++q) v[q] *= activate_slope<ACT>(s[q]);
+                store_acc<T, V>(dz + i * cols + j, v);
             }
-            sum += v;
+#pragma unroll
+            for (int q = 0; q < V; ++q) sum[q] += v[q];
         }
-    sm[lane][threadIdx.x % 32] = sum;
-    __syncthreads();
-    if (lane == 0 && j < cols && sums) {
-        for (int q = 1; q < 8; ++q) sum += sm[q][threadIdx.x];
-        sums[blockIdx.x * cols + j] = sum;
     }
+    if (!sums) return;
+#pragma unroll
+    for (int q = 0; q < V; ++q) sm[threadIdx.x * V + q] = sum[q];
+    __syncthreads();
+    int width = 1;
+    while (width < row_lanes) width <<= 1;
+    for (int off = width >> 1; off > 0; off >>= 1) {
+        const int other = threadIdx.x + off * lanes;
+        if (live && row_lane < off && row_lane + off < row_lanes) {
+#pragma unroll
+            for (int q = 0; q < V; ++q) sm[threadIdx.x * V + q] = sum[q] += sm[other * V + q];
+        }
+        __syncthreads();
+    }
+    if (live && row_lane == 0)
+#pragma unroll
+        for (int q = 0; q < V; ++q) sums[blockIdx.x * cols + j + q] = sum[q];
 }
 
-constexpr int64_t kMaxBands = 512;
-int64_t band_rows(int64_t rows) { return rows <= 64 * kMaxBands ? 64 : ceil_div(rows, kMaxBands); }
-int64_t band_count(int64_t rows) { return ceil_div(rows, band_rows(rows)); }
+// Bands of at least 32 rows, eight blocks per SM at most.
+int64_t band_count(int64_t rows) {
+    const int64_t wanted = ceil_div(rows, 32);
+    return wanted < kSMs * 8 ? (wanted < 1 ? 1 : wanted) : kSMs * 8;
+}
+
+template <typename T, int V>
+int slope_pass(int64_t m, int64_t n, int act, const T* dy, int64_t ldd, const T* z, T* dz, acc_t<T>* sums, cudaStream_t stream) {
+    const int64_t vectors = n / V, lanes = vectors < kThreads ? vectors : kThreads, gy = ceil_div(vectors, lanes);
+    if (gy > 65535) return NB200_ERR_TOO_LARGE;
+    const int64_t bands = band_count(m);
+    return NB200_DISPATCH_ACT(act, (slope_kernel<T, V, ACT><<<dim3(bands, gy), kThreads, 0, stream>>>(
+                                        m, n, static_cast<int>(lanes), ceil_div(m, bands), dy, ldd, z, dz, sums), launch_status()));
+}
+
+template <typename T>
+int join_parts(int64_t size, int64_t parts, const acc_t<T>* partial, T* out, cudaStream_t stream) {
+    const int64_t blocks = ceil_div(size, 32);
+    if (blocks > INT32_MAX) return NB200_ERR_TOO_LARGE;
+    join_parts_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(size, static_cast<int>(parts), partial, out);
+    return launch_status();
+}
 
 // Whether a product runs on the tensor cores.
 template <typename T>
@@ -178,14 +229,11 @@ int backward(int64_t m, int64_t k, int64_t n, const T* dy, int64_t ldd, const T*
     A* partial = reinterpret_cast<A*>(work + lay.partial);
     int rc = NB200_OK;
     if (dz || db) {
-        const int64_t bands = band_count(m), gy = ceil_div(n, 32);
-        if (gy > 65535) return NB200_ERR_TOO_LARGE;
-        rc = NB200_DISPATCH_ACT(act, (slope_kernel<T, ACT><<<dim3(bands, gy), kThreads, 0, stream>>>(m, n, band_rows(m), dy, ldd, z, dz,
-                                                                                                db ? sums : nullptr), launch_status()));
-        if (rc == NB200_OK && db) {
-            join_splits_kernel<T><<<static_cast<unsigned>(ceil_div(n, kThreads)), kThreads, 0, stream>>>(n, static_cast<int>(bands), sums, db);
-            rc = launch_status();
-        }
+        constexpr int V = 16 / sizeof(T);
+        const bool vector = n % V == 0 && ldd % V == 0 && aligned16(dy) && aligned16(z);
+        rc = vector ? slope_pass<T, V>(m, n, act, dy, ldd, z, dz, db ? sums : nullptr, stream)
+                    : slope_pass<T, 1>(m, n, act, dy, ldd, z, dz, db ? sums : nullptr, stream);
+        if (rc == NB200_OK && db) rc = join_parts<T>(n, band_count(m), sums, db, stream);
         if (rc != NB200_OK) return rc;
     }
     const T* g = dz ? dz : dy;
@@ -200,10 +248,7 @@ int backward(int64_t m, int64_t k, int64_t n, const T* dy, int64_t ldd, const T*
         rc = product<T, false, false, NB200_ACT_NONE>(k, n, m, split, x, ldx, g, ldg, {nullptr, nullptr, 0, nullptr, nullptr, partial}, status,
                                                       stream);
         if (rc != NB200_OK) return rc;
-        const int64_t blocks = ceil_div(k * n, kThreads);
-        join_splits_kernel<T><<<static_cast<unsigned>(blocks < kSMs * 8 ? blocks : kSMs * 8), kThreads, 0, stream>>>(
-            k * n, static_cast<int>(split.parts), partial, dw);
-        rc = launch_status();
+        if (rc == NB200_OK) rc = join_parts<T>(k * n, split.parts, partial, dw, stream);
     }
     return rc;
 }

@@ -38,6 +38,7 @@ static_assert(kEpilogueWarps * kEpilogueRegisters + kLoaderWarps * kLoaderRegist
 constexpr int kPieceBytes = kMmaTile * kMmaChunk * 2;              // one piece of one operand's chunk: 16 KB
 constexpr int kUnits = kMmaTile * kMmaChunk / 8 / kLoaders;        // units of eight values per loader thread
 constexpr int kDrainChunks = 2;
+constexpr int kAhead = 4;
 
 template <typename T> struct Traits {                              // 16-bit types
     static constexpr int pieces = 1, a_slots = 4, b_slots = 8, accumulators = 1;
@@ -244,6 +245,28 @@ __device__ __forceinline__ void load_split(const Args<T>& g, uint32_t a_ring, ui
         if (threadIdx.x % 32 == 0) tc::mbar_arrive(&ctl->full[ring.slot]);
         w.next_chunk();
         if (g.resident && w.chunk == 0) with_b = false;
+    }
+}
+
+// Float operands on their way: one thread asks for the boxes that the loaders will need kAhead chunks later to be
+// brought into L2, so that the loaders, whose registers hold one chunk, wait for L2 and not for memory.
+template <typename T, bool A_K, bool B_K>
+__device__ __forceinline__ void prefetch_role(const Args<T>& g, const void* map_a, const void* map_b, Control* ctl) {
+    constexpr int S = Traits<T>::a_slots;
+    Walk<T> w(g), ahead(g);
+    auto ask = [&]() {
+        if (A_K) tc::tile_prefetch(map_a, static_cast<int>(ahead.k0()), static_cast<int>(ahead.i0()));
+        else tc::tile_prefetch(map_a, static_cast<int>(ahead.i0()), static_cast<int>(ahead.k0()));
+        if (!g.resident) {
+            if (B_K) tc::tile_prefetch(map_b, static_cast<int>(ahead.k0()), static_cast<int>(ahead.j0()));
+            else tc::tile_prefetch(map_b, static_cast<int>(ahead.j0()), static_cast<int>(ahead.k0()));
+        }
+        ahead.next_chunk();
+    };
+    for (int q = 0; q < kAhead && ahead.live(); ++q) ask();
+    for (Ring<S> ring; w.live() && ahead.live(); ring.next(), w.next_chunk()) {
+        if (!tc::mbar_wait(&ctl->full[ring.slot], ring.parity, &ctl->gave_up)) return;
+        ask();
     }
 }
 
@@ -524,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
     const int warp = threadIdx.x / 32;
     if (threadIdx.x == 0) {
         for (int s = 0; s < Tr::a_slots; ++s) {
-            tc::mbar_init(&ctl.full[s], g.tiled ? 1 : kLoaderWarps);
+            tc::mbar_init(&ctl.full[s], Tr::pieces == 1 && g.tiled ? 1 : kLoaderWarps);
             tc::mbar_init(&ctl.empty[s], 1);
         }
         for (int s = 0; s < 2; ++s) {
@@ -557,6 +580,8 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
     } else {
         if constexpr (Tr::pieces == 3) tc::registers_down<kProductRegisters>();
         if (threadIdx.x == (kEpilogueWarps + kLoaderWarps) * 32) product_role<T, A_K, B_K>(g, a_ring, b_ring, tmem, &ctl);
+        if (Tr::pieces == 3 && g.tiled && threadIdx.x == (kEpilogueWarps + kLoaderWarps + 1) * 32)
+            prefetch_role<T, A_K, B_K>(g, &map_a, &map_b, &ctl);
     }
     __syncwarp();
     tc::fence_before_sync();
@@ -583,17 +608,22 @@ EncodeTiled encode_tiled() {
     return fn;
 }
 
-// Boxes of 64 contiguous values by `lines` rows of a [outer, inner] array with row stride ld.
+// Boxes of `lines` rows of a [outer, inner] array with row stride ld: 64 contiguous 16-bit values in the tensor
+// cores' order, or the floats of a whole chunk.
 template <typename T>
 bool make_map(CUtensorMap* map, const T* p, int64_t inner, int64_t outer, int64_t ld, int lines) {
+    constexpr bool split = std::is_same<T, float>::value;
     const EncodeTiled encode = encode_tiled();
     if (!encode || inner > INT32_MAX || outer > INT32_MAX || ld * int64_t(sizeof(T)) >= (int64_t(1) << 40)) return false;
     const cuuint64_t size[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
     const cuuint64_t stride[1] = {static_cast<cuuint64_t>(ld) * sizeof(T)};
-    const cuuint32_t box[2] = {kMmaChunk, static_cast<cuuint32_t>(lines)}, step[2] = {1, 1};
-    return encode(map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
-                  const_cast<T*>(p), size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint32_t box[2] = {split ? static_cast<cuuint32_t>(kMmaTile * kMmaChunk / lines) : kMmaChunk, static_cast<cuuint32_t>(lines)};
+    const cuuint32_t step[2] = {1, 1};
+    const CUtensorMapDataType type = split ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                           : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return encode(map, type, 2, const_cast<T*>(p), size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  split ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace
@@ -621,12 +651,10 @@ int mma_product(int64_t rows, int64_t cols, int64_t depth, int64_t splits, int64
     auto fits = [&](const void* p) { return !p || reinterpret_cast<uintptr_t>(p) % wide == 0; };
     g.vector_out = cols % 4 == 0 && fits(ep.z) && fits(ep.y) && fits(ep.residual) && (!ep.residual || ep.ldr % 4 == 0);
     CUtensorMap map_a{}, map_b{};
-    g.tiled = false;
-    if constexpr (!std::is_same<T, float>::value) {
-        g.tiled = g.a.vector && g.b.vector &&
-                  (A_K ? make_map(&map_a, a, depth, rows, as, kMmaTile) : make_map(&map_a, a, rows, depth, as, kMmaChunk)) &&
-                  (B_K ? make_map(&map_b, b, depth, cols, bs, kMmaTile) : make_map(&map_b, b, cols, depth, bs, kMmaChunk));
-    }
+    // 16-bit types: boxes that the tensor cores read; float: boxes for the prefetches
+    g.tiled = g.a.vector && g.b.vector &&
+              (A_K ? make_map(&map_a, a, depth, rows, as, kMmaTile) : make_map(&map_a, a, rows, depth, as, kMmaChunk)) &&
+              (B_K ? make_map(&map_b, b, depth, cols, bs, kMmaTile) : make_map(&map_b, b, cols, depth, bs, kMmaChunk));
     // a block keeps to one column of tiles when the grid is a multiple of their number
     int64_t grid = g.items < kSMs ? g.items : kSMs;
     g.resident = false;

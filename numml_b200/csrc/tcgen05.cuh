@@ -99,6 +99,11 @@ __device__ __forceinline__ void tile_load(uint32_t dst, const void* map, int x, 
                  :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
 }
 
+// The same box into L2 only.
+__device__ __forceinline__ void tile_prefetch(const void* map, int x, int y) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" :: "l"(map), "r"(x), "r"(y) : "memory");
+}
+
 // ---- registers: moved between warpgroups; the sum after all moves must not exceed the sum at launch ---------
 template <int N> __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N)); }
 template <int N> __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N)); }
