@@ -1,10 +1,11 @@
 // Dense products on the 5th-generation tensor cores (tcgen05.mma, accumulators in tensor memory).
 //
 // float: the tensor cores multiply 8-bit significands (bfloat16) exactly and add in 32 bits, so a float is
-// split into three bfloat16 pieces of 8 bits each, x = x0 + x1 + x2 (each piece the rounding of what the
-// ones before leave, exact to 24 bits), and a product takes the six pairs of pieces whose weight is not
-// below the last bit: x0y0, x0y1, x1y0, x1y1, x0y2, x2y0.  What is dropped is below 2^-25 of |x||y| per
-// term, under the rounding of one float multiply-add.  bfloat16 and half go in as they are.
+// cut into three bfloat16 pieces of 8 bits each, x = x0 + x1 + x2 (each piece the rounding of what the ones
+// before leave: exact to 24 bits), and a product takes the six pairs of pieces whose weight is not below the
+// last bit: x0y0, x0y1, x1y0, x1y1, x0y2, x2y0.  What is dropped, x1y2 + x2y1 + x2y2, is below 2^-23 |x||y|
+// and 2^-26 |x||y| on average, of either sign.  (Pieces cut off instead of rounded would cost fewer
+// instructions, but drop up to 2^-20, always of one sign.)  bfloat16 and half go in as they are.
 //
 // One persistent block per SM, warps specialised: eight loader warps bring chunks of 64 terms of both
 // operands into shared memory (float: through registers, split on the way; 16-bit types: one thread issues
@@ -68,7 +69,7 @@ template <typename T>
 struct Operand {
     const T* p;
     int64_t ld, extent;       // row stride; rows (A) or columns (B) in all
-    bool vector;              // base and stride are multiples of 16 bytes
+    bool vector, wide;        // base and stride are multiples of 16, of 32 bytes
 };
 
 template <typename T>
@@ -103,22 +104,35 @@ struct UnitPlace {
     }
 };
 
+// The units of one thread of a chunk at (m0, k0).  A chunk that lies inside the operand needs no more than one
+// address; `wide`: rows start on 32-byte boundaries.
 template <bool K_MAJOR>
-__device__ __forceinline__ void fetch(const Operand<float>& o, int64_t m, int64_t k, int64_t k_end, float (&v)[8]) {
+struct ChunkFetch {
     using U = UnitPlace<float, K_MAJOR>;
-    const int valid = U::valid(m, k, o.extent, k_end);
-    const float* p = U::address(o, m, k);
-    if (valid == 8 && o.vector) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-#pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = q < valid ? __ldg(p + q) : 0.f;
+    const float* p;
+    int64_t step;
+    int64_t m, k, extent, k_end;
+    bool inside;
+    __device__ __forceinline__ ChunkFetch(const Operand<float>& o, int t, int64_t m0, int64_t k0, int64_t end)
+        : m(m0 + U::mn(t, 0)), k(k0 + U::k(t, 0)), extent(o.extent), k_end(end) {
+        p = U::address(o, m, k);
+        step = (K_MAJOR ? kLoaders / 8 : kLoaders / 16) * o.ld;
+        inside = o.wide && m0 + kMmaTile <= extent && k0 + kMmaChunk <= k_end;
     }
-}
+    __device__ __forceinline__ void operator()(int q, float (&v)[8]) const {
+        const float* s = p + q * step;
+        if (inside) {
+            asm volatile("ld.global.nc.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                         : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "l"(s));
+            return;
+        }
+        const int valid = U::valid(K_MAJOR ? m + q * (kLoaders / 8) : m, K_MAJOR ? k : k + q * (kLoaders / 16), extent, k_end);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < valid ? __ldg(s + e) : 0.f;
+    }
+};
 
-// Eight floats as three pieces of eight bfloat16.
+// Eight floats as three pieces of eight bfloat16.  What a piece leaves is exact in 32 bits and formed two at a time.
 __device__ __forceinline__ void split_store(uint32_t addr, const float (&v)[8]) {
     uint32_t piece[3][4];
 #pragma unroll
@@ -129,8 +143,10 @@ __device__ __forceinline__ void split_store(uint32_t addr, const float (&v)[8]) 
             const __nv_bfloat162 r = __floats2bfloat162_rn(lo, hi);
             const uint32_t bits = *reinterpret_cast<const uint32_t*>(&r);
             piece[s][q] = bits;
-            lo -= __uint_as_float(bits << 16);
-            hi -= __uint_as_float(bits & 0xFFFF0000u);
+            if (s == 2) break;
+            asm("{\n\t.reg .b64 x, y, m;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tmov.b64 m, {%4, %4};\n\t"
+                "fma.rn.f32x2 x, y, m, x;\n\tmov.b64 {%0, %1}, x;\n\t}"
+                : "+f"(lo), "+f"(hi) : "r"(bits << 16), "r"(bits & 0xFFFF0000u), "r"(0xBF800000u));      // times -1
         }
     }
 #pragma unroll
@@ -210,17 +226,15 @@ __device__ __forceinline__ void load_split(const Args<T>& g, uint32_t a_ring, ui
     float ra[kUnits][8], rb[kUnits][8];
     Walk<T> w(g), ahead(g);
     bool with_b = true, ahead_b = true;                  // a resident operand is loaded with the block's first item
-    auto fetch_a = [&](int q) {
-        fetch<A_K>(g.a, ahead.i0() + UnitPlace<T, A_K>::mn(t, q), ahead.k0() + UnitPlace<T, A_K>::k(t, q), ahead.k_end(), ra[q]);
-    };
-    auto fetch_b = [&](int q) {
-        fetch<B_K>(g.b, ahead.j0() + UnitPlace<T, B_K>::mn(t, q), ahead.k0() + UnitPlace<T, B_K>::k(t, q), ahead.k_end(), rb[q]);
-    };
     if (!w.live()) return;
+    {
+        const ChunkFetch<A_K> fa(g.a, t, ahead.i0(), ahead.k0(), ahead.k_end());
+        const ChunkFetch<B_K> fb(g.b, t, ahead.j0(), ahead.k0(), ahead.k_end());
 #pragma unroll
-    for (int q = 0; q < kUnits; ++q) {
-        fetch_a(q);
-        fetch_b(q);
+        for (int q = 0; q < kUnits; ++q) {
+            fa(q, ra[q]);
+            fb(q, rb[q]);
+        }
     }
     for (Ring<Traits<T>::a_slots> ring; w.live(); ring.next()) {
         if (ring.wrapped && !tc::mbar_wait(&ctl->empty[ring.slot], ring.parity ^ 1, &ctl->gave_up)) return;
@@ -228,16 +242,20 @@ __device__ __forceinline__ void load_split(const Args<T>& g, uint32_t a_ring, ui
         if (g.resident && ahead.chunk == 0) ahead_b = false;
         const bool more = ahead.live();
         const uint32_t a_slot = a_ring + ring.slot * slot_bytes<T>(), b_slot = b_ring + (g.resident ? w.chunk : ring.slot) * slot_bytes<T>();
+        {
+            const ChunkFetch<A_K> fa(g.a, t, ahead.i0(), ahead.k0(), ahead.k_end());
 #pragma unroll
-        for (int q = 0; q < kUnits; ++q) {
-            split_store(a_slot + UnitPlace<T, A_K>::offset(t, q), ra[q]);
-            if (more) fetch_a(q);
+            for (int q = 0; q < kUnits; ++q) {
+                split_store(a_slot + UnitPlace<T, A_K>::offset(t, q), ra[q]);
+                if (more) fa(q, ra[q]);
+            }
         }
         if (with_b) {
+            const ChunkFetch<B_K> fb(g.b, t, ahead.j0(), ahead.k0(), ahead.k_end());
 #pragma unroll
             for (int q = 0; q < kUnits; ++q) {
                 split_store(b_slot + UnitPlace<T, B_K>::offset(t, q), rb[q]);
-                if (more && ahead_b) fetch_b(q);
+                if (more && ahead_b) fb(q, rb[q]);
             }
         }
         tc::fence_smem_for_async();
@@ -381,7 +399,7 @@ __device__ __noinline__ void repair(const Args<T>& g, uint32_t stage, int64_t ro
         asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
         if (isfinite(v) || i >= g.rows || j >= g.cols) continue;
         v = 0.f;
-        for (int64_t k = k_begin; k < k_end; ++k)
+        for (int64_t k = k_begin; k < k_end && !isnan(v); ++k)
             v = fmaf(to_acc(A_K ? g.a.p[i * g.a.ld + k] : g.a.p[k * g.a.ld + i]), to_acc(B_K ? g.b.p[j * g.b.ld + k] : g.b.p[k * g.b.ld + j]), v);
         asm volatile("st.shared.f32 [%0], %1;" :: "r"(addr), "f"(v) : "memory");
     }
@@ -590,7 +608,9 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
     if (threadIdx.x == 0 && ctl.gave_up && g.status) atomicMax(g.status, static_cast<int>(NB200_ERR_WAIT_BUDGET));
 }
 
-bool multiple16(const void* p, int64_t ld, size_t size) { return aligned16(p) && (ld * size) % 16 == 0; }
+bool multiple_of(size_t bytes, const void* p, int64_t ld, size_t size) {
+    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && (ld * size) % bytes == 0;
+}
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -636,8 +656,8 @@ int mma_product(int64_t rows, int64_t cols, int64_t depth, int64_t splits, int64
         row_tiles * col_tiles * splits > INT32_MAX / 2)
         return NB200_ERR_TOO_LARGE;
     Args<T> g;
-    g.a = {a, as, rows, multiple16(a, as, sizeof(T))};
-    g.b = {b, bs, cols, multiple16(b, bs, sizeof(T))};
+    g.a = {a, as, rows, multiple_of(16, a, as, sizeof(T)), multiple_of(32, a, as, sizeof(T))};
+    g.b = {b, bs, cols, multiple_of(16, b, bs, sizeof(T)), multiple_of(32, b, bs, sizeof(T))};
     g.rows = rows;
     g.cols = cols;
     g.depth = depth;
