@@ -3,7 +3,7 @@
 // with z = x w + bias as the forward pass left it.  x [m, k], w [k, n], y [m, n].
 //
 // This file holds the entry points, the products that run on the CUDA cores (double, for which the tensor
-// cores of this GPU are no faster, and empty sums) and the passes around the products; linear_mma.cu holds
+// cores of this GPU are no faster, and empty sums) and the passes around the products; linear_mma_kernel.cuh holds
 // the products on the tensor cores.
 #include <type_traits>
 

@@ -1,4 +1,4 @@
-// Interface of the tensor-core product (linear_mma.cu) to the entry points in linear.cu.
+// Interface of the tensor-core product (linear_mma_kernel.cuh) to the entry points in linear.cu.
 #pragma once
 #include "dense_common.cuh"
 

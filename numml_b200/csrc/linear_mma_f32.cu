@@ -1,0 +1,6 @@
+// Tensor-core products of float operands; one file per type so that they compile side by side.
+#include "linear_mma_kernel.cuh"
+
+namespace nb200 {
+NB200_MMA_TYPE(float)
+}  // namespace nb200

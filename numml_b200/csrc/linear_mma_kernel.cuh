@@ -15,10 +15,11 @@
 // one before.  When a tile's second operand fits beside the ring of the first (the weights of a layer with
 // few channels), it is loaded and split once per block and the rows stream past it.
 //
-// The tensor cores truncate where they add, always towards zero.  For float the products of leading pieces
-// therefore have an accumulator of their own, into which one addition goes per 16 terms (the five smaller ones
-// go to a second, where a truncation weighs 2^-8 as much), and both are taken out every kDrainChunks chunks
-// and added up in registers with rounding to nearest.
+// The tensor cores truncate where they add, always towards zero.  For float a chunk's products therefore go in
+// order of size, the twenty small ones first, where a truncation weighs 2^-8 as much, then the four of the leading
+// pieces, and the sums over chunks are formed by the epilogue warps with rounding to nearest (the running sums
+// stay in tensor memory).
+#pragma once
 #include <cuda.h>
 
 #include <atomic>
@@ -32,26 +33,27 @@ namespace {
 
 constexpr int kEpilogueWarps = 8, kLoaderWarps = 8, kLoaders = kLoaderWarps * 32;
 constexpr int kThreads = (kEpilogueWarps + kLoaderWarps + 4) * 32;   // whole warpgroups; three warps of the last are idle
-// Registers per thread at launch (float; checked on the host) and after the warpgroups have shared them out anew.
-constexpr int kLaunchRegisters = 96, kEpilogueRegisters = 104, kLoaderRegisters = 112, kProductRegisters = 48;
-static_assert(kEpilogueWarps * kEpilogueRegisters + kLoaderWarps * kLoaderRegisters + 4 * kProductRegisters <=
-              (kEpilogueWarps + kLoaderWarps + 4) * kLaunchRegisters, "registers beyond the block's own would be waited for for ever");
+constexpr int kLaunchRegisters = 96;                               // per thread; checked on the host
 constexpr int kPieceBytes = kMmaTile * kMmaChunk * 2;              // one piece of one operand's chunk: 16 KB
 constexpr int kUnits = kMmaTile * kMmaChunk / 8 / kLoaders;        // units of eight values per loader thread
-constexpr int kDrainChunks = 2;
 constexpr int kAhead = 4;
 
+// Registers per thread after the warpgroups have shared them out anew: the float loaders hold a chunk of both
+// operands and the epilogue the sums of 64 columns; for 16-bit types the epilogue holds twice as many columns of a
+// block and the loaders next to nothing.
 template <typename T> struct Traits {                              // 16-bit types
-    static constexpr int pieces = 1, a_slots = 4, b_slots = 8, accumulators = 1;
-    static constexpr bool drains = false;
+    static constexpr int epilogue_registers = 160, loader_registers = 56, product_registers = 48;
+    static constexpr int pieces = 1, a_slots = 4, b_slots = 8, buffers = 4;
 };
 template <> struct Traits<float> {
-    static constexpr int pieces = 3, a_slots = 2, b_slots = 2, accumulators = 2;
-    static constexpr bool drains = true;
+    static constexpr int epilogue_registers = 120, loader_registers = 96, product_registers = 48;
+    static constexpr int pieces = 3, a_slots = 2, b_slots = 2, buffers = 3;
 };
 
-template <typename T>
-constexpr uint32_t tmem_columns() { return 2 * Traits<T>::accumulators * kMmaTile; }      // two buffers of each
+// What leaves: y; y and z; a product without a forward epilogue; float parts of a sum.
+enum Kind { kForward, kForwardZ, kPlain, kParts };
+
+constexpr uint32_t kTmemColumns = 512;            // float: three accumulators and the running sums; 16-bit: four accumulators
 template <typename T>
 constexpr int slot_bytes() { return Traits<T>::pieces * kPieceBytes; }
 template <typename T>
@@ -60,7 +62,7 @@ constexpr int smem_bytes() {
 }
 
 struct Control {
-    uint64_t full[8], empty[8], acc_full[2], acc_empty[2], done;
+    uint64_t full[8], empty[8], acc_full[4], acc_empty[4], done;
     uint32_t tmem;
     int gave_up;
 };
@@ -78,7 +80,9 @@ struct Args {
     int64_t rows, cols, depth;
     int row_tiles, col_tiles, items;
     int chunks;               // chunks of a part of the sum (the last part may have fewer)
-    bool resident, vector_out, tiled;
+    bool resident;            // a block's second operand stays in shared memory
+    bool tiled;               // operands have rows that bulk copies can address
+    bool vector_out, vector_bias;       // four neighbouring values can be moved at once
     Epilogue<T> ep;
     int32_t* status;
 };
@@ -339,39 +343,35 @@ __device__ void product_role(const Args<T>& g, uint32_t a_ring, uint32_t b_ring,
     constexpr uint32_t idesc = tc::instruction_descriptor(!std::is_same<T, __half>::value, !A_K, !B_K, kMmaTile);
     constexpr uint32_t a_step = A_K ? 32 : 2048, b_step = B_K ? 32 : 2048;       // bytes from one 16-term step to the next
     Ring<S> ring;
-    Ring<2> buffers;
+    Ring<Tr::buffers> buffers;
     bool ok = true;
     for (Walk<T> w(g); ok && w.live(); w.next_item()) {
         for (int c = 0; ok && c < w.chunks; ++c, ring.next()) {
-            const bool fresh = Tr::drains ? c % kDrainChunks == 0 : c == 0;
-            const bool last = c + 1 == w.chunks || (Tr::drains && (c + 1) % kDrainChunks == 0);
+            const bool fresh = Tr::pieces == 3 || c == 0, last = Tr::pieces == 3 || c + 1 == w.chunks;
             if (fresh && buffers.wrapped) ok = tc::mbar_wait(&ctl->acc_empty[buffers.slot], buffers.parity ^ 1, &ctl->gave_up);
             ok = ok && tc::mbar_wait(&ctl->full[ring.slot], ring.parity, &ctl->gave_up);
             if (!ok) break;
             tc::fence_after_sync();
             const uint32_t a = a_ring + ring.slot * slot_bytes<T>(), b = b_ring + (g.resident ? c : ring.slot) * slot_bytes<T>();
-            const uint32_t d = tmem + buffers.slot * Tr::accumulators * kMmaTile;
-            bool accumulate[2] = {!fresh, !fresh};
+            const uint32_t d = tmem + buffers.slot * kMmaTile;
+            bool accumulate = !fresh;
+            auto products = [&](int pa, int pb) {
+                const uint64_t da = tc::smem_descriptor(a + pa * kPieceBytes, A_K ? 16 : kPieceBytes / 2, 1024);
+                const uint64_t db = tc::smem_descriptor(b + pb * kPieceBytes, B_K ? 16 : kPieceBytes / 2, 1024);
 #pragma unroll
-            for (int k = 0; k < kMmaChunk / 16; ++k) {
-                auto product = [&](int pa, int pb) {
-                    const uint64_t da = A_K ? tc::smem_descriptor(a + pa * kPieceBytes + k * a_step, 16, 1024)
-                                            : tc::smem_descriptor(a + pa * kPieceBytes + k * a_step, kPieceBytes / 2, 1024);
-                    const uint64_t db = B_K ? tc::smem_descriptor(b + pb * kPieceBytes + k * b_step, 16, 1024)
-                                            : tc::smem_descriptor(b + pb * kPieceBytes + k * b_step, kPieceBytes / 2, 1024);
-                    const int into = pa + pb > 0 ? 1 : 0;
-                    tc::mma_f16(d + into * kMmaTile, da, db, idesc, accumulate[into]);
-                    accumulate[into] = true;
-                };
-                if (Tr::pieces == 3) {
-                    product(2, 0);
-                    product(0, 2);
-                    product(1, 1);
-                    product(1, 0);
-                    product(0, 1);
+                for (int k = 0; k < kMmaChunk / 16; ++k) {         // the address field counts 16 bytes
+                    tc::mma_f16(d, da + k * (a_step / 16), db + k * (b_step / 16), idesc, accumulate);
+                    accumulate = true;
                 }
-                product(0, 0);
+            };
+            if (Tr::pieces == 3) {
+                products(2, 0);
+                products(0, 2);
+                products(1, 1);
+                products(1, 0);
+                products(0, 1);
             }
+            products(0, 0);
             tc::commit(&ctl->empty[ring.slot]);
             if (last) {
                 tc::commit(&ctl->acc_full[buffers.slot]);
@@ -386,174 +386,241 @@ __device__ void product_role(const Args<T>& g, uint32_t a_ring, uint32_t b_ring,
     while (!tc::mbar_try(addr, 0) && clock64() - t0 < tc::kWaitCycles) {}
 }
 
-// The elements of a staged 32 x 32 block that are not finite, again in plain 32-bit arithmetic: the pieces of an
-// infinity, or of a value that rounds to one in 16 bits, make a NaN where the product may be neither.
+// A value again in plain 32-bit arithmetic: the pieces of an infinity, or of a value that rounds to one in 16 bits,
+// make a NaN where the product may be neither.
 template <typename T, bool A_K, bool B_K>
-__device__ __noinline__ void repair(const Args<T>& g, uint32_t stage, int64_t row0, int64_t col0, int64_t k_begin, int64_t k_end) {
-    const int lane = threadIdx.x % 32;
-    const int64_t i = row0 + lane;
-    for (int q = 0; q < 32; ++q) {
-        const int64_t j = col0 + q;
-        const uint32_t addr = stage + lane * 128 + (((q / 4) ^ (lane % 8)) * 16) + (q % 4) * 4;
-        float v;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-        if (isfinite(v) || i >= g.rows || j >= g.cols) continue;
-        v = 0.f;
-        for (int64_t k = k_begin; k < k_end && !isnan(v); ++k)
-            v = fmaf(to_acc(A_K ? g.a.p[i * g.a.ld + k] : g.a.p[k * g.a.ld + i]), to_acc(B_K ? g.b.p[j * g.b.ld + k] : g.b.p[k * g.b.ld + j]), v);
-        asm volatile("st.shared.f32 [%0], %1;" :: "r"(addr), "f"(v) : "memory");
-    }
+__device__ __forceinline__ float plain_value(const Args<T>& g, int64_t i, int64_t j, int64_t k_begin, int64_t k_end) {
+    float v = 0.f;
+#pragma unroll 1
+    for (int64_t k = k_begin; k < k_end && !isnan(v); ++k)
+        v = fmaf(to_acc(A_K ? g.a.p[i * g.a.ld + k] : g.a.p[k * g.a.ld + i]), to_acc(B_K ? g.b.p[j * g.b.ld + k] : g.b.p[k * g.b.ld + j]), v);
+    return v;
 }
 
-// A staged 32 x 32 block to memory: eight lanes cover a row's 32 columns, a warp four rows at a time.
-template <typename T, int ACT>
-__device__ __forceinline__ void write_block(const Args<T>& g, int split, uint32_t stage, int64_t row0, int64_t col0) {
-    const int lane = threadIdx.x % 32, first = lane / 8, unit = lane % 8;
-    const int64_t j = col0 + unit * 4, i0 = row0 + first;
-    const Epilogue<T>& ep = g.ep;
-    if (j >= g.cols) return;
-    const int width = g.cols - j < 4 ? static_cast<int>(g.cols - j) : 4;
-    const int count = static_cast<int>(min(int64_t(8), (g.rows - i0 + 3) / 4));       // rows of this lane
-    auto staged = [&](int e, float (&v)[4]) {
-        const int r = first + 4 * e;
-        asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
-                     : "r"(stage + r * 128 + ((unit ^ (r % 8)) * 16)));
-    };
-    if (ep.partial) {
-        float* out = reinterpret_cast<float*>(ep.partial) + (split * g.rows + i0) * g.cols + j;
+// What an epilogue warp does with blocks of 32 rows x CB columns, CB columns being a 128-byte line of the output type
+// O.  Accumulators come out of tensor memory one row to a thread; a block goes through 4 KB of shared memory (32 rows
+// of 32 floats, or for 16-bit types twice 16 rows of 64) so that a row's line is written by neighbouring lanes at
+// once: lines written in halves or quarters cost up to twice the time (measured with a row per thread and with
+// 64-byte bulk stores).  Bias, activation, residual and rounding follow behind the turn, when a lane holds four
+// neighbouring columns of eight rows.
+template <typename T, typename O, int ACT, int KIND>
+struct Writer {
+    static constexpr int CB = 128 / sizeof(O);                               // columns of a block
+    static constexpr int kLanes = CB / 4, kStep = 32 / kLanes;               // lanes of a row, rows of a warp's access
+    static constexpr int kPhases = CB / 32, kRows = 32 / kPhases;            // turns through the stage, rows of each
+    const Args<T>& g;
+    float* const stage;
+    const int lane;
+
+    __device__ __forceinline__ Writer(const Args<T>& args, float* s) : g(args), stage(s), lane(threadIdx.x % 32) {}
+    // 16-byte unit u of row r of the stage; swizzled so that neither side of the turn has bank conflicts
+    __device__ __forceinline__ float4* place(int r, int u) const { return reinterpret_cast<float4*>(stage + r * CB) + (u ^ (r & 7)); }
+
+    // What this lane will add to a turn's rows; asked for before the turn, so that its way overlaps.
+    __device__ __forceinline__ void fetch_residual(int64_t row0, int64_t col0, Pack<T, 4> (&next)[8]) const {
+        const int64_t i = row0 + lane / kLanes, j = col0 + lane % kLanes * 4;
+        const int count = j < g.cols ? rows_of_lane(i) : 0;
+        const T* p = g.ep.residual + i * g.ep.ldr + j;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float v[4];
-            staged(e, v);
-            if (e >= count) continue;
-            float* p = out + e * 4 * g.cols;
-            if (g.vector_out) {
-                *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-            } else {
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (q < width) p[q] = v[q];
-            }
-        }
-        return;
+        for (int e = 0; e < 8; ++e, p += kStep * g.ep.ldr)
+            if (e < count) next[e] = *reinterpret_cast<const Pack<T, 4>*>(p);
     }
-    float bias[4] = {};
-    if (ep.bias)
+    __device__ __forceinline__ int rows_of_lane(int64_t i) const {
+        return static_cast<int>(min(int64_t(8), (g.rows - i + kStep - 1) / kStep));
+    }
+
+    // One turn: rows row0 .. row0 + kRows, staged.
+    template <bool RESIDUAL>
+    __device__ __forceinline__ void write(int split, int64_t row0, int64_t col0, const Pack<T, 4> (&next)[8]) const {
+        const Epilogue<T>& ep = g.ep;
+        const int unit = lane % kLanes, first = lane / kLanes;
+        const int64_t j = col0 + unit * 4, i = row0 + first;
+        if (j >= g.cols) return;
+        const int count = rows_of_lane(i);
+        const int64_t at = (split * g.rows + i) * g.cols + j, stride = kStep * g.cols;
+        if constexpr (KIND == kParts) {
+            float* out = ep.partial + at;
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (q < width) bias[q] = to_acc(ep.bias[j + q]);
-    const int64_t out = i0 * g.cols + j;
-    const T* res = ep.residual ? ep.residual + i0 * ep.ldr + j : nullptr;
-    if (g.vector_out) {
+            for (int e = 0; e < 8; ++e, out += stride)
+                if (e < count) *reinterpret_cast<float4*>(out) = *place(first + kStep * e, unit);
+        } else {
+            float bias[4] = {};
+            if (KIND != kPlain && ep.bias) {
+                if (g.vector_bias) {
+                    load_acc<T, 4>(g.ep.bias + j, bias);
+                } else {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            Pack<T, 4> r[4];
-            if (res)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (half * 4 + e < count) r[e] = *reinterpret_cast<const Pack<T, 4>*>(res + (half * 4 + e) * 4 * ep.ldr);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = half * 4 + e;
-                float v[4];
-                staged(row, v);
-                Pack<T, 4> z, y;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float s = v[q] + bias[q];
-                    z.v[q] = rounded_z<T, ACT>(s);
-                    const float t = activate<ACT>(s);
-                    y.v[q] = from_acc<T>(res ? t + to_acc(r[e].v[q]) : t);
+                    for (int q = 0; q < 4; ++q) bias[q] = to_acc(g.ep.bias[j + q]);
                 }
-                if (row >= count) continue;
-                if (ep.z) *reinterpret_cast<Pack<T, 4>*>(ep.z + out + row * 4 * g.cols) = z;
-                *reinterpret_cast<Pack<T, 4>*>(ep.y + out + row * 4 * g.cols) = y;
             }
-        }
-    } else {
-        for (int e = 0; e < count; ++e) {
-            float v[4];
-            staged(e, v);
+            T *out_y = ep.y + at, *out_z = KIND == kForwardZ ? ep.z + at : nullptr;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                if (q >= width) break;
-                const float s = v[q] + bias[q];
-                if (ep.z) ep.z[out + e * 4 * g.cols + q] = rounded_z<T, ACT>(s);
-                float t = activate<ACT>(s);
-                if (res) t += to_acc(res[e * 4 * ep.ldr + q]);
-                ep.y[out + e * 4 * g.cols + q] = from_acc<T>(t);
+            for (int e = 0; e < 8; ++e) {
+                const float4 u = *place(first + kStep * e, unit);
+                float v[4] = {u.x, u.y, u.z, u.w};
+                if constexpr (KIND != kPlain) {
+                    Pack<T, 4> z;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        v[q] += bias[q];
+                        if (KIND == kForwardZ) z.v[q] = rounded_z<T, ACT>(v[q]);
+                        v[q] = activate<ACT>(v[q]);
+                        if (RESIDUAL) v[q] += to_acc(next[e].v[q]);
+                    }
+                    if (KIND == kForwardZ && e < count) *reinterpret_cast<Pack<T, 4>*>(out_z) = z;
+                }
+                if (e < count) store_acc<T, 4>(out_y, v);
+                out_y += stride;
+                if (KIND == kForwardZ) out_z += stride;
             }
         }
     }
-}
+    // The same for rows that start anywhere: a lane per column.
+    __device__ __forceinline__ void write_columns(int split, int64_t row0, int64_t col0) const {
+        const Epilogue<T>& ep = g.ep;
+        const int rows = static_cast<int>(min(int64_t(kRows), g.rows - row0));
+#pragma unroll 1
+        for (int c = lane; c < CB && col0 + c < g.cols; c += 32) {
+            const float bias = KIND != kParts && KIND != kPlain && ep.bias ? to_acc(ep.bias[col0 + c]) : 0.f;
+#pragma unroll 4
+            for (int r = 0; r < rows; ++r) {
+                const float v = reinterpret_cast<const float*>(place(r, c / 4))[c % 4] + bias;
+                const int64_t o = (split * g.rows + row0 + r) * g.cols + col0 + c;
+                if constexpr (KIND == kParts) {
+                    ep.partial[o] = v;
+                } else {
+                    if (KIND == kForwardZ) ep.z[o] = rounded_z<T, ACT>(v);
+                    float t = activate<ACT>(v);
+                    if (KIND != kPlain && ep.residual) t += to_acc(ep.residual[(row0 + r) * ep.ldr + col0 + c]);
+                    ep.y[o] = from_acc<T>(t);
+                }
+            }
+        }
+    }
 
-template <typename T, bool A_K, bool B_K, int ACT>
-__device__ __forceinline__ void epilogue_role(const Args<T>& g, uint32_t staging, uint32_t tmem, Control* ctl) {
+    // This thread's row of a block, and whoever's it is in the other lanes.
+    __device__ __forceinline__ void block(const float (&v)[CB], int split, int64_t row0, int64_t col0) const {
+#pragma unroll
+        for (int phase = 0; phase < kPhases; ++phase) {
+            if (row0 + phase * kRows >= g.rows) break;
+            const bool residual = (KIND == kForward || KIND == kForwardZ) && g.vector_out && g.ep.residual;
+            Pack<T, 4> next[8];
+            if (residual) fetch_residual(row0 + phase * kRows, col0, next);
+            __syncwarp();                            // the turn before has been read
+            if (kPhases == 1 || lane / kRows == phase)
+#pragma unroll
+                for (int u = 0; u < CB / 4; ++u) *place(lane % kRows, u) = make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+            __syncwarp();
+            if (!g.vector_out)
+                write_columns(split, row0 + phase * kRows, col0);
+            else if (residual)
+                write<true>(split, row0 + phase * kRows, col0, next);
+            else
+                write<false>(split, row0 + phase * kRows, col0, next);
+        }
+    }
+};
+
+// The accumulators of one item (float: one per chunk).
+template <typename T, typename O, bool A_K, bool B_K, int ACT, int KIND>
+__device__ __forceinline__ bool epilogue_item(const Args<T>& g, const Walk<T>& w, const Writer<T, O, ACT, KIND>& out,
+                                              Ring<Traits<T>::buffers>& buffers, uint32_t tmem, Control* ctl) {
     using Tr = Traits<T>;
+    constexpr int CB = Writer<T, O, ACT, KIND>::CB;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int quarter = warp % 4, half = warp / 4;                 // tensor memory lanes and columns of this warp
-    const uint32_t stage = staging + warp * 4096;
-    Ring<2> buffers;
-    for (Walk<T> w(g); w.live(); w.next_item()) {
-        float acc[4][16];                                          // sums of the parts that were taken out (float only)
-        const int parts = Tr::drains ? (w.chunks + kDrainChunks - 1) / kDrainChunks : 1;
-        for (int part = 0; part < parts; ++part, buffers.next()) {
-            const bool final = part + 1 == parts;
-            if (!tc::mbar_wait(&ctl->acc_full[buffers.slot], buffers.parity, &ctl->gave_up)) return;
-            tc::fence_after_sync();
+    const int64_t row0 = w.i0() + quarter * 32, col0 = w.j0() + half * 64;
+    auto present = [&](int block) { return row0 < g.rows && col0 + block * CB < g.cols; };
+    const uint32_t mine = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * 64, sums = mine + Tr::buffers * kMmaTile;
+    auto arrived = [&]() {
+        if (!tc::mbar_wait(&ctl->acc_full[buffers.slot], buffers.parity, &ctl->gave_up)) return false;
+        tc::fence_after_sync();
+        return true;
+    };
+    auto release = [&]() {                                         // everything has left the accumulator
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&ctl->acc_empty[buffers.slot]);
+        buffers.next();
+    };
+    if constexpr (Tr::pieces == 3) {
+        for (int part = 0; part + 1 < w.chunks; ++part) {
+            if (!arrived()) return false;
+            const uint32_t from = mine + buffers.slot * kMmaTile;
+#pragma unroll 2
+            for (int c = 0; c < 64 && present(c / CB); c += 16) {
+                float v[16], sum[16];
+                tc::tmem_load16(from + c, v);
+                if (part > 0) tc::tmem_load16(sums + c, sum);
+                tc::tmem_wait16(v);
+                if (part > 0) {
+                    tc::tmem_wait16(sum);
 #pragma unroll
-            for (int block = 0; block < 4; ++block) {
-                const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buffers.slot * Tr::accumulators * kMmaTile +
-                                      half * 64 + block * 16;
-                float v[16];
-                tc::tmem_load16(from, v);
-                tc::tmem_wait(v);
-                if constexpr (Tr::accumulators == 2) {
-#pragma unroll
-                    for (int q = 0; q < 16; ++q) acc[block][q] = part == 0 ? v[q] : acc[block][q] + v[q];
-                    tc::tmem_load16(from + kMmaTile, v);
-                    tc::tmem_wait(v);
-#pragma unroll
-                    for (int q = 0; q < 16; ++q) v[q] = acc[block][q] += v[q];
-                    if (!final) continue;
+                    for (int q = 0; q < 16; ++q) v[q] += sum[q];
                 }
-                bool finite = true;
-                if constexpr (Tr::pieces == 3) {
-                    float t = 0.f;                                 // NaN if any of the values is not finite
-#pragma unroll
-                    for (int q = 0; q < 16; ++q) t = fmaf(v[q], 0.f, t);
-                    finite = t == t;
-                }
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" :: "r"(stage + lane * 128 + (((block % 2 * 4 + q) ^ (lane % 8)) * 16)),
-                                 "f"(v[4 * q]), "f"(v[4 * q + 1]), "f"(v[4 * q + 2]), "f"(v[4 * q + 3]) : "memory");
-                if (block == 3) {                                  // everything has left tensor memory
-                    tc::fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(&ctl->acc_empty[buffers.slot]);
-                }
-                const int64_t row0 = w.i0() + quarter * 32, col0 = w.j0() + half * 64 + block / 2 * 32;
-                if (Tr::pieces == 3 && __any_sync(0xFFFFFFFFu, !finite)) {
-                    __syncwarp();
-                    repair<T, A_K, B_K>(g, stage, row0, col0, w.k_begin(), w.k_end());
-                }
-                if (block % 2 == 1) {
-                    __syncwarp();
-                    write_block<T, ACT>(g, w.split, stage, row0, col0);
-                    __syncwarp();
-                }
+                tc::tmem_store16(sums + c, v);
             }
-            if (!final) {
-                tc::fence_before_sync();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&ctl->acc_empty[buffers.slot]);
-            }
+            tc::tmem_stores_done();
+            release();
         }
     }
+    if (!arrived()) return false;
+    const uint32_t from = mine + buffers.slot * kMmaTile;
+#pragma unroll 1
+    for (int block = 0; block < 64 / CB; ++block) {
+        if (!present(block)) break;
+        const int64_t col = col0 + block * CB;
+        float v[CB];
+#pragma unroll
+        for (int q = 0; q < CB; q += 16) tc::tmem_load16(from + block * CB + q, *reinterpret_cast<float(*)[16]>(v + q));
+        if (Tr::pieces == 3 && w.chunks > 1) {
+#pragma unroll
+            for (int h = 0; h < CB; h += 16) {
+                float sum[16];
+                tc::tmem_load16(sums + block * CB + h, sum);
+                tc::tmem_wait16(v + h);
+                tc::tmem_wait16(sum);
+#pragma unroll
+                for (int q = 0; q < 16; ++q) v[h + q] += sum[q];
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < CB; q += 16) tc::tmem_wait16(v + q);
+        }
+        if (block + 1 == 64 / CB || !present(block + 1)) release();
+        if constexpr (Tr::pieces == 3) {
+            float t = 0.f;                                         // NaN if any of the values is not finite
+#pragma unroll
+            for (int q = 0; q < CB; ++q) t = fmaf(v[q], 0.f, t);
+            if (t != t && row0 + lane < g.rows) {
+                float* row = out.stage + lane * CB;                // the loop's index picks from memory, not from registers
+#pragma unroll
+                for (int q = 0; q < CB; ++q) row[q] = v[q];
+#pragma unroll 1
+                for (int q = 0; q < CB && col + q < g.cols; ++q)
+                    if (!isfinite(row[q])) row[q] = plain_value<T, A_K, B_K>(g, row0 + lane, col + q, w.k_begin(), w.k_end());
+#pragma unroll
+                for (int q = 0; q < CB; ++q) v[q] = row[q];
+            }
+            __syncwarp();
+        }
+        out.block(v, w.split, row0, col);
+    }
+    if (!present(0)) release();
+    return true;
 }
 
-template <typename T, bool A_K, bool B_K, int ACT>
+template <typename T, bool A_K, bool B_K, int ACT, int KIND>
+__device__ __forceinline__ void epilogue_role(const Args<T>& g, float* staging, uint32_t tmem, Control* ctl) {
+    using O = typename std::conditional<KIND == kParts, float, T>::type;
+    const int warp = threadIdx.x / 32;
+    const Writer<T, O, ACT, KIND> out(g, staging + warp * 1024);
+    Ring<Traits<T>::buffers> buffers;
+    Walk<T> w(g);
+    for (bool ok = true; ok && w.live(); w.next_item()) ok = epilogue_item<T, O, A_K, B_K, ACT, KIND>(g, w, out, buffers, tmem, ctl);
+}
+
+template <typename T, bool A_K, bool B_K, int ACT, int KIND>
 __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant__ Args<T> g,
                                                           const __grid_constant__ CUtensorMap map_a,
                                                           const __grid_constant__ CUtensorMap map_b) {
@@ -568,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
             tc::mbar_init(&ctl.full[s], Tr::pieces == 1 && g.tiled ? 1 : kLoaderWarps);
             tc::mbar_init(&ctl.empty[s], 1);
         }
-        for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < Tr::buffers; ++s) {
             tc::mbar_init(&ctl.acc_full[s], 1);
             tc::mbar_init(&ctl.acc_empty[s], kEpilogueWarps);
         }
@@ -576,27 +643,29 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
         ctl.gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kEpilogueWarps + kLoaderWarps) tc::tmem_alloc(&ctl.tmem, tmem_columns<T>());
+    if (warp == kEpilogueWarps + kLoaderWarps) tc::tmem_alloc(&ctl.tmem, kTmemColumns);
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = ctl.tmem;
-    // Float: the loaders hold a chunk of both operands and the epilogue the sums of 64 columns, so registers move to
-    // them from the products' warpgroup.
+    static_assert(kEpilogueWarps * Tr::epilogue_registers + kLoaderWarps * Tr::loader_registers + 4 * Tr::product_registers <=
+                  (kEpilogueWarps + kLoaderWarps + 4) * kLaunchRegisters, "registers beyond the block's own would be waited for for ever");
     if (warp < kEpilogueWarps) {
-        if constexpr (Tr::pieces == 3) tc::registers_up<kEpilogueRegisters>();
-        epilogue_role<T, A_K, B_K, ACT>(g, staging, tmem, &ctl);
+        tc::registers_up<Tr::epilogue_registers>();
+        epilogue_role<T, A_K, B_K, ACT, KIND>(g, reinterpret_cast<float*>(raw + (staging - tc::smem_u32(raw))), tmem, &ctl);
     } else if (warp < kEpilogueWarps + kLoaderWarps) {
         if constexpr (Tr::pieces == 3) {
-            tc::registers_up<kLoaderRegisters>();
+            tc::registers_up<Tr::loader_registers>();
             load_split<T, A_K, B_K>(g, a_ring, b_ring, &ctl);
-        } else if (!g.tiled) {
-            load_gathered<T, A_K, B_K>(g, a_ring, b_ring, &ctl);
-        } else if (threadIdx.x == kEpilogueWarps * 32) {
-            load_tiled<T, A_K, B_K>(g, &map_a, &map_b, a_ring, b_ring, &ctl);
+        } else {
+            tc::registers_down<Tr::loader_registers>();
+            if (!g.tiled)
+                load_gathered<T, A_K, B_K>(g, a_ring, b_ring, &ctl);
+            else if (threadIdx.x == kEpilogueWarps * 32)
+                load_tiled<T, A_K, B_K>(g, &map_a, &map_b, a_ring, b_ring, &ctl);
         }
     } else {
-        if constexpr (Tr::pieces == 3) tc::registers_down<kProductRegisters>();
+        tc::registers_down<Tr::product_registers>();
         if (threadIdx.x == (kEpilogueWarps + kLoaderWarps) * 32) product_role<T, A_K, B_K>(g, a_ring, b_ring, tmem, &ctl);
         if (Tr::pieces == 3 && g.tiled && threadIdx.x == (kEpilogueWarps + kLoaderWarps + 1) * 32)
             prefetch_role<T, A_K, B_K>(g, &map_a, &map_b, &ctl);
@@ -604,7 +673,7 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
     __syncwarp();
     tc::fence_before_sync();
     __syncthreads();
-    if (warp == kEpilogueWarps + kLoaderWarps) tc::tmem_dealloc(tmem, tmem_columns<T>());
+    if (warp == kEpilogueWarps + kLoaderWarps) tc::tmem_dealloc(tmem, kTmemColumns);
     if (threadIdx.x == 0 && ctl.gave_up && g.status) atomicMax(g.status, static_cast<int>(NB200_ERR_WAIT_BUDGET));
 }
 
@@ -646,10 +715,8 @@ bool make_map(CUtensorMap* map, const T* p, int64_t inner, int64_t outer, int64_
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-}  // namespace
-
-template <typename T, bool A_K, bool B_K, int ACT>
-int mma_product(int64_t rows, int64_t cols, int64_t depth, int64_t splits, int64_t per, const T* a, int64_t as, const T* b, int64_t bs,
+template <typename T, bool A_K, bool B_K, int ACT, int KIND>
+int launch(int64_t rows, int64_t cols, int64_t depth, int64_t splits, int64_t per, const T* a, int64_t as, const T* b, int64_t bs,
                 const Epilogue<T>& ep, int32_t* status, cudaStream_t stream) {
     const int64_t row_tiles = ceil_div(rows, kMmaTile), col_tiles = ceil_div(cols, kMmaTile);
     if (row_tiles > INT32_MAX || col_tiles > INT32_MAX || row_tiles * col_tiles > INT32_MAX / 2 ||
@@ -667,10 +734,11 @@ int mma_product(int64_t rows, int64_t cols, int64_t depth, int64_t splits, int64
     g.chunks = static_cast<int>(ceil_div(per < depth ? per : depth, kMmaChunk));
     g.ep = ep;
     g.status = status;
-    const size_t wide = 4 * sizeof(T) < 16 ? 4 * sizeof(T) : 16;
-    auto fits = [&](const void* p) { return !p || reinterpret_cast<uintptr_t>(p) % wide == 0; };
-    g.vector_out = cols % 4 == 0 && fits(ep.z) && fits(ep.y) && fits(ep.residual) && (!ep.residual || ep.ldr % 4 == 0);
     CUtensorMap map_a{}, map_b{};
+    auto fits = [](const void* p, size_t size) { return reinterpret_cast<uintptr_t>(p) % (4 * size) == 0; };
+    g.vector_out = cols % 4 == 0 && (KIND == kParts ? fits(ep.partial, 4) : fits(ep.z, sizeof(T)) && fits(ep.y, sizeof(T))) &&
+                   (!ep.residual || (fits(ep.residual, sizeof(T)) && ep.ldr % 4 == 0));
+    g.vector_bias = fits(ep.bias, sizeof(T));
     // 16-bit types: boxes that the tensor cores read; float: boxes for the prefetches
     g.tiled = g.a.vector && g.b.vector &&
               (A_K ? make_map(&map_a, a, depth, rows, as, kMmaTile) : make_map(&map_a, a, rows, depth, as, kMmaChunk)) &&
@@ -691,19 +759,35 @@ int mma_product(int64_t rows, int64_t cols, int64_t depth, int64_t splits, int64
     if (cudaGetDevice(&device) != cudaSuccess) return NB200_ERR_CUDA;
     if (device >= 64 || !(prepared.load(std::memory_order_acquire) >> device & 1)) {
         cudaFuncAttributes attr;
-        if (cudaFuncSetAttribute(mma_kernel<T, A_K, B_K, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
-            cudaFuncGetAttributes(&attr, mma_kernel<T, A_K, B_K, ACT>) != cudaSuccess)
+        if (cudaFuncSetAttribute(mma_kernel<T, A_K, B_K, ACT, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+            cudaFuncGetAttributes(&attr, mma_kernel<T, A_K, B_K, ACT, KIND>) != cudaSuccess)
             return NB200_ERR_CUDA;
-        if (Traits<T>::pieces == 3 && attr.numRegs != kLaunchRegisters) return NB200_ERR_PRECONDITION;
+        if (attr.numRegs != kLaunchRegisters) return NB200_ERR_PRECONDITION;
         if (device < 64) prepared.fetch_or(uint64_t(1) << device, std::memory_order_release);
     }
-    mma_kernel<T, A_K, B_K, ACT><<<static_cast<unsigned>(grid), kThreads, smem, stream>>>(g, map_a, map_b);
+    mma_kernel<T, A_K, B_K, ACT, KIND><<<static_cast<unsigned>(grid), kThreads, smem, stream>>>(g, map_a, map_b);
     return launch_status();
+}
+
+}  // namespace
+
+template <typename T, bool A_K, bool B_K, int ACT>
+int mma_product(int64_t rows, int64_t cols, int64_t depth, int64_t splits, int64_t per, const T* a, int64_t as, const T* b, int64_t bs,
+                const Epilogue<T>& ep, int32_t* status, cudaStream_t stream) {
+    if constexpr (!A_K) {
+        return launch<T, A_K, B_K, ACT, kParts>(rows, cols, depth, splits, per, a, as, b, bs, ep, status, stream);
+    } else if constexpr (B_K) {
+        return launch<T, A_K, B_K, ACT, kPlain>(rows, cols, depth, splits, per, a, as, b, bs, ep, status, stream);
+    } else {
+        return ep.z ? launch<T, A_K, B_K, ACT, kForwardZ>(rows, cols, depth, splits, per, a, as, b, bs, ep, status, stream)
+                    : launch<T, A_K, B_K, ACT, kForward>(rows, cols, depth, splits, per, a, as, b, bs, ep, status, stream);
+    }
 }
 
 #define NB200_MMA(T, A_K, B_K, ACT)                                                                                            \
     template int mma_product<T, A_K, B_K, ACT>(int64_t, int64_t, int64_t, int64_t, int64_t, const T*, int64_t, const T*, int64_t, \
                                                const Epilogue<T>&, int32_t*, cudaStream_t);
+// The three products of a layer in one type: forward with every activation, dx, dw.
 #define NB200_MMA_TYPE(T)                     \
     NB200_MMA(T, true, false, NB200_ACT_NONE) \
     NB200_MMA(T, true, false, NB200_ACT_RELU) \
@@ -712,8 +796,5 @@ int mma_product(int64_t rows, int64_t cols, int64_t depth, int64_t splits, int64
     NB200_MMA(T, true, false, NB200_ACT_TANH) \
     NB200_MMA(T, true, true, NB200_ACT_NONE)  \
     NB200_MMA(T, false, false, NB200_ACT_NONE)
-NB200_MMA_TYPE(float)
-NB200_MMA_TYPE(__nv_bfloat16)
-NB200_MMA_TYPE(__half)
 
 }  // namespace nb200
