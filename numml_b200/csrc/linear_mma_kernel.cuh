@@ -10,9 +10,10 @@
 // One persistent block per SM, warps specialised: eight loader warps bring chunks of 64 terms of both
 // operands into shared memory (float: through registers, split on the way; 16-bit types: one thread issues
 // tiled bulk copies, or, where rows do not start on 16-byte boundaries, all gather them), one thread issues
-// the products, eight epilogue warps take finished accumulators out of tensor memory, turn them so that a row is written in whole 128-byte lines, and apply bias, activation, residual
-// and rounding.  Accumulators are double-buffered, so the products of a tile run under the epilogue of the
-// one before.  When a tile's second operand fits beside the ring of the first (the weights of a layer with
+// the products, eight epilogue warps take finished accumulators out of tensor memory, apply bias, activation,
+// residual and rounding, and send the rows off in bulk stores of whole 128-byte lines (lines written in halves or
+// quarters took up to twice the time).  There are several accumulators, so the products of a tile run under the
+// epilogue of the one before.  When a tile's second operand fits beside the ring of the first (the weights of a layer with
 // few channels), it is loaded and split once per block and the rows stream past it.
 //
 // The tensor cores truncate where they add, always towards zero.  For float a chunk's products therefore go in
@@ -82,7 +83,8 @@ struct Args {
     int chunks;               // chunks of a part of the sum (the last part may have fewer)
     bool resident;            // a block's second operand stays in shared memory
     bool tiled;               // operands have rows that bulk copies can address
-    bool vector_out, vector_bias;       // four neighbouring values can be moved at once
+    bool tiled_out;           // so have the outputs
+    bool vector_residual, vector_bias;                   // rows of 16-byte units
     Epilogue<T> ep;
     int32_t* status;
 };
@@ -108,31 +110,41 @@ struct UnitPlace {
     }
 };
 
-// The units of one thread of a chunk at (m0, k0).  A chunk that lies inside the operand needs no more than one
-// address; `wide`: rows start on 32-byte boundaries.
+// The units of one thread of a chunk at (m0, k0): a run of eight values of every second, fourth, ... line.  All runs
+// of a thread begin at the same place of their lines, so whether they are whole is asked once; a whole run is one
+// 32-byte load, or two of 16 bytes.
 template <bool K_MAJOR>
 struct ChunkFetch {
     using U = UnitPlace<float, K_MAJOR>;
     const float* p;
     int64_t step;
-    int64_t m, k, extent, k_end;
-    bool inside;
-    __device__ __forceinline__ ChunkFetch(const Operand<float>& o, int t, int64_t m0, int64_t k0, int64_t end)
-        : m(m0 + U::mn(t, 0)), k(k0 + U::k(t, 0)), extent(o.extent), k_end(end) {
+    int lines, run;           // lines left from the first on, values of a run that exist
+    bool wide, vector;
+    __device__ __forceinline__ ChunkFetch(const Operand<float>& o, int t, int64_t m0, int64_t k0, int64_t end) {
+        const int64_t m = m0 + U::mn(t, 0), k = k0 + U::k(t, 0);
+        const int64_t lines_left = K_MAJOR ? o.extent - m : end - k, run_left = K_MAJOR ? end - k : o.extent - m;
+        lines = static_cast<int>(min(lines_left, int64_t(1) << 20));
+        run = static_cast<int>(min(run_left, int64_t(8)));
         p = U::address(o, m, k);
-        step = (K_MAJOR ? kLoaders / 8 : kLoaders / 16) * o.ld;
-        inside = o.wide && m0 + kMmaTile <= extent && k0 + kMmaChunk <= k_end;
+        step = kLineStep * o.ld;
+        wide = o.wide && run == 8;
+        vector = o.vector && run == 8;
     }
+    static constexpr int kLineStep = K_MAJOR ? kLoaders / 8 : kLoaders / 16;
     __device__ __forceinline__ void operator()(int q, float (&v)[8]) const {
         const float* s = p + q * step;
-        if (inside) {
+        const bool exists = q * kLineStep < lines;
+        if (wide && exists) {
             asm volatile("ld.global.nc.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                          : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "l"(s));
-            return;
-        }
-        const int valid = U::valid(K_MAJOR ? m + q * (kLoaders / 8) : m, K_MAJOR ? k : k + q * (kLoaders / 16), extent, k_end);
+        } else if (vector && exists) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(s)), b = __ldg(reinterpret_cast<const float4*>(s) + 1);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = e < valid ? __ldg(s + e) : 0.f;
+            for (int e = 0; e < 8; ++e) v[e] = exists && e < run ? __ldg(s + e) : 0.f;
+        }
     }
 };
 
@@ -340,12 +352,14 @@ template <typename T, bool A_K, bool B_K>
 __device__ void product_role(const Args<T>& g, uint32_t a_ring, uint32_t b_ring, uint32_t tmem, Control* ctl) {
     using Tr = Traits<T>;
     constexpr int S = Tr::a_slots;
-    constexpr uint32_t idesc = tc::instruction_descriptor(!std::is_same<T, __half>::value, !A_K, !B_K, kMmaTile);
+    constexpr uint32_t whole = tc::instruction_descriptor(!std::is_same<T, __half>::value, !A_K, !B_K, kMmaTile);
+    constexpr uint32_t part = tc::instruction_descriptor(!std::is_same<T, __half>::value, !A_K, !B_K, kMmaTile / 2);
     constexpr uint32_t a_step = A_K ? 32 : 2048, b_step = B_K ? 32 : 2048;       // bytes from one 16-term step to the next
     Ring<S> ring;
     Ring<Tr::buffers> buffers;
     bool ok = true;
     for (Walk<T> w(g); ok && w.live(); w.next_item()) {
+        const uint32_t idesc = g.cols - w.j0() > kMmaTile / 2 ? whole : part;      // columns that do not exist are not multiplied
         for (int c = 0; ok && c < w.chunks; ++c, ring.next()) {
             const bool fresh = Tr::pieces == 3 || c == 0, last = Tr::pieces == 3 || c + 1 == w.chunks;
             if (fresh && buffers.wrapped) ok = tc::mbar_wait(&ctl->acc_empty[buffers.slot], buffers.parity ^ 1, &ctl->gave_up);
@@ -397,126 +411,165 @@ __device__ __forceinline__ float plain_value(const Args<T>& g, int64_t i, int64_
     return v;
 }
 
-// What an epilogue warp does with blocks of 32 rows x CB columns, CB columns being a 128-byte line of the output type
-// O.  Accumulators come out of tensor memory one row to a thread; a block goes through 4 KB of shared memory (32 rows
-// of 32 floats, or for 16-bit types twice 16 rows of 64) so that a row's line is written by neighbouring lanes at
-// once: lines written in halves or quarters cost up to twice the time (measured with a row per thread and with
-// 64-byte bulk stores).  Bias, activation, residual and rounding follow behind the turn, when a lane holds four
-// neighbouring columns of eight rows.
+// 128 bytes of the output type from floats, rounded once.
+__device__ __forceinline__ void pack_line(const float (&s)[32], uint32_t (&w)[32], float) {
+#pragma unroll
+    for (int q = 0; q < 32; ++q) w[q] = __float_as_uint(s[q]);
+}
+__device__ __forceinline__ void pack_line(const float (&s)[64], uint32_t (&w)[32], __nv_bfloat16) {
+#pragma unroll
+    for (int q = 0; q < 32; ++q) {
+        const __nv_bfloat162 r = __floats2bfloat162_rn(s[2 * q], s[2 * q + 1]);
+        w[q] = *reinterpret_cast<const uint32_t*>(&r);
+    }
+}
+__device__ __forceinline__ void pack_line(const float (&s)[64], uint32_t (&w)[32], __half) {
+#pragma unroll
+    for (int q = 0; q < 32; ++q) {
+        const __half2 r = __floats2half2_rn(s[2 * q], s[2 * q + 1]);
+        w[q] = *reinterpret_cast<const uint32_t*>(&r);
+    }
+}
+// Value q (0..3 or 0..7) of a 16-byte unit.
+__device__ __forceinline__ float unit_value(const uint32_t (&w)[4], int q, float) { return __uint_as_float(w[q]); }
+__device__ __forceinline__ float unit_value(const uint32_t (&w)[4], int q, __nv_bfloat16) {
+    return __uint_as_float(q & 1 ? w[q / 2] & 0xFFFF0000u : w[q / 2] << 16);
+}
+__device__ __forceinline__ float unit_value(const uint32_t (&w)[4], int q, __half) {
+    const __half2 h = *reinterpret_cast<const __half2*>(&w[q / 2]);
+    return q & 1 ? __high2float(h) : __low2float(h);
+}
+__device__ __forceinline__ void shared_store16(uint32_t addr, const uint32_t* w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" :: "r"(addr), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+__device__ __forceinline__ void shared_load16(uint32_t addr, uint32_t (&w)[4]) {
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr) : "memory");
+}
+
+// What an epilogue warp does with blocks of 32 rows x CB columns, CB columns being 128 bytes of the output type O.
+// Accumulators come out of tensor memory one row to a thread; bias, activation, residual and rounding are applied
+// there, where a thread has a row's values in registers and no address to compute, and a bulk store takes the block
+// from a 4 KB stage to memory, cutting off what lies outside the array.  16-byte unit u of row r of the stage is at
+// unit u ^ (r % 8): the order of the bulk store's 128-byte swizzle, and free of bank conflicts.
 template <typename T, typename O, int ACT, int KIND>
 struct Writer {
-    static constexpr int CB = 128 / sizeof(O);                               // columns of a block
-    static constexpr int kLanes = CB / 4, kStep = 32 / kLanes;               // lanes of a row, rows of a warp's access
-    static constexpr int kPhases = CB / 32, kRows = 32 / kPhases;            // turns through the stage, rows of each
+    static constexpr int CB = 128 / sizeof(O), U = 16 / sizeof(O);           // columns of a block, of a unit
     const Args<T>& g;
-    float* const stage;
+    const void *map_y, *map_z;
+    const uint32_t stage;
     const int lane;
 
-    __device__ __forceinline__ Writer(const Args<T>& args, float* s) : g(args), stage(s), lane(threadIdx.x % 32) {}
-    // 16-byte unit u of row r of the stage; swizzled so that neither side of the turn has bank conflicts
-    __device__ __forceinline__ float4* place(int r, int u) const { return reinterpret_cast<float4*>(stage + r * CB) + (u ^ (r & 7)); }
+    __device__ __forceinline__ Writer(const Args<T>& args, const void* my, const void* mz, uint32_t s)
+        : g(args), map_y(my), map_z(mz), stage(s), lane(threadIdx.x % 32) {}
+    __device__ __forceinline__ uint32_t place(int r, int u) const { return stage + r * 128 + ((u ^ (r & 7)) * 16); }
 
-    // What this lane will add to a turn's rows; asked for before the turn, so that its way overlaps.
-    __device__ __forceinline__ void fetch_residual(int64_t row0, int64_t col0, Pack<T, 4> (&next)[8]) const {
-        const int64_t i = row0 + lane / kLanes, j = col0 + lane % kLanes * 4;
-        const int count = j < g.cols ? rows_of_lane(i) : 0;
+    // Eight lanes read a row's 128 bytes, a warp four rows at a time; asked for early, so that the way overlaps.
+    __device__ __forceinline__ void fetch_residual(int64_t row0, int64_t col0, uint32_t (&next)[8][4]) const {
+        const int64_t i = row0 + lane / 8, j = col0 + lane % 8 * U;
+        const int count = j < g.cols ? static_cast<int>(min(int64_t(8), (g.rows - i + 3) / 4)) : 0;
         const T* p = g.ep.residual + i * g.ep.ldr + j;
 #pragma unroll
-        for (int e = 0; e < 8; ++e, p += kStep * g.ep.ldr)
-            if (e < count) next[e] = *reinterpret_cast<const Pack<T, 4>*>(p);
-    }
-    __device__ __forceinline__ int rows_of_lane(int64_t i) const {
-        return static_cast<int>(min(int64_t(8), (g.rows - i + kStep - 1) / kStep));
-    }
-
-    // One turn: rows row0 .. row0 + kRows, staged.
-    template <bool RESIDUAL>
-    __device__ __forceinline__ void write(int split, int64_t row0, int64_t col0, const Pack<T, 4> (&next)[8]) const {
-        const Epilogue<T>& ep = g.ep;
-        const int unit = lane % kLanes, first = lane / kLanes;
-        const int64_t j = col0 + unit * 4, i = row0 + first;
-        if (j >= g.cols) return;
-        const int count = rows_of_lane(i);
-        const int64_t at = (split * g.rows + i) * g.cols + j, stride = kStep * g.cols;
-        if constexpr (KIND == kParts) {
-            float* out = ep.partial + at;
-#pragma unroll
-            for (int e = 0; e < 8; ++e, out += stride)
-                if (e < count) *reinterpret_cast<float4*>(out) = *place(first + kStep * e, unit);
-        } else {
-            float bias[4] = {};
-            if (KIND != kPlain && ep.bias) {
-                if (g.vector_bias) {
-                    load_acc<T, 4>(g.ep.bias + j, bias);
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) bias[q] = to_acc(g.ep.bias[j + q]);
-                }
+        for (int e = 0; e < 8; ++e, p += 4 * g.ep.ldr)
+            if (e < count) {
+                const uint4 u = *reinterpret_cast<const uint4*>(p);
+                next[e][0] = u.x; next[e][1] = u.y; next[e][2] = u.z; next[e][3] = u.w;
             }
-            T *out_y = ep.y + at, *out_z = KIND == kForwardZ ? ep.z + at : nullptr;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float4 u = *place(first + kStep * e, unit);
-                float v[4] = {u.x, u.y, u.z, u.w};
-                if constexpr (KIND != kPlain) {
-                    Pack<T, 4> z;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        v[q] += bias[q];
-                        if (KIND == kForwardZ) z.v[q] = rounded_z<T, ACT>(v[q]);
-                        v[q] = activate<ACT>(v[q]);
-                        if (RESIDUAL) v[q] += to_acc(next[e].v[q]);
-                    }
-                    if (KIND == kForwardZ && e < count) *reinterpret_cast<Pack<T, 4>*>(out_z) = z;
-                }
-                if (e < count) store_acc<T, 4>(out_y, v);
-                out_y += stride;
-                if (KIND == kForwardZ) out_z += stride;
-            }
-        }
     }
-    // The same for rows that start anywhere: a lane per column.
-    __device__ __forceinline__ void write_columns(int split, int64_t row0, int64_t col0) const {
-        const Epilogue<T>& ep = g.ep;
-        const int rows = static_cast<int>(min(int64_t(kRows), g.rows - row0));
-#pragma unroll 1
-        for (int c = lane; c < CB && col0 + c < g.cols; c += 32) {
-            const float bias = KIND != kParts && KIND != kPlain && ep.bias ? to_acc(ep.bias[col0 + c]) : 0.f;
-#pragma unroll 4
-            for (int r = 0; r < rows; ++r) {
-                const float v = reinterpret_cast<const float*>(place(r, c / 4))[c % 4] + bias;
-                const int64_t o = (split * g.rows + row0 + r) * g.cols + col0 + c;
-                if constexpr (KIND == kParts) {
-                    ep.partial[o] = v;
-                } else {
-                    if (KIND == kForwardZ) ep.z[o] = rounded_z<T, ACT>(v);
-                    float t = activate<ACT>(v);
-                    if (KIND != kPlain && ep.residual) t += to_acc(ep.residual[(row0 + r) * ep.ldr + col0 + c]);
-                    ep.y[o] = from_acc<T>(t);
-                }
-            }
-        }
+    // The stage may be written: the last store has read it.
+    __device__ __forceinline__ void open() const {
+        if (g.tiled_out && lane == 0) tc::stores_read();
+        __syncwarp();
     }
-
-    // This thread's row of a block, and whoever's it is in the other lanes.
-    __device__ __forceinline__ void block(const float (&v)[CB], int split, int64_t row0, int64_t col0) const {
+    // This thread's row of the block to the stage, and from there to memory.
+    __device__ __forceinline__ void close(const float (&s)[CB], O* base, const void* map, int split, int64_t row0, int64_t col0) const {
+        uint32_t w[32];
+        pack_line(s, w, O());
 #pragma unroll
-        for (int phase = 0; phase < kPhases; ++phase) {
-            if (row0 + phase * kRows >= g.rows) break;
-            const bool residual = (KIND == kForward || KIND == kForwardZ) && g.vector_out && g.ep.residual;
-            Pack<T, 4> next[8];
-            if (residual) fetch_residual(row0 + phase * kRows, col0, next);
-            __syncwarp();                            // the turn before has been read
-            if (kPhases == 1 || lane / kRows == phase)
-#pragma unroll
-                for (int u = 0; u < CB / 4; ++u) *place(lane % kRows, u) = make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+        for (int u = 0; u < 8; ++u) shared_store16(place(lane, u), w + 4 * u);
+        if (g.tiled_out) {
+            tc::fence_smem_for_async();
             __syncwarp();
-            if (!g.vector_out)
-                write_columns(split, row0 + phase * kRows, col0);
-            else if (residual)
-                write<true>(split, row0 + phase * kRows, col0, next);
-            else
-                write<false>(split, row0 + phase * kRows, col0, next);
+            if (lane == 0) tc::tile_store(map, static_cast<int>(col0), static_cast<int>(row0), split, stage);
+        } else {                                     // rows that start anywhere: a lane per column
+            __syncwarp();
+            const int rows = static_cast<int>(min(int64_t(32), g.rows - row0));
+#pragma unroll 1
+            for (int c = lane; c < CB && col0 + c < g.cols; c += 32) {
+                O* out = base + (split * g.rows + row0) * g.cols + col0 + c;
+#pragma unroll 4
+                for (int r = 0; r < rows; ++r, out += g.cols) {
+                    const uint32_t addr = place(r, c / U) + c % U * sizeof(O);
+                    if constexpr (sizeof(O) == 4) {
+                        float v;
+                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+                        *out = v;
+                    } else {
+                        unsigned short v;
+                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
+                        *reinterpret_cast<unsigned short*>(out) = v;
+                    }
+                }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void block(float (&v)[CB], int split, int64_t row0, int64_t col0, const uint32_t (&next)[8][4]) const {
+        const Epilogue<T>& ep = g.ep;
+        if constexpr (KIND == kParts) {
+            open();
+            close(v, ep.partial, map_y, split, row0, col0);
+        } else if constexpr (KIND == kPlain) {
+            open();
+            close(v, ep.y, map_y, 0, row0, col0);
+        } else {
+            if (ep.bias) {
+                if (g.vector_bias && col0 + CB <= g.cols) {
+#pragma unroll
+                    for (int u = 0; u < CB; u += U) {
+                        const uint4 b4 = *reinterpret_cast<const uint4*>(ep.bias + col0 + u);
+                        const uint32_t b[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+                        for (int q = 0; q < U; ++q) v[u + q] += unit_value(b, q, O());
+                    }
+                } else {
+#pragma unroll
+                    for (int q = 0; q < CB; ++q) v[q] += col0 + q < g.cols ? to_acc(ep.bias[col0 + q]) : 0.f;
+                }
+            }
+            if constexpr (KIND == kForwardZ) {
+                open();
+                if constexpr (ACT == NB200_ACT_RELU && sizeof(T) == 2) {   // only relu's slope needs more than the rounded value
+                    float t[CB];
+#pragma unroll
+                    for (int q = 0; q < CB; ++q) t[q] = to_acc(rounded_z<T, ACT>(v[q]));
+                    close(t, ep.z, map_z, 0, row0, col0);
+                } else {
+                    close(v, ep.z, map_z, 0, row0, col0);
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < CB; ++q) v[q] = activate<ACT>(v[q]);
+            open();
+            if (ep.residual) {
+                if (g.vector_residual) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) shared_store16(place(lane / 8 + 4 * e, lane % 8), next[e]);
+                    __syncwarp();
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        uint32_t r[4];
+                        shared_load16(place(lane, u), r);
+#pragma unroll
+                        for (int q = 0; q < U; ++q) v[u * U + q] += unit_value(r, q, O());
+                    }
+                } else if (row0 + lane < g.rows) {
+                    const T* p = ep.residual + (row0 + lane) * ep.ldr + col0;
+#pragma unroll
+                    for (int q = 0; q < CB; ++q)
+                        if (col0 + q < g.cols) v[q] += to_acc(p[q]);
+                }
+            }
+            close(v, ep.y, map_y, 0, row0, col0);
         }
     }
 };
@@ -570,6 +623,8 @@ __device__ __forceinline__ bool epilogue_item(const Args<T>& g, const Walk<T>& w
     for (int block = 0; block < 64 / CB; ++block) {
         if (!present(block)) break;
         const int64_t col = col0 + block * CB;
+        uint32_t residual[8][4];
+        if ((KIND == kForward || KIND == kForwardZ) && g.ep.residual && g.vector_residual) out.fetch_residual(row0, col, residual);
         float v[CB];
 #pragma unroll
         for (int q = 0; q < CB; q += 16) tc::tmem_load16(from + block * CB + q, *reinterpret_cast<float(*)[16]>(v + q));
@@ -593,37 +648,42 @@ __device__ __forceinline__ bool epilogue_item(const Args<T>& g, const Walk<T>& w
 #pragma unroll
             for (int q = 0; q < CB; ++q) t = fmaf(v[q], 0.f, t);
             if (t != t && row0 + lane < g.rows) {
-                float* row = out.stage + lane * CB;                // the loop's index picks from memory, not from registers
-#pragma unroll
-                for (int q = 0; q < CB; ++q) row[q] = v[q];
+                // one value in turn, so that the loop needs no index into registers
 #pragma unroll 1
-                for (int q = 0; q < CB && col + q < g.cols; ++q)
-                    if (!isfinite(row[q])) row[q] = plain_value<T, A_K, B_K>(g, row0 + lane, col + q, w.k_begin(), w.k_end());
+                for (int q = 0; q < CB; ++q) {
+                    float first = v[0];
+                    if (!isfinite(first) && col + q < g.cols) first = plain_value<T, A_K, B_K>(g, row0 + lane, col + q, w.k_begin(), w.k_end());
 #pragma unroll
-                for (int q = 0; q < CB; ++q) v[q] = row[q];
+                    for (int r = 0; r + 1 < CB; ++r) v[r] = v[r + 1];
+                    v[CB - 1] = first;
+                }
             }
             __syncwarp();
         }
-        out.block(v, w.split, row0, col);
+        out.block(v, w.split, row0, col, residual);
     }
     if (!present(0)) release();
     return true;
 }
 
 template <typename T, bool A_K, bool B_K, int ACT, int KIND>
-__device__ __forceinline__ void epilogue_role(const Args<T>& g, float* staging, uint32_t tmem, Control* ctl) {
+__device__ __forceinline__ void epilogue_role(const Args<T>& g, const void* map_y, const void* map_z, uint32_t staging, uint32_t tmem,
+                                              Control* ctl) {
     using O = typename std::conditional<KIND == kParts, float, T>::type;
     const int warp = threadIdx.x / 32;
-    const Writer<T, O, ACT, KIND> out(g, staging + warp * 1024);
+    const Writer<T, O, ACT, KIND> out(g, map_y, map_z, staging + warp * 4096);
     Ring<Traits<T>::buffers> buffers;
     Walk<T> w(g);
     for (bool ok = true; ok && w.live(); w.next_item()) ok = epilogue_item<T, O, A_K, B_K, ACT, KIND>(g, w, out, buffers, tmem, ctl);
+    if (threadIdx.x % 32 == 0) tc::stores_done();
 }
 
 template <typename T, bool A_K, bool B_K, int ACT, int KIND>
 __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant__ Args<T> g,
                                                           const __grid_constant__ CUtensorMap map_a,
-                                                          const __grid_constant__ CUtensorMap map_b) {
+                                                          const __grid_constant__ CUtensorMap map_b,
+                                                          const __grid_constant__ CUtensorMap map_y,
+                                                          const __grid_constant__ CUtensorMap map_z) {
     using Tr = Traits<T>;
     extern __shared__ char raw[];
     __shared__ Control ctl;
@@ -652,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
                   (kEpilogueWarps + kLoaderWarps + 4) * kLaunchRegisters, "registers beyond the block's own would be waited for for ever");
     if (warp < kEpilogueWarps) {
         tc::registers_up<Tr::epilogue_registers>();
-        epilogue_role<T, A_K, B_K, ACT, KIND>(g, reinterpret_cast<float*>(raw + (staging - tc::smem_u32(raw))), tmem, &ctl);
+        epilogue_role<T, A_K, B_K, ACT, KIND>(g, &map_y, &map_z, staging, tmem, &ctl);
     } else if (warp < kEpilogueWarps + kLoaderWarps) {
         if constexpr (Tr::pieces == 3) {
             tc::registers_up<Tr::loader_registers>();
@@ -715,6 +775,20 @@ bool make_map(CUtensorMap* map, const T* p, int64_t inner, int64_t outer, int64_
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Boxes of 32 rows by 128 bytes of a [parts, rows, cols] array, for the epilogue's stores.
+template <typename O>
+bool make_output_map(CUtensorMap* map, O* p, int64_t rows, int64_t cols, int64_t parts) {
+    const EncodeTiled encode = encode_tiled();
+    const uint64_t line = static_cast<uint64_t>(cols) * sizeof(O), part = static_cast<uint64_t>(rows) * line;
+    if (!encode || !aligned16(p) || line % 16 != 0 || rows > INT32_MAX || cols > INT32_MAX || part >= (uint64_t(1) << 40)) return false;
+    const cuuint64_t size[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(parts)};
+    const cuuint64_t stride[2] = {line, part};
+    const cuuint32_t box[3] = {128 / sizeof(O), 32, 1}, step[3] = {1, 1, 1};
+    const CUtensorMapDataType type = sizeof(O) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+    return encode(map, type, 3, p, size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, bool A_K, bool B_K, int ACT, int KIND>
 int launch(int64_t rows, int64_t cols, int64_t depth, int64_t splits, int64_t per, const T* a, int64_t as, const T* b, int64_t bs,
                 const Epilogue<T>& ep, int32_t* status, cudaStream_t stream) {
@@ -734,11 +808,11 @@ int launch(int64_t rows, int64_t cols, int64_t depth, int64_t splits, int64_t pe
     g.chunks = static_cast<int>(ceil_div(per < depth ? per : depth, kMmaChunk));
     g.ep = ep;
     g.status = status;
-    CUtensorMap map_a{}, map_b{};
-    auto fits = [](const void* p, size_t size) { return reinterpret_cast<uintptr_t>(p) % (4 * size) == 0; };
-    g.vector_out = cols % 4 == 0 && (KIND == kParts ? fits(ep.partial, 4) : fits(ep.z, sizeof(T)) && fits(ep.y, sizeof(T))) &&
-                   (!ep.residual || (fits(ep.residual, sizeof(T)) && ep.ldr % 4 == 0));
-    g.vector_bias = fits(ep.bias, sizeof(T));
+    CUtensorMap map_a{}, map_b{}, map_y{}, map_z{};
+    g.tiled_out = KIND == kParts ? make_output_map(&map_y, ep.partial, rows, cols, splits)
+                                 : make_output_map(&map_y, ep.y, rows, cols, 1) && (!ep.z || make_output_map(&map_z, ep.z, rows, cols, 1));
+    g.vector_residual = (cols * sizeof(T)) % 16 == 0 && multiple_of(16, ep.residual, ep.ldr, sizeof(T));
+    g.vector_bias = aligned16(ep.bias);
     // 16-bit types: boxes that the tensor cores read; float: boxes for the prefetches
     g.tiled = g.a.vector && g.b.vector &&
               (A_K ? make_map(&map_a, a, depth, rows, as, kMmaTile) : make_map(&map_a, a, rows, depth, as, kMmaChunk)) &&
@@ -765,7 +839,7 @@ int launch(int64_t rows, int64_t cols, int64_t depth, int64_t splits, int64_t pe
         if (attr.numRegs != kLaunchRegisters) return NB200_ERR_PRECONDITION;
         if (device < 64) prepared.fetch_or(uint64_t(1) << device, std::memory_order_release);
     }
-    mma_kernel<T, A_K, B_K, ACT, KIND><<<static_cast<unsigned>(grid), kThreads, smem, stream>>>(g, map_a, map_b);
+    mma_kernel<T, A_K, B_K, ACT, KIND><<<static_cast<unsigned>(grid), kThreads, smem, stream>>>(g, map_a, map_b, map_y, map_z);
     return launch_status();
 }
 

@@ -105,6 +105,16 @@ __device__ __forceinline__ void tile_load(uint32_t dst, const void* map, int x, 
                  :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
 }
 
+// A box from shared memory to element (x, y, z); what lies outside the array is not written.  Groups of stores are
+// counted per thread.
+__device__ __forceinline__ void tile_store(const void* map, int x, int y, int z, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];"
+                 :: "l"(map), "r"(x), "r"(y), "r"(z), "r"(src) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// The thread's stores have read their shared memory / are done.
+__device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 // The same box into L2 only.
 __device__ __forceinline__ void tile_prefetch(const void* map, int x, int y) {
     asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" :: "l"(map), "r"(x), "r"(y) : "memory");
