@@ -44,10 +44,6 @@ __device__ __forceinline__ void store_acc(T* p, const acc_t<T> (&in)[V]) {
 }
 
 // ---- activations ---------------------------------------------------------------------------------
-__device__ __forceinline__ float exp_acc(float v) { return expf(v); }
-__device__ __forceinline__ double exp_acc(double v) { return exp(v); }
-__device__ __forceinline__ float erf_acc(float v) { return erff(v); }
-__device__ __forceinline__ double erf_acc(double v) { return erf(v); }
 __device__ __forceinline__ float tanh_acc(float v) { return tanhf(v); }
 __device__ __forceinline__ double tanh_acc(double v) { return tanh(v); }
 
@@ -59,11 +55,30 @@ __device__ __forceinline__ double logistic(double z) { return 1.0 / (1.0 + exp(-
 constexpr double kRootHalf = 0.70710678118654752440;     // 1 / sqrt(2)
 constexpr double kInvRoot2Pi = 0.39894228040143267794;   // 1 / sqrt(2 pi)
 
+// The normal distribution function at z and exp(-z^2 / 2).  In 32 bits by Abramowitz and Stegun, Handbook of
+// Mathematical Functions, 7.1.26: erf(x) = 1 - (a1 t + ... + a5 t^5) exp(-x^2) with t = 1 / (1 + p x), x >= 0, off by
+// at most 1.5e-7, so the result is off by little more than a rounding of a number near one.  It has no branches, and
+// its exponential is the one that the density needs: slope and value together cost a third of erff and expf.
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+    const float x = fabsf(z) * static_cast<float>(kRootHalf), t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
+    e = __expf(-x * x);
+    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    const float tail = 0.5f * poly * e;
+    return z > 0.f ? 1.f - tail : tail;
+}
+__device__ __forceinline__ double normal_cdf(double z, double& e) {
+    e = exp(-0.5 * z * z);
+    return 0.5 * erfc(-z * kRootHalf);
+}
+
 template <int ACT, typename A>
 __device__ __forceinline__ A activate(A z) {
     if constexpr (ACT == NB200_ACT_RELU) return z > A(0) ? z : (z != z ? z : A(0));
     if constexpr (ACT == NB200_ACT_SILU) return z * logistic(z);
-    if constexpr (ACT == NB200_ACT_GELU) return A(0.5) * z * (A(1) + erf_acc(z * A(kRootHalf)));
+    if constexpr (ACT == NB200_ACT_GELU) {
+        A e;
+        return z * normal_cdf(z, e);
+    }
     if constexpr (ACT == NB200_ACT_TANH) return tanh_acc(z);
     return z;
 }
@@ -76,11 +91,14 @@ __device__ __forceinline__ A activate_slope(A z) {
         const A s = logistic(z);
         return s * (A(1) + z * (A(1) - s));
     }
-    if constexpr (ACT == NB200_ACT_GELU)
-        return A(0.5) * (A(1) + erf_acc(z * A(kRootHalf))) + z * A(kInvRoot2Pi) * exp_acc(A(-0.5) * z * z);
-    if constexpr (ACT == NB200_ACT_TANH) {
-        const A t = tanh_acc(z);
-        return A(1) - t * t;
+    if constexpr (ACT == NB200_ACT_GELU) {
+        A e;
+        const A cdf = normal_cdf(z, e);
+        return cdf + z * A(kInvRoot2Pi) * e;
+    }
+    if constexpr (ACT == NB200_ACT_TANH) {                        // 1 - tanh^2 = 4 s (1 - s) with s = logistic(2 z)
+        const A s = logistic(A(2) * z);
+        return A(4) * s * (A(1) - s);
     }
     return A(1);
 }

@@ -37,66 +37,108 @@ __device__ __forceinline__ Words philox(uint64_t block, uint64_t offset, uint32_
     return {{c0, c1, c2, c3}};
 }
 
-// Bit q set: element q of the block of eight is kept.
-__device__ __forceinline__ uint32_t keep_bits(uint64_t block, uint64_t offset, uint64_t seed, uint32_t t_high, uint32_t t_low) {
+// Which of a block's eight elements are kept.  `high` holds the threshold's high half in its upper 16 bits (zeros
+// below): a word's upper half is above it where the word is above high | 0xFFFF, its lower half where the word
+// shifted up is above high, so no half is taken out.  A half that equals the threshold's makes a zero half in
+// word ^ pattern; one test finds it in all four words.
+struct Threshold {
+    uint32_t high, pattern, low;
+};
+__device__ __forceinline__ void keep_flags(uint64_t block, uint64_t offset, uint64_t seed, const Threshold& t, bool (&keep)[8]) {
     const Words a = philox(block, offset, 0, seed);
-    uint32_t keep = 0, tie = 0;
+    uint32_t zero = 0;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-        const uint32_t h = (q & 1) ? a.w[q / 2] >> 16 : a.w[q / 2] & 0xFFFFu;
-        keep |= (h > t_high ? 1u : 0u) << q;
-        tie |= (h == t_high ? 1u : 0u) << q;
+    for (int q = 0; q < 4; ++q) {
+        keep[2 * q] = (a.w[q] << 16) > t.high;
+        keep[2 * q + 1] = a.w[q] > (t.high | 0xFFFFu);
+        const uint32_t z = a.w[q] ^ t.pattern;
+        zero |= (z - 0x00010001u) & ~z;
     }
-    if (tie) {
+    if (zero & 0x80008000u) {                        // at most a few in 65536: a carry may report a half that is none
         const Words b = philox(block, offset, 1, seed);
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-            const uint32_t l = (q & 1) ? b.w[q / 2] >> 16 : b.w[q / 2] & 0xFFFFu;
-            if ((tie >> q & 1u) && l >= t_low) keep |= 1u << q;
+            const uint32_t h = (q & 1) ? a.w[q / 2] >> 16 : a.w[q / 2] & 0xFFFFu, l = (q & 1) ? b.w[q / 2] >> 16 : b.w[q / 2] & 0xFFFFu;
+            if (h == t.high >> 16) keep[q] = l >= t.low;
         }
     }
-    return keep;
 }
 
-// A thread owns blocks of eight consecutive elements; `state` (device int64[2]: seed, offset) overrides
-// the arguments when given, so that a captured graph can be replayed with new numbers.
+template <typename T>
+constexpr int batch() { return sizeof(T) == 8 ? 1 : sizeof(T) == 4 ? 2 : 4; }
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, acc_t<T> (&v)[8]) {
+    constexpr int V = 16 / sizeof(T);
+#pragma unroll
+    for (int q = 0; q < 8; q += V) load_acc<T, V>(p + q, *reinterpret_cast<acc_t<T>(*)[V]>(v + q));
+}
+
+// A thread has kBatch blocks of eight consecutive elements, all of whose loads are under way before the first is used;
+// `state` (device int64[2]: seed, offset) overrides the arguments when given, so that a captured graph can be
+// replayed with new numbers.
 template <typename T, bool RESIDUAL>
 __global__ void __launch_bounds__(256) dropout_kernel(int64_t n, const T* __restrict__ x, const T* __restrict__ residual,
-                                                      T* __restrict__ y, uint64_t threshold, acc_t<T> scale, uint64_t seed,
+                                                      T* __restrict__ y, Threshold threshold, acc_t<T> scale, uint64_t seed,
                                                       uint64_t offset, const int64_t* __restrict__ state) {
     using A = acc_t<T>;
-    constexpr int V = 16 / sizeof(T) < 8 ? 16 / sizeof(T) : 8;
+    constexpr int V = 16 / sizeof(T), kBatch = batch<T>();
     if (state) {
         seed = static_cast<uint64_t>(state[0]);
         offset = static_cast<uint64_t>(state[1]);
     }
-    // T = 2^32 (p = 1) keeps nothing: no half-word exceeds 0x10000
-    const uint32_t t_high = static_cast<uint32_t>(threshold >> 16), t_low = static_cast<uint32_t>(threshold & 0xFFFFu);
-    const int64_t blocks = (n + 7) / 8;
-    for (int64_t b = blockIdx.x * int64_t(blockDim.x) + threadIdx.x; b < blocks; b += int64_t(gridDim.x) * blockDim.x) {
-        const int64_t base = b * 8;
-        if (base + 8 <= n) {
+    const int64_t whole = n / 8;
+    constexpr int64_t stride = 256;
+    int64_t b = blockIdx.x * (kBatch * stride) + threadIdx.x;
+    const int64_t limit = min(whole, (blockIdx.x + int64_t(1)) * (kBatch * stride));
+    auto finish = [&](int64_t block, A (&xv)[8], const A (&rv)[8]) {
+        bool keep[8];
+        keep_flags(block, offset, seed, threshold, keep);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            xv[q] = keep[q] ? xv[q] * scale : A(0);
+            if (RESIDUAL) xv[q] += rv[q];
+        }
+#pragma unroll
+        for (int q = 0; q < 8; q += V) store_acc<T, V>(y + block * 8 + q, *reinterpret_cast<A(*)[V]>(xv + q));
+    };
+    if (b + (kBatch - 1) * stride < whole) {
+        Pack<T, V> xr[kBatch][8 / V], rr[kBatch][8 / V];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+            for (int q = 0; q < 8 / V; ++q) {
+                xr[u][q] = *reinterpret_cast<const Pack<T, V>*>(x + (b + u * stride) * 8 + q * V);
+                if (RESIDUAL) rr[u][q] = *reinterpret_cast<const Pack<T, V>*>(residual + (b + u * stride) * 8 + q * V);
+            }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
             A xv[8], rv[8];
 #pragma unroll
-            for (int q = 0; q < 8; q += V) {
-                load_acc<T, V>(x + base + q, *reinterpret_cast<A(*)[V]>(xv + q));
-                if (RESIDUAL) load_acc<T, V>(residual + base + q, *reinterpret_cast<A(*)[V]>(rv + q));
-            }
-            const uint32_t keep = keep_bits(b, offset, seed, t_high, t_low);
-#pragma unroll
             for (int q = 0; q < 8; ++q) {
-                xv[q] = (keep >> q & 1u) ? xv[q] * scale : A(0);
-                if (RESIDUAL) xv[q] += rv[q];
+                xv[q] = to_acc(xr[u][q / V].v[q % V]);
+                rv[q] = RESIDUAL ? to_acc(rr[u][q / V].v[q % V]) : A(0);
             }
+            finish(b + u * stride, xv, rv);
+        }
+        return;
+    }
+    for (; b < limit; b += stride) {
+        A xv[8], rv[8] = {};
+        load8(x + b * 8, xv);
+        if (RESIDUAL) load8(residual + b * 8, rv);
+        finish(b, xv, rv);
+    }
+    if (b == whole && n % 8 != 0 && b < (blockIdx.x + int64_t(1)) * (kBatch * stride)) {          // the last, partial block
+        bool keep[8];
+        keep_flags(whole, offset, seed, threshold, keep);
 #pragma unroll
-            for (int q = 0; q < 8; q += V) store_acc<T, V>(y + base + q, *reinterpret_cast<A(*)[V]>(xv + q));
-        } else {
-            const uint32_t keep = keep_bits(b, offset, seed, t_high, t_low);
-            for (int64_t i = base; i < n; ++i) {
-                A v = (keep >> (i - base) & 1u) ? to_acc(x[i]) * scale : A(0);
-                if (RESIDUAL) v += to_acc(residual[i]);
-                y[i] = from_acc<T>(v);
-            }
+        for (int q = 0; q < 7; ++q) {
+            const int64_t i = whole * 8 + q;
+            if (i >= n) break;
+            A v = keep[q] ? to_acc(x[i]) * scale : A(0);
+            if (RESIDUAL) v += to_acc(residual[i]);
+            y[i] = from_acc<T>(v);
         }
     }
 }
@@ -104,10 +146,15 @@ __global__ void __launch_bounds__(256) dropout_kernel(int64_t n, const T* __rest
 template <typename T>
 int launch_dropout(int64_t n, const void* x, const void* residual, void* y, double p, uint64_t seed, uint64_t offset,
                    const int64_t* state, cudaStream_t stream) {
-    const uint64_t threshold = static_cast<uint64_t>(std::nearbyint(p * 4294967296.0));
+    const uint64_t bar = static_cast<uint64_t>(std::nearbyint(p * 4294967296.0));
+    // 2^32 (p = 1) keeps nothing: no half is above 0xFFFF and no lower half reaches 0x10000
+    const uint32_t half = bar >> 32 ? 0xFFFFu : static_cast<uint32_t>(bar >> 16);
+    const Threshold threshold{half << 16, half << 16 | half, bar >> 32 ? 0x10000u : static_cast<uint32_t>(bar & 0xFFFFu)};
     const acc_t<T> scale = p < 1.0 ? static_cast<acc_t<T>>(1.0 / (1.0 - p)) : acc_t<T>(0);
-    const int64_t blocks = ceil_div(n, 8);
-    const int grid = static_cast<int>(ceil_div(blocks, 256) < kSMs * 8 ? ceil_div(blocks, 256) : kSMs * 8);
+    constexpr int kBatch = batch<T>();
+    const int64_t blocks = ceil_div(ceil_div(n, 8), 256 * kBatch);
+    if (blocks > INT32_MAX) return NB200_ERR_TOO_LARGE;
+    const unsigned grid = static_cast<unsigned>(blocks);
     const T* xt = static_cast<const T*>(x);
     if (residual)
         dropout_kernel<T, true><<<grid, 256, 0, stream>>>(n, xt, static_cast<const T*>(residual), static_cast<T*>(y), threshold,

@@ -86,7 +86,8 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(Shape sh, const T* __re
         if (live) {
             int64_t r = row + row_lane;
             if (r < end) load_acc<T, V>(x + r * sh.channels + c, k);
-#pragma unroll 4
+            n = static_cast<A>(r < end ? (end - r + row_lanes - 1) / row_lanes : 0);
+#pragma unroll 8
             for (; r < end; r += row_lanes) {
                 A v[V];
                 load_acc<T, V>(x + r * sh.channels + c, v);
@@ -96,7 +97,6 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(Shape sh, const T* __re
                     sum[q] += d;
                     sq[q] += d * d;
                 }
-                n += A(1);
             }
         }
         A mean[V], m2[V];
@@ -146,42 +146,60 @@ __device__ __forceinline__ int64_t piece_rows(int64_t begin, int64_t end, int64_
     return min(end, (b + 1) * chunk) - max(begin, b * chunk);
 }
 
-// One team of TEAM threads per (segment, group).
+// One team of TEAM threads per (segment, group): the mean from the pieces' means weighted by their entries, then the
+// sum of squared deviations from it, sum of m2 + entries (piece's mean - mean)^2, all in 64 bits.
+template <int TEAM>
+__device__ __forceinline__ double team_sum(double v, double* sm) {
+    const int t = threadIdx.x % TEAM;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, off);
+    if (TEAM == 32) return v;
+    __syncthreads();
+    if (t % 32 == 0) sm[t / 32] = v;
+    __syncthreads();
+    double total = 0;
+#pragma unroll
+    for (int q = 0; q < TEAM / 32; ++q) total += sm[q];
+    return total;
+}
+
+constexpr int join_threads(int team) { return team < kThreads ? kThreads : team; }
+
 template <typename A, int TEAM>
-__global__ void __launch_bounds__(kThreads) stats_join_kernel(Shape sh, const A* __restrict__ part, double eps,
+__global__ void __launch_bounds__(join_threads(TEAM)) stats_join_kernel(Shape sh, const A* __restrict__ part, double eps,
                                                               A* __restrict__ mean_out, A* __restrict__ rstd_out) {
-    __shared__ double sm[3][kThreads];
+    __shared__ double sm[join_threads(TEAM) / 32];
     const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM;
-    const int64_t item = blockIdx.x * int64_t(kThreads / TEAM) + team;
+    const int64_t item = blockIdx.x * int64_t(join_threads(TEAM) / TEAM) + team;
     const bool live = item < sh.segments * sh.groups;
     const int64_t s = live ? item / sh.groups : 0;
     const int g = static_cast<int>(live ? item % sh.groups : 0), width = sh.channels / sh.groups;
     const int64_t begin = segment_begin(sh, s), end = max(begin, segment_begin(sh, s + 1));
-    double n = 0, mean = 0, m2 = 0;
-    if (live && end > begin) {
-        const int64_t first = begin / sh.chunk, last = (end - 1) / sh.chunk, work = (last - first + 1) * width;
-        for (int64_t e = t; e < work; e += TEAM) {
-            const int64_t b = first + e / width;
-            const A* p = part + (b + s) * 2 * sh.channels + g * width + e % width;
-            join(n, mean, m2, static_cast<double>(piece_rows(begin, end, b, sh.chunk)), static_cast<double>(p[0]),
-                 static_cast<double>(p[sh.channels]));
-        }
-    }
-    sm[0][threadIdx.x] = n;
-    sm[1][threadIdx.x] = mean;
-    sm[2][threadIdx.x] = m2;
-    __syncthreads();
-    for (int off = TEAM / 2; off > 0; off >>= 1) {
-        if (t < off) {
-            join(n, mean, m2, sm[0][threadIdx.x + off], sm[1][threadIdx.x + off], sm[2][threadIdx.x + off]);
-            sm[0][threadIdx.x] = n;
-            sm[1][threadIdx.x] = mean;
-            sm[2][threadIdx.x] = m2;
-        }
-        __syncthreads();
-    }
+    const int64_t first = begin / sh.chunk, last = end > begin ? (end - 1) / sh.chunk : first - 1;
+    const int64_t pieces = live ? last - first + 1 : 0;
+    const A* base = part + (first + s) * 2 * sh.channels + g * width;
+    // the team's threads go along the channels first; what does not divide is idle
+    const int per = width < TEAM ? width : TEAM, lanes = TEAM / per, lane = t / per;
+    double sum = 0;
+    for (int c = t % per; c < width; c += per)
+        if (lane < lanes)
+#pragma unroll 4
+            for (int64_t b = lane; b < pieces; b += lanes)
+                sum += static_cast<double>(piece_rows(begin, end, first + b, sh.chunk)) * static_cast<double>(base[b * 2 * sh.channels + c]);
+    const double n = static_cast<double>(end - begin) * width;
+    const double mean = team_sum<TEAM>(sum, sm) / (n > 0 ? n : 1.0);
+    double m2 = 0;
+    for (int c = t % per; c < width; c += per)
+        if (lane < lanes)
+#pragma unroll 4
+            for (int64_t b = lane; b < pieces; b += lanes) {
+                const A* p = base + b * 2 * sh.channels + c;
+                const double d = static_cast<double>(p[0]) - mean;
+                m2 += static_cast<double>(p[sh.channels]) + static_cast<double>(piece_rows(begin, end, first + b, sh.chunk)) * d * d;
+            }
+    m2 = team_sum<TEAM>(m2, sm);
     if (live && t == 0) {
-        mean_out[item] = static_cast<A>(mean);
+        mean_out[item] = static_cast<A>(n > 0 ? mean : 0.0);
         rstd_out[item] = n > 0 ? static_cast<A>(1.0 / sqrt(m2 / n + eps)) : A(0);
     }
 }
@@ -263,7 +281,7 @@ __global__ void __launch_bounds__(kThreads) grad_sums_kernel(Shape sh, const T* 
                 m[q] = mean[s * sh.groups + cp.group[q]];
                 rs[q] = rstd[s * sh.groups + cp.group[q]];
             }
-#pragma unroll 2
+#pragma unroll 4
             for (int64_t r = row + row_lane; r < end; r += row_lanes) {
                 A v[V], g[V];
                 load_acc<T, V>(x + r * sh.channels + c, v);
@@ -320,36 +338,35 @@ __global__ void __launch_bounds__(kThreads) grad_sums_kernel(Shape sh, const T* 
 
 // mean(h) and mean(h xhat) of every (segment, group), from the per-channel sums of its pieces.
 template <typename T, int TEAM>
-__global__ void __launch_bounds__(kThreads) grad_join_kernel(Shape sh, const acc_t<T>* __restrict__ part, const T* __restrict__ w,
+__global__ void __launch_bounds__(join_threads(TEAM)) grad_join_kernel(Shape sh, const acc_t<T>* __restrict__ part, const T* __restrict__ w,
                                                              acc_t<T>* __restrict__ coef) {
-    __shared__ double sm[2][kThreads];
+    __shared__ double sm[join_threads(TEAM) / 32];
     const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM;
-    const int64_t item = blockIdx.x * int64_t(kThreads / TEAM) + team;
+    const int64_t item = blockIdx.x * int64_t(join_threads(TEAM) / TEAM) + team;
     const bool live = item < sh.segments * sh.groups;
     const int64_t s = live ? item / sh.groups : 0;
     const int g = static_cast<int>(live ? item % sh.groups : 0), width = sh.channels / sh.groups;
     const int64_t begin = segment_begin(sh, s), end = max(begin, segment_begin(sh, s + 1));
+    const int64_t first = begin / sh.chunk, last = end > begin ? (end - 1) / sh.chunk : first - 1;
+    const int64_t pieces = live ? last - first + 1 : 0;
+    const acc_t<T>* base = part + (first + s) * 2 * sh.channels + g * width;
+    const int per = width < TEAM ? width : TEAM, lanes = TEAM / per, lane = t / per;
     double a = 0, b = 0;
-    if (live && end > begin) {
-        const int64_t first = begin / sh.chunk, last = (end - 1) / sh.chunk, work = (last - first + 1) * width;
-        for (int64_t e = t; e < work; e += TEAM) {
-            const int c = g * width + static_cast<int>(e % width);
-            const acc_t<T>* p = part + (first + e / width + s) * 2 * sh.channels + c;
-            const double gamma = w ? static_cast<double>(to_acc(w[c])) : 1.0;
-            a += gamma * static_cast<double>(p[0]);
-            b += gamma * static_cast<double>(p[sh.channels]);
-        }
+    for (int c = t % per; c < width; c += per) {
+        double ca = 0, cb = 0;
+        if (lane < lanes)
+#pragma unroll 4
+            for (int64_t q = lane; q < pieces; q += lanes) {
+                const acc_t<T>* p = base + q * 2 * sh.channels + c;
+                ca += static_cast<double>(p[0]);
+                cb += static_cast<double>(p[sh.channels]);
+            }
+        const double gamma = w ? static_cast<double>(to_acc(w[g * width + c])) : 1.0;
+        a += gamma * ca;
+        b += gamma * cb;
     }
-    sm[0][threadIdx.x] = a;
-    sm[1][threadIdx.x] = b;
-    __syncthreads();
-    for (int off = TEAM / 2; off > 0; off >>= 1) {
-        if (t < off) {
-            sm[0][threadIdx.x] = a += sm[0][threadIdx.x + off];
-            sm[1][threadIdx.x] = b += sm[1][threadIdx.x + off];
-        }
-        __syncthreads();
-    }
+    a = team_sum<TEAM>(a, sm);
+    b = team_sum<TEAM>(b, sm);
     if (live && t == 0) {
         const double n = static_cast<double>(end - begin) * width;
         coef[2 * item] = static_cast<acc_t<T>>(n > 0 ? a / n : 0.0);
@@ -357,21 +374,27 @@ __global__ void __launch_bounds__(kThreads) grad_join_kernel(Shape sh, const acc
     }
 }
 
-// dbeta and dgamma: columns of block_sums [blocks][2][channels] added up; 32 columns x 8 rows of threads.
+// dbeta and dgamma: columns of sums [parts][2][channels] added up; 32 columns x 32 lanes of a block, in an order
+// that depends on the sizes alone.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) column_sums_kernel(int64_t blocks, int channels, const acc_t<T>* __restrict__ block_sums,
-                                                               T* __restrict__ dbeta, T* __restrict__ dgamma) {
-    __shared__ double sm[8][33];
-    const int col = blockIdx.x * 32 + threadIdx.x % 32, part = threadIdx.x / 32;
+__global__ void __launch_bounds__(1024) column_sums_kernel(int64_t parts, int channels, const acc_t<T>* __restrict__ sums,
+                                                           T* __restrict__ dbeta, T* __restrict__ dgamma) {
+    __shared__ double sm[32][33];
+    const int col = blockIdx.x * 32 + threadIdx.x % 32, lane = threadIdx.x / 32;
     double a = 0;
     if (col < 2 * channels)
-        for (int64_t b = part; b < blocks; b += 8) a += static_cast<double>(block_sums[b * 2 * channels + col]);
-    sm[part][threadIdx.x % 32] = a;
+#pragma unroll 8
+        for (int64_t b = lane; b < parts; b += 32) a += static_cast<double>(sums[b * 2 * channels + col]);
+    sm[lane][threadIdx.x % 32] = a;
     __syncthreads();
-    if (part == 0 && col < 2 * channels) {
-        for (int q = 1; q < 8; ++q) a += sm[q][threadIdx.x % 32];
-        T* out = col < channels ? dbeta : dgamma;
-        if (out) out[col % channels] = from_acc<T>(static_cast<acc_t<T>>(a));
+    // transposed, so that a warp adds the 32 lanes of one column
+    a = sm[threadIdx.x % 32][lane];
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) a += __shfl_xor_sync(0xFFFFFFFFu, a, off);
+    const int mine = blockIdx.x * 32 + lane;
+    if (threadIdx.x % 32 == 0 && mine < 2 * channels) {
+        T* out = mine < channels ? dbeta : dgamma;
+        if (out) out[mine % channels] = from_acc<T>(static_cast<acc_t<T>>(a));
     }
 }
 
@@ -403,8 +426,9 @@ __global__ void __launch_bounds__(kThreads) grad_apply_kernel(Shape sh, const T*
             c1[q] = coef[2 * item];
             c2[q] = coef[2 * item + 1];
         }
-#pragma unroll 2
-        for (int64_t r = row + row_lane; r < end; r += row_lanes) {
+        // backwards: what the first pass read last is still in L2
+#pragma unroll 4
+        for (int64_t r = end - 1 - row_lane; r >= row; r -= row_lanes) {
             A v[V], g[V];
             load_acc<T, V>(x + r * sh.channels + c, v);
             load_acc<T, V>(dy + r * sh.channels + c, g);
@@ -419,10 +443,309 @@ __global__ void __launch_bounds__(kThreads) grad_apply_kernel(Shape sh, const T*
     }
 }
 
+// ---- short segments: one block per (segment, slab of whole groups), one launch per direction -------------------
+// The rows of a short segment stay in L1 / L2 between the passes over them, so the block simply reads them again:
+// once for the mean, once for the squared deviations from it, once to apply (backward: sums, then apply).
+struct Slab {
+    int channels, lanes;          // channels of a slab (whole groups), vectors of its row
+    int pad_blocks;               // blocks that write the rows outside every segment
+};
+
+constexpr int kSlabGroups = 256;                    // most groups of a slab
+constexpr int kKeep = 8;                            // rows per row lane that a thread can keep in registers
+
+// Sum over the block's row lanes and over the channels of each group of the slab; entries [row lane][channel] of sm.
+// The block's warps share the groups, several to a group when there are few; out holds `parts` sums per group.
+template <typename A>
+struct GroupSums {
+    A out[kSlabGroups + kThreads / 32];
+    static __device__ __forceinline__ int parts(int groups) { return groups < kThreads / 32 ? kThreads / 32 / groups : 1; }
+    __device__ __forceinline__ void form(const A* sm, int rows, int channels, int width) {
+        const int groups = channels / width, p = parts(groups), lane = threadIdx.x % 32;
+        const int per = width < 32 ? width : 32, lanes = 32 / per, row = lane / per, column = lane % per;
+        for (int item = threadIdx.x / 32; item < groups * p; item += kThreads / 32) {
+            const int g = item / p;
+            A v = 0;
+            if (row < lanes)
+                for (int r = item % p * lanes + row; r < rows; r += p * lanes)
+                    for (int c = column; c < width; c += per) v += sm[r * channels + g * width + c];
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, off);
+            if (lane == 0) out[item] = v;
+        }
+    }
+    __device__ __forceinline__ A total(int g, int groups) const {
+        const int p = parts(groups);
+        A v = out[g * p];
+        for (int q = 1; q < p; ++q) v += out[g * p + q];
+        return v;
+    }
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void zero_outside(const Shape& sh, int64_t first, int64_t blocks, T* out) {
+    const acc_t<T> zero[V] = {};
+    const int64_t before = segment_begin(sh, 0), behind = max(before, segment_begin(sh, sh.segments));
+    const int64_t vectors = sh.channels / V, count = (before + sh.rows - behind) * vectors;
+    for (int64_t e = first * kThreads + threadIdx.x; e < count; e += blocks * kThreads) {
+        const int64_t r = e / vectors;
+        store_acc<T, V>(out + (r < before ? r : r - before + behind) * sh.channels + e % vectors * V, zero);
+    }
+}
+
+// The rows of this thread: kept in registers when a row lane has at most kKeep of them, read again otherwise.
+template <typename T, int V, int N>
+struct Rows {
+    Pack<T, V> kept[N][kKeep];
+    const T* base[N];
+    int64_t rows, step;
+    int first, stride;
+    bool keep;
+    __device__ __forceinline__ void load() {
+        keep = rows <= int64_t(kKeep) * stride;
+        if (keep)
+#pragma unroll
+            for (int e = 0; e < kKeep; ++e)
+                if (first + e * stride < rows)
+#pragma unroll
+                    for (int a = 0; a < N; ++a) kept[a][e] = *reinterpret_cast<const Pack<T, V>*>(base[a] + e * step);
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F&& f) const {
+        if (keep) {
+#pragma unroll
+            for (int e = 0; e < kKeep; ++e)
+                if (first + e * stride < rows) {
+                    acc_t<T> v[N][V];
+#pragma unroll
+                    for (int a = 0; a < N; ++a)
+#pragma unroll
+                        for (int q = 0; q < V; ++q) v[a][q] = to_acc(kept[a][e].v[q]);
+                    f(v, e * step);
+                }
+        } else {
+            int64_t at = 0;
+#pragma unroll 2
+            for (int64_t r = first; r < rows; r += stride, at += step) {
+                acc_t<T> v[N][V];
+#pragma unroll
+                for (int a = 0; a < N; ++a) load_acc<T, V>(base[a] + at, v[a]);
+                f(v, at);
+            }
+        }
+    }
+};
+
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads) short_forward_kernel(Shape sh, Slab slab, const T* __restrict__ x, const T* __restrict__ w,
+                                                                 const T* __restrict__ bias, double eps, acc_t<T>* __restrict__ mean,
+                                                                 acc_t<T>* __restrict__ rstd, T* __restrict__ y) {
+    using A = acc_t<T>;
+    __shared__ A sm[kThreads * V], centre[kSlabGroups], scale[kSlabGroups];
+    __shared__ GroupSums<A> sums;
+    if (blockIdx.x >= sh.segments) {
+        if (blockIdx.y == 0) zero_outside<T, V>(sh, blockIdx.x - sh.segments, slab.pad_blocks, y);
+        return;
+    }
+    const int64_t s = blockIdx.x, begin = segment_begin(sh, s), end = max(begin, segment_begin(sh, s + 1));
+    const int width = sh.channels / sh.groups, first = blockIdx.y * slab.channels, mine = slab.channels;
+    const int groups = mine / width, g0 = first / width;
+    if (end == begin) {
+        for (int g = threadIdx.x; g < groups; g += kThreads) mean[s * sh.groups + g0 + g] = rstd[s * sh.groups + g0 + g] = A(0);
+        return;
+    }
+    const int lane = threadIdx.x % slab.lanes, row_lane = threadIdx.x / slab.lanes, row_lanes = kThreads / slab.lanes;
+    const int c = lane * V;                                            // inside the slab
+    const bool live = row_lane < row_lanes;
+    const int used = static_cast<int>(min(int64_t(row_lanes), end - begin));       // row lanes that have a row
+    const int64_t at = (begin + row_lane) * sh.channels + first + c;
+    Rows<T, V, 1> rows;
+    rows.base[0] = x + at;
+    rows.rows = live ? end - begin : 0;
+    rows.step = int64_t(row_lanes) * sh.channels;
+    rows.first = row_lane;
+    rows.stride = row_lanes;
+    rows.load();
+    int group[V];
+    A shift[V], sum[V] = {};
+#pragma unroll
+    for (int q = 0; q < V; ++q) {
+        group[q] = (c + q) / width < groups ? (c + q) / width : 0;
+        shift[q] = to_acc(x[begin * sh.channels + first + group[q] * width]);      // the group's first value
+    }
+    rows.each([&](const A (&v)[1][V], int64_t) {
+#pragma unroll
+        for (int q = 0; q < V; ++q) sum[q] += v[0][q] - shift[q];
+    });
+    if (live)
+#pragma unroll
+        for (int q = 0; q < V; ++q) sm[row_lane * mine + c + q] = sum[q];
+    __syncthreads();
+    sums.form(sm, used, mine, width);
+    __syncthreads();
+    const A n = static_cast<A>(end - begin) * width;
+    A m[V];
+#pragma unroll
+    for (int q = 0; q < V; ++q) {
+        m[q] = shift[q] + sums.total(group[q], groups) / n;
+        sum[q] = 0;
+    }
+    rows.each([&](const A (&v)[1][V], int64_t) {
+#pragma unroll
+        for (int q = 0; q < V; ++q) sum[q] += (v[0][q] - m[q]) * (v[0][q] - m[q]);
+    });
+    if (live)
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+            sm[row_lane * mine + c + q] = sum[q];
+            if (row_lane == 0 && (c + q) % width == 0) centre[group[q]] = m[q];
+        }
+    __syncthreads();
+    sums.form(sm, used, mine, width);
+    __syncthreads();
+    for (int g = threadIdx.x; g < groups; g += kThreads) {
+        scale[g] = static_cast<A>(1.0 / sqrt(static_cast<double>(sums.total(g, groups)) / static_cast<double>(n) + eps));
+        mean[s * sh.groups + g0 + g] = centre[g];
+        rstd[s * sh.groups + g0 + g] = scale[g];
+    }
+    __syncthreads();
+    A a[V], b[V];
+    if (live)
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+            a[q] = scale[group[q]] * (w ? to_acc(w[first + c + q]) : A(1));
+            b[q] = bias ? to_acc(bias[first + c + q]) : A(0);
+        }
+    rows.each([&](const A (&v)[1][V], int64_t offset) {
+        A out[V];
+#pragma unroll
+        for (int q = 0; q < V; ++q) out[q] = activate<ACT>((v[0][q] - m[q]) * a[q] + b[q]);
+        store_acc<T, V>(y + at + offset, out);
+    });
+}
+
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads) short_backward_kernel(Shape sh, Slab slab, const T* __restrict__ x, const T* __restrict__ dy,
+                                                                  const T* __restrict__ w, const T* __restrict__ bias,
+                                                                  const acc_t<T>* __restrict__ mean, const acc_t<T>* __restrict__ rstd,
+                                                                  acc_t<T>* __restrict__ channel_sums, T* __restrict__ dx) {
+    using A = acc_t<T>;
+    __shared__ A sm[2][kThreads * V];
+    __shared__ GroupSums<A> sums[2];
+    if (blockIdx.x >= sh.segments) {
+        if (dx && blockIdx.y == 0) zero_outside<T, V>(sh, blockIdx.x - sh.segments, slab.pad_blocks, dx);
+        return;
+    }
+    const int64_t s = blockIdx.x, begin = segment_begin(sh, s), end = max(begin, segment_begin(sh, s + 1));
+    const int width = sh.channels / sh.groups, first = blockIdx.y * slab.channels, mine = slab.channels, groups = mine / width;
+    const int lane = threadIdx.x % slab.lanes, row_lane = threadIdx.x / slab.lanes, row_lanes = kThreads / slab.lanes;
+    const int c = lane * V;
+    const bool live = row_lane < row_lanes;
+    const int used = static_cast<int>(min(int64_t(row_lanes), end - begin));
+    const int64_t at = (begin + row_lane) * sh.channels + first + c;
+    Rows<T, V, 2> rows;
+    rows.base[0] = x + at;
+    rows.base[1] = dy + at;
+    rows.rows = live ? end - begin : 0;
+    rows.step = int64_t(row_lanes) * sh.channels;
+    rows.first = row_lane;
+    rows.stride = row_lanes;
+    rows.load();
+    A gamma[V], beta[V], m[V], rs[V];
+    int group[V];
+#pragma unroll
+    for (int q = 0; q < V; ++q) {
+        group[q] = (c + q) / width < groups ? (c + q) / width : 0;
+        gamma[q] = w ? to_acc(w[first + c + q]) : A(1);
+        beta[q] = bias ? to_acc(bias[first + c + q]) : A(0);
+        m[q] = mean[s * sh.groups + first / width + group[q]];
+        rs[q] = rstd[s * sh.groups + first / width + group[q]];
+    }
+    A s1[V] = {}, s2[V] = {};
+    rows.each([&](const A (&v)[2][V], int64_t) {
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+            const A xhat = (v[0][q] - m[q]) * rs[q];
+            const A dz = v[1][q] * activate_slope<ACT>(xhat * gamma[q] + beta[q]);
+            s1[q] += dz;
+            s2[q] += dz * xhat;
+        }
+    });
+    if (live)
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+            sm[0][row_lane * mine + c + q] = s1[q];
+            sm[1][row_lane * mine + c + q] = s2[q];
+        }
+    __syncthreads();
+    // sums over the row lanes: per channel for dgamma and dbeta, then weighted per group for dx
+    for (int e = threadIdx.x; e < 2 * mine; e += kThreads) {
+        const int part = e >= mine, ch = e - part * mine;
+        A v = 0;
+#pragma unroll 8
+        for (int r = 0; r < used; ++r) v += sm[part][r * mine + ch];
+        channel_sums[s * 2 * sh.channels + part * sh.channels + first + ch] = v;
+        sm[part][ch] = v * (w ? to_acc(w[first + ch]) : A(1));          // row 0 of this channel has been added up
+    }
+    if (!dx) return;
+    __syncthreads();
+    sums[0].form(sm[0], 1, mine, width);
+    sums[1].form(sm[1], 1, mine, width);
+    __syncthreads();
+    A c1[V], c2[V];
+    const A n = static_cast<A>(end - begin) * width;
+#pragma unroll
+    for (int q = 0; q < V; ++q) {
+        c1[q] = sums[0].total(group[q], groups) / n;
+        c2[q] = sums[1].total(group[q], groups) / n;
+    }
+    rows.each([&](const A (&v)[2][V], int64_t offset) {
+        A out[V];
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+            const A xhat = (v[0][q] - m[q]) * rs[q];
+            const A h = v[1][q] * activate_slope<ACT>(xhat * gamma[q] + beta[q]) * gamma[q];
+            out[q] = rs[q] * (h - c1[q] - xhat * c2[q]);
+        }
+        store_acc<T, V>(dx + at + offset, out);
+    });
+}
+
 // ---- host side ------------------------------------------------------------------------------------------
 int64_t block_count(int64_t rows) {
     const int64_t wanted = ceil_div(rows, 32);
     return wanted < kSMs * 8 ? (wanted < 1 ? 1 : wanted) : kSMs * 8;
+}
+
+// Whether the one-block-per-segment kernels run, and with which slabs of channels.  They need segments that stay in
+// a block's L1 on average (a slab of one up to 128 KB) and an array in which even one segment that has all rows is
+// read by a single block in about 0.1 ms (slabs up to 8 MB); beyond that the row chunks, which are balanced however
+// long a segment is, take over.  Slabs are made narrower (whole groups) until there are two blocks for every SM, down
+// to rows of 32 bytes, or until they are light enough, down to 64.  Measured on 512 graphs of 120 rows x 128 bfloat16 channels: see the figures at the end.
+bool short_segments(int64_t rows, int64_t channels, int64_t groups, int64_t segments, size_t size, int V, Slab* slab) {
+    if (segments < 1 || segments > 65535 * 16) return false;
+    const int64_t width = channels / groups;
+    auto divisor = [&](int64_t most) {                                 // the largest divisor of groups up to it whose rows are whole vectors
+        for (int64_t d = most; d >= 1; --d)
+            if (groups % d == 0 && d * width % V == 0) return d;
+        return int64_t(0);
+    };
+    const int64_t room = kThreads * V / width < kSlabGroups ? kThreads * V / width : kSlabGroups;
+    int64_t in_slab = divisor(groups < room ? groups : room);
+    if (in_slab == 0) return false;
+    for (;;) {
+        const int64_t d = divisor(in_slab - 1), d_line = d * width * int64_t(size);
+        const bool few = segments * (groups / in_slab) < 2 * kSMs && d_line >= 32;
+        const bool heavy = rows * in_slab * width * int64_t(size) > 8 * 1024 * 1024 && d_line >= 64;
+        if (d == 0 || !(few || heavy)) break;
+        in_slab = d;
+    }
+    const int64_t line = in_slab * width * int64_t(size);
+    if (rows / segments * line > 128 * 1024 || rows * line > 8 * 1024 * 1024) return false;
+    if (groups / in_slab > 65535) return false;
+    slab->channels = static_cast<int>(in_slab * width);
+    slab->lanes = static_cast<int>(in_slab * width / V);
+    return true;
 }
 
 // Partial results of the pieces, of the blocks, and the two coefficients per (segment, group).
@@ -457,13 +780,20 @@ template <typename T, int V>
 int forward(const Launch& l, const T* x, const T* w, const T* b, double eps, int act, T* y, acc_t<T>* mean, acc_t<T>* rstd,
             acc_t<T>* part, cudaStream_t stream) {
     using A = acc_t<T>;
+    Slab slab;
+    if (short_segments(l.sh.rows, l.sh.channels, l.sh.groups, l.sh.segments, sizeof(T), V, &slab)) {
+        slab.pad_blocks = l.sh.ptr ? kSMs / 4 : 0;
+        const dim3 grid(static_cast<unsigned>(l.sh.segments + slab.pad_blocks), static_cast<unsigned>(l.sh.channels / slab.channels));
+        return NB200_DISPATCH_ACT(act, (short_forward_kernel<T, V, ACT><<<grid, kThreads, 0, stream>>>(l.sh, slab, x, w, b, eps, mean, rstd, y),
+                                        launch_status()));
+    }
     stats_kernel<T, V><<<l.grid, kThreads, 0, stream>>>(l.sh, x, part);
     const int64_t items = l.sh.segments * l.sh.groups;
     if (items > 0) {
         if (items > kSMs * 8)
             stats_join_kernel<A, 32><<<static_cast<unsigned>(ceil_div(items, kThreads / 32)), kThreads, 0, stream>>>(l.sh, part, eps, mean, rstd);
         else
-            stats_join_kernel<A, kThreads><<<static_cast<unsigned>(items), kThreads, 0, stream>>>(l.sh, part, eps, mean, rstd);
+            stats_join_kernel<A, 1024><<<static_cast<unsigned>(items), 1024, 0, stream>>>(l.sh, part, eps, mean, rstd);
     }
     return NB200_DISPATCH_ACT(act, (apply_kernel<T, V, ACT><<<l.grid, kThreads, 0, stream>>>(l.sh, x, w, b, mean, rstd, y), launch_status()));
 }
@@ -472,13 +802,24 @@ template <typename T, int V>
 int backward(const Launch& l, const T* dy, const T* x, const T* w, const T* b, const acc_t<T>* mean, const acc_t<T>* rstd, int act,
              T* dx, T* dw, T* db, acc_t<T>* part, cudaStream_t stream) {
     using A = acc_t<T>;
+    Slab slab;
+    if (short_segments(l.sh.rows, l.sh.channels, l.sh.groups, l.sh.segments, sizeof(T), V, &slab)) {
+        slab.pad_blocks = l.sh.ptr && dx ? kSMs / 4 : 0;
+        const dim3 grid(static_cast<unsigned>(l.sh.segments + slab.pad_blocks), static_cast<unsigned>(l.sh.channels / slab.channels));
+        const int rc = NB200_DISPATCH_ACT(act, (short_backward_kernel<T, V, ACT><<<grid, kThreads, 0, stream>>>(
+                                                    l.sh, slab, x, dy, w, b, mean, rstd, part, dx), launch_status()));
+        if (rc != NB200_OK || !(dw || db)) return rc;
+        column_sums_kernel<T><<<static_cast<unsigned>(ceil_div(2 * l.sh.channels, 32)), 1024, 0, stream>>>(l.sh.segments, l.sh.channels, part,
+                                                                                                         db, dw);
+        return launch_status();
+    }
     A* block_sums = part + part_elements(l.sh.rows, l.sh.channels, l.sh.segments);
     A* coef = block_sums + size_t(block_count(l.sh.rows)) * 2 * l.sh.channels;
     int rc = NB200_DISPATCH_ACT(act, (grad_sums_kernel<T, V, ACT><<<l.grid, kThreads, 0, stream>>>(l.sh, x, dy, w, b, mean, rstd, part,
                                                                                                  block_sums), launch_status()));
     if (rc != NB200_OK) return rc;
     if (dw || db)
-        column_sums_kernel<T><<<static_cast<unsigned>(ceil_div(2 * l.sh.channels, 32)), kThreads, 0, stream>>>(
+        column_sums_kernel<T><<<static_cast<unsigned>(ceil_div(2 * l.sh.channels, 32)), 1024, 0, stream>>>(
             l.grid.x, l.sh.channels, block_sums, db, dw);
     if (!dx) return launch_status();
     const int64_t items = l.sh.segments * l.sh.groups;
@@ -486,7 +827,7 @@ int backward(const Launch& l, const T* dy, const T* x, const T* w, const T* b, c
         if (items > kSMs * 8)
             grad_join_kernel<T, 32><<<static_cast<unsigned>(ceil_div(items, kThreads / 32)), kThreads, 0, stream>>>(l.sh, part, w, coef);
         else
-            grad_join_kernel<T, kThreads><<<static_cast<unsigned>(items), kThreads, 0, stream>>>(l.sh, part, w, coef);
+            grad_join_kernel<T, 1024><<<static_cast<unsigned>(items), 1024, 0, stream>>>(l.sh, part, w, coef);
     }
     return NB200_DISPATCH_ACT(act, (grad_apply_kernel<T, V, ACT><<<l.grid, kThreads, 0, stream>>>(l.sh, x, dy, w, b, mean, rstd, coef, dx),
                                     launch_status()));
