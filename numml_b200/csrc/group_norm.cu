@@ -451,24 +451,24 @@ struct Slab {
     int pad_blocks;               // blocks that write the rows outside every segment
 };
 
+constexpr int kShort = 512;                         // threads of these blocks: the longest segment of a batch sets the time
 constexpr int kSlabGroups = 256;                    // most groups of a slab
-constexpr int kKeep = 8;                            // rows per row lane that a thread can keep in registers
 
-// Sum over the block's row lanes and over the channels of each group of the slab; entries [row lane][channel] of sm.
-// The block's warps share the groups, several to a group when there are few; out holds `parts` sums per group.
+// Sum over the row lanes and over the columns of each group of sm [rows][groups * width].  The block's warps share the
+// groups, several to a group when there are few; out holds `parts` sums per group.
 template <typename A>
 struct GroupSums {
-    A out[kSlabGroups + kThreads / 32];
-    static __device__ __forceinline__ int parts(int groups) { return groups < kThreads / 32 ? kThreads / 32 / groups : 1; }
-    __device__ __forceinline__ void form(const A* sm, int rows, int channels, int width) {
-        const int groups = channels / width, p = parts(groups), lane = threadIdx.x % 32;
+    A out[kSlabGroups + kShort / 32];
+    static __device__ __forceinline__ int parts(int groups) { return groups < kShort / 32 ? kShort / 32 / groups : 1; }
+    __device__ __forceinline__ void form(const A* sm, int rows, int groups, int width) {
+        const int p = parts(groups), lane = threadIdx.x % 32, line = groups * width;
         const int per = width < 32 ? width : 32, lanes = 32 / per, row = lane / per, column = lane % per;
-        for (int item = threadIdx.x / 32; item < groups * p; item += kThreads / 32) {
+        for (int item = threadIdx.x / 32; item < groups * p; item += kShort / 32) {
             const int g = item / p;
             A v = 0;
             if (row < lanes)
                 for (int r = item % p * lanes + row; r < rows; r += p * lanes)
-                    for (int c = column; c < width; c += per) v += sm[r * channels + g * width + c];
+                    for (int c = column; c < width; c += per) v += sm[r * line + g * width + c];
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, off);
             if (lane == 0) out[item] = v;
@@ -487,150 +487,113 @@ __device__ __forceinline__ void zero_outside(const Shape& sh, int64_t first, int
     const acc_t<T> zero[V] = {};
     const int64_t before = segment_begin(sh, 0), behind = max(before, segment_begin(sh, sh.segments));
     const int64_t vectors = sh.channels / V, count = (before + sh.rows - behind) * vectors;
-    for (int64_t e = first * kThreads + threadIdx.x; e < count; e += blocks * kThreads) {
+    for (int64_t e = first * kShort + threadIdx.x; e < count; e += blocks * kShort) {
         const int64_t r = e / vectors;
         store_acc<T, V>(out + (r < before ? r : r - before + behind) * sh.channels + e % vectors * V, zero);
     }
 }
 
-// The rows of this thread: kept in registers when a row lane has at most kKeep of them, read again otherwise.
-template <typename T, int V, int N>
-struct Rows {
-    Pack<T, V> kept[N][kKeep];
-    const T* base[N];
-    int64_t rows, step;
-    int first, stride;
-    bool keep;
-    __device__ __forceinline__ void load() {
-        keep = rows <= int64_t(kKeep) * stride;
-        if (keep)
-#pragma unroll
-            for (int e = 0; e < kKeep; ++e)
-                if (first + e * stride < rows)
-#pragma unroll
-                    for (int a = 0; a < N; ++a) kept[a][e] = *reinterpret_cast<const Pack<T, V>*>(base[a] + e * step);
-    }
-    template <typename F>
-    __device__ __forceinline__ void each(F&& f) const {
-        if (keep) {
-#pragma unroll
-            for (int e = 0; e < kKeep; ++e)
-                if (first + e * stride < rows) {
-                    acc_t<T> v[N][V];
-#pragma unroll
-                    for (int a = 0; a < N; ++a)
-#pragma unroll
-                        for (int q = 0; q < V; ++q) v[a][q] = to_acc(kept[a][e].v[q]);
-                    f(v, e * step);
-                }
-        } else {
-            int64_t at = 0;
-#pragma unroll 2
-            for (int64_t r = first; r < rows; r += stride, at += step) {
-                acc_t<T> v[N][V];
-#pragma unroll
-                for (int a = 0; a < N; ++a) load_acc<T, V>(base[a] + at, v[a]);
-                f(v, at);
-            }
-        }
-    }
-};
-
-template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads) short_forward_kernel(Shape sh, Slab slab, const T* __restrict__ x, const T* __restrict__ w,
-                                                                 const T* __restrict__ bias, double eps, acc_t<T>* __restrict__ mean,
-                                                                 acc_t<T>* __restrict__ rstd, T* __restrict__ y) {
+// ONE: a vector of channels belongs to one group (V divides channels / groups), so that a thread has one mean and one
+// sum instead of V.
+template <typename T, int V, int ACT, bool ONE>
+__global__ void __launch_bounds__(kShort) short_forward_kernel(Shape sh, Slab slab, const T* __restrict__ x, const T* __restrict__ w,
+                                                               const T* __restrict__ bias, double eps, acc_t<T>* __restrict__ mean,
+                                                               acc_t<T>* __restrict__ rstd, T* __restrict__ y) {
     using A = acc_t<T>;
-    __shared__ A sm[kThreads * V], centre[kSlabGroups], scale[kSlabGroups];
+    constexpr int G = ONE ? 1 : V;                                     // groups that a thread may touch
+    __shared__ A sm[kShort * G], scale[kSlabGroups];
     __shared__ GroupSums<A> sums;
     if (blockIdx.x >= sh.segments) {
         if (blockIdx.y == 0) zero_outside<T, V>(sh, blockIdx.x - sh.segments, slab.pad_blocks, y);
         return;
     }
     const int64_t s = blockIdx.x, begin = segment_begin(sh, s), end = max(begin, segment_begin(sh, s + 1));
-    const int width = sh.channels / sh.groups, first = blockIdx.y * slab.channels, mine = slab.channels;
-    const int groups = mine / width, g0 = first / width;
+    const int width = sh.channels / sh.groups, first = blockIdx.y * slab.channels;
+    const int groups = slab.channels / width, g0 = first / width;
     if (end == begin) {
-        for (int g = threadIdx.x; g < groups; g += kThreads) mean[s * sh.groups + g0 + g] = rstd[s * sh.groups + g0 + g] = A(0);
+        for (int g = threadIdx.x; g < groups; g += kShort) mean[s * sh.groups + g0 + g] = rstd[s * sh.groups + g0 + g] = A(0);
         return;
     }
-    const int lane = threadIdx.x % slab.lanes, row_lane = threadIdx.x / slab.lanes, row_lanes = kThreads / slab.lanes;
+    const int lane = threadIdx.x % slab.lanes, row_lane = threadIdx.x / slab.lanes, row_lanes = kShort / slab.lanes;
     const int c = lane * V;                                            // inside the slab
-    const bool live = row_lane < row_lanes;
     const int used = static_cast<int>(min(int64_t(row_lanes), end - begin));       // row lanes that have a row
+    const int64_t rows = row_lane < row_lanes ? end - begin : 0, step = int64_t(row_lanes) * sh.channels;
     const int64_t at = (begin + row_lane) * sh.channels + first + c;
-    Rows<T, V, 1> rows;
-    rows.base[0] = x + at;
-    rows.rows = live ? end - begin : 0;
-    rows.step = int64_t(row_lanes) * sh.channels;
-    rows.first = row_lane;
-    rows.stride = row_lanes;
-    rows.load();
-    int group[V];
-    A shift[V], sum[V] = {};
+    // columns of sm: one per vector (ONE) or per channel
+    const int line = ONE ? slab.lanes : slab.channels, columns = ONE ? width / V : width;
+    int group[G];
+    A m[G], sum[G] = {};
 #pragma unroll
-    for (int q = 0; q < V; ++q) {
-        group[q] = (c + q) / width < groups ? (c + q) / width : 0;
-        shift[q] = to_acc(x[begin * sh.channels + first + group[q] * width]);      // the group's first value
+    for (int q = 0; q < G; ++q) {
+        group[q] = (c + q) / width;
+        m[q] = to_acc(x[begin * sh.channels + first + group[q] * width]);          // the group's first value
     }
-    rows.each([&](const A (&v)[1][V], int64_t) {
+    auto over_rows = [&](auto&& f) {
+        const T* p = x + at;
+#pragma unroll 4
+        for (int64_t r = row_lane; r < rows; r += row_lanes, p += step) {
+            A v[V];
+            load_acc<T, V>(p, v);
+            f(v, p - x);
+        }
+    };
+    auto join = [&]() {
+        if (rows > 0)
 #pragma unroll
-        for (int q = 0; q < V; ++q) sum[q] += v[0][q] - shift[q];
-    });
-    if (live)
-#pragma unroll
-        for (int q = 0; q < V; ++q) sm[row_lane * mine + c + q] = sum[q];
-    __syncthreads();
-    sums.form(sm, used, mine, width);
-    __syncthreads();
+            for (int q = 0; q < G; ++q) sm[row_lane * line + (ONE ? lane : c + q)] = sum[q];
+        __syncthreads();
+        sums.form(sm, used, groups, columns);
+        __syncthreads();
+    };
     const A n = static_cast<A>(end - begin) * width;
-    A m[V];
+    over_rows([&](const A (&v)[V], int64_t) {
 #pragma unroll
-    for (int q = 0; q < V; ++q) {
-        m[q] = shift[q] + sums.total(group[q], groups) / n;
-        sum[q] = 0;
-    }
-    rows.each([&](const A (&v)[1][V], int64_t) {
-#pragma unroll
-        for (int q = 0; q < V; ++q) sum[q] += (v[0][q] - m[q]) * (v[0][q] - m[q]);
+        for (int q = 0; q < V; ++q) sum[ONE ? 0 : q] += v[q] - m[ONE ? 0 : q];
     });
-    if (live)
+    join();
+#pragma unroll
+    for (int q = 0; q < G; ++q) {
+        m[q] += sums.total(group[q], groups) / n;
+        sum[q] = 0;
+        if (row_lane == 0 && (c + q) % width == 0) mean[s * sh.groups + g0 + group[q]] = m[q];
+    }
+    over_rows([&](const A (&v)[V], int64_t) {
 #pragma unroll
         for (int q = 0; q < V; ++q) {
-            sm[row_lane * mine + c + q] = sum[q];
-            if (row_lane == 0 && (c + q) % width == 0) centre[group[q]] = m[q];
+            const A d = v[q] - m[ONE ? 0 : q];
+            sum[ONE ? 0 : q] += d * d;
         }
-    __syncthreads();
-    sums.form(sm, used, mine, width);
-    __syncthreads();
-    for (int g = threadIdx.x; g < groups; g += kThreads) {
+    });
+    join();
+    for (int g = threadIdx.x; g < groups; g += kShort) {
         scale[g] = static_cast<A>(1.0 / sqrt(static_cast<double>(sums.total(g, groups)) / static_cast<double>(n) + eps));
-        mean[s * sh.groups + g0 + g] = centre[g];
         rstd[s * sh.groups + g0 + g] = scale[g];
     }
     __syncthreads();
     A a[V], b[V];
-    if (live)
+    if (rows > 0)
 #pragma unroll
         for (int q = 0; q < V; ++q) {
-            a[q] = scale[group[q]] * (w ? to_acc(w[first + c + q]) : A(1));
+            a[q] = scale[group[ONE ? 0 : q]] * (w ? to_acc(w[first + c + q]) : A(1));
             b[q] = bias ? to_acc(bias[first + c + q]) : A(0);
         }
-    rows.each([&](const A (&v)[1][V], int64_t offset) {
+    over_rows([&](const A (&v)[V], int64_t offset) {
         A out[V];
 #pragma unroll
-        for (int q = 0; q < V; ++q) out[q] = activate<ACT>((v[0][q] - m[q]) * a[q] + b[q]);
-        store_acc<T, V>(y + at + offset, out);
+        for (int q = 0; q < V; ++q) out[q] = activate<ACT>((v[q] - m[ONE ? 0 : q]) * a[q] + b[q]);
+        store_acc<T, V>(y + offset, out);
     });
 }
 
-template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads) short_backward_kernel(Shape sh, Slab slab, const T* __restrict__ x, const T* __restrict__ dy,
-                                                                  const T* __restrict__ w, const T* __restrict__ bias,
-                                                                  const acc_t<T>* __restrict__ mean, const acc_t<T>* __restrict__ rstd,
-                                                                  acc_t<T>* __restrict__ channel_sums, T* __restrict__ dx) {
+template <typename T, int V, int ACT, bool ONE>
+__global__ void __launch_bounds__(kShort) short_backward_kernel(Shape sh, Slab slab, const T* __restrict__ x, const T* __restrict__ dy,
+                                                                const T* __restrict__ w, const T* __restrict__ bias,
+                                                                const acc_t<T>* __restrict__ mean, const acc_t<T>* __restrict__ rstd,
+                                                                acc_t<T>* __restrict__ channel_sums, T* __restrict__ dx) {
     using A = acc_t<T>;
-    __shared__ A sm[2][kThreads * V];
+    constexpr int G = ONE ? 1 : V;
+    __shared__ A sm[kShort * V];
+    __shared__ A weighted[2][kThreads * V];                            // a slab has at most kThreads vectors
     __shared__ GroupSums<A> sums[2];
     if (blockIdx.x >= sh.segments) {
         if (dx && blockIdx.y == 0) zero_outside<T, V>(sh, blockIdx.x - sh.segments, slab.pad_blocks, dx);
@@ -638,77 +601,83 @@ __global__ void __launch_bounds__(kThreads) short_backward_kernel(Shape sh, Slab
     }
     const int64_t s = blockIdx.x, begin = segment_begin(sh, s), end = max(begin, segment_begin(sh, s + 1));
     const int width = sh.channels / sh.groups, first = blockIdx.y * slab.channels, mine = slab.channels, groups = mine / width;
-    const int lane = threadIdx.x % slab.lanes, row_lane = threadIdx.x / slab.lanes, row_lanes = kThreads / slab.lanes;
+    const int lane = threadIdx.x % slab.lanes, row_lane = threadIdx.x / slab.lanes, row_lanes = kShort / slab.lanes;
     const int c = lane * V;
-    const bool live = row_lane < row_lanes;
     const int used = static_cast<int>(min(int64_t(row_lanes), end - begin));
+    const int64_t rows = row_lane < row_lanes ? end - begin : 0, step = int64_t(row_lanes) * sh.channels;
     const int64_t at = (begin + row_lane) * sh.channels + first + c;
-    Rows<T, V, 2> rows;
-    rows.base[0] = x + at;
-    rows.base[1] = dy + at;
-    rows.rows = live ? end - begin : 0;
-    rows.step = int64_t(row_lanes) * sh.channels;
-    rows.first = row_lane;
-    rows.stride = row_lanes;
-    rows.load();
-    A gamma[V], beta[V], m[V], rs[V];
-    int group[V];
+    A gamma[V], beta[V], m[G], rs[G];
+    int group[G];
 #pragma unroll
     for (int q = 0; q < V; ++q) {
-        group[q] = (c + q) / width < groups ? (c + q) / width : 0;
         gamma[q] = w ? to_acc(w[first + c + q]) : A(1);
         beta[q] = bias ? to_acc(bias[first + c + q]) : A(0);
+    }
+#pragma unroll
+    for (int q = 0; q < G; ++q) {
+        group[q] = (c + q) / width;
         m[q] = mean[s * sh.groups + first / width + group[q]];
         rs[q] = rstd[s * sh.groups + first / width + group[q]];
     }
     A s1[V] = {}, s2[V] = {};
-    rows.each([&](const A (&v)[2][V], int64_t) {
+    {
+        const T *px = x + at, *pg = dy + at;
+#pragma unroll 2
+        for (int64_t r = row_lane; r < rows; r += row_lanes, px += step, pg += step) {
+            A v[V], g[V];
+            load_acc<T, V>(px, v);
+            load_acc<T, V>(pg, g);
 #pragma unroll
-        for (int q = 0; q < V; ++q) {
-            const A xhat = (v[0][q] - m[q]) * rs[q];
-            const A dz = v[1][q] * activate_slope<ACT>(xhat * gamma[q] + beta[q]);
-            s1[q] += dz;
-            s2[q] += dz * xhat;
+            for (int q = 0; q < V; ++q) {
+                const A xhat = (v[q] - m[ONE ? 0 : q]) * rs[ONE ? 0 : q];
+                const A dz = g[q] * activate_slope<ACT>(xhat * gamma[q] + beta[q]);
+                s1[q] += dz;
+                s2[q] += dz * xhat;
+            }
         }
-    });
-    if (live)
+    }
+    // sums over the row lanes: per channel for dbeta and dgamma, weighted with gamma per group for dx
 #pragma unroll
-        for (int q = 0; q < V; ++q) {
-            sm[0][row_lane * mine + c + q] = s1[q];
-            sm[1][row_lane * mine + c + q] = s2[q];
-        }
-    __syncthreads();
-    // sums over the row lanes: per channel for dgamma and dbeta, then weighted per group for dx
-    for (int e = threadIdx.x; e < 2 * mine; e += kThreads) {
-        const int part = e >= mine, ch = e - part * mine;
-        A v = 0;
+    for (int part = 0; part < 2; ++part) {
+        if (row_lane < row_lanes)
+#pragma unroll
+            for (int q = 0; q < V; ++q) sm[row_lane * mine + c + q] = part == 0 ? s1[q] : s2[q];
+        __syncthreads();
+        for (int ch = threadIdx.x; ch < mine; ch += kShort) {
+            A v = 0;
 #pragma unroll 8
-        for (int r = 0; r < used; ++r) v += sm[part][r * mine + ch];
-        channel_sums[s * 2 * sh.channels + part * sh.channels + first + ch] = v;
-        sm[part][ch] = v * (w ? to_acc(w[first + ch]) : A(1));          // row 0 of this channel has been added up
+            for (int r = 0; r < used; ++r) v += sm[r * mine + ch];
+            channel_sums[s * 2 * sh.channels + part * sh.channels + first + ch] = v;
+            weighted[part][ch] = v * (w ? to_acc(w[first + ch]) : A(1));
+        }
+        __syncthreads();
     }
     if (!dx) return;
+    sums[0].form(weighted[0], 1, groups, width);
+    sums[1].form(weighted[1], 1, groups, width);
     __syncthreads();
-    sums[0].form(sm[0], 1, mine, width);
-    sums[1].form(sm[1], 1, mine, width);
-    __syncthreads();
-    A c1[V], c2[V];
+    A c1[G], c2[G];
     const A n = static_cast<A>(end - begin) * width;
 #pragma unroll
-    for (int q = 0; q < V; ++q) {
+    for (int q = 0; q < G; ++q) {
         c1[q] = sums[0].total(group[q], groups) / n;
         c2[q] = sums[1].total(group[q], groups) / n;
     }
-    rows.each([&](const A (&v)[2][V], int64_t offset) {
-        A out[V];
+    const T *px = x + at, *pg = dy + at;
+    T* out = dx + at;
+#pragma unroll 2
+    for (int64_t r = row_lane; r < rows; r += row_lanes, px += step, pg += step, out += step) {
+        A v[V], g[V];
+        load_acc<T, V>(px, v);
+        load_acc<T, V>(pg, g);
 #pragma unroll
         for (int q = 0; q < V; ++q) {
-            const A xhat = (v[0][q] - m[q]) * rs[q];
-            const A h = v[1][q] * activate_slope<ACT>(xhat * gamma[q] + beta[q]) * gamma[q];
-            out[q] = rs[q] * (h - c1[q] - xhat * c2[q]);
+            const A xhat = (v[q] - m[ONE ? 0 : q]) * rs[ONE ? 0 : q];
+            const A h = g[q] * activate_slope<ACT>(xhat * gamma[q] + beta[q]) * gamma[q];
+            v[q] = rs[ONE ? 0 : q] * (h - c1[ONE ? 0 : q] - xhat * c2[ONE ? 0 : q]);
         }
-        store_acc<T, V>(dx + at + offset, out);
-    });
+        store_acc<T, V>(out, v);
+    }
 }
 
 // ---- host side ------------------------------------------------------------------------------------------
@@ -784,8 +753,11 @@ int forward(const Launch& l, const T* x, const T* w, const T* b, double eps, int
     if (short_segments(l.sh.rows, l.sh.channels, l.sh.groups, l.sh.segments, sizeof(T), V, &slab)) {
         slab.pad_blocks = l.sh.ptr ? kSMs / 4 : 0;
         const dim3 grid(static_cast<unsigned>(l.sh.segments + slab.pad_blocks), static_cast<unsigned>(l.sh.channels / slab.channels));
-        return NB200_DISPATCH_ACT(act, (short_forward_kernel<T, V, ACT><<<grid, kThreads, 0, stream>>>(l.sh, slab, x, w, b, eps, mean, rstd, y),
-                                        launch_status()));
+        if (l.sh.channels / l.sh.groups % V == 0)
+            return NB200_DISPATCH_ACT(act, (short_forward_kernel<T, V, ACT, true><<<grid, kShort, 0, stream>>>(l.sh, slab, x, w, b, eps, mean,
+                                                                                                            rstd, y), launch_status()));
+        return NB200_DISPATCH_ACT(act, (short_forward_kernel<T, V, ACT, false><<<grid, kShort, 0, stream>>>(l.sh, slab, x, w, b, eps, mean,
+                                                                                                         rstd, y), launch_status()));
     }
     stats_kernel<T, V><<<l.grid, kThreads, 0, stream>>>(l.sh, x, part);
     const int64_t items = l.sh.segments * l.sh.groups;
@@ -806,8 +778,11 @@ int backward(const Launch& l, const T* dy, const T* x, const T* w, const T* b, c
     if (short_segments(l.sh.rows, l.sh.channels, l.sh.groups, l.sh.segments, sizeof(T), V, &slab)) {
         slab.pad_blocks = l.sh.ptr && dx ? kSMs / 4 : 0;
         const dim3 grid(static_cast<unsigned>(l.sh.segments + slab.pad_blocks), static_cast<unsigned>(l.sh.channels / slab.channels));
-        const int rc = NB200_DISPATCH_ACT(act, (short_backward_kernel<T, V, ACT><<<grid, kThreads, 0, stream>>>(
-                                                    l.sh, slab, x, dy, w, b, mean, rstd, part, dx), launch_status()));
+        const int rc = l.sh.channels / l.sh.groups % V == 0
+                           ? NB200_DISPATCH_ACT(act, (short_backward_kernel<T, V, ACT, true><<<grid, kShort, 0, stream>>>(
+                                                          l.sh, slab, x, dy, w, b, mean, rstd, part, dx), launch_status()))
+                           : NB200_DISPATCH_ACT(act, (short_backward_kernel<T, V, ACT, false><<<grid, kShort, 0, stream>>>(
+                                                          l.sh, slab, x, dy, w, b, mean, rstd, part, dx), launch_status()));
         if (rc != NB200_OK || !(dw || db)) return rc;
         column_sums_kernel<T><<<static_cast<unsigned>(ceil_div(2 * l.sh.channels, 32)), 1024, 0, stream>>>(l.sh.segments, l.sh.channels, part,
                                                                                                          db, dw);
