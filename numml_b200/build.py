@@ -73,7 +73,7 @@ def build(force=False, verbose=False, ptxas_info=False):
     return LIB_PATH
 
 
-EXT_SRC = os.path.join(PKG, "csrc_ext", "ops_ext.cpp")
+EXT_DIR = os.path.join(PKG, "csrc_ext")
 EXT_NAME = "numml_b200_ext"
 
 
@@ -83,28 +83,33 @@ def extension_path():
 
 
 def build_extension(force=False, verbose=False):
-    """Compile the torch extension with the per-call path of the SpMV / SpMM operators
-    (``csrc_ext/ops_ext.cpp``) against the installed torch and link it to ``libnumml_b200.so`` (found at
-    run time next to itself).  Returns its path."""
+    """Compile the torch extension with the per-call path of the SpMV / SpMM operators and of the dense
+    operators (``csrc_ext/*.cpp``, one compiler run per file, side by side) against the installed torch and
+    link it to ``libnumml_b200.so`` (found at run time next to itself).  Returns its path."""
     import sysconfig
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
     build()
     out = extension_path()
-    newest = max(os.path.getmtime(EXT_SRC), os.path.getmtime(HEADER))
+    sources = sorted(glob.glob(os.path.join(EXT_DIR, "*.cpp")))
+    newest = max(os.path.getmtime(f) for f in sources + glob.glob(os.path.join(EXT_DIR, "*.h")) + [HEADER])
     if os.path.exists(out) and not force and os.path.getmtime(out) >= newest:
         return out
     cuda_home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     incs = ["-I" + p for p in include_paths()] + ["-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(cuda_home, "include")]
     libdirs = library_paths()
-    cmd = (["g++", "-std=c++17", "-O2", "-fPIC", "-w", "-shared", "-DNDEBUG", "-DTORCH_EXTENSION_NAME=" + EXT_NAME,
-            "-DTORCH_API_INCLUDE_EXTENSION_H", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
-           + incs + [EXT_SRC, "-o", out] + ["-L" + d for d in libdirs] + ["-Wl,-rpath," + d for d in libdirs]
-           + ["-L" + LIB_DIR, "-Wl,-rpath,$ORIGIN", "-lnumml_b200", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda",
-              "-ltorch", "-ltorch_python"])
+    flags = ["-std=c++17", "-O2", "-fPIC", "-w", "-DNDEBUG", "-DTORCH_EXTENSION_NAME=" + EXT_NAME, "-DTORCH_API_INCLUDE_EXTENSION_H",
+             "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
+    objects = [os.path.join(OBJ_DIR, os.path.basename(f) + ".o") for f in sources]
+    commands = [["g++"] + flags + incs + ["-c", f, "-o", o] for f, o in zip(sources, objects)]
+    link = (["g++", "-shared"] + objects + ["-o", out] + ["-L" + d for d in libdirs] + ["-Wl,-rpath," + d for d in libdirs]
+            + ["-L" + LIB_DIR, "-Wl,-rpath,$ORIGIN", "-lnumml_b200", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda",
+               "-ltorch", "-ltorch_python"])
     if verbose:
-        print(" ".join(cmd), flush=True)
-    subprocess.check_call(cmd)
+        print("\n".join(" ".join(c) for c in commands + [link]), flush=True)
+    with ThreadPoolExecutor(max_workers=len(commands)) as ex:
+        list(ex.map(subprocess.check_call, commands))
+    subprocess.check_call(link)
     return out
 
 

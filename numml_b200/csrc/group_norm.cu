@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(kShort) short_forward_kernel(Shape sh, Slab sl
     }
     auto over_rows = [&](auto&& f) {
         const T* p = x + at;
-#pragma unroll 4
+#pragma unroll 1
         for (int64_t r = row_lane; r < rows; r += row_lanes, p += step) {
             A v[V];
             load_acc<T, V>(p, v);
@@ -622,7 +622,7 @@ __global__ void __launch_bounds__(kShort) short_backward_kernel(Shape sh, Slab s
     A s1[V] = {}, s2[V] = {};
     {
         const T *px = x + at, *pg = dy + at;
-#pragma unroll 2
+#pragma unroll 1
         for (int64_t r = row_lane; r < rows; r += row_lanes, px += step, pg += step) {
             A v[V], g[V];
             load_acc<T, V>(px, v);
@@ -665,7 +665,7 @@ __global__ void __launch_bounds__(kShort) short_backward_kernel(Shape sh, Slab s
     }
     const T *px = x + at, *pg = dy + at;
     T* out = dx + at;
-#pragma unroll 2
+#pragma unroll 1
     for (int64_t r = row_lane; r < rows; r += row_lanes, px += step, pg += step, out += step) {
         A v[V], g[V];
         load_acc<T, V>(px, v);

@@ -5,6 +5,8 @@
 // This file holds the entry points, the products that run on the CUDA cores (double, for which the tensor
 // cores of this GPU are no faster, and empty sums) and the passes around the products; linear_mma_kernel.cuh holds
 // the products on the tensor cores.
+#include <cooperative_groups.h>
+
 #include <type_traits>
 
 #include "linear_mma.cuh"
@@ -72,6 +74,103 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(int64_t rows, int64_t co
             ep.y[i * cols + j] = from_acc<T>(v);
         }
     }
+}
+
+// Few rows (the features of a node or two): the call is the reading of w.  A block has kSkinnyCols columns and a
+// share of the rows of w, eight columns to a thread, so that a warp reads lines of w; up to four rows of x go along.
+// The blocks that share a column of blocks are a thread-block cluster and add their parts up through distributed
+// shared memory in order of rank: one launch, no workspace, no atomics.
+constexpr int kSkinnyCols = 64, kSkinnyRows = 4, kSkinnyMost = 16;
+
+template <typename T, bool VECTOR, int ACT>
+__global__ void __launch_bounds__(kThreads) skinny_kernel(int rows, int64_t cols, int64_t depth, int64_t share, const T* __restrict__ x,
+                                                          int64_t ldx, const T* __restrict__ w, int64_t ldw, Epilogue<T> ep) {
+    using A = acc_t<T>;
+    constexpr int V = 8, kLanes = kSkinnyCols / V, kRowLanes = kThreads / kLanes, kWarps = kThreads / 32;
+    __shared__ A part[kWarps][kSkinnyRows][kSkinnyCols];
+    const unsigned rank = cooperative_groups::this_cluster().block_rank(), ranks = cooperative_groups::this_cluster().num_blocks();
+    const int lane = threadIdx.x % kLanes, row_lane = threadIdx.x / kLanes;
+    const int64_t j = blockIdx.x / ranks * int64_t(kSkinnyCols) + lane * V;
+    const int i0 = blockIdx.y * kSkinnyRows, count = min(kSkinnyRows, rows - i0);
+    const int64_t k_end = min(depth, (rank + 1) * share);
+    A acc[kSkinnyRows][V] = {};
+#pragma unroll 4
+    for (int64_t k = rank * share + row_lane; k < k_end; k += kRowLanes) {
+        A wv[V] = {};
+        if (VECTOR) {
+            constexpr int U = 16 / sizeof(T) < V ? 16 / sizeof(T) : V;
+            if (j < cols)
+#pragma unroll
+                for (int q = 0; q < V; q += U) load_acc<T, U>(w + k * ldw + j + q, *reinterpret_cast<A(*)[U]>(wv + q));
+        } else {
+#pragma unroll
+            for (int q = 0; q < V; ++q)
+                if (j + q < cols) wv[q] = to_acc(w[k * ldw + j + q]);
+        }
+#pragma unroll
+        for (int i = 0; i < kSkinnyRows; ++i) {
+            if (i >= count) break;
+            const A xv = to_acc(x[(i0 + i) * ldx + k]);
+#pragma unroll
+            for (int q = 0; q < V; ++q) acc[i][q] += xv * wv[q];
+        }
+    }
+    // row lanes of a warp, then the warps, then the blocks
+#pragma unroll
+    for (int i = 0; i < kSkinnyRows; ++i)
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+            A v = acc[i][q];
+#pragma unroll
+            for (int off = kLanes; off < 32; off <<= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, off);
+            if (threadIdx.x % 32 < kLanes) part[threadIdx.x / 32][i][lane * V + q] = v;
+        }
+    __syncthreads();
+    A* sums = &part[0][0][0];
+    for (int e = threadIdx.x; e < kSkinnyRows * kSkinnyCols; e += kThreads) {
+        A v = sums[e];
+        for (int q = 1; q < kWarps; ++q) v += sums[q * kSkinnyRows * kSkinnyCols + e];
+        sums[e] = v;
+    }
+    auto cluster = cooperative_groups::this_cluster();
+    cluster.sync();
+    for (int e = rank * kThreads + threadIdx.x; e < kSkinnyRows * kSkinnyCols; e += ranks * kThreads) {
+        const int i = i0 + e / kSkinnyCols;
+        const int64_t col = blockIdx.x / ranks * int64_t(kSkinnyCols) + e % kSkinnyCols;
+        if (i >= rows || col >= cols) continue;
+        A v = 0;
+        for (unsigned r = 0; r < ranks; ++r) v += *cluster.map_shared_rank(sums + e, r);
+        if (ep.bias) v += to_acc(ep.bias[col]);
+        if (ep.z) ep.z[i * cols + col] = rounded_z<T, ACT>(v);
+        v = activate<ACT>(v);
+        if (ep.residual) v += to_acc(ep.residual[i * ep.ldr + col]);
+        ep.y[i * cols + col] = from_acc<T>(v);
+    }
+    cluster.sync();                                  // nobody leaves while its sums are being read
+}
+
+template <typename T, int ACT>
+int skinny(int64_t rows, int64_t cols, int64_t depth, const T* x, int64_t ldx, const T* w, int64_t ldw, const Epilogue<T>& ep,
+           cudaStream_t stream) {
+    unsigned ranks = 1;                              // a share of at least 64 rows of w
+    while (ranks < 8 && depth > int64_t(ranks) * 64) ranks *= 2;
+    const int64_t blocks = ceil_div(cols, kSkinnyCols) * ranks;
+    if (blocks > INT32_MAX) return NB200_ERR_TOO_LARGE;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(ceil_div(rows, kSkinnyRows)));
+    config.blockDim = dim3(kThreads);
+    config.stream = stream;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeClusterDimension;
+    attribute[0].val.clusterDim = {ranks, 1, 1};
+    config.attrs = attribute;
+    config.numAttrs = 1;
+    const bool vector = cols % 8 == 0 && aligned16(w) && ldw * sizeof(T) % 16 == 0;
+    const cudaError_t e = vector ? cudaLaunchKernelEx(&config, skinny_kernel<T, true, ACT>, static_cast<int>(rows), cols, depth,
+                                                      ceil_div(depth, int64_t(ranks)), x, ldx, w, ldw, ep)
+                                 : cudaLaunchKernelEx(&config, skinny_kernel<T, false, ACT>, static_cast<int>(rows), cols, depth,
+                                                      ceil_div(depth, int64_t(ranks)), x, ldx, w, ldw, ep);
+    return e == cudaSuccess ? launch_status() : NB200_ERR_CUDA;
 }
 
 // Sums over the leading index of partial [parts][size]: 32 columns x 8 lanes per block, lane l adds parts l, l + 8,
@@ -271,6 +370,9 @@ extern "C" int nb200_linear_forward(int64_t m, int64_t k, int64_t n, const void*
     if ((k > 0 && (!x || !w)) || !y || ldx < k || ldw < n || (residual && ldr < n)) return NB200_ERR_BAD_ARG;
     return NB200_DISPATCH_DENSE(dtype, ([&]() -> int {
         const Epilogue<T> ep{static_cast<const T*>(bias), static_cast<const T*>(residual), ldr, static_cast<T*>(z), static_cast<T*>(y), nullptr};
+        if (m <= kSkinnyMost)
+            return NB200_DISPATCH_ACT(activation, (skinny<T, ACT>(m, n, k, static_cast<const T*>(x), ldx, static_cast<const T*>(w), ldw, ep,
+                                                                  as_stream(stream))));
         return NB200_DISPATCH_ACT(activation, (product<T, true, false, ACT>(m, n, k, whole(k), static_cast<const T*>(x), ldx,
                                                                            static_cast<const T*>(w), ldw, ep, status, as_stream(stream))));
     }()));

@@ -18,6 +18,7 @@
 #include <vector>
 
 #include "../../include/numml_b200.h"
+#include "dense_ops.h"
 
 namespace {
 
@@ -280,7 +281,8 @@ int values_state(const at::Tensor& indices, const at::Tensor& indptr) {
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-    m.doc() = "compiled per-call path of numml_b200's SpMV / SpMM operators over libnumml_b200";
+    m.doc() = "compiled per-call path of numml_b200's SpMV / SpMM operators and dense operators over libnumml_b200";
+    register_dense_ops(m);
     m.def("spgemv_forward", &spgemv_forward);
     m.def("spgemv_backward", &spgemv_backward);
     m.def("spdmm_forward", &spdmm_forward);

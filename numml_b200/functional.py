@@ -10,13 +10,17 @@ array.  Values are float32, float64, bfloat16 or float16 (one type per call); su
 activations are held in 32 bits (64 for float64) and every result is rounded once.  All tensors are on
 one CUDA device (there is no CPU path); calls run on that device's current stream.  Results do not
 depend on the run: no operator adds with atomics.
+
+Calls go through the compiled extension (``csrc_ext/dense_ops.cpp``) when it has been built; the Python
+functions below do the same work otherwise, with identical results (see
+``numml_torch_cpp.use_compiled_shim``).
 """
 import math
 
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _cabi
+from . import _cabi, numml_torch_cpp
 from .numml_torch_cpp import _on, _ptr, _require_cuda, _status_word, _stream
 
 _DTYPES = {torch.float32: _cabi.F32, torch.float64: _cabi.F64, torch.bfloat16: _cabi.BF16, torch.float16: _cabi.F16}
@@ -59,6 +63,14 @@ def _aligned(t):
     """Contiguous and on a 16-byte boundary, as the vector loads need it."""
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _shim(*operands):
+    """The compiled per-call path, or None when it has not been built; operands of it are tensors."""
+    for t in operands:
+        if t is not None and not isinstance(t, torch.Tensor):
+            raise RuntimeError(f"expected a torch.Tensor, got {type(t)}")
+    return numml_torch_cpp.compiled_shim()
 
 
 def _wants_grad(*tensors):
@@ -129,6 +141,9 @@ def linear(X, weights, bias=None, activation=None, residual=None):
     activation: None / 'none', 'relu', 'silu', 'gelu' (the erf form) or 'tanh'.  X, weights and residual
     may be 2-D views with any row stride.  float32 products are as exact as float32 multiply-adds."""
     act = _activation_code(activation)
+    ext = _shim(X, weights, bias, residual)
+    if ext is not None:
+        return ext.linear(X, weights, bias, residual, act)
     _check_operands(X, weights=weights, bias=bias, residual=residual)
     if X.ndim < 2:
         raise RuntimeError(f"expected node features [..., channels] with at least 2 dimensions, got {X.ndim}")
@@ -218,6 +233,9 @@ def group_norm(X, groups, weight=None, bias=None, eps=1e-5, activation=None, ptr
     which graph g has rows ``ptr[g]:ptr[g+1]``; graphs may be empty, and rows outside every graph give zeros
     and receive no gradient.  weight and bias: [channels] or None."""
     act = _activation_code(activation)
+    ext = _shim(X, weight, bias, ptr)
+    if ext is not None:
+        return ext.group_norm(X, int(groups), weight, bias, float(eps), act, ptr)
     _check_operands(X, weight=weight, bias=bias)
     if X.ndim < 2 or X.shape[-1] < 1:
         raise RuntimeError(f"expected features [..., channels] with at least 2 dimensions and one channel, got {tuple(X.shape)}")
@@ -285,23 +303,26 @@ def dropout(X, p, seed, offset=0, residual=None):
             raise RuntimeError("the dropout of a sparse tensor takes no residual")
         from .sparse import SparseCSRTensor
         return SparseCSRTensor((dropout(X.data, p, seed, offset), X.indices, X.indptr), X.shape, clone=False)
-    _check_operands(X, residual=residual)
-    p = float(p)
-    if not 0.0 <= p <= 1.0:
-        raise RuntimeError(f"dropout probability must be in [0, 1], got {p}")
-    if residual is not None and residual.shape != X.shape:
-        raise RuntimeError(f"residual must have the shape {tuple(X.shape)}, got {tuple(residual.shape)}")
-    state = None
+    p, state = float(p), None
     if isinstance(seed, torch.Tensor):
-        _require_cuda(X, seed)
-        if seed.dtype != torch.int64 or tuple(seed.shape) != (2,) or not seed.is_contiguous():
-            raise RuntimeError(f"a seed tensor must hold two int64 words [seed, offset], got {seed.dtype} {tuple(seed.shape)}")
         if offset != 0:
             raise RuntimeError("with a seed tensor the offset is its second word; leave the offset argument at 0")
         state, seed = seed, 0
     seed, offset = int(seed), int(offset)
     if not (0 <= seed < 1 << 64 and 0 <= offset < 1 << 63):
         raise RuntimeError(f"seed must be in [0, 2**64) and offset in [0, 2**63), got {seed} and {offset}")
+    ext = _shim(X, residual, state)
+    if ext is not None:
+        return ext.dropout(X, p, seed, offset, state, residual)
+    _check_operands(X, residual=residual)
+    if not 0.0 <= p <= 1.0:
+        raise RuntimeError(f"dropout probability must be in [0, 1], got {p}")
+    if residual is not None and residual.shape != X.shape:
+        raise RuntimeError(f"residual must have the shape {tuple(X.shape)}, got {tuple(residual.shape)}")
+    if state is not None:
+        _require_cuda(X, state)
+        if state.dtype != torch.int64 or tuple(state.shape) != (2,) or not state.is_contiguous():
+            raise RuntimeError(f"a seed tensor must hold two int64 words [seed, offset], got {state.dtype} {tuple(state.shape)}")
     if _wants_grad(X, residual):
         return dropout_fn.apply(X, residual, p, seed, offset, state)
     return _dropout_run(X, p, seed, offset, state, residual)

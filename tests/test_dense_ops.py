@@ -13,6 +13,15 @@ import torch
 import numml_b200.functional as F
 import numml_b200.nn as nn
 import numml_b200.sparse as sp
+from numml_b200 import numml_torch_cpp
+
+
+@pytest.fixture(autouse=True, params=["compiled", "python"])
+def shim(request, monkeypatch):
+    """Every test runs through the compiled per-call path and through the Python one."""
+    monkeypatch.setattr(numml_torch_cpp, "use_compiled_shim", request.param == "compiled")
+    return request.param
+
 
 TYPES = [torch.float32, torch.float64, torch.bfloat16, torch.float16]
 gpu = pytest.mark.gpu
