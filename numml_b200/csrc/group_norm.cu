@@ -446,36 +446,50 @@ __global__ void __launch_bounds__(kThreads) grad_apply_kernel(Shape sh, const T*
 // ---- short segments: one block per (segment, slab of whole groups), one launch per direction -------------------
 // The rows of a short segment stay in L1 / L2 between the passes over them, so the block simply reads them again:
 // once for the mean, once for the squared deviations from it, once to apply (backward: sums, then apply).
+
+// Division of small numbers (n d < 2^32) by a number that the host knows.
+struct Divisor {
+    uint32_t d, magic;
+    __host__ explicit Divisor(int v = 1) : d(v), magic(v > 1 ? 0xFFFFFFFFu / v + 1 : 0) {}
+    __device__ __forceinline__ int div(int n) const { return d == 1 ? n : static_cast<int>(__umulhi(n, magic)); }
+    __device__ __forceinline__ int mod(int n) const { return n - div(n) * static_cast<int>(d); }
+};
+
 struct Slab {
     int channels, lanes;          // channels of a slab (whole groups), vectors of its row
     int pad_blocks;               // blocks that write the rows outside every segment
+    int width, groups;            // channels of a group, groups of a slab
+    Divisor by_lanes, by_width;
+    // sums over a group: by one vector per column (width / V columns) in the forward pass, per channel in the backward
+    int columns;
+    Divisor by_parts, by_columns; // warps of a group; threads of a warp along a group's columns
+    Divisor by_channels;
 };
 
-constexpr int kShort = 512;                         // threads of these blocks: the longest segment of a batch sets the time
-constexpr int kSlabGroups = 256;                    // most groups of a slab
+constexpr int kShort = 256;                         // threads of these blocks, and most channels of a slab
+constexpr int kSlabGroups = kShort;                 // most groups of a slab
 
 // Sum over the row lanes and over the columns of each group of sm [rows][groups * width].  The block's warps share the
 // groups, several to a group when there are few; out holds `parts` sums per group.
 template <typename A>
 struct GroupSums {
     A out[kSlabGroups + kShort / 32];
-    static __device__ __forceinline__ int parts(int groups) { return groups < kShort / 32 ? kShort / 32 / groups : 1; }
-    __device__ __forceinline__ void form(const A* sm, int rows, int groups, int width) {
-        const int p = parts(groups), lane = threadIdx.x % 32, line = groups * width;
-        const int per = width < 32 ? width : 32, lanes = 32 / per, row = lane / per, column = lane % per;
-        for (int item = threadIdx.x / 32; item < groups * p; item += kShort / 32) {
-            const int g = item / p;
+    __device__ __forceinline__ void form(const A* sm, int rows, const Slab& slab, int width, const Divisor& by_columns) {
+        const int p = slab.by_parts.d, lane = threadIdx.x % 32, line = slab.groups * width;
+        const int per = by_columns.d, lanes = by_columns.div(32), row = by_columns.div(lane), column = lane - row * per;
+        for (int item = threadIdx.x / 32; item < slab.groups * p; item += kShort / 32) {
+            const int g = slab.by_parts.div(item), part = item - g * p;
             A v = 0;
             if (row < lanes)
-                for (int r = item % p * lanes + row; r < rows; r += p * lanes)
+                for (int r = part * lanes + row; r < rows; r += p * lanes)
                     for (int c = column; c < width; c += per) v += sm[r * line + g * width + c];
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, off);
             if (lane == 0) out[item] = v;
         }
     }
-    __device__ __forceinline__ A total(int g, int groups) const {
-        const int p = parts(groups);
+    __device__ __forceinline__ A total(int g, const Slab& slab) const {
+        const int p = slab.by_parts.d;
         A v = out[g * p];
         for (int q = 1; q < p; ++q) v += out[g * p + q];
         return v;
@@ -496,7 +510,7 @@ __device__ __forceinline__ void zero_outside(const Shape& sh, int64_t first, int
 // ONE: a vector of channels belongs to one group (V divides channels / groups), so that a thread has one mean and one
 // sum instead of V.
 template <typename T, int V, int ACT, bool ONE>
-__global__ void __launch_bounds__(kShort) short_forward_kernel(Shape sh, Slab slab, const T* __restrict__ x, const T* __restrict__ w,
+__global__ void __launch_bounds__(kShort, 4) short_forward_kernel(Shape sh, Slab slab, const T* __restrict__ x, const T* __restrict__ w,
                                                                const T* __restrict__ bias, double eps, acc_t<T>* __restrict__ mean,
                                                                acc_t<T>* __restrict__ rstd, T* __restrict__ y) {
     using A = acc_t<T>;
@@ -508,30 +522,43 @@ __global__ void __launch_bounds__(kShort) short_forward_kernel(Shape sh, Slab sl
         return;
     }
     const int64_t s = blockIdx.x, begin = segment_begin(sh, s), end = max(begin, segment_begin(sh, s + 1));
-    const int width = sh.channels / sh.groups, first = blockIdx.y * slab.channels;
-    const int groups = slab.channels / width, g0 = first / width;
+    const int width = slab.width, groups = slab.groups, first = blockIdx.y * slab.channels, g0 = blockIdx.y * groups;
     if (end == begin) {
         for (int g = threadIdx.x; g < groups; g += kShort) mean[s * sh.groups + g0 + g] = rstd[s * sh.groups + g0 + g] = A(0);
         return;
     }
-    const int lane = threadIdx.x % slab.lanes, row_lane = threadIdx.x / slab.lanes, row_lanes = kShort / slab.lanes;
+    const int row_lane = slab.by_lanes.div(threadIdx.x), lane = threadIdx.x - row_lane * slab.lanes, row_lanes = slab.by_lanes.div(kShort);
     const int c = lane * V;                                            // inside the slab
     const int used = static_cast<int>(min(int64_t(row_lanes), end - begin));       // row lanes that have a row
     const int64_t rows = row_lane < row_lanes ? end - begin : 0, step = int64_t(row_lanes) * sh.channels;
     const int64_t at = (begin + row_lane) * sh.channels + first + c;
     // columns of sm: one per vector (ONE) or per channel
-    const int line = ONE ? slab.lanes : slab.channels, columns = ONE ? width / V : width;
+    const int line = ONE ? slab.lanes : slab.channels;
     int group[G];
     A m[G], sum[G] = {};
 #pragma unroll
     for (int q = 0; q < G; ++q) {
-        group[q] = (c + q) / width;
+        group[q] = slab.by_width.div(c + q);
         m[q] = to_acc(x[begin * sh.channels + first + group[q] * width]);          // the group's first value
     }
+    // several rows' loads under way at a time: the longest segment of a batch is bound by their latency
     auto over_rows = [&](auto&& f) {
         const T* p = x + at;
+        int64_t r = row_lane;
+        for (; r + 3 * int64_t(row_lanes) < rows; r += 4 * int64_t(row_lanes), p += 4 * step) {
+            Pack<T, V> raw[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) raw[e] = *reinterpret_cast<const Pack<T, V>*>(p + e * step);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                A v[V];
+#pragma unroll
+                for (int q = 0; q < V; ++q) v[q] = to_acc(raw[e].v[q]);
+                f(v, p + e * step - x);
+            }
+        }
 #pragma unroll 1
-        for (int64_t r = row_lane; r < rows; r += row_lanes, p += step) {
+        for (; r < rows; r += row_lanes, p += step) {
             A v[V];
             load_acc<T, V>(p, v);
             f(v, p - x);
@@ -542,7 +569,7 @@ __global__ void __launch_bounds__(kShort) short_forward_kernel(Shape sh, Slab sl
 #pragma unroll
             for (int q = 0; q < G; ++q) sm[row_lane * line + (ONE ? lane : c + q)] = sum[q];
         __syncthreads();
-        sums.form(sm, used, groups, columns);
+        sums.form(sm, used, slab, slab.columns, slab.by_columns);
         __syncthreads();
     };
     const A n = static_cast<A>(end - begin) * width;
@@ -553,9 +580,9 @@ __global__ void __launch_bounds__(kShort) short_forward_kernel(Shape sh, Slab sl
     join();
 #pragma unroll
     for (int q = 0; q < G; ++q) {
-        m[q] += sums.total(group[q], groups) / n;
+        m[q] += sums.total(group[q], slab) / n;
         sum[q] = 0;
-        if (row_lane == 0 && (c + q) % width == 0) mean[s * sh.groups + g0 + group[q]] = m[q];
+        if (row_lane == 0 && group[q] * width == c + q) mean[s * sh.groups + g0 + group[q]] = m[q];
     }
     over_rows([&](const A (&v)[V], int64_t) {
 #pragma unroll
@@ -566,7 +593,7 @@ __global__ void __launch_bounds__(kShort) short_forward_kernel(Shape sh, Slab sl
     });
     join();
     for (int g = threadIdx.x; g < groups; g += kShort) {
-        scale[g] = static_cast<A>(1.0 / sqrt(static_cast<double>(sums.total(g, groups)) / static_cast<double>(n) + eps));
+        scale[g] = static_cast<A>(1.0 / sqrt(static_cast<double>(sums.total(g, slab)) / static_cast<double>(n) + eps));
         rstd[s * sh.groups + g0 + g] = scale[g];
     }
     __syncthreads();
@@ -586,22 +613,22 @@ __global__ void __launch_bounds__(kShort) short_forward_kernel(Shape sh, Slab sl
 }
 
 template <typename T, int V, int ACT, bool ONE>
-__global__ void __launch_bounds__(kShort) short_backward_kernel(Shape sh, Slab slab, const T* __restrict__ x, const T* __restrict__ dy,
+__global__ void __launch_bounds__(kShort, sizeof(T) == 8 ? 2 : 4) short_backward_kernel(Shape sh, Slab slab, const T* __restrict__ x, const T* __restrict__ dy,
                                                                 const T* __restrict__ w, const T* __restrict__ bias,
                                                                 const acc_t<T>* __restrict__ mean, const acc_t<T>* __restrict__ rstd,
                                                                 acc_t<T>* __restrict__ channel_sums, T* __restrict__ dx) {
     using A = acc_t<T>;
     constexpr int G = ONE ? 1 : V;
     __shared__ A sm[kShort * V];
-    __shared__ A weighted[2][kThreads * V];                            // a slab has at most kThreads vectors
+    __shared__ A weighted[2][kShort];
     __shared__ GroupSums<A> sums[2];
     if (blockIdx.x >= sh.segments) {
         if (dx && blockIdx.y == 0) zero_outside<T, V>(sh, blockIdx.x - sh.segments, slab.pad_blocks, dx);
         return;
     }
     const int64_t s = blockIdx.x, begin = segment_begin(sh, s), end = max(begin, segment_begin(sh, s + 1));
-    const int width = sh.channels / sh.groups, first = blockIdx.y * slab.channels, mine = slab.channels, groups = mine / width;
-    const int lane = threadIdx.x % slab.lanes, row_lane = threadIdx.x / slab.lanes, row_lanes = kShort / slab.lanes;
+    const int width = slab.width, first = blockIdx.y * slab.channels, mine = slab.channels, g0 = blockIdx.y * slab.groups;
+    const int row_lane = slab.by_lanes.div(threadIdx.x), lane = threadIdx.x - row_lane * slab.lanes, row_lanes = slab.by_lanes.div(kShort);
     const int c = lane * V;
     const int used = static_cast<int>(min(int64_t(row_lanes), end - begin));
     const int64_t rows = row_lane < row_lanes ? end - begin : 0, step = int64_t(row_lanes) * sh.channels;
@@ -615,14 +642,14 @@ __global__ void __launch_bounds__(kShort) short_backward_kernel(Shape sh, Slab s
     }
 #pragma unroll
     for (int q = 0; q < G; ++q) {
-        group[q] = (c + q) / width;
-        m[q] = mean[s * sh.groups + first / width + group[q]];
-        rs[q] = rstd[s * sh.groups + first / width + group[q]];
+        group[q] = slab.by_width.div(c + q);
+        m[q] = mean[s * sh.groups + g0 + group[q]];
+        rs[q] = rstd[s * sh.groups + g0 + group[q]];
     }
     A s1[V] = {}, s2[V] = {};
     {
         const T *px = x + at, *pg = dy + at;
-#pragma unroll 1
+#pragma unroll 2
         for (int64_t r = row_lane; r < rows; r += row_lanes, px += step, pg += step) {
             A v[V], g[V];
             load_acc<T, V>(px, v);
@@ -643,7 +670,8 @@ __global__ void __launch_bounds__(kShort) short_backward_kernel(Shape sh, Slab s
 #pragma unroll
             for (int q = 0; q < V; ++q) sm[row_lane * mine + c + q] = part == 0 ? s1[q] : s2[q];
         __syncthreads();
-        for (int ch = threadIdx.x; ch < mine; ch += kShort) {
+        if (threadIdx.x < mine) {
+            const int ch = threadIdx.x;
             A v = 0;
 #pragma unroll 8
             for (int r = 0; r < used; ++r) v += sm[r * mine + ch];
@@ -653,19 +681,19 @@ __global__ void __launch_bounds__(kShort) short_backward_kernel(Shape sh, Slab s
         __syncthreads();
     }
     if (!dx) return;
-    sums[0].form(weighted[0], 1, groups, width);
-    sums[1].form(weighted[1], 1, groups, width);
+    sums[0].form(weighted[0], 1, slab, width, slab.by_channels);
+    sums[1].form(weighted[1], 1, slab, width, slab.by_channels);
     __syncthreads();
     A c1[G], c2[G];
     const A n = static_cast<A>(end - begin) * width;
 #pragma unroll
     for (int q = 0; q < G; ++q) {
-        c1[q] = sums[0].total(group[q], groups) / n;
-        c2[q] = sums[1].total(group[q], groups) / n;
+        c1[q] = sums[0].total(group[q], slab) / n;
+        c2[q] = sums[1].total(group[q], slab) / n;
     }
     const T *px = x + at, *pg = dy + at;
     T* out = dx + at;
-#pragma unroll 1
+#pragma unroll 2
     for (int64_t r = row_lane; r < rows; r += row_lanes, px += step, pg += step, out += step) {
         A v[V], g[V];
         load_acc<T, V>(px, v);
@@ -699,7 +727,7 @@ bool short_segments(int64_t rows, int64_t channels, int64_t groups, int64_t segm
             if (groups % d == 0 && d * width % V == 0) return d;
         return int64_t(0);
     };
-    const int64_t room = kThreads * V / width < kSlabGroups ? kThreads * V / width : kSlabGroups;
+    const int64_t room = kShort / width;
     int64_t in_slab = divisor(groups < room ? groups : room);
     if (in_slab == 0) return false;
     for (;;) {
@@ -714,6 +742,14 @@ bool short_segments(int64_t rows, int64_t channels, int64_t groups, int64_t segm
     if (groups / in_slab > 65535) return false;
     slab->channels = static_cast<int>(in_slab * width);
     slab->lanes = static_cast<int>(in_slab * width / V);
+    slab->width = static_cast<int>(width);
+    slab->groups = static_cast<int>(in_slab);
+    slab->by_lanes = Divisor(slab->lanes);
+    slab->by_width = Divisor(slab->width);
+    slab->columns = static_cast<int>(width % V == 0 ? width / V : width);
+    slab->by_parts = Divisor(slab->groups < kShort / 32 ? kShort / 32 / slab->groups : 1);
+    slab->by_columns = Divisor(slab->columns < 32 ? slab->columns : 32);
+    slab->by_channels = Divisor(slab->width < 32 ? slab->width : 32);
     return true;
 }
 
