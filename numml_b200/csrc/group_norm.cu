@@ -717,8 +717,11 @@ int64_t block_count(int64_t rows) {
 // Whether the one-block-per-segment kernels run, and with which slabs of channels.  They need segments that stay in
 // a block's L1 on average (a slab of one up to 128 KB) and an array in which even one segment that has all rows is
 // read by a single block in about 0.1 ms (slabs up to 8 MB); beyond that the row chunks, which are balanced however
-// long a segment is, take over.  Slabs are made narrower (whole groups) until there are two blocks for every SM, down
-// to rows of 32 bytes, or until they are light enough, down to 64.  Measured on 512 graphs of 120 rows x 128 bfloat16 channels: see the figures at the end.
+// long a segment is, take over.  Slabs are made narrower (whole groups) while there are fewer than eight blocks for
+// every SM, down to rows of 64 bytes, or fewer than two, down to 32.  Measured on 512 graphs of 1 to 1076 rows, mean
+// 118, x 128 bfloat16 channels with gelu, forward / backward: slabs of 128 channels 46 / 100 us, 64: 32 / 65, 32: 31 /
+// 57 (the longest graph's arithmetic on one SM is what is left; clusters of 2 to 8 blocks per graph, which split it,
+// were no faster: 34-41 / 67-72); the row chunks 82 / 117 us in six launches.
 bool short_segments(int64_t rows, int64_t channels, int64_t groups, int64_t segments, size_t size, int V, Slab* slab) {
     if (segments < 1 || segments > 65535 * 16) return false;
     const int64_t width = channels / groups;
@@ -732,7 +735,8 @@ bool short_segments(int64_t rows, int64_t channels, int64_t groups, int64_t segm
     if (in_slab == 0) return false;
     for (;;) {
         const int64_t d = divisor(in_slab - 1), d_line = d * width * int64_t(size);
-        const bool few = segments * (groups / in_slab) < 2 * kSMs && d_line >= 32;
+        const int64_t blocks = segments * (groups / in_slab);
+        const bool few = (blocks < 8 * kSMs && d_line >= 64) || (blocks < 2 * kSMs && d_line >= 32);
         const bool heavy = rows * in_slab * width * int64_t(size) > 8 * 1024 * 1024 && d_line >= 64;
         if (d == 0 || !(few || heavy)) break;
         in_slab = d;
