@@ -2,9 +2,9 @@
 //   dz = dy act'(z),  dx = dz w^T,  dw = x^T dz,  dbias = column sums of dz
 // with z = x w + bias as the forward pass left it.  x [m, k], w [k, n], y [m, n].
 //
-// This file holds the entry points, the products that run on the CUDA cores (double, for which the tensor
-// cores of this GPU are no faster, and empty sums) and the passes around the products; linear_mma_kernel.cuh holds
-// the products on the tensor cores.
+// This file holds the entry points, the products of few rows, those of double (the 5th-generation tensor
+// instructions do not take it) and the passes around the products; linear_mma_kernel.cuh holds the products of the
+// other types.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -16,63 +16,116 @@ namespace {
 
 constexpr int kTile = 64, kDepth = 16, kThreads = 256;
 
-// C[i, j] = sum_k A(i, k) B(k, j), one 64 x 64 tile per block, blockIdx.z cuts the sum.  A(i, k) is
-// a[i * as + k] with A_K (k contiguous) or a[i + k * as]; B(k, j) is b[k + j * bs] with B_K or b[k * bs + j].
-template <typename T, bool A_K, bool B_K, int ACT>
-__global__ void __launch_bounds__(kThreads) tile_kernel(int64_t rows, int64_t cols, int64_t depth, int64_t depth_per_split,
-                                                        const T* __restrict__ a, int64_t as, const T* __restrict__ b, int64_t bs,
-                                                        Epilogue<T> ep) {
-    using A = acc_t<T>;
-    __shared__ A sa[kDepth][kTile + 1], sb[kDepth][kTile + 1];
-    const int64_t i0 = blockIdx.x * int64_t(kTile), j0 = blockIdx.y * int64_t(kTile);
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    const int64_t k_begin = blockIdx.z * depth_per_split, k_end = min(depth, k_begin + depth_per_split);
-    A acc[4][4] = {};
-    for (int64_t k0 = k_begin; k0 < k_end; k0 += kDepth) {
+// ---- double: the double-precision tensor instruction (mma.sync, 16 x 8 x 8) ----------------------------------
+// C[i, j] = sum_k A(i, k) B(k, j) on tiles of 64 rows x 32 WN columns, a warp per 32 x 32; blockIdx.z cuts the sum.
+// A(i, k) is a[i * as + k] with A_K (k contiguous) or a[i + k * as]; B(k, j) is b[k + j * bs] with B_K or
+// b[k * bs + j].  Sixteen terms of both operands are staged at a time, the next sixteen on their way in registers.
+// Lines of 64 + 4 doubles: the sixteen lanes of a half-warp, four k by four rows, then touch sixteen banks.
+constexpr int kLine = 64 + 4;
+
+__device__ __forceinline__ void mma_f64(double (&c)[4], const double (&a)[4], const double (&b)[2]) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f64.f64.f64.f64 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+d"(c[0]), "+d"(c[1]), "+d"(c[2]), "+d"(c[3])
+                 : "d"(a[0]), "d"(a[1]), "d"(a[2]), "d"(a[3]), "d"(b[0]), "d"(b[1]));
+}
+
+template <bool A_K, bool B_K, int ACT, int WN>
+__global__ void __launch_bounds__(64 * WN) double_kernel(int64_t rows, int64_t cols, int64_t depth, int64_t per,
+                                                         const double* __restrict__ a, int64_t as, const double* __restrict__ b, int64_t bs,
+                                                         Epilogue<double> ep) {
+    constexpr int kBlock = 64 * WN, kCols = 32 * WN;
+    constexpr int NA = kTile * kDepth / kBlock, NB = kCols * kDepth / kBlock;          // values per thread and step
+    __shared__ double sa[2][kDepth][kLine], sb[2][kDepth][kLine];
+    const int64_t i0 = blockIdx.x * int64_t(kTile), j0 = blockIdx.y * int64_t(kCols);
+    const int t = threadIdx.x, lane = t % 32, g = lane / 4, q4 = lane % 4;
+    const int wi = t / 32 % 2 * 32, wj = t / 64 * 32;                                  // the warp's corner in the tile
+    const int64_t k_begin = blockIdx.z * per, k_end = min(depth, k_begin + per);
+    double ra[NA], rb[NB];
+    auto fetch = [&](int64_t k0) {
 #pragma unroll
-        for (int e = threadIdx.x; e < kTile * kDepth; e += kThreads) {
-            const int ai = A_K ? e / kDepth : e % kTile, ak = A_K ? e % kDepth : e / kTile;
-            const int64_t i = i0 + ai, k = k0 + ak;
-            sa[ak][ai] = i < rows && k < k_end ? to_acc(A_K ? a[i * as + k] : a[i + k * as]) : A(0);
-            const int bj = B_K ? e / kDepth : e % kTile, bk = B_K ? e % kDepth : e / kTile;
-            const int64_t j = j0 + bj, kb = k0 + bk;
-            sb[bk][bj] = j < cols && kb < k_end ? to_acc(B_K ? b[kb + j * bs] : b[kb * bs + j]) : A(0);
+        for (int e = 0; e < NA; ++e) {
+            const int x = t + e * kBlock, m = A_K ? x / kDepth : x % kTile, k = A_K ? x % kDepth : x / kTile;
+            ra[e] = i0 + m < rows && k0 + k < k_end ? (A_K ? a[(i0 + m) * as + k0 + k] : a[i0 + m + (k0 + k) * as]) : 0.0;
         }
-        __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kDepth; ++k) {
-            A av[4], bv[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                av[q] = sa[k][ty + 16 * q];
-                bv[q] = sb[k][tx + 16 * q];
-            }
-#pragma unroll
-            for (int p = 0; p < 4; ++p)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) acc[p][q] += av[p] * bv[q];
+        for (int e = 0; e < NB; ++e) {
+            const int x = t + e * kBlock, n = B_K ? x / kDepth : x % kCols, k = B_K ? x % kDepth : x / kCols;
+            rb[e] = j0 + n < cols && k0 + k < k_end ? (B_K ? b[k0 + k + (j0 + n) * bs] : b[(k0 + k) * bs + j0 + n]) : 0.0;
         }
+    };
+    auto stage = [&](int s) {
+#pragma unroll
+        for (int e = 0; e < NA; ++e) {
+            const int x = t + e * kBlock;
+            sa[s][A_K ? x % kDepth : x / kTile][A_K ? x / kDepth : x % kTile] = ra[e];
+        }
+#pragma unroll
+        for (int e = 0; e < NB; ++e) {
+            const int x = t + e * kBlock;
+            sb[s][B_K ? x % kDepth : x / kCols][B_K ? x / kDepth : x % kCols] = rb[e];
+        }
+    };
+    double acc[2][4][4] = {};
+    if (k_begin < k_end) {
+        fetch(k_begin);
+        stage(0);
+    }
+    __syncthreads();
+    int s = 0;
+    for (int64_t k0 = k_begin; k0 < k_end; k0 += kDepth, s ^= 1) {
+        const bool more = k0 + kDepth < k_end;
+        if (more) fetch(k0 + kDepth);
+#pragma unroll
+        for (int k = 0; k < kDepth; k += 8) {
+            double af[2][4], bf[4][2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) af[u][r] = sa[s][k + q4 + (r / 2) * 4][wi + u * 16 + g + (r % 2) * 8];
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) bf[v][r] = sb[s][k + q4 + r * 4][wj + v * 8 + g];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) mma_f64(acc[u][v], af[u], bf[v]);
+        }
+        if (more) stage(s ^ 1);
         __syncthreads();
     }
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
-        const int64_t i = i0 + ty + 16 * p;
-        if (i >= rows) continue;
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int64_t j = j0 + tx + 16 * q;
-            if (j >= cols) continue;
-            A v = acc[p][q];
-            if (ep.partial) {
-                ep.partial[(blockIdx.z * rows + i) * cols + j] = v;
-                continue;
+        for (int v = 0; v < 4; ++v)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int64_t i = i0 + wi + u * 16 + g + (r / 2) * 8, j = j0 + wj + v * 8 + q4 * 2 + r % 2;
+                if (i >= rows || j >= cols) continue;
+                double c = acc[u][v][r];
+                if (ep.partial) {
+                    ep.partial[(blockIdx.z * rows + i) * cols + j] = c;
+                    continue;
+                }
+                if (ep.bias) c += ep.bias[j];
+                if (ep.z) ep.z[i * cols + j] = c;
+                c = activate<ACT>(c);
+                if (ep.residual) c += ep.residual[i * ep.ldr + j];
+                ep.y[i * cols + j] = c;
             }
-            if (ep.bias) v += to_acc(ep.bias[j]);
-            if (ep.z) ep.z[i * cols + j] = rounded_z<T, ACT>(v);
-            v = activate<ACT>(v);
-            if (ep.residual) v += to_acc(ep.residual[i * ep.ldr + j]);
-            ep.y[i * cols + j] = from_acc<T>(v);
-        }
+}
+
+// A product whose sum is empty (no input channels): act(bias) + residual.
+template <typename T, int ACT>
+__global__ void __launch_bounds__(kThreads) empty_sum_kernel(int64_t rows, int64_t cols, Epilogue<T> ep) {
+    using A = acc_t<T>;
+    for (int64_t e = blockIdx.x * int64_t(kThreads) + threadIdx.x; e < rows * cols; e += int64_t(gridDim.x) * kThreads) {
+        const int64_t i = e / cols, j = e % cols;
+        A v = ep.bias ? to_acc(ep.bias[j]) : A(0);
+        if (ep.z) ep.z[e] = rounded_z<T, ACT>(v);
+        v = activate<ACT>(v);
+        if (ep.residual) v += to_acc(ep.residual[i * ep.ldr + j]);
+        ep.y[e] = from_acc<T>(v);
     }
 }
 
@@ -274,10 +327,6 @@ int join_parts(int64_t size, int64_t parts, const acc_t<T>* partial, T* out, cud
     return launch_status();
 }
 
-// Whether a product runs on the tensor cores.
-template <typename T>
-constexpr bool on_tensor_cores(int64_t depth) { return !std::is_same<T, double>::value && depth > 0; }
-
 // Into how many parts the sum over the rows is cut for dw, so that there is work for every SM, and how long one is.
 struct Split {
     int64_t parts, per;
@@ -315,13 +364,24 @@ BackwardLayout backward_layout(int64_t m, int64_t k, int64_t n, int act, int dty
 template <typename T, bool A_K, bool B_K, int ACT>
 int product(int64_t rows, int64_t cols, int64_t depth, Split split, const T* a, int64_t as, const T* b, int64_t bs,
             const Epilogue<T>& ep, int32_t* status, cudaStream_t stream) {
-    if constexpr (!std::is_same<T, double>::value)
-        if (on_tensor_cores<T>(depth))
-            return mma_product<T, A_K, B_K, ACT>(rows, cols, depth, split.parts, split.per, a, as, b, bs, ep, status, stream);
-    const int64_t gx = ceil_div(rows, kTile), gy = ceil_div(cols, kTile);
-    if (gx > INT32_MAX || gy > 65535) return NB200_ERR_TOO_LARGE;
-    tile_kernel<T, A_K, B_K, ACT><<<dim3(gx, gy, split.parts), kThreads, 0, stream>>>(rows, cols, depth, split.per, a, as, b, bs, ep);
-    return launch_status();
+    if (depth == 0) {
+        const int64_t blocks = ceil_div(rows * cols, kThreads);
+        empty_sum_kernel<T, ACT><<<static_cast<unsigned>(blocks < kSMs * 8 ? blocks : kSMs * 8), kThreads, 0, stream>>>(rows, cols, ep);
+        return launch_status();
+    }
+    if constexpr (!std::is_same<T, double>::value) {
+        return mma_product<T, A_K, B_K, ACT>(rows, cols, depth, split.parts, split.per, a, as, b, bs, ep, status, stream);
+    } else {
+        const bool narrow = cols <= 32;
+        const int64_t gx = ceil_div(rows, kTile), gy = ceil_div(cols, narrow ? 32 : 64);
+        if (gx > INT32_MAX || gy > 65535 || split.parts > 65535) return NB200_ERR_TOO_LARGE;
+        const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(gy), static_cast<unsigned>(split.parts));
+        if (narrow)
+            double_kernel<A_K, B_K, ACT, 1><<<grid, 64, 0, stream>>>(rows, cols, depth, split.per, a, as, b, bs, ep);
+        else
+            double_kernel<A_K, B_K, ACT, 2><<<grid, 128, 0, stream>>>(rows, cols, depth, split.per, a, as, b, bs, ep);
+        return launch_status();
+    }
 }
 
 Split whole(int64_t depth) { return {1, depth > 0 ? ceil_div(depth, kMmaChunk) * kMmaChunk : kMmaChunk}; }
