@@ -30,7 +30,7 @@ __device__ __forceinline__ void mma_f64(double (&c)[4], const double (&a)[4], co
 }
 
 template <bool A_K, bool B_K, int ACT, int WN>
-__global__ void __launch_bounds__(64 * WN) double_kernel(int64_t rows, int64_t cols, int64_t depth, int64_t per,
+__global__ void __launch_bounds__(64 * WN, 4) double_kernel(int64_t rows, int64_t cols, int64_t depth, int64_t per,
                                                          const double* __restrict__ a, int64_t as, const double* __restrict__ b, int64_t bs,
                                                          Epilogue<double> ep) {
     constexpr int kBlock = 64 * WN, kCols = 32 * WN;
