@@ -233,25 +233,37 @@ int skinny(int64_t rows, int64_t cols, int64_t depth, const T* x, int64_t ldx, c
     return e == cudaSuccess ? launch_status() : NB200_ERR_CUDA;
 }
 
-// Sums over the leading index of partial [parts][size]: 32 columns x 8 lanes per block, lane l adds parts l, l + 8,
-// ..., then the lanes are added in order.  The order depends on the sizes alone.
+// Sums over the leading index of partial [parts][size]: a block has 256 / lanes columns; lane l adds parts l, l + lanes,
+// ..., then the lanes are added in order.  More lanes for more parts (4, 8 or 32), so that neither the loads of a
+// lane follow one another for long nor lanes are idle.  The order depends on the sizes alone.  Up to two arrays in one
+// launch.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) join_parts_kernel(int64_t size, int parts, const acc_t<T>* __restrict__ partial,
-                                                              T* __restrict__ out) {
+struct Join {
+    int64_t size = 0;
+    int parts = 0;
+    const acc_t<T>* partial = nullptr;
+    T* out = nullptr;
+    __host__ __device__ int lanes() const { return parts <= 16 ? 4 : parts <= 64 ? 8 : 32; }
+    int64_t blocks() const { return ceil_div(size, kThreads / lanes()); }
+};
+template <typename T>
+__global__ void __launch_bounds__(kThreads) join_parts_kernel(Join<T> first, Join<T> second, unsigned first_blocks) {
     using A = acc_t<T>;
-    __shared__ A sm[8][33];
-    const int64_t e = blockIdx.x * int64_t(32) + threadIdx.x % 32;
-    const int lane = threadIdx.x / 32;
+    __shared__ A sm[kThreads];
+    const bool is_first = blockIdx.x < first_blocks;
+    const Join<T>& j = is_first ? first : second;
+    const int lanes = j.lanes(), columns = kThreads / lanes, lane = threadIdx.x / columns;
+    const int64_t e = (blockIdx.x - (is_first ? 0 : first_blocks)) * int64_t(columns) + threadIdx.x % columns;
     A v = 0;
-    if (e < size)
+    if (e < j.size)
 #pragma unroll 8
-        for (int s = lane; s < parts; s += 8) v += partial[s * size + e];
-    sm[lane][threadIdx.x % 32] = v;
+        for (int s = lane; s < j.parts; s += lanes) v += j.partial[s * j.size + e];
+    sm[threadIdx.x] = v;
     __syncthreads();
-    if (lane == 0 && e < size) {
-#pragma unroll
-        for (int q = 1; q < 8; ++q) v += sm[q][threadIdx.x];
-        out[e] = from_acc<T>(v);
+    if (lane == 0 && e < j.size) {
+#pragma unroll 4
+        for (int q = 1; q < lanes; ++q) v += sm[q * columns + threadIdx.x];
+        j.out[e] = from_acc<T>(v);
     }
 }
 
@@ -320,10 +332,11 @@ int slope_pass(int64_t m, int64_t n, int act, const T* dy, int64_t ldd, const T*
 }
 
 template <typename T>
-int join_parts(int64_t size, int64_t parts, const acc_t<T>* partial, T* out, cudaStream_t stream) {
-    const int64_t blocks = ceil_div(size, 32);
-    if (blocks > INT32_MAX) return NB200_ERR_TOO_LARGE;
-    join_parts_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(size, static_cast<int>(parts), partial, out);
+int join_parts(const Join<T>& first, const Join<T>& second, cudaStream_t stream) {
+    const int64_t a = first.blocks(), b = second.blocks();
+    if (a + b > INT32_MAX) return NB200_ERR_TOO_LARGE;
+    if (a + b == 0) return NB200_OK;
+    join_parts_kernel<T><<<static_cast<unsigned>(a + b), kThreads, 0, stream>>>(first, second, static_cast<unsigned>(a));
     return launch_status();
 }
 
@@ -393,14 +406,15 @@ int backward(int64_t m, int64_t k, int64_t n, const T* dy, int64_t ldd, const T*
     T* dz = act == NB200_ACT_NONE ? nullptr : reinterpret_cast<T*>(work + lay.dz);
     A* sums = reinterpret_cast<A*>(work + lay.sums);
     A* partial = reinterpret_cast<A*>(work + lay.partial);
+    Join<T> join_db, join_dw;
     int rc = NB200_OK;
     if (dz || db) {
         constexpr int V = 16 / sizeof(T);
         const bool vector = n % V == 0 && ldd % V == 0 && aligned16(dy) && aligned16(z);
         rc = vector ? slope_pass<T, V>(m, n, act, dy, ldd, z, dz, db ? sums : nullptr, stream)
                     : slope_pass<T, 1>(m, n, act, dy, ldd, z, dz, db ? sums : nullptr, stream);
-        if (rc == NB200_OK && db) rc = join_parts<T>(n, band_count(m), sums, db, stream);
         if (rc != NB200_OK) return rc;
+        if (db) join_db = Join<T>{n, static_cast<int>(band_count(m)), sums, db};
     }
     const T* g = dz ? dz : dy;
     const int64_t ldg = dz ? n : ldd;
@@ -414,9 +428,10 @@ int backward(int64_t m, int64_t k, int64_t n, const T* dy, int64_t ldd, const T*
         rc = product<T, false, false, NB200_ACT_NONE>(k, n, m, split, x, ldx, g, ldg, {nullptr, nullptr, 0, nullptr, nullptr, partial}, status,
                                                       stream);
         if (rc != NB200_OK) return rc;
-        if (rc == NB200_OK) rc = join_parts<T>(k * n, split.parts, partial, dw, stream);
+        if (rc != NB200_OK) return rc;
+        join_dw = Join<T>{k * n, static_cast<int>(split.parts), partial, dw};
     }
-    return rc;
+    return join_parts<T>(join_dw, join_db, stream);
 }
 
 bool bad_sizes(int64_t m, int64_t k, int64_t n) {
