@@ -33,22 +33,21 @@ namespace nb200 {
 namespace {
 
 constexpr int kEpilogueWarps = 8, kLoaderWarps = 8, kLoaders = kLoaderWarps * 32;
-constexpr int kThreads = (kEpilogueWarps + kLoaderWarps + 4) * 32;   // whole warpgroups; three warps of the last are idle
+constexpr int kThreads = (kEpilogueWarps + kLoaderWarps + 4) * 32;   // whole warpgroups; the last has products, prefetches and two idle warps
 constexpr int kLaunchRegisters = 96;                               // per thread; checked on the host
 constexpr int kPieceBytes = kMmaTile * kMmaChunk * 2;              // one piece of one operand's chunk: 16 KB
 constexpr int kUnits = kMmaTile * kMmaChunk / 8 / kLoaders;        // units of eight values per loader thread
-constexpr int kAhead = 4;
 
 // Registers per thread after the warpgroups have shared them out anew: the float loaders hold a chunk of both
 // operands and the epilogue the sums of 64 columns; for 16-bit types the epilogue holds twice as many columns of a
 // block and the loaders next to nothing.
 template <typename T> struct Traits {                              // 16-bit types
     static constexpr int epilogue_registers = 160, loader_registers = 56, product_registers = 48;
-    static constexpr int pieces = 1, a_slots = 4, b_slots = 8, buffers = 4;
+    static constexpr int pieces = 1, a_slots = 4, b_slots = 8, buffers = 4, ahead = 12;
 };
 template <> struct Traits<float> {
     static constexpr int epilogue_registers = 120, loader_registers = 96, product_registers = 48;
-    static constexpr int pieces = 3, a_slots = 2, b_slots = 2, buffers = 3;
+    static constexpr int pieces = 3, a_slots = 2, b_slots = 2, buffers = 3, ahead = 4;
 };
 
 // What leaves: y; y and z; a product without a forward epilogue; float parts of a sum.
@@ -66,6 +65,7 @@ struct Control {
     uint64_t full[8], empty[8], acc_full[4], acc_empty[4], done;
     uint32_t tmem;
     int gave_up;
+    int progress;             // chunks whose products have been issued
 };
 
 template <typename T>
@@ -282,25 +282,38 @@ __device__ __forceinline__ void load_split(const Args<T>& g, uint32_t a_ring, ui
     }
 }
 
-// Float operands on their way: one thread asks for the boxes that the loaders will need kAhead chunks later to be
-// brought into L2, so that the loaders, whose registers hold one chunk, wait for L2 and not for memory.
-template <typename T, bool A_K, bool B_K>
+// One warp walks kAhead chunks in front of the products and asks for what will be needed to be brought into L2: float
+// operands (the loaders' registers hold one chunk, so they should wait for L2 and not for memory) and the rows of the
+// residual (which the epilogue asks for only a block ahead).  It goes by a counter that only grows, so it may fall
+// behind without missing anything, and nobody waits for it.
+template <typename T, bool A_K, bool B_K, int KIND>
 __device__ __forceinline__ void prefetch_role(const Args<T>& g, const void* map_a, const void* map_b, Control* ctl) {
-    constexpr int S = Traits<T>::a_slots;
-    Walk<T> w(g), ahead(g);
-    auto ask = [&]() {
-        if (A_K) tc::tile_prefetch(map_a, static_cast<int>(ahead.k0()), static_cast<int>(ahead.i0()));
-        else tc::tile_prefetch(map_a, static_cast<int>(ahead.i0()), static_cast<int>(ahead.k0()));
-        if (!g.resident) {
-            if (B_K) tc::tile_prefetch(map_b, static_cast<int>(ahead.k0()), static_cast<int>(ahead.j0()));
-            else tc::tile_prefetch(map_b, static_cast<int>(ahead.j0()), static_cast<int>(ahead.k0()));
+    const int lane = threadIdx.x % 32;
+    const bool operands = Traits<T>::pieces == 3 && g.tiled, residual = (KIND == kForward || KIND == kForwardZ) && g.ep.residual;
+    if (!operands && !residual) return;
+    const long long t0 = clock64();
+    int asked = 0;
+    for (Walk<T> ahead(g); ahead.live(); ahead.next_chunk(), ++asked) {
+        while (asked >= *static_cast<volatile int*>(&ctl->progress) + Traits<T>::ahead) {
+            if (*static_cast<volatile int*>(&ctl->gave_up) || clock64() - t0 > 64 * tc::kWaitCycles) return;
+            __nanosleep(100);
         }
-        ahead.next_chunk();
-    };
-    for (int q = 0; q < kAhead && ahead.live(); ++q) ask();
-    for (Ring<S> ring; w.live() && ahead.live(); ring.next(), w.next_chunk()) {
-        if (!tc::mbar_wait(&ctl->full[ring.slot], ring.parity, &ctl->gave_up)) return;
-        ask();
+        if (operands && lane == 0) {
+            if (A_K) tc::tile_prefetch(map_a, static_cast<int>(ahead.k0()), static_cast<int>(ahead.i0()));
+            else tc::tile_prefetch(map_a, static_cast<int>(ahead.i0()), static_cast<int>(ahead.k0()));
+            if (!g.resident) {
+                if (B_K) tc::tile_prefetch(map_b, static_cast<int>(ahead.k0()), static_cast<int>(ahead.j0()));
+                else tc::tile_prefetch(map_b, static_cast<int>(ahead.j0()), static_cast<int>(ahead.k0()));
+            }
+        }
+        if (residual && ahead.chunk == 0) {
+            const int64_t columns = min(int64_t(kMmaTile), g.cols - ahead.j0());
+            for (int r = lane; r < kMmaTile && ahead.i0() + r < g.rows; r += 32) {
+                const char* p = reinterpret_cast<const char*>(g.ep.residual + (ahead.i0() + r) * g.ep.ldr + ahead.j0());
+                for (int64_t c = 0; c < columns * int64_t(sizeof(T)); c += 128)
+                    asm volatile("prefetch.global.L2 [%0];" :: "l"(p + c));
+            }
+        }
     }
 }
 
@@ -357,6 +370,7 @@ __device__ void product_role(const Args<T>& g, uint32_t a_ring, uint32_t b_ring,
     constexpr uint32_t a_step = A_K ? 32 : 2048, b_step = B_K ? 32 : 2048;       // bytes from one 16-term step to the next
     Ring<S> ring;
     Ring<Tr::buffers> buffers;
+    int issued = 0;
     bool ok = true;
     for (Walk<T> w(g); ok && w.live(); w.next_item()) {
         const uint32_t idesc = g.cols - w.j0() > kMmaTile / 2 ? whole : part;      // columns that do not exist are not multiplied
@@ -387,6 +401,7 @@ __device__ void product_role(const Args<T>& g, uint32_t a_ring, uint32_t b_ring,
             }
             products(0, 0);
             tc::commit(&ctl->empty[ring.slot]);
+            *static_cast<volatile int*>(&ctl->progress) = ++issued;
             if (last) {
                 tc::commit(&ctl->acc_full[buffers.slot]);
                 buffers.next();
@@ -701,6 +716,7 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
         }
         tc::mbar_init(&ctl.done, 1);
         ctl.gave_up = 0;
+        ctl.progress = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kEpilogueWarps + kLoaderWarps) tc::tmem_alloc(&ctl.tmem, kTmemColumns);
@@ -727,8 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
     } else {
         tc::registers_down<Tr::product_registers>();
         if (threadIdx.x == (kEpilogueWarps + kLoaderWarps) * 32) product_role<T, A_K, B_K>(g, a_ring, b_ring, tmem, &ctl);
-        if (Tr::pieces == 3 && g.tiled && threadIdx.x == (kEpilogueWarps + kLoaderWarps + 1) * 32)
-            prefetch_role<T, A_K, B_K>(g, &map_a, &map_b, &ctl);
+        if (warp == kEpilogueWarps + kLoaderWarps + 1) prefetch_role<T, A_K, B_K, KIND>(g, &map_a, &map_b, &ctl);
     }
     __syncwarp();
     tc::fence_before_sync();
