@@ -103,6 +103,58 @@ __device__ __forceinline__ A activate_slope(A z) {
     return A(1);
 }
 
+// ---- two floats at a time: one instruction for a pair of additions, products or multiply-adds ---------------
+struct Pair {
+    unsigned long long bits;
+    __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ explicit Pair(unsigned long long v) : bits(v) {}
+    __device__ __forceinline__ void to(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(bits)); }
+};
+__device__ __forceinline__ Pair operator+(const Pair& a, const Pair& b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.bits), "l"(b.bits));
+    return Pair(r);
+}
+__device__ __forceinline__ Pair operator*(const Pair& a, const Pair& b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.bits), "l"(b.bits));
+    return Pair(r);
+}
+__device__ __forceinline__ Pair fma(const Pair& a, const Pair& b, const Pair& c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+    return Pair(r);
+}
+__device__ __forceinline__ Pair both(float v) { return Pair(v, v); }
+
+// activate() of two values: the same formulas, the parts outside the special functions done in pairs.
+template <int ACT>
+__device__ __forceinline__ void activate_pair(float& a, float& b) {
+    if constexpr (ACT == NB200_ACT_SILU) {
+        float ea = __expf(-a), eb = __expf(-b);
+        (Pair(ea, eb) + both(1.f)).to(ea, eb);
+        (Pair(a, b) * Pair(__fdividef(1.f, ea), __fdividef(1.f, eb))).to(a, b);
+    } else if constexpr (ACT == NB200_ACT_GELU) {
+        const Pair z(a, b), x = Pair(fabsf(a), fabsf(b)) * both(static_cast<float>(kRootHalf));
+        float ta, tb, ea, eb;
+        fma(x, both(0.3275911f), both(1.f)).to(ta, tb);
+        const Pair t(__fdividef(1.f, ta), __fdividef(1.f, tb));
+        (x * x).to(ea, eb);
+        Pair poly = fma(t, both(1.061405429f), both(-1.453152027f));
+        poly = fma(t, poly, both(1.421413741f));
+        poly = fma(t, poly, both(-0.284496736f));
+        poly = fma(t, poly, both(0.254829592f));
+        const Pair tail = t * poly * Pair(0.5f * __expf(-ea), 0.5f * __expf(-eb));
+        float ca, cb, na, nb;
+        tail.to(ca, cb);
+        fma(tail, both(-1.f), both(1.f)).to(na, nb);
+        (z * Pair(a > 0.f ? na : ca, b > 0.f ? nb : cb)).to(a, b);
+    } else {
+        a = activate<ACT>(a);
+        b = activate<ACT>(b);
+    }
+}
+
 inline bool known_activation(int act) { return act >= NB200_ACT_NONE && act <= NB200_ACT_TANH; }
 inline bool known_dense_dtype(int dtype) { return dtype >= NB200_F32 && dtype <= NB200_F16; }
 inline size_t dense_dtype_size(int dtype) { return dtype == NB200_F64 ? 8 : dtype == NB200_F32 ? 4 : 2; }

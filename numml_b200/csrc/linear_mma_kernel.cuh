@@ -544,7 +544,8 @@ struct Writer {
                         const uint4 b4 = *reinterpret_cast<const uint4*>(ep.bias + col0 + u);
                         const uint32_t b[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
-                        for (int q = 0; q < U; ++q) v[u + q] += unit_value(b, q, O());
+                        for (int q = 0; q < U; q += 2)
+                            (Pair(v[u + q], v[u + q + 1]) + Pair(unit_value(b, q, O()), unit_value(b, q + 1, O()))).to(v[u + q], v[u + q + 1]);
                     }
                 } else {
 #pragma unroll
@@ -563,7 +564,7 @@ struct Writer {
                 }
             }
 #pragma unroll
-            for (int q = 0; q < CB; ++q) v[q] = activate<ACT>(v[q]);
+            for (int q = 0; q < CB; q += 2) activate_pair<ACT>(v[q], v[q + 1]);
             open();
             if (ep.residual) {
                 if (g.vector_residual) {
@@ -575,7 +576,9 @@ struct Writer {
                         uint32_t r[4];
                         shared_load16(place(lane, u), r);
 #pragma unroll
-                        for (int q = 0; q < U; ++q) v[u * U + q] += unit_value(r, q, O());
+                        for (int q = 0; q < U; q += 2)
+                            (Pair(v[u * U + q], v[u * U + q + 1]) + Pair(unit_value(r, q, O()), unit_value(r, q + 1, O())))
+                                .to(v[u * U + q], v[u * U + q + 1]);
                     }
                 } else if (row0 + lane < g.rows) {
                     const T* p = ep.residual + (row0 + lane) * ep.ldr + col0;
@@ -624,7 +627,7 @@ __device__ __forceinline__ bool epilogue_item(const Args<T>& g, const Walk<T>& w
                 if (part > 0) {
                     tc::tmem_wait16(sum);
 #pragma unroll
-                    for (int q = 0; q < 16; ++q) v[q] += sum[q];
+                    for (int q = 0; q < 16; q += 2) (Pair(v[q], v[q + 1]) + Pair(sum[q], sum[q + 1])).to(v[q], v[q + 1]);
                 }
                 tc::tmem_store16(sums + c, v);
             }
@@ -651,7 +654,8 @@ __device__ __forceinline__ bool epilogue_item(const Args<T>& g, const Walk<T>& w
                 tc::tmem_wait16(v + h);
                 tc::tmem_wait16(sum);
 #pragma unroll
-                for (int q = 0; q < 16; ++q) v[h + q] += sum[q];
+                for (int q = 0; q < 16; q += 2)
+                    (Pair(v[h + q], v[h + q + 1]) + Pair(sum[q], sum[q + 1])).to(v[h + q], v[h + q + 1]);
             }
         } else {
 #pragma unroll
@@ -659,9 +663,12 @@ __device__ __forceinline__ bool epilogue_item(const Args<T>& g, const Walk<T>& w
         }
         if (block + 1 == 64 / CB || !present(block + 1)) release();
         if constexpr (Tr::pieces == 3) {
-            float t = 0.f;                                         // NaN if any of the values is not finite
+            Pair zeros = both(0.f);                                // NaN if any of the values is not finite
 #pragma unroll
-            for (int q = 0; q < CB; ++q) t = fmaf(v[q], 0.f, t);
+            for (int q = 0; q < CB; q += 2) zeros = fma(Pair(v[q], v[q + 1]), both(0.f), zeros);
+            float t, t2;
+            zeros.to(t, t2);
+            t += t2;
             if (t != t && row0 + lane < g.rows) {
                 // one value in turn, so that the loop needs no index into registers
 #pragma unroll 1
