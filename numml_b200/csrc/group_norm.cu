@@ -249,7 +249,8 @@ __global__ void __launch_bounds__(kThreads) apply_kernel(Shape sh, const T* __re
             A v[V];
             load_acc<T, V>(x + r * sh.channels + c, v);
 #pragma unroll
-            for (int q = 0; q < V; ++q) v[q] = activate<ACT>((v[q] - m[q]) * a[q] + cp.beta[q]);
+            for (int q = 0; q < V; ++q) v[q] = (v[q] - m[q]) * a[q] + cp.beta[q];
+            activate_all<ACT>(v);
             store_acc<T, V>(y + r * sh.channels + c, v);
         }
     }
@@ -432,12 +433,15 @@ __global__ void __launch_bounds__(kThreads) grad_apply_kernel(Shape sh, const T*
             A v[V], g[V];
             load_acc<T, V>(x + r * sh.channels + c, v);
             load_acc<T, V>(dy + r * sh.channels + c, g);
+            A slope[V];
 #pragma unroll
             for (int q = 0; q < V; ++q) {
-                const A xhat = (v[q] - m[q]) * rs[q];
-                const A h = g[q] * activate_slope<ACT>(xhat * cp.gamma[q] + cp.beta[q]) * cp.gamma[q];
-                v[q] = rs[q] * (h - c1[q] - xhat * c2[q]);
+                v[q] = (v[q] - m[q]) * rs[q];
+                slope[q] = v[q] * cp.gamma[q] + cp.beta[q];
             }
+            slope_all<ACT>(slope);
+#pragma unroll
+            for (int q = 0; q < V; ++q) v[q] = rs[q] * (g[q] * slope[q] * cp.gamma[q] - c1[q] - v[q] * c2[q]);
             store_acc<T, V>(dx + r * sh.channels + c, v);
         }
     }
@@ -607,7 +611,8 @@ __global__ void __launch_bounds__(kShort, 4) short_forward_kernel(Shape sh, Slab
     over_rows([&](const A (&v)[V], int64_t offset) {
         A out[V];
 #pragma unroll
-        for (int q = 0; q < V; ++q) out[q] = activate<ACT>((v[q] - m[ONE ? 0 : q]) * a[q] + b[q]);
+        for (int q = 0; q < V; ++q) out[q] = (v[q] - m[ONE ? 0 : q]) * a[q] + b[q];
+        activate_all<ACT>(out);
         store_acc<T, V>(y + offset, out);
     });
 }
@@ -654,12 +659,18 @@ __global__ void __launch_bounds__(kShort, sizeof(T) == 8 ? 2 : 4) short_backward
             A v[V], g[V];
             load_acc<T, V>(px, v);
             load_acc<T, V>(pg, g);
+            A slope[V];
 #pragma unroll
             for (int q = 0; q < V; ++q) {
-                const A xhat = (v[q] - m[ONE ? 0 : q]) * rs[ONE ? 0 : q];
-                const A dz = g[q] * activate_slope<ACT>(xhat * gamma[q] + beta[q]);
+                v[q] = (v[q] - m[ONE ? 0 : q]) * rs[ONE ? 0 : q];
+                slope[q] = v[q] * gamma[q] + beta[q];
+            }
+            slope_all<ACT>(slope);
+#pragma unroll
+            for (int q = 0; q < V; ++q) {
+                const A dz = g[q] * slope[q];
                 s1[q] += dz;
-                s2[q] += dz * xhat;
+                s2[q] += dz * v[q];
             }
         }
     }
@@ -698,12 +709,15 @@ __global__ void __launch_bounds__(kShort, sizeof(T) == 8 ? 2 : 4) short_backward
         A v[V], g[V];
         load_acc<T, V>(px, v);
         load_acc<T, V>(pg, g);
+        A slope[V];
 #pragma unroll
         for (int q = 0; q < V; ++q) {
-            const A xhat = (v[q] - m[ONE ? 0 : q]) * rs[ONE ? 0 : q];
-            const A h = g[q] * activate_slope<ACT>(xhat * gamma[q] + beta[q]) * gamma[q];
-            v[q] = rs[ONE ? 0 : q] * (h - c1[ONE ? 0 : q] - xhat * c2[ONE ? 0 : q]);
+            v[q] = (v[q] - m[ONE ? 0 : q]) * rs[ONE ? 0 : q];
+            slope[q] = v[q] * gamma[q] + beta[q];
         }
+        slope_all<ACT>(slope);
+#pragma unroll
+        for (int q = 0; q < V; ++q) v[q] = rs[ONE ? 0 : q] * (g[q] * slope[q] * gamma[q] - c1[ONE ? 0 : q] - v[q] * c2[ONE ? 0 : q]);
         store_acc<T, V>(out, v);
     }
 }

@@ -289,8 +289,9 @@ __global__ void __launch_bounds__(kThreads) slope_kernel(int64_t rows, int64_t c
             if (ACT != NB200_ACT_NONE) {
                 A s[V];
                 load_acc<T, V>(z + i * cols + j, s);
+                slope_all<ACT>(s);
 #pragma unroll
-                for (int q = 0; q < V; ++q) v[q] *= activate_slope<ACT>(s[q]);
+                for (int q = 0; q < V; ++q) v[q] *= s[q];
                 store_acc<T, V>(dz + i * cols + j, v);
             }
 #pragma unroll

@@ -73,6 +73,14 @@ def _shim(*operands):
     return numml_torch_cpp.compiled_shim()
 
 
+def _status_pointer(dev):
+    """The device's status word; none while a graph is being captured that would otherwise come to own it."""
+    key = dev.index if dev.index is not None else torch.cuda.current_device()
+    if key not in numml_torch_cpp._status_words and torch.cuda.is_current_stream_capturing():
+        return None
+    return _ptr(_status_word(dev))
+
+
 def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -92,7 +100,7 @@ def _linear_forward(X, weights, bias, residual, act, keep_z):
         y = torch.empty(X.shape[:-1] + (N,), dtype=X.dtype, device=X.device)
         z = torch.empty((M, N), dtype=X.dtype, device=X.device) if keep_z and act else None
         _cabi.call("nb200_linear_forward", M, K, N, _ptr(x), ldx, _ptr(w), ldw, _ptr(b), _ptr(r), ldr, act, _ptr(z), _ptr(y),
-                   _ptr(_status_word(X.device)), _DTYPES[X.dtype], _stream())
+                   _status_pointer(X.device), _DTYPES[X.dtype], _stream())
     return y, z
 
 
@@ -109,7 +117,7 @@ def _linear_backward(dY, X, weights, z, act, want_x, want_w, want_b):
         db = torch.empty((N,), dtype=X.dtype, device=X.device) if want_b else None
         work = torch.empty(_cabi.lib().nb200_linear_backward_workspace_bytes(M, K, N, act, code), dtype=torch.uint8, device=X.device)
         _cabi.call("nb200_linear_backward", M, K, N, _ptr(g), ldg, _ptr(x), ldx, _ptr(w), ldw, _ptr(z), act, _ptr(dx), _ptr(dw),
-                   _ptr(db), _ptr(work), work.numel(), _ptr(_status_word(X.device)), code, _stream())
+                   _ptr(db), _ptr(work), work.numel(), _status_pointer(X.device), code, _stream())
     return dx, dw, db
 
 

@@ -5,6 +5,7 @@ accumulation type (float32 for the narrow types), a sum of n terms in it is off 
 sum of their magnitudes (the factor 2 covers accumulators that truncate), and an activation passes an error
 of its argument on with a factor of at most 1.13 (the largest slope, gelu's) and its slope with at most 0.8
 (the largest curvature, gelu's)."""
+import itertools
 import math
 
 import pytest
@@ -133,7 +134,7 @@ def run_linear(m, k, n, dtype, act, bias, residual, seed=0, integers=False):
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 64, 40), (3, 129, 7), (17, 5, 300), (64, 64, 64), (127, 65, 129), (128, 128, 128),
                                    (130, 256, 16), (257, 33, 65), (1000, 16, 200), (2049, 96, 130), (5, 1024, 1024), (16, 700, 24),
-                                   (33, 512, 513)])
+                                   (33, 512, 513), (513, 64, 64), (700, 200, 36), (640, 33, 140), (1025, 520, 260), (900, 1, 1)])
 def test_linear_sizes(m, k, n, dtype):
     run_linear(m, k, n, dtype, "gelu", True, True, seed=m + k + n)
 
@@ -145,11 +146,12 @@ def test_linear_sizes(m, k, n, dtype):
 def test_linear_parts(act, bias, residual, dtype):
     run_linear(200, 72, 56, dtype, act, bias, residual, seed=7)
     run_linear(2, 72, 56, dtype, act, bias, residual, seed=8)
+    run_linear(600, 136, 72, dtype, act, bias, residual, seed=9)          # tiles of more than 512 rows, three chunks
 
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("m", [2, 300])
+@pytest.mark.parametrize("m", [2, 300, 700])
 def test_linear_relu(m, dtype):
     run_linear(m, 24, 40, dtype, "relu", True, True, seed=3, integers=True)
 
@@ -167,15 +169,16 @@ def test_linear_many_rows(dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-def test_linear_views(dtype):
+@pytest.mark.parametrize("rows", [150, 1200])
+def test_linear_views(rows, dtype):
     """Row-strided, odd-offset, transposed and 3-D operands give what their contiguous copies give, bit for bit."""
-    big = normal((150, 201), 0, dtype).cuda()
+    big = normal((rows, 201), 0, dtype).cuda()
     W = normal((101, 90), 1, dtype, 0.1).cuda()
-    R = normal((150, 100), 2, dtype).cuda()
+    R = normal((rows, 100), 2, dtype).cuda()
     b = normal((90,), 3, dtype).cuda()
-    for X, w, r in ((big[:, :101], W, R[:, 3:93]), (big[:, 97:198], W[:, :], R[:, :90]), (big[::2, 1:102], W, R[:75, 10:]),
+    for X, w, r in ((big[:, :101], W, R[:, 3:93]), (big[:, 97:198], W[:, :], R[:, :90]), (big[::2, 1:102], W, R[:rows // 2, 10:]),
                     (big[:, 5:55], normal((70, 50), 4, dtype, 0.1).cuda().T[:, :70], R[:, :70]),
-                    (big[:, 0:1].expand(150, 101), W, R[:, :90]), (big[:, 100:].view(150, 101)[:, :101], W, None)):
+                    (big[:, 0:1].expand(rows, 101), W, R[:, :90]), (big[:, 100:].view(rows, 101)[:, :101], W, None)):
         bias = b[:w.shape[1]]
         got = F.linear(X, w, bias, "silu", r)
         want = F.linear(X.contiguous(), w.contiguous(), bias.clone(), "silu", r.contiguous() if r is not None else None)
@@ -210,7 +213,7 @@ def test_linear_empty(m, k, n, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("m", [1, 5, 200])
+@pytest.mark.parametrize("m", [1, 5, 200, 600])
 def test_linear_infinities_and_nan_stay_in_their_rows_and_columns(m, dtype):
     """An infinity times a positive weight is an infinity, a NaN a NaN, and other rows do not notice."""
     X = normal((m, 130), 1, dtype).cuda()
@@ -232,12 +235,27 @@ def test_linear_infinities_and_nan_stay_in_their_rows_and_columns(m, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("m", [100, 600])
+@pytest.mark.parametrize("power", [-36, -38, 37])
+def test_linear_float32_ends_of_the_range(power, m):
+    """Values whose low-order pieces are subnormal in 16 bits, and values near the largest: products with weights near
+    one keep float32's error relative to the sum of magnitudes, down to the spacing of the smallest normal number."""
+    X = (normal((m, 40), 1, torch.float64) * 10.0 ** power).float()
+    W = normal((40, 70), 2, torch.float32, 0.5)
+    ref, mag = X.double() @ W.double(), X.double().abs() @ W.double().abs()
+    keep = mag < 3e38
+    y = F.linear(X.cuda(), W.cuda()).cpu().double()
+    bound = 2 * 42 * units(torch.float32)[1] * mag + 40 * torch.finfo(torch.float32).tiny * 2 ** -23
+    assert ((y - ref).abs() <= bound)[keep].all(), ((y - ref).abs() / bound)[keep].max()
+
+
+@gpu
 def test_linear_float32_keeps_small_and_large_values():
     """float32 inputs use their whole range: products of very large and very small factors, and values with all
     24 bits, whose sums with few terms are off by a few units in the last place only."""
     ua = units(torch.float32)[1]
-    for k in (3, 64, 200):
-        X = normal((150, k), k, torch.float64).mul(10.0 ** torch.linspace(-30, 30, k, dtype=torch.float64)).float()
+    for m, k in ((150, 3), (150, 64), (600, 3), (600, 64), (600, 200)):
+        X = normal((m, k), k, torch.float64).mul(10.0 ** torch.linspace(-30, 30, k, dtype=torch.float64)).float()
         W = normal((k, 90), k + 1, torch.float64).mul(10.0 ** torch.linspace(30, -30, k, dtype=torch.float64)[:, None] * 1e-3).float()
         y = F.linear(X.cuda(), W.cuda())
         ref, mag = X.double() @ W.double(), X.double().abs() @ W.double().abs()
@@ -397,6 +415,28 @@ def test_group_norm_batch(dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("C,groups", [(600, 2), (303, 1)])
+def test_group_norm_batch_in_row_chunks(C, groups, dtype):
+    """Groups too wide for the one-block-per-graph kernels: pieces of graphs in chunks of rows."""
+    sizes = [0, 40, 1, 0, 0, 63, 700, 64, 2, 33, 0, 1500, 31, 0]
+    ptr = [3]
+    for s in sizes:
+        ptr.append(ptr[-1] + s)
+    X = normal((ptr[-1] + 77, C), 9, dtype, 1.0, -2.0)
+    run_group_norm(X, groups, dtype, "silu", ptr=ptr, seed=5)
+    run_group_norm(X[:1000], groups, dtype, "gelu", affine=False, seed=6)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_group_norm_long_graphs(dtype):
+    """Graphs of tens of thousands of rows beside short ones."""
+    ptr = [0, 70000, 70000, 70003, 140000, 140100, 150000]
+    run_group_norm(normal((150010, 64), 9, dtype, 1.0, 3.0), 1, dtype, "tanh", ptr=ptr, seed=5)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_group_norm_many_small_graphs(dtype):
     gen = torch.Generator().manual_seed(3)
     ptr = [0] + torch.cumsum(torch.randint(0, 12, (700,), generator=gen), 0).tolist()
@@ -444,8 +484,9 @@ def test_group_norm_nan_stays_in_its_graph_and_group(dtype):
 @gpu
 def test_group_norm_broken_row_pointers_touch_nothing_else():
     """Row numbers out of order or out of range: values are unspecified, the rest of memory is not touched."""
-    for ptr in ([5, 2, 40, 10], [-7, 20, 1 << 40, 30], [0, 100, 100, 100000], [60, 50, 40, 30], [90, 90, 90, 90]):
-        arena = torch.full((3, 60, 16), 7.0, device="cuda")
+    for C, ptr in itertools.product((16, 1600), ([5, 2, 40, 10], [-7, 20, 1 << 40, 30], [0, 100, 100, 100000], [60, 50, 40, 30],
+                                                 [90, 90, 90, 90])):
+        arena = torch.full((3, 60, C), 7.0, device="cuda")
         x = arena[1].requires_grad_(True)
         y = F.group_norm(x, 4, ptr=torch.tensor(ptr, device="cuda"))
         torch.autograd.grad(y.sum(), x)
@@ -809,3 +850,26 @@ def test_on_another_stream():
         got = F.linear(F.dropout(F.group_norm(X, 4, activation="gelu"), 0.3, 1), W)
     s.synchronize()
     assert torch.equal(got, want)
+
+
+@gpu
+def test_two_streams_at_once():
+    """Calls of the same operators that overlap on two streams do not see one another."""
+    data = [(normal((4000, 96), q, torch.float32).cuda(), normal((96, 120), q + 9, torch.float32).cuda()) for q in range(2)]
+    dY = normal((4000, 120), 5, torch.float32).cuda()
+
+    def step(X, W):
+        x, w = X.detach().requires_grad_(True), W.detach().requires_grad_(True)
+        y = F.group_norm(F.linear(F.dropout(x, 0.2, 4), w, activation="gelu"), 8)
+        return [y.detach(), *torch.autograd.grad(y, (x, w), dY)]
+
+    want = [step(*d) for d in data]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [None, None]
+    for _ in range(5):
+        for q in range(2):
+            with torch.cuda.stream(streams[q]):
+                got[q] = step(*data[q])
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(a, b) for a, b in zip(w, g))
