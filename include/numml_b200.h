@@ -616,7 +616,8 @@ typedef enum {
  * receives x w + bias, [m, n] contiguous, which the backward pass reads when there is an activation.
  *
  * Backward, dz = dy act'(z):  dx = dz w^T [m, k],  dw = x^T dz [k, n],  dbias = column sums of dz [n], each
- * contiguous and each skipped when NULL; the residual's gradient is dy itself.  z may be NULL for NB200_ACT_NONE.
+ * contiguous and each skipped when NULL; the residual's gradient is dy itself.  float factors below 2^-102 may count
+ * as up to 2^-125 less than they are (their low-order pieces are below the smallest normal number).  z may be NULL for NB200_ACT_NONE.
  * `status` (device word, may be NULL) receives NB200_ERR_WAIT_BUDGET if a bounded wait of a kernel ever runs out.
  * No alignment is required of any array but `work` (16 bytes); aligned rows are read faster.  Results do not depend on the run: sums are cut at
  * places that depend on the sizes alone and joined in order. */

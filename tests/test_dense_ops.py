@@ -238,14 +238,15 @@ def test_linear_infinities_and_nan_stay_in_their_rows_and_columns(m, dtype):
 @pytest.mark.parametrize("m", [100, 600])
 @pytest.mark.parametrize("power", [-36, -38, 37])
 def test_linear_float32_ends_of_the_range(power, m):
-    """Values whose low-order pieces are subnormal in 16 bits, and values near the largest: products with weights near
-    one keep float32's error relative to the sum of magnitudes, down to the spacing of the smallest normal number."""
+    """Values whose low-order pieces are subnormal in 16 bits, and values near the largest.  A piece below 2^-126 counts
+    as zero, so of a value at most 2^-126 is lost per piece: two pieces of x times |w|, and two of w times |x|."""
     X = (normal((m, 40), 1, torch.float64) * 10.0 ** power).float()
     W = normal((40, 70), 2, torch.float32, 0.5)
     ref, mag = X.double() @ W.double(), X.double().abs() @ W.double().abs()
     keep = mag < 3e38
     y = F.linear(X.cuda(), W.cuda()).cpu().double()
-    bound = 2 * 42 * units(torch.float32)[1] * mag + 40 * torch.finfo(torch.float32).tiny * 2 ** -23
+    lost = 2.0 ** -125 * (W.double().abs().sum(0)[None, :] + X.double().abs().sum(1)[:, None] + 40)
+    bound = 2 * 42 * units(torch.float32)[1] * mag + lost
     assert ((y - ref).abs() <= bound)[keep].all(), ((y - ref).abs() / bound)[keep].max()
 
 
