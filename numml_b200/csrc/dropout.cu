@@ -11,6 +11,10 @@
 // that equals T's high half, which happens once in 65536 elements; only then is stream 1 evaluated.  So
 // one generator call serves eight elements (with a word per element the ten rounds would cost as much
 // issue time as the bytes of a 16-bit type take to arrive) while p keeps a resolution of 2^-32.
+//
+// Measured (a pass; copy 6548 GB/s): 14.6 M doubles 37 us = 6.3 TB/s (0.96); 67 M bfloat16 with a residual 69 us = 5.8 TB/s
+// (0.89), without 64 us = 4.2 TB/s: for two bytes each way the generator's instructions are the bound (61 % of the issue
+// slots, the rest waits for the multiplier).
 #include <cmath>
 #include <type_traits>
 

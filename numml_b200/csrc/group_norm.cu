@@ -14,6 +14,10 @@
 // Variances come from differences: a thread sums (x - k) and (x - k)^2 with k the first value it meets
 // of its channel in the piece, and partial results are joined as (count, mean, sum of squared
 // deviations), the join over pieces in 64 bits.  E[x^2] - E[x]^2 never appears.
+//
+// Measured on a million rows of 128 floats in 32 groups, silu (537 MB an array; copy 6548 GB/s): stats 104 us = 5.2 TB/s,
+// apply 173 us = 6.2, gradient sums 204 us = 5.3, gradient 265 us = 6.1, joins 6-10 us each: bound by memory.  An array
+// that does not fit on chip is read twice in each direction.
 #include "dense_common.cuh"
 
 namespace nb200 {

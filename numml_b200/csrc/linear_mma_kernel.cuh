@@ -20,6 +20,13 @@
 // order of size, the twenty small ones first, where a truncation weighs 2^-8 as much, then the four of the leading
 // pieces, and the sums over chunks are formed by the epilogue warps with rounding to nearest (the running sums
 // stay in tensor memory).
+//
+// Measured on a B200 (copy 6548 GB/s, dense bfloat16 1651 TFLOP/s; cold L2): float, a million rows of 128 -> 128: plain
+// forward 220 us = 4.9 TB/s, with silu and z kept 345 us = 4.7 TB/s, dx 177 us = 6.1 TB/s, dw 225 us = 4.8 TB/s: the
+// epilogue's instructions and the shared-memory traffic of six products take turns with memory as the bound.  65,536 x
+// 1024 -> 1024: 773 us = 178 TFLOP/s of float, 1.07 PFLOP/s of products (0.65).  bfloat16, a million rows of 128 -> 128:
+// 86 us = 6.2 TB/s; 131,072 x 512 -> 512: 107 us, bound by L2 reads of the first operand, once per column of tiles;
+// 16,384 x 4096 -> 4096: 600 us = 0.92 PFLOP/s (0.56).
 #pragma once
 #include <cuda.h>
 
