@@ -738,7 +738,7 @@ int64_t block_count(int64_t rows) {
 // long a segment is, take over.  Slabs are made narrower (whole groups) while there are fewer than eight blocks for
 // every SM, down to rows of 64 bytes, or fewer than two, down to 32.  Measured on 512 graphs of 1 to 1076 rows, mean
 // 118, x 128 bfloat16 channels with gelu, forward / backward: slabs of 128 channels 46 / 100 us, 64: 32 / 65, 32: 31 /
-// 57 (the longest graph's arithmetic on one SM is what is left; clusters of 2 to 8 blocks per graph, which split it,
+// 57, with four channels to a thread 31 / 51 (the longest graph's arithmetic on one SM is what is left; clusters of 2 to 8 blocks per graph, which split it,
 // were no faster: 34-41 / 67-72); the row chunks 82 / 117 us in six launches.
 bool short_segments(int64_t rows, int64_t channels, int64_t groups, int64_t segments, size_t size, int V, Slab* slab) {
     if (segments < 1 || segments > 65535 * 16) return false;
@@ -786,15 +786,18 @@ bool bad_shape(int64_t rows, int64_t channels, int64_t groups, int64_t segments,
 struct Launch {
     Shape sh;
     dim3 grid;
-    bool vector;
 };
 
+// Channels of a thread.  16-bit types: four, where a thread of eight would hold so much that too few are resident
+// (a million rows of 128 bfloat16 forward 199 us against 234; the batch of short graphs backward 51 against 57), but
+// eight in the backward pass over row chunks (392 us against 449).
 template <typename T>
+constexpr int few_channels() { return sizeof(T) == 2 ? 4 : 16 / sizeof(T); }
+
+template <int V>
 Launch make_launch(int64_t rows, int64_t channels, int64_t groups, int64_t segments, const int64_t* ptr) {
     Launch l;
-    constexpr int V = 16 / sizeof(T);
-    l.vector = channels % V == 0;
-    const int vectors = static_cast<int>(l.vector ? channels / V : channels);
+    const int vectors = static_cast<int>(channels / V);
     const int64_t blocks = block_count(rows), chunk = ceil_div(rows, blocks);
     const int lanes = vectors < kThreads ? vectors : kThreads;
     l.sh = {rows, chunk, static_cast<int>(channels), static_cast<int>(groups), lanes, segments, ptr,
@@ -829,23 +832,25 @@ int forward(const Launch& l, const T* x, const T* w, const T* b, double eps, int
 }
 
 template <typename T, int V>
-int backward(const Launch& l, const T* dy, const T* x, const T* w, const T* b, const acc_t<T>* mean, const acc_t<T>* rstd, int act,
+int backward_short(const Launch& l, Slab slab, const T* dy, const T* x, const T* w, const T* b, const acc_t<T>* mean, const acc_t<T>* rstd,
+                   int act, T* dx, T* dw, T* db, acc_t<T>* part, cudaStream_t stream) {
+    slab.pad_blocks = l.sh.ptr && dx ? kSMs / 4 : 0;
+    const dim3 grid(static_cast<unsigned>(l.sh.segments + slab.pad_blocks), static_cast<unsigned>(l.sh.channels / slab.channels));
+    const int rc = l.sh.channels / l.sh.groups % V == 0
+                       ? NB200_DISPATCH_ACT(act, (short_backward_kernel<T, V, ACT, true><<<grid, kShort, 0, stream>>>(
+                                                      l.sh, slab, x, dy, w, b, mean, rstd, part, dx), launch_status()))
+                       : NB200_DISPATCH_ACT(act, (short_backward_kernel<T, V, ACT, false><<<grid, kShort, 0, stream>>>(
+                                                      l.sh, slab, x, dy, w, b, mean, rstd, part, dx), launch_status()));
+    if (rc != NB200_OK || !(dw || db)) return rc;
+    column_sums_kernel<T><<<static_cast<unsigned>(ceil_div(2 * l.sh.channels, 32)), 1024, 0, stream>>>(l.sh.segments, l.sh.channels, part, db,
+                                                                                                     dw);
+    return launch_status();
+}
+
+template <typename T, int V>
+int backward_chunks(const Launch& l, const T* dy, const T* x, const T* w, const T* b, const acc_t<T>* mean, const acc_t<T>* rstd, int act,
              T* dx, T* dw, T* db, acc_t<T>* part, cudaStream_t stream) {
     using A = acc_t<T>;
-    Slab slab;
-    if (short_segments(l.sh.rows, l.sh.channels, l.sh.groups, l.sh.segments, sizeof(T), V, &slab)) {
-        slab.pad_blocks = l.sh.ptr && dx ? kSMs / 4 : 0;
-        const dim3 grid(static_cast<unsigned>(l.sh.segments + slab.pad_blocks), static_cast<unsigned>(l.sh.channels / slab.channels));
-        const int rc = l.sh.channels / l.sh.groups % V == 0
-                           ? NB200_DISPATCH_ACT(act, (short_backward_kernel<T, V, ACT, true><<<grid, kShort, 0, stream>>>(
-                                                          l.sh, slab, x, dy, w, b, mean, rstd, part, dx), launch_status()))
-                           : NB200_DISPATCH_ACT(act, (short_backward_kernel<T, V, ACT, false><<<grid, kShort, 0, stream>>>(
-                                                          l.sh, slab, x, dy, w, b, mean, rstd, part, dx), launch_status()));
-        if (rc != NB200_OK || !(dw || db)) return rc;
-        column_sums_kernel<T><<<static_cast<unsigned>(ceil_div(2 * l.sh.channels, 32)), 1024, 0, stream>>>(l.sh.segments, l.sh.channels, part,
-                                                                                                         db, dw);
-        return launch_status();
-    }
     A* block_sums = part + part_elements(l.sh.rows, l.sh.channels, l.sh.segments);
     A* coef = block_sums + size_t(block_count(l.sh.rows)) * 2 * l.sh.channels;
     int rc = NB200_DISPATCH_ACT(act, (grad_sums_kernel<T, V, ACT><<<l.grid, kThreads, 0, stream>>>(l.sh, x, dy, w, b, mean, rstd, part,
@@ -896,13 +901,14 @@ extern "C" int nb200_group_norm_forward(int64_t rows, int64_t channels, int64_t 
     }
     return NB200_DISPATCH_DENSE(dtype, ([&]() -> int {
         using A = acc_t<T>;
-        const Launch l = make_launch<T>(rows, channels, groups, segments, ptr);
         const T *xt = static_cast<const T*>(x), *wt = static_cast<const T*>(weight), *bt = static_cast<const T*>(bias);
         A *m = static_cast<A*>(mean), *rs = static_cast<A*>(rstd), *part = static_cast<A*>(work);
         T* yt = static_cast<T*>(y);
-        constexpr int V = 16 / sizeof(T);
-        return l.vector ? forward<T, V>(l, xt, wt, bt, eps, activation, yt, m, rs, part, as_stream(stream))
-                        : forward<T, 1>(l, xt, wt, bt, eps, activation, yt, m, rs, part, as_stream(stream));
+        constexpr int V = few_channels<T>();
+        return channels % V == 0 ? forward<T, V>(make_launch<V>(rows, channels, groups, segments, ptr), xt, wt, bt, eps, activation, yt, m, rs,
+                                                 part, as_stream(stream))
+                                 : forward<T, 1>(make_launch<1>(rows, channels, groups, segments, ptr), xt, wt, bt, eps, activation, yt, m, rs,
+                                                 part, as_stream(stream));
     }()));
 }
 
@@ -924,14 +930,24 @@ extern "C" int nb200_group_norm_backward(int64_t rows, int64_t channels, int64_t
     if (!aligned16(x) || !aligned16(dy) || !aligned16(work) || (dx && !aligned16(dx))) return NB200_ERR_ALIGN;
     return NB200_DISPATCH_DENSE(dtype, ([&]() -> int {
         using A = acc_t<T>;
-        const Launch l = make_launch<T>(rows, channels, groups, segments, ptr);
         const T *xt = static_cast<const T*>(x), *gt = static_cast<const T*>(dy), *wt = static_cast<const T*>(weight),
                 *bt = static_cast<const T*>(bias);
         const A *m = static_cast<const A*>(mean), *rs = static_cast<const A*>(rstd);
         A* part = static_cast<A*>(work);
         T *dxt = static_cast<T*>(dx), *dwt = static_cast<T*>(dweight), *dbt = static_cast<T*>(dbias);
-        constexpr int V = 16 / sizeof(T);
-        return l.vector ? backward<T, V>(l, gt, xt, wt, bt, m, rs, activation, dxt, dwt, dbt, part, as_stream(stream))
-                        : backward<T, 1>(l, gt, xt, wt, bt, m, rs, activation, dxt, dwt, dbt, part, as_stream(stream));
+        constexpr int V = few_channels<T>(), W = 16 / sizeof(T);
+        Slab slab;
+        if (channels % V == 0) {
+            if (short_segments(rows, channels, groups, segments, sizeof(T), V, &slab))
+                return backward_short<T, V>(make_launch<V>(rows, channels, groups, segments, ptr), slab, gt, xt, wt, bt, m, rs, activation, dxt,
+                                            dwt, dbt, part, as_stream(stream));
+        } else if (short_segments(rows, channels, groups, segments, sizeof(T), 1, &slab)) {
+            return backward_short<T, 1>(make_launch<1>(rows, channels, groups, segments, ptr), slab, gt, xt, wt, bt, m, rs, activation, dxt,
+                                        dwt, dbt, part, as_stream(stream));
+        }
+        return channels % W == 0 ? backward_chunks<T, W>(make_launch<W>(rows, channels, groups, segments, ptr), gt, xt, wt, bt, m, rs, activation,
+                                                         dxt, dwt, dbt, part, as_stream(stream))
+                                 : backward_chunks<T, 1>(make_launch<1>(rows, channels, groups, segments, ptr), gt, xt, wt, bt, m, rs, activation,
+                                                         dxt, dwt, dbt, part, as_stream(stream));
     }()));
 }
