@@ -738,8 +738,8 @@ int64_t block_count(int64_t rows) {
 // long a segment is, take over.  Slabs are made narrower (whole groups) while there are fewer than eight blocks for
 // every SM, down to rows of 64 bytes, or fewer than two, down to 32.  Measured on 512 graphs of 1 to 1076 rows, mean
 // 118, x 128 bfloat16 channels with gelu, forward / backward: slabs of 128 channels 46 / 100 us, 64: 32 / 65, 32: 31 /
-// 57, with four channels to a thread 31 / 51 (the longest graph's arithmetic on one SM is what is left; clusters of 2 to 8 blocks per graph, which split it,
-// were no faster: 34-41 / 67-72); the row chunks 82 / 117 us in six launches.
+// 57, with four channels to a thread 31 / 51 (the longest graph's arithmetic on one SM is what is left; clusters of 2 to
+// 8 blocks per graph, which split it, were no faster: 34-41 / 67-72); the row chunks 82 / 117 us in six launches.
 bool short_segments(int64_t rows, int64_t channels, int64_t groups, int64_t segments, size_t size, int V, Slab* slab) {
     if (segments < 1 || segments > 65535 * 16) return false;
     const int64_t width = channels / groups;

@@ -5,7 +5,9 @@
 
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 
 #include "../../include/numml_b200.h"
 
@@ -100,6 +102,28 @@ struct Needs {
     bool operator()(bool present) { return present && ctx->needs_input_grad(next++); }
 };
 
+// A backward pass under capture may not hand a gradient to a leaf that a live eager graph holds on another stream: the
+// engine would make that stream wait for the capture, which invalidates it or ends the process.  Raised here instead.
+void refuse_foreign_accumulation() {
+    const auto current = at::cuda::getCurrentCUDAStream();
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(current, &capturing) != cudaSuccess || capturing == cudaStreamCaptureStatusNone) return;
+    const auto node = torch::autograd::get_current_node();
+    if (!node) return;
+    const auto* info = torch::autograd::get_current_graph_task_exec_info();
+    for (const auto& edge : node->next_edges()) {
+        if (!edge.is_valid() || dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get()) == nullptr) continue;
+        if (info != nullptr && !info->empty()) {                 // torch.autograd.grad: only the leaves that were asked for
+            const auto it = info->find(edge.function.get());
+            if (it == info->end() || !it->second.should_execute()) continue;
+        }
+        const auto stream = edge.function->stream();
+        TORCH_CHECK(!stream.has_value() || *stream == current.unwrap(),
+                    "a backward pass is being captured into a CUDA graph while an eager graph of the same leaf is alive on another "
+                    "stream; drop the eager results first, or make the leaf inside the capture");
+    }
+}
+
 // ---- linear ---------------------------------------------------------------------------------------------
 std::pair<Tensor, Tensor> linear_forward(const Tensor& X, const Tensor& W, const Tensor& bias, const Tensor& residual, int act, bool keep_z) {
     const int64_t M = row_count(X), K = W.size(0), N = W.size(1);
@@ -125,6 +149,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        refuse_foreign_accumulation();
         const auto saved = ctx->get_saved_variables();
         const Tensor &X = saved[0], &W = saved[1], &z = saved[2], &dY = grads[0];
         const int act = static_cast<int>(ctx->saved_data["act"].toInt());
@@ -198,6 +223,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        refuse_foreign_accumulation();
         const auto saved = ctx->get_saved_variables();
         const Tensor &X = saved[0], &stats = saved[4];
         const int64_t groups = ctx->saved_data["groups"].toInt();
@@ -270,6 +296,7 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
         return dropout_run(X, p, static_cast<uint64_t>(seed), static_cast<uint64_t>(offset), or_empty(state), or_empty(residual));
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        refuse_foreign_accumulation();
         const Tensor state = ctx->get_saved_variables()[0];
         Tensor dx;
         Needs needs{ctx};

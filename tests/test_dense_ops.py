@@ -841,6 +841,38 @@ def test_captured_and_replayed():
 
 
 @gpu
+def test_capture_beside_a_live_eager_graph(shim):
+    """A captured backward pass into leaves that a live eager graph holds on another stream raises and leaves the capture
+    intact (the compiled path alone can ask the engine what it is about to run)."""
+    if shim == "python":
+        return
+    x = normal((700, 32), 1, torch.float32).cuda().requires_grad_(True)
+    w = normal((32, 48), 2, torch.float32).cuda().requires_grad_(True)
+    alive = F.linear(x, w, activation="gelu")
+    torch.cuda.synchronize()
+    for make in (lambda: F.linear(x, w), lambda: F.dropout(x, 0.5, 1), lambda: F.group_norm(x, 4)):
+        for backward in (lambda y: y.backward(torch.ones_like(y)), lambda y: torch.autograd.grad(y, x, torch.ones_like(y))):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                y = make()
+                with pytest.raises(RuntimeError, match="eager graph of the same leaf"):
+                    backward(y)
+                y = y.detach() + 1
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, make().detach() + 1)
+    assert x.grad is None and w.grad is None
+    del alive, y
+    x2 = x.detach().requires_grad_(True)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):                                     # with no eager graph of the leaf the same capture works
+        (dx,) = torch.autograd.grad(F.linear(x2, w.detach()), x2, torch.ones(700, 48, device="cuda"))
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(dx, torch.autograd.grad(F.linear(x2, w.detach()), x2, torch.ones(700, 48, device="cuda"))[0])
+
+
+@gpu
 def test_on_another_stream():
     X = normal((500, 64), 1, torch.float32).cuda()
     W = normal((64, 48), 2, torch.float32).cuda()
