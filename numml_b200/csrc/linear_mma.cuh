@@ -15,10 +15,22 @@ struct Epilogue {
     acc_t<T>* partial;    // instead of all of the above: [splits, rows, cols]
 };
 
-// z as the backward pass will read it.  Rounding to 16 bits keeps the sign, which is all that relu's slope
-// needs, except that a positive z below half the smallest fp16 number would become zero.
+// The largest finite number of a 16-bit type.
+template <typename T> __device__ __forceinline__ float largest_finite();
+template <> __device__ __forceinline__ float largest_finite<__nv_bfloat16>() { return 3.3895313892515355e38f; }
+template <> __device__ __forceinline__ float largest_finite<__half>() { return 65504.f; }
+
+// Whether the slope of an activation is a number times z: at an infinity it is then 0 * infinity.
+template <int ACT> constexpr bool slope_has_z() { return ACT == NB200_ACT_SILU || ACT == NB200_ACT_GELU; }
+
+// z as the backward pass will read it, one rounding of the 32-bit value that the activation was applied to.  A finite z
+// stays finite in 16 bits: beyond their range the slopes are constant, so the largest number stands for it, where an
+// infinity would make a NaN.  For relu only the sign counts, and rounding keeps it, except that a positive z below half
+// the smallest fp16 number would become zero.
 template <typename T, int ACT>
 __device__ __forceinline__ T rounded_z(acc_t<T> v) {
+    if constexpr (slope_has_z<ACT>() && sizeof(T) == 2)
+        if (isfinite(v)) v = fminf(fmaxf(v, -largest_finite<T>()), largest_finite<T>());
     T r = from_acc<T>(v);
     if constexpr (ACT == NB200_ACT_RELU && sizeof(T) == 2)
         if (v > 0.f && to_acc(r) == 0.f) r = from_acc<T>(5.9604644775390625e-8f);   // 2^-24, representable in both types

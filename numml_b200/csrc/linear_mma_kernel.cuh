@@ -452,15 +452,15 @@ __device__ __forceinline__ void pack_line(const float (&s)[64], uint32_t (&w)[32
         w[q] = *reinterpret_cast<const uint32_t*>(&r);
     }
 }
-// Value q (0..3 or 0..7) of a 16-byte unit.
-__device__ __forceinline__ float unit_value(const uint32_t (&w)[4], int q, float) { return __uint_as_float(w[q]); }
-__device__ __forceinline__ float unit_value(const uint32_t (&w)[4], int q, __nv_bfloat16) {
-    return __uint_as_float(q & 1 ? w[q / 2] & 0xFFFF0000u : w[q / 2] << 16);
-}
-__device__ __forceinline__ float unit_value(const uint32_t (&w)[4], int q, __half) {
-    const __half2 h = *reinterpret_cast<const __half2*>(&w[q / 2]);
+// Half q % 2 of a word of two values, value q (0..3 or 0..7) of a 16-byte unit.
+__device__ __forceinline__ float unit_value(uint32_t w, int q, __nv_bfloat16) { return __uint_as_float(q & 1 ? w & 0xFFFF0000u : w << 16); }
+__device__ __forceinline__ float unit_value(uint32_t w, int q, __half) {
+    const __half2 h = *reinterpret_cast<const __half2*>(&w);
     return q & 1 ? __high2float(h) : __low2float(h);
 }
+__device__ __forceinline__ float unit_value(const uint32_t (&w)[4], int q, float) { return __uint_as_float(w[q]); }
+template <typename T>
+__device__ __forceinline__ float unit_value(const uint32_t (&w)[4], int q, T type) { return unit_value(w[q / 2], q, type); }
 __device__ __forceinline__ void shared_store16(uint32_t addr, const uint32_t* w) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" :: "r"(addr), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
 }
@@ -506,6 +506,9 @@ struct Writer {
     __device__ __forceinline__ void close(const float (&s)[CB], O* base, const void* map, int split, int64_t row0, int64_t col0) const {
         uint32_t w[32];
         pack_line(s, w, O());
+        send(w, base, map, split, row0, col0);
+    }
+    __device__ __forceinline__ void send(const uint32_t (&w)[32], O* base, const void* map, int split, int64_t row0, int64_t col0) const {
 #pragma unroll
         for (int u = 0; u < 8; ++u) shared_store16(place(lane, u), w + 4 * u);
         if (g.tiled_out) {
@@ -561,11 +564,22 @@ struct Writer {
             }
             if constexpr (KIND == kForwardZ) {
                 open();
-                if constexpr (ACT == NB200_ACT_RELU && sizeof(T) == 2) {   // only relu's slope needs more than the rounded value
+                if constexpr (ACT == NB200_ACT_RELU && sizeof(T) == 2) {   // relu's slope needs more than the rounded value
                     float t[CB];
 #pragma unroll
                     for (int q = 0; q < CB; ++q) t[q] = to_acc(rounded_z<T, ACT>(v[q]));
                     close(t, ep.z, map_z, 0, row0, col0);
+                } else if constexpr (slope_has_z<ACT>() && sizeof(T) == 2) {
+                    uint32_t w[32];
+                    pack_line(v, w, O());
+                    float most = 0.f;
+#pragma unroll
+                    for (int q = 0; q < CB; ++q) most = fmaxf(most, fabsf(v[q]));
+                    if (most > largest_finite<T>())          // hardly ever; the bits of the largest number are those of infinity less one
+#pragma unroll
+                        for (int q = 0; q < CB; ++q)
+                            if (isfinite(v[q]) && isinf(unit_value(w[q / 2], q, O()))) w[q / 2] -= q & 1 ? 0x10000u : 1u;
+                    send(w, ep.z, map_z, 0, row0, col0);
                 } else {
                     close(v, ep.z, map_z, 0, row0, col0);
                 }
