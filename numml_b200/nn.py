@@ -137,7 +137,11 @@ class Dropout(torch.nn.Module):
     ``seed`` (drawn from torch's generator when None) and a counter of the calls made so far name the mask.
     They live on the host, where a captured CUDA graph would freeze them, so a call under capture raises
     unless the layer was made with ``capturable=True``: then they are a buffer on the device that every
-    call advances, and a replayed graph takes new masks."""
+    call advances, and a replayed graph takes new masks.
+
+    A forward pass that is run again inside the backward pass (``torch.utils.checkpoint``) has to see the mask of
+    the first run, and the layer cannot tell which call that was.  Take ``call = layer.next_call()`` in front of the
+    recomputed region and call ``layer(A, X, call)`` inside it; a call of the layer that names no mask raises there."""
 
     def __init__(self, p=0.5, seed=None, capturable=False):
         super().__init__()
@@ -153,18 +157,33 @@ class Dropout(torch.nn.Module):
         else:
             self.state = None
 
-    def forward(self, A, X):
-        if not self.training:
-            return X
+    def _refuse_capture(self):
+        if self.state is None and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("Dropout under CUDA graph capture needs capturable=True: "
+                               "the captured graph would repeat one mask for ever")
+
+    def next_call(self):
+        """The name of the next call's mask (a number, or the words [seed, number] on the device); counts the call."""
+        self._refuse_capture()
         if self.state is None:
-            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("Dropout under CUDA graph capture needs capturable=True: "
-                                   "the captured graph would repeat one mask for ever")
             self.calls += 1
-            return F.dropout(X, self.p, self.seed, self.calls - 1)
+            return self.calls - 1
         now = self.state.clone()
         self.state[1] += 1
-        return F.dropout(X, self.p, now)
+        return now
+
+    def forward(self, A, X, call=None):
+        """call: what ``next_call`` gave, or None for a mask of its own."""
+        if not self.training:
+            return X
+        if call is None:
+            if torch._C._current_graph_task_id() != -1:
+                raise RuntimeError("Dropout is being run inside a backward pass, as a recomputed forward pass is, where another mask "
+                                   "would belong to the gradients than to the output; take call = layer.next_call() in front of "
+                                   "the recomputed region and give it to the layer: layer(A, X, call)")
+            call = self.next_call()
+        self._refuse_capture()
+        return F.dropout(X, self.p, call) if isinstance(call, torch.Tensor) else F.dropout(X, self.p, self.seed, call)
 
 
 class SeqWrapper(torch.nn.Module):

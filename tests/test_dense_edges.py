@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import numml_b200.functional as F
+import numml_b200.nn as nn
 from numml_b200 import numml_torch_cpp
 from test_dense_ops import CURVE, act64, check, normal, tiny, units
 
@@ -66,3 +67,54 @@ def test_linear_backward_beyond_the_range_of_16_bits(m, n, act, dtype, big):
         assert y[1, 5] == -1 and y[2, 5] == 1
     else:
         assert y[1, 5] == 0 and y[2, 5] == math.inf
+
+
+# ---------------------------------------------------------------------------------------------------------
+# forward passes that are run again in order to be differentiated
+# ---------------------------------------------------------------------------------------------------------
+def _dropout_on_the_host(X, p, seed, offset=0, residual=None):
+    """A stand-in for the kernel: another mask for another (seed, offset)."""
+    if isinstance(seed, torch.Tensor):
+        seed, offset = seed.tolist()
+    gen = torch.Generator().manual_seed(seed * 1000 + offset)
+    return X * (torch.rand(X.shape, generator=gen, dtype=X.dtype) >= p)
+
+
+def _checkpointed_mask(drop, X, use_reentrant, named):
+    """Masks of the output and of the gradient of x -> dropout(x) in a checkpointed region, for two regions in turn."""
+    from torch.utils.checkpoint import checkpoint
+    masks = []
+    for _ in range(2):
+        x = X.detach().requires_grad_(True)
+        call = drop.next_call() if named else None
+        y = checkpoint(lambda t: drop(None, t, call) * t.detach(), x, use_reentrant=use_reentrant)
+        y.sum().backward()
+        masks.append((y.detach() != 0, x.grad != 0))
+    return masks
+
+
+@pytest.mark.parametrize("use_reentrant", [False, True])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_dropout_recomputed_on_the_host(use_reentrant, capturable, monkeypatch):
+    monkeypatch.setattr(nn.F, "dropout", _dropout_on_the_host)
+    drop = nn.Dropout(0.5, seed=11, capturable=capturable)
+    X = torch.ones(40, 5)
+    (y0, g0), (y1, g1) = _checkpointed_mask(drop, X, use_reentrant, True)
+    assert torch.equal(y0, g0) and torch.equal(y1, g1) and not torch.equal(y0, y1)
+    with pytest.raises(RuntimeError, match="next_call"):
+        _checkpointed_mask(drop, X, use_reentrant, False)
+    want = _dropout_on_the_host(X, 0.5, 11, 3) != 0            # the refused call has advanced the counter once, in its forward pass
+    assert torch.equal(drop(None, X) != 0, want)
+
+
+@gpu
+@pytest.mark.parametrize("use_reentrant", [False, True])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_dropout_recomputed(use_reentrant, capturable):
+    drop = nn.Dropout(0.5, seed=11, capturable=capturable).cuda()
+    X = normal((300, 17), 1, torch.float32).cuda().abs() + 1
+    (y0, g0), (y1, g1) = _checkpointed_mask(drop, X, use_reentrant, True)
+    assert torch.equal(y0, g0) and torch.equal(y1, g1) and not torch.equal(y0, y1)
+    assert torch.equal(y1, F.dropout(X, 0.5, 11, 1) != 0)
+    with pytest.raises(RuntimeError, match="next_call"):
+        _checkpointed_mask(drop, X, use_reentrant, False)
