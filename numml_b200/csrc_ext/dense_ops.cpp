@@ -4,6 +4,7 @@
 #include "dense_ops.h"
 
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -64,6 +65,12 @@ int64_t row_count(const Tensor& X) {
 }
 Tensor or_empty(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 Tensor contiguous_or_empty(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+// Tangents of forward-mode differentiation are refused: no operator passes them on, and a result without one reads as zero.
+void refuse_tangents(std::initializer_list<std::reference_wrapper<const Tensor>> operands) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor& t : operands)
+        TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), "the dense operators have no forward-mode derivative; an operand carries a tangent");
+}
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
 // One int32 device word per GPU into which kernels with bounded waits report a failure.
@@ -188,6 +195,7 @@ Tensor linear(const Tensor& X, const Tensor& W, const OptTensor& bias_, const Op
         for (int64_t d = 0; same && d + 1 < X.dim(); ++d) same = residual.size(d) == X.size(d);
         TORCH_CHECK(same, "residual must have the output's shape ", X.sizes().slice(0, X.dim() - 1), " + ", W.size(1), ", got ", residual.sizes());
     }
+    refuse_tangents({X, W, bias, residual});
     if (at::GradMode::is_enabled() && (wants_grad(X) || wants_grad(W) || wants_grad(bias) || wants_grad(residual)))
         return LinearNode::apply(X, W, option(bias), option(residual), act);
     return linear_forward(X, W, bias, residual, static_cast<int>(act), false).first;
@@ -270,6 +278,7 @@ Tensor group_norm(const Tensor& X, int64_t groups, const OptTensor& weight_, con
                     "ptr must be a 1-D int64 tensor of graphs + 1 row numbers, got ", p.scalar_type(), " ", p.sizes());
         TORCH_CHECK(X.dim() == 2, "with ptr the features must be [nodes, channels], got ", X.sizes());
     }
+    refuse_tangents({X, weight, bias});
     if (at::GradMode::is_enabled() && (wants_grad(X) || wants_grad(weight) || wants_grad(bias)))
         return NormNode::apply(X, option(weight), option(bias), option(p), groups, eps, act);
     return norm_forward(X, groups, weight, bias, eps, static_cast<int>(act), p).first;
@@ -322,6 +331,7 @@ Tensor dropout(const Tensor& X, double p, uint64_t seed, uint64_t offset, const 
         TORCH_CHECK(state.scalar_type() == at::kLong && state.dim() == 1 && state.numel() == 2 && state.is_contiguous(),
                     "a seed tensor must hold two int64 words [seed, offset], got ", state.scalar_type(), " ", state.sizes());
     }
+    refuse_tangents({X, residual});
     if (at::GradMode::is_enabled() && (wants_grad(X) || wants_grad(residual)))
         return DropoutNode::apply(X, option(residual), option(state), p, static_cast<int64_t>(seed), static_cast<int64_t>(offset));
     return dropout_run(X, p, seed, offset, state, residual);

@@ -9,7 +9,7 @@ channels-last, ``[nodes, channels]``; a batch of graphs is a concatenation of th
 array.  Values are float32, float64, bfloat16 or float16 (one type per call); sums, statistics and
 activations are held in 32 bits (64 for float64) and every result is rounded once.  All tensors are on
 one CUDA device (there is no CPU path); calls run on that device's current stream.  Results do not
-depend on the run: no operator adds with atomics.
+depend on the run: no operator adds with atomics.  Gradients of gradients and forward-mode tangents are refused.
 
 Calls go through the compiled extension (``csrc_ext/dense_ops.cpp``) when it has been built; the Python
 functions below do the same work otherwise, with identical results (see
@@ -18,6 +18,7 @@ functions below do the same work otherwise, with identical results (see
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _cabi, numml_torch_cpp
@@ -79,6 +80,15 @@ def _status_pointer(dev):
     if key not in numml_torch_cpp._status_words and torch.cuda.is_current_stream_capturing():
         return None
     return _ptr(_status_word(dev))
+
+
+def _refuse_tangents(*tensors):
+    """Tangents of forward-mode differentiation: no operator passes them on, and a result without one reads as zero."""
+    if not torch._C._is_fwd_grad_enabled() or forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("the dense operators have no forward-mode derivative; an operand carries a tangent")
 
 
 def _wants_grad(*tensors):
@@ -163,6 +173,7 @@ def linear(X, weights, bias=None, activation=None, residual=None):
     out_shape = tuple(X.shape[:-1]) + (weights.shape[1],)
     if residual is not None and tuple(residual.shape) != out_shape:
         raise RuntimeError(f"residual must have the output's shape {out_shape}, got {tuple(residual.shape)}")
+    _refuse_tangents(X, weights, bias, residual)
     if _wants_grad(X, weights, bias, residual):
         return linear_fn.apply(X, weights, bias, residual, act)
     return _linear_forward(X, weights, bias, residual, act, False)[0]
@@ -264,6 +275,7 @@ def group_norm(X, groups, weight=None, bias=None, eps=1e-5, activation=None, ptr
             raise RuntimeError(f"ptr must be a 1-D int64 tensor of graphs + 1 row numbers, got {ptr.dtype} {tuple(ptr.shape)}")
         if X.ndim != 2:
             raise RuntimeError(f"with ptr the features must be [nodes, channels], got {tuple(X.shape)}")
+    _refuse_tangents(X, weight, bias)
     if _wants_grad(X, weight, bias):
         return group_norm_fn.apply(X, weight, bias, ptr, groups, eps, act)
     return _group_norm_forward(X, groups, weight, bias, eps, act, ptr)[0]
@@ -332,6 +344,7 @@ def dropout(X, p, seed, offset=0, residual=None):
         _require_cuda(X, state)
         if state.dtype != torch.int64 or tuple(state.shape) != (2,) or not state.is_contiguous():
             raise RuntimeError(f"a seed tensor must hold two int64 words [seed, offset], got {state.dtype} {tuple(state.shape)}")
+    _refuse_tangents(X, residual)
     if _wants_grad(X, residual):
         return dropout_fn.apply(X, residual, p, seed, offset, state)
     return _dropout_run(X, p, seed, offset, state, residual)

@@ -118,3 +118,22 @@ def test_dropout_recomputed(use_reentrant, capturable):
     assert torch.equal(y1, F.dropout(X, 0.5, 11, 1) != 0)
     with pytest.raises(RuntimeError, match="next_call"):
         _checkpointed_mask(drop, X, use_reentrant, False)
+
+
+@gpu
+@pytest.mark.parametrize("leaf", [False, True])
+def test_forward_mode_tangents_are_refused(leaf):
+    import torch.autograd.forward_ad as fw
+    X, W, v, R = (normal(s, q, torch.float32).cuda() for q, s in enumerate(((20, 8), (8, 8), (8,), (20, 8))))
+    calls = [(X, lambda t: F.linear(t, W)), (W, lambda t: F.linear(X, t)), (v, lambda t: F.linear(X, W, t)),
+             (R, lambda t: F.linear(X, W, residual=t)), (X, lambda t: F.group_norm(t, 2)), (v, lambda t: F.group_norm(X, 2, t)),
+             (v, lambda t: F.group_norm(X, 2, None, t)), (X, lambda t: F.dropout(t, 0.5, 1)), (R, lambda t: F.dropout(X, 0.5, 1, residual=t))]
+    for operand, call in calls:
+        operand = operand.clone().requires_grad_(leaf)
+        with fw.dual_level():
+            dual = fw.make_dual(operand, torch.ones_like(operand))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(dual)
+            with torch.inference_mode():                         # no derivative of any kind is formed there
+                quiet = call(dual)
+            assert torch.equal(quiet, call(operand))             # without a tangent all is as before
