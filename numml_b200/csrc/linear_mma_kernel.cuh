@@ -31,6 +31,7 @@
 #include <cuda.h>
 
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "linear_mma.cuh"
@@ -721,6 +722,17 @@ __device__ __forceinline__ void epilogue_role(const Args<T>& g, const void* map_
     if (threadIdx.x % 32 == 0) tc::stores_done();
 }
 
+// After a wait that ran out: NaN over all that this block was to write, so that nothing passes for a result.  The
+// epilogue warps do it, once all stores are done: the others have given registers away.
+template <typename T, typename O>
+__device__ __forceinline__ void write_nan(const Args<T>& g, O* out) {
+    for (Walk<T> w(g); w.live(); w.next_item()) {
+        const int64_t columns = min(int64_t(kMmaTile), g.cols - w.j0()), rows = min(int64_t(kMmaTile), g.rows - w.i0());
+        O* corner = out + (w.split * g.rows + w.i0()) * g.cols + w.j0();
+        for (int e = threadIdx.x; e < rows * columns; e += kEpilogueWarps * 32) corner[e / columns * g.cols + e % columns] = from_acc<O>(NAN);
+    }
+}
+
 template <typename T, bool A_K, bool B_K, int ACT, int KIND>
 __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant__ Args<T> g,
                                                           const __grid_constant__ CUtensorMap map_a,
@@ -777,7 +789,12 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
     tc::fence_before_sync();
     __syncthreads();
     if (warp == kEpilogueWarps + kLoaderWarps) tc::tmem_dealloc(tmem, kTmemColumns);
-    if (threadIdx.x == 0 && ctl.gave_up && g.status) atomicMax(g.status, static_cast<int>(NB200_ERR_WAIT_BUDGET));
+    if (ctl.gave_up && warp < kEpilogueWarps) {
+        if (threadIdx.x == 0 && g.status) atomicMax(g.status, static_cast<int>(NB200_ERR_WAIT_BUDGET));
+        if constexpr (KIND == kParts) write_nan<T, float>(g, g.ep.partial);
+        else write_nan<T, T>(g, g.ep.y);
+        if constexpr (KIND == kForwardZ) write_nan<T, T>(g, g.ep.z);
+    }
 }
 
 bool multiple_of(size_t bytes, const void* p, int64_t ld, size_t size) {

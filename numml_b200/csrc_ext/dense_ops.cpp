@@ -73,21 +73,36 @@ void refuse_tangents(std::initializer_list<std::reference_wrapper<const Tensor>>
 }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
-// One int32 device word per GPU into which kernels with bounded waits report a failure.
+// The device's int32 status word, into which kernels with bounded waits report a failure and which
+// numml_torch_cpp.check_status reads: the Python module owns one per GPU for good and hands it over at the first call.
+py::function* status_source = nullptr;                   // device index -> tensor; never destroyed, like the words
+
+Tensor* known_status_words() {
+    static Tensor* words = new Tensor[64];               // never destroyed: the context may be gone by then
+    return words;
+}
+
 int32_t* status_word(const Tensor& like) {
     static std::mutex mutex;
-    static std::vector<Tensor>* words = new std::vector<Tensor>(64);      // never destroyed: the context may be gone by then
     const auto device = static_cast<size_t>(like.get_device());
-    if (device >= words->size()) return nullptr;
-    std::lock_guard<std::mutex> lock(mutex);
-    Tensor& w = (*words)[device];
-    if (!w.defined()) {
-        // a capture may not own it: left out until the first call outside one
-        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing(at::cuda::getCurrentCUDAStream(), &capturing) != cudaSuccess || capturing != cudaStreamCaptureStatusNone)
-            return nullptr;
-        w = at::zeros({1}, like.options().dtype(at::kInt));
+    if (device >= 64 || status_source == nullptr) return nullptr;
+    Tensor& w = known_status_words()[device];
+    {
+        std::lock_guard<std::mutex> lock(mutex);
+        if (w.defined()) return w.data_ptr<int32_t>();
     }
+    // a capture may not come to own it: left out until the first call outside one
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(at::cuda::getCurrentCUDAStream(like.get_device()), &capturing) != cudaSuccess ||
+        capturing != cudaStreamCaptureStatusNone)
+        return nullptr;
+    Tensor word;
+    {
+        py::gil_scoped_acquire gil;                      // not under the mutex
+        word = (*status_source)(like.get_device()).cast<Tensor>();
+    }
+    std::lock_guard<std::mutex> lock(mutex);
+    if (!w.defined()) w = word;
     return w.data_ptr<int32_t>();
 }
 
@@ -344,4 +359,6 @@ void register_dense_ops(py::module_& m) {
     m.def("linear", &linear, free_gil);
     m.def("group_norm", &group_norm, free_gil);
     m.def("dropout", &dropout, free_gil);
+    m.def("set_status_source", [](py::function f) { status_source = new py::function(std::move(f)); });
+    m.def("known_status_word", [](int64_t device) { return device >= 0 && device < 64 ? known_status_words()[device] : Tensor(); });
 }

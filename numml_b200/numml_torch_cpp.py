@@ -145,6 +145,7 @@ def compiled_shim():
             mod = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(mod)
             mod.set_planner(_planner)
+            mod.set_status_source(lambda index: _status_word(torch.device("cuda", index)))
             _ext = mod
     return _ext
 

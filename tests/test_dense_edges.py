@@ -137,3 +137,25 @@ def test_forward_mode_tangents_are_refused(leaf):
             with torch.inference_mode():                         # no derivative of any kind is formed there
                 quiet = call(dual)
             assert torch.equal(quiet, call(operand))             # without a tangent all is as before
+
+
+# ---------------------------------------------------------------------------------------------------------
+# waits that run out
+# ---------------------------------------------------------------------------------------------------------
+@gpu
+def test_a_wait_that_ran_out_is_seen_by_check_status(shim):
+    """The kernels of the compiled path report into the word that check_status reads (written here by the host)."""
+    X, W = normal((700, 40), 1, torch.float32).cuda(), normal((40, 24), 2, torch.float32).cuda()
+    want = F.linear(X, W)
+    numml_torch_cpp.check_status()
+    if shim == "compiled":
+        word = numml_torch_cpp.compiled_shim().known_status_word(X.device.index)
+        assert word.data_ptr() == numml_torch_cpp._status_word(X.device).data_ptr()
+    else:
+        word = numml_torch_cpp._status_word(X.device)
+    word.fill_(5)
+    with pytest.raises(RuntimeError, match="status 5"):
+        numml_torch_cpp.check_status()
+    numml_torch_cpp.check_status()                               # read and cleared
+    assert torch.equal(F.linear(X, W), want)
+    numml_torch_cpp.check_status()
