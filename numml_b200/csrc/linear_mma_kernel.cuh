@@ -241,6 +241,11 @@ struct Ring {
             wrapped = true;
         }
     }
+    // Whether slot s has been used, and the parity of its latest use.
+    __device__ __forceinline__ bool used(int s, unsigned& last) const {
+        last = s < slot ? parity : parity ^ 1;
+        return s < slot || wrapped;
+    }
 };
 
 template <typename T, bool A_K, bool B_K>
@@ -261,7 +266,7 @@ __device__ __forceinline__ void load_split(const Args<T>& g, uint32_t a_ring, ui
         }
     }
     for (Ring<Traits<T>::a_slots> ring; w.live(); ring.next()) {
-        if (ring.wrapped && !tc::mbar_wait(&ctl->empty[ring.slot], ring.parity ^ 1, &ctl->gave_up)) return;
+        if (ring.wrapped && !tc::mbar_wait_warp(&ctl->empty[ring.slot], ring.parity ^ 1, &ctl->gave_up)) return;
         ahead.next_chunk();
         if (g.resident && ahead.chunk == 0) ahead_b = false;
         const bool more = ahead.live();
@@ -332,9 +337,14 @@ __device__ __forceinline__ void load_gathered(const Args<T>& g, uint32_t a_ring,
     Walk<T> w(g);
     bool with_b = true;
     for (Ring<Traits<T>::a_slots> ring; w.live(); ring.next()) {
-        if (ring.wrapped && !tc::mbar_wait(&ctl->empty[ring.slot], ring.parity ^ 1, &ctl->gave_up)) return;
-        gather_units<T, A_K>(g.a, a_ring + ring.slot * slot_bytes<T>(), t, w.i0(), w.k0(), w.k_end());
-        if (with_b) gather_units<T, B_K>(g.b, b_ring + (g.resident ? w.chunk : ring.slot) * slot_bytes<T>(), t, w.j0(), w.k0(), w.k_end());
+        const bool ok = !ring.wrapped || tc::mbar_wait(&ctl->empty[ring.slot], ring.parity ^ 1, &ctl->gave_up);
+        if (ok) {
+            gather_units<T, A_K>(g.a, a_ring + ring.slot * slot_bytes<T>(), t, w.i0(), w.k0(), w.k_end());
+            if (with_b) gather_units<T, B_K>(g.b, b_ring + (g.resident ? w.chunk : ring.slot) * slot_bytes<T>(), t, w.j0(), w.k0(), w.k_end());
+        }
+        // the warp leaves together; asked behind the loads: dw of a million rows of 100 x 128 bfloat16 takes 313 us, with the
+        // question in front of them 398
+        if (!__all_sync(0xFFFFFFFFu, ok)) return;
         tc::fence_smem_for_async();
         __syncwarp();
         if (threadIdx.x % 32 == 0) tc::mbar_arrive(&ctl->full[ring.slot]);
@@ -358,14 +368,24 @@ template <typename T, bool A_K, bool B_K>
 __device__ __forceinline__ void load_tiled(const Args<T>& g, const void* map_a, const void* map_b, uint32_t a_ring, uint32_t b_ring, Control* ctl) {
     Walk<T> w(g);
     bool with_b = true;
-    for (Ring<Traits<T>::a_slots> ring; w.live(); ring.next()) {
-        if (ring.wrapped && !tc::mbar_wait(&ctl->empty[ring.slot], ring.parity ^ 1, &ctl->gave_up)) return;
+    Ring<Traits<T>::a_slots> ring;
+    for (; w.live(); ring.next()) {
+        if (ring.wrapped && !tc::mbar_wait(&ctl->empty[ring.slot], ring.parity ^ 1, &ctl->gave_up)) break;
         uint64_t* bar = &ctl->full[ring.slot];
         tc::mbar_expect(bar, with_b ? 2 * kPieceBytes : kPieceBytes);
         load_boxes<A_K>(a_ring + ring.slot * slot_bytes<T>(), map_a, w.i0(), w.k0(), bar);
         if (with_b) load_boxes<B_K>(b_ring + (g.resident ? w.chunk : ring.slot) * slot_bytes<T>(), map_b, w.j0(), w.k0(), bar);
         w.next_chunk();
         if (g.resident && w.chunk == 0) with_b = false;
+    }
+    // no copy of this thread's may be under way when the block ends, whether its products were ever formed or not
+#pragma unroll 1
+    for (int s = 0; s < Traits<T>::a_slots; ++s) {
+        unsigned last;
+        if (!ring.used(s, last)) continue;
+        const uint32_t addr = tc::smem_u32(&ctl->full[s]);
+        const long long t0 = clock64();
+        while (!tc::mbar_try(addr, last) && clock64() - t0 < tc::kWaitCycles) {}
     }
 }
 
@@ -626,7 +646,7 @@ __device__ __forceinline__ bool epilogue_item(const Args<T>& g, const Walk<T>& w
     auto present = [&](int block) { return row0 < g.rows && col0 + block * CB < g.cols; };
     const uint32_t mine = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * 64, sums = mine + Tr::buffers * kMmaTile;
     auto arrived = [&]() {
-        if (!tc::mbar_wait(&ctl->acc_full[buffers.slot], buffers.parity, &ctl->gave_up)) return false;
+        if (!tc::mbar_wait_warp(&ctl->acc_full[buffers.slot], buffers.parity, &ctl->gave_up)) return false;
         tc::fence_after_sync();
         return true;
     };

@@ -36,6 +36,12 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, unsigned parity, volati
     return true;
 }
 
+// The same for a whole warp, which leaves together: a lane that was let through would go on to instructions that the
+// warp has to run as one.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, unsigned parity, volatile int* gave_up) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, gave_up));
+}
+
 // ---- tensor memory ------------------------------------------------------------------------------------
 // Whole warp; `columns` a power of two, 32..512.
 __device__ __forceinline__ void tmem_alloc(uint32_t* where, uint32_t columns) {
