@@ -31,6 +31,7 @@
 #include <cuda.h>
 
 #include <atomic>
+#include <climits>
 #include <cmath>
 #include <type_traits>
 
@@ -74,6 +75,7 @@ struct Control {
     uint32_t tmem;
     int gave_up;
     int progress;             // chunks whose products have been issued
+    int odd_first, odd_last;  // float: between which items sums were not finite
 };
 
 template <typename T>
@@ -443,17 +445,6 @@ __device__ void product_role(const Args<T>& g, uint32_t a_ring, uint32_t b_ring,
     while (!tc::mbar_try(addr, 0) && clock64() - t0 < tc::kWaitCycles) {}
 }
 
-// A value again in plain 32-bit arithmetic: the pieces of an infinity, or of a value that rounds to one in 16 bits,
-// make a NaN where the product may be neither.
-template <typename T, bool A_K, bool B_K>
-__device__ __forceinline__ float plain_value(const Args<T>& g, int64_t i, int64_t j, int64_t k_begin, int64_t k_end) {
-    float v = 0.f;
-#pragma unroll 1
-    for (int64_t k = k_begin; k < k_end && !isnan(v); ++k)
-        v = fmaf(to_acc(A_K ? g.a.p[i * g.a.ld + k] : g.a.p[k * g.a.ld + i]), to_acc(B_K ? g.b.p[j * g.b.ld + k] : g.b.p[k * g.b.ld + j]), v);
-    return v;
-}
-
 // 128 bytes of the output type from floats, rounded once.
 __device__ __forceinline__ void pack_line(const float (&s)[32], uint32_t (&w)[32], float) {
 #pragma unroll
@@ -635,7 +626,7 @@ struct Writer {
 };
 
 // The accumulators of one item (float: one per chunk).
-template <typename T, typename O, bool A_K, bool B_K, int ACT, int KIND>
+template <typename T, typename O, int ACT, int KIND>
 __device__ __forceinline__ bool epilogue_item(const Args<T>& g, const Walk<T>& w, const Writer<T, O, ACT, KIND>& out,
                                               Ring<Traits<T>::buffers>& buffers, uint32_t tmem, Control* ctl) {
     using Tr = Traits<T>;
@@ -711,18 +702,14 @@ __device__ __forceinline__ bool epilogue_item(const Args<T>& g, const Walk<T>& w
             float t, t2;
             zeros.to(t, t2);
             t += t2;
-            if (t != t && row0 + lane < g.rows) {
-                // one value in turn, so that the loop needs no index into registers
-#pragma unroll 1
-                for (int q = 0; q < CB; ++q) {
-                    float first = v[0];
-                    if (!isfinite(first) && col + q < g.cols) first = plain_value<T, A_K, B_K>(g, row0 + lane, col + q, w.k_begin(), w.k_end());
-#pragma unroll
-                    for (int r = 0; r + 1 < CB; ++r) v[r] = v[r + 1];
-                    v[CB - 1] = first;
-                }
+            if (t != t && row0 + lane < g.rows) {                  // left as it is for now; see form_again
+                atomicMin(&ctl->odd_first, w.item);
+                atomicMax(&ctl->odd_last, w.item);
             }
             __syncwarp();
+            // the values are settled before bias and residual are called for (left to the compiler, 27 registers go to memory)
+#pragma unroll
+            for (int q = 0; q < CB; ++q) asm volatile("" : "+f"(v[q]));
         }
         out.block(v, w.split, row0, col, residual);
     }
@@ -730,7 +717,7 @@ __device__ __forceinline__ bool epilogue_item(const Args<T>& g, const Walk<T>& w
     return true;
 }
 
-template <typename T, bool A_K, bool B_K, int ACT, int KIND>
+template <typename T, int ACT, int KIND>
 __device__ __forceinline__ void epilogue_role(const Args<T>& g, const void* map_y, const void* map_z, uint32_t staging, uint32_t tmem,
                                               Control* ctl) {
     using O = typename std::conditional<KIND == kParts, float, T>::type;
@@ -738,8 +725,115 @@ __device__ __forceinline__ void epilogue_role(const Args<T>& g, const void* map_
     const Writer<T, O, ACT, KIND> out(g, map_y, map_z, staging + warp * 4096);
     Ring<Traits<T>::buffers> buffers;
     Walk<T> w(g);
-    for (bool ok = true; ok && w.live(); w.next_item()) ok = epilogue_item<T, O, A_K, B_K, ACT, KIND>(g, w, out, buffers, tmem, ctl);
+    for (bool ok = true; ok && w.live(); w.next_item()) ok = epilogue_item<T, O, ACT, KIND>(g, w, out, buffers, tmem, ctl);
     if (threadIdx.x % 32 == 0) tc::stores_done();
+}
+
+// Float sums again in plain 32-bit arithmetic: the pieces of an infinity, or of a value that rounds to one in 16 bits,
+// make a NaN where the product may be neither.  Either the lanes of a warp share the terms of one value (128 at a time),
+// or each has the value of its own row (eight terms at a time): whichever takes fewer trips to memory for the `count`
+// values of a column.  A sum that is NaN stays so and ends early.
+template <typename T, bool A_K, bool B_K>
+struct Plain {
+    const Args<T>& g;
+    const int64_t k_begin, k_end;
+    __device__ __forceinline__ float a(int64_t i, int64_t k) const { return to_acc(A_K ? g.a.p[i * g.a.ld + k] : g.a.p[k * g.a.ld + i]); }
+    __device__ __forceinline__ float b(int64_t k, int64_t j) const { return to_acc(B_K ? g.b.p[j * g.b.ld + k] : g.b.p[k * g.b.ld + j]); }
+    __device__ __forceinline__ bool share_terms(int count) const {
+        const int64_t terms = k_end - k_begin;
+        return count * ((terms + 127) / 128) <= (terms + 7) / 8;
+    }
+    // The value at (i, j), the same for all lanes.
+    __device__ __forceinline__ float shared(int64_t i, int64_t j) const {
+        const int lane = threadIdx.x % 32;
+        float v = 0.f;
+#pragma unroll 1
+        for (int64_t k = k_begin + lane; k - lane < k_end; k += 128) {
+            float x[4], y[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {                              // without conditions: the loads go out together
+                const int64_t there = min(k + 32 * u, k_end - 1);
+                x[u] = a(i, there);
+                y[u] = b(there, j);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v = k + 32 * u < k_end ? fmaf(x[u], y[u], v) : v;
+            if (__any_sync(0xFFFFFFFFu, isnan(v))) break;
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, off);
+        return v;
+    }
+    // The value at (i, j) of every lane that wants one; j is the same for all.
+    __device__ __forceinline__ float own(int64_t i, int64_t j, bool wanted) const {
+        float v = 0.f;
+        i = min(i, g.rows - 1);
+#pragma unroll 1
+        for (int64_t k = k_begin; k < k_end; k += 8) {
+            float x[8], y[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int64_t there = min(k + u, k_end - 1);
+                x[u] = a(i, there);
+                y[u] = b(there, j);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v = k + u < k_end ? fmaf(x[u], y[u], v) : v;
+            if (__all_sync(0xFFFFFFFFu, !wanted || isnan(v))) break;
+        }
+        return v;
+    }
+};
+
+// Forms again what is not finite of the items among which the epilogue has met such sums.  It runs when everything else
+// of the block is done, so nobody waits for it however long the sums are.  Its eight warps take pieces of 32 x 32 values,
+// a row to a lane.  Measured, forward, dx and dw of a million rows of 128 floats, 0.66 ms: 2.6 ms with one infinity in x
+// (128 sums of 7000 terms), 39 ms with a row of them (every entry of dw), 12 ms with nothing but NaN.
+template <typename T, bool A_K, bool B_K, int ACT, int KIND>
+__device__ __noinline__ void form_again(const Args<T>& g, const Control* ctl) {
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int first = ctl->odd_first, last = ctl->odd_last;
+    for (Walk<T> w(g); w.live() && w.item <= last; w.next_item()) {
+        if (w.item < first) continue;
+        const Plain<T, A_K, B_K> plain{g, w.k_begin(), w.k_end()};
+        for (int piece = warp; piece < 16; piece += kEpilogueWarps) {
+            const int64_t i = w.i0() + piece % 4 * 32 + lane, j0 = w.j0() + piece / 4 * 32;
+            for (int64_t j = j0; j < j0 + 32 && j < g.cols; ++j) {
+                const int64_t e = i * g.cols + j;
+                float* part = KIND == kParts ? g.ep.partial + w.split * g.rows * g.cols + e : nullptr;
+                bool wanted = false;
+                if (i < g.rows) {
+                    const float seen = KIND == kParts ? *part : to_acc(KIND == kForwardZ ? g.ep.z[e] : g.ep.y[e]);
+                    wanted = !isfinite(seen);
+                }
+                unsigned left = __ballot_sync(0xFFFFFFFFu, wanted);
+                if (left == 0) continue;
+                float v = 0.f;
+                if (plain.share_terms(__popc(left))) {
+#pragma unroll 1
+                    for (; left != 0; left &= left - 1) {
+                        const int row = __ffs(left) - 1;
+                        const float again = plain.shared(i - lane + row, j);
+                        if (lane == row) v = again;
+                    }
+                } else {
+                    v = plain.own(i, j, wanted);
+                }
+                if (!wanted) continue;
+                if constexpr (KIND == kParts) {
+                    *part = v;
+                } else if constexpr (KIND == kPlain) {
+                    g.ep.y[e] = from_acc<T>(v);
+                } else {
+                    if (g.ep.bias) v += to_acc(g.ep.bias[j]);
+                    if constexpr (KIND == kForwardZ) g.ep.z[e] = rounded_z<T, ACT>(v);
+                    v = activate<ACT>(v);
+                    if (g.ep.residual) v += to_acc(g.ep.residual[i * g.ep.ldr + j]);
+                    g.ep.y[e] = from_acc<T>(v);
+                }
+            }
+        }
+    }
 }
 
 // After a wait that ran out: NaN over all that this block was to write, so that nothing passes for a result.  The
@@ -778,6 +872,8 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
         tc::mbar_init(&ctl.done, 1);
         ctl.gave_up = 0;
         ctl.progress = 0;
+        ctl.odd_first = INT_MAX;
+        ctl.odd_last = -1;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kEpilogueWarps + kLoaderWarps) tc::tmem_alloc(&ctl.tmem, kTmemColumns);
@@ -789,7 +885,7 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
                   (kEpilogueWarps + kLoaderWarps + 4) * kLaunchRegisters, "registers beyond the block's own would be waited for for ever");
     if (warp < kEpilogueWarps) {
         tc::registers_up<Tr::epilogue_registers>();
-        epilogue_role<T, A_K, B_K, ACT, KIND>(g, &map_y, &map_z, staging, tmem, &ctl);
+        epilogue_role<T, ACT, KIND>(g, &map_y, &map_z, staging, tmem, &ctl);
     } else if (warp < kEpilogueWarps + kLoaderWarps) {
         if constexpr (Tr::pieces == 3) {
             tc::registers_up<Tr::loader_registers>();
@@ -810,6 +906,11 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
     tc::fence_before_sync();
     __syncthreads();
     if (warp == kEpilogueWarps + kLoaderWarps) tc::tmem_dealloc(tmem, kTmemColumns);
+    if constexpr (Tr::pieces == 3)
+        if (ctl.odd_last >= 0 && warp < kEpilogueWarps) {
+            asm volatile("fence.proxy.async;" ::: "memory");         // the bulk stores are done; what they wrote is read
+            form_again<T, A_K, B_K, ACT, KIND>(g, &ctl);
+        }
     if (ctl.gave_up && warp < kEpilogueWarps) {
         if (threadIdx.x == 0 && g.status) atomicMax(g.status, static_cast<int>(NB200_ERR_WAIT_BUDGET));
         if constexpr (KIND == kParts) write_nan<T, float>(g, g.ep.partial);

@@ -159,3 +159,58 @@ def test_a_wait_that_ran_out_is_seen_by_check_status(shim):
     numml_torch_cpp.check_status()                               # read and cleared
     assert torch.equal(F.linear(X, W), want)
     numml_torch_cpp.check_status()
+
+
+# ---------------------------------------------------------------------------------------------------------
+# infinities and NaN in the sums of the backward pass
+# ---------------------------------------------------------------------------------------------------------
+def _products(X, W, dY):
+    x, w = X.detach().requires_grad_(True), W.detach().requires_grad_(True)
+    b = torch.zeros(W.shape[1], dtype=X.dtype, device=X.device, requires_grad=True)
+    return torch.autograd.grad(F.linear(x, w, b), (x, w, b), dY)
+
+
+def _same_but(got, clean, row=None, column=None, value=None, what=""):
+    """`got` is `clean`, bit for bit, but for one row or column, which is `value`."""
+    want = clean.clone()
+    if row is not None:
+        want[row] = value
+    else:
+        want[:, column] = value
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(1.5), want.nan_to_num(1.5)), what
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("m,k,n", [(700, 40, 24), (20011, 40, 130), (3000, 1700, 1601)])
+def test_linear_infinities_in_the_backward_pass(m, k, n, dtype):
+    """One infinity in x: a row of dW infinite with the signs of dY's row (an infinity times a number), all else as it was;
+    one in dY: a row of dX and a column of dW; NaN and infinities of both signs: NaN.  The last size has more tiles of dW
+    than the GPU has multiprocessors, so its sum over the rows is one piece, behind which other tiles wait."""
+    X, W, dY = normal((m, k), 1, dtype).cuda(), normal((k, n), 2, dtype, 0.1).cuda(), normal((m, n), 3, dtype).cuda()
+    X[X == 0], W[W == 0], dY[dY == 0] = 1, 1, 1
+    clean = _products(X, W, dY)
+    inf = float("inf")
+    i, r, c = m - 2, k // 2, n - 1
+    Xi = X.clone()
+    Xi[i, r] = inf
+    dx, dw, db = _products(Xi, W, dY)
+    assert torch.equal(dx, clean[0]) and torch.equal(db, clean[2])
+    _same_but(dw, clean[1], row=r, value=dY[i].sign() * inf, what="infinity in x")
+    Xi[3, r] = -inf                                              # NaN where the two meet with opposite signs
+    meet = dY[i].sign() * inf - dY[3].sign() * inf
+    _same_but(_products(Xi, W, dY)[1], clean[1], row=r, value=meet, what="two infinities in x")
+    Xi = X.clone()
+    Xi[i, r] = float("nan")
+    _same_but(_products(Xi, W, dY)[1], clean[1], row=r, value=float("nan"), what="NaN in x")
+    Gi = dY.clone()
+    Gi[i, c] = -inf
+    dx, dw, db = _products(X, W, Gi)
+    _same_but(dx, clean[0], row=i, value=-W[:, c].sign() * inf, what="infinity in dY, dX")
+    _same_but(dw, clean[1], column=c, value=-X[i].sign() * inf, what="infinity in dY, dW")
+    assert db[c] == -inf and torch.equal(db[:c], clean[2][:c])
+    Xi = X.clone()
+    Xi[:, r] = inf                                               # every term of a row of dW
+    both = (dY.sign().amax(0) > 0) & (dY.sign().amin(0) < 0)
+    _same_but(_products(Xi, W, dY)[1], clean[1], row=r, value=torch.where(both, float("nan"), dY[0].sign() * inf).to(dtype), what="a column of infinities")
+    numml_torch_cpp.check_status()
