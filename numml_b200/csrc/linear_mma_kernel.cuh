@@ -19,7 +19,7 @@
 // The tensor cores truncate where they add, always towards zero.  For float a chunk's products therefore go in
 // order of size, the twenty small ones first, where a truncation weighs 2^-8 as much, then the four of the leading
 // pieces, and the sums over chunks are formed by the epilogue warps with rounding to nearest (the running sums
-// stay in tensor memory).
+// stay in tensor memory).  16-bit types have the same every 4096 terms.
 //
 // Measured on a B200 (copy 6548 GB/s, dense bfloat16 1651 TFLOP/s; cold L2): float, a million rows of 128 -> 128: plain
 // forward 220 us = 4.9 TB/s, with silu and z kept 345 us = 4.7 TB/s, dx 177 us = 6.1 TB/s, dw 225 us = 4.8 TB/s: the
@@ -47,22 +47,37 @@ constexpr int kLaunchRegisters = 96;                               // per thread
 constexpr int kPieceBytes = kMmaTile * kMmaChunk * 2;              // one piece of one operand's chunk: 16 KB
 constexpr int kUnits = kMmaTile * kMmaChunk / 8 / kLoaders;        // units of eight values per loader thread
 
-// Registers per thread after the warpgroups have shared them out anew: the float loaders hold a chunk of both
-// operands and the epilogue the sums of 64 columns; for 16-bit types the epilogue holds twice as many columns of a
-// block and the loaders next to nothing.
+// run: chunks whose products go into one accumulator.  The tensor cores cut off what they add there: measured, a sum that
+// grows evenly is short by 6.3e-9 of itself per term (2^-22.2 of the sum so far with every sixteen: two additions of
+// eight terms, say), always towards zero; 2^20 terms in one accumulator lost 6.6e-3, more than a bfloat16 step.  64 chunks =
+// 4096 terms lose 2.5e-5, a twentieth of float16's rounding; the sums of further runs are added with rounding to nearest
+// (in the columns of an accumulator, of which there is one less then).
 template <typename T> struct Traits {                              // 16-bit types
-    static constexpr int epilogue_registers = 160, loader_registers = 56, product_registers = 48;
-    static constexpr int pieces = 1, a_slots = 4, b_slots = 8, buffers = 4, ahead = 12;
+    static constexpr int pieces = 1, a_slots = 4, b_slots = 8, ahead = 12, run = 64;
 };
 template <> struct Traits<float> {
-    static constexpr int epilogue_registers = 120, loader_registers = 96, product_registers = 48;
-    static constexpr int pieces = 3, a_slots = 2, b_slots = 2, buffers = 3, ahead = 4;
+    static constexpr int pieces = 3, a_slots = 2, b_slots = 2, ahead = 4, run = 1;
 };
 
 // What leaves: y; y and z; a product without a forward epilogue; float parts of a sum.
 enum Kind { kForward, kForwardZ, kPlain, kParts };
 
-constexpr uint32_t kTmemColumns = 512;            // float: three accumulators and the running sums; 16-bit: four accumulators
+// Registers per thread after the warpgroups have shared them out anew.  With float outputs the epilogue holds 32 columns of
+// a block, and the loaders keep what they were launched with (a chunk of both float operands, or more of the values that they
+// gather: dw of a million rows of 100 x 128 bfloat16 348 us, with 56 registers to a loader 448); with 16-bit outputs the
+// epilogue holds twice as many columns and the loaders next to nothing.
+template <typename T, int KIND>
+struct Shares {
+    static constexpr bool floats = sizeof(T) == 4 || KIND == kParts;
+    static constexpr int epilogue = floats ? 120 : 160, loader = floats ? kLaunchRegisters : 56, product = 48;
+    static_assert(kEpilogueWarps * epilogue + kLoaderWarps * loader + 4 * product <= (kEpilogueWarps + kLoaderWarps + 4) * kLaunchRegisters,
+                  "registers beyond the block's own would be waited for for ever");
+};
+
+// Tensor memory: four blocks of columns, all of them accumulators or three and the running sums.
+constexpr uint32_t kTmemColumns = 512;
+constexpr int kSumsBlock = 3;
+template <bool LONG> constexpr int buffer_count() { return LONG ? kSumsBlock : kSumsBlock + 1; }
 template <typename T>
 constexpr int slot_bytes() { return Traits<T>::pieces * kPieceBytes; }
 template <typename T>
@@ -344,8 +359,7 @@ __device__ __forceinline__ void load_gathered(const Args<T>& g, uint32_t a_ring,
             gather_units<T, A_K>(g.a, a_ring + ring.slot * slot_bytes<T>(), t, w.i0(), w.k0(), w.k_end());
             if (with_b) gather_units<T, B_K>(g.b, b_ring + (g.resident ? w.chunk : ring.slot) * slot_bytes<T>(), t, w.j0(), w.k0(), w.k_end());
         }
-        // the warp leaves together; asked behind the loads: dw of a million rows of 100 x 128 bfloat16 takes 313 us, with the
-        // question in front of them 398
+        // the warp leaves together; asked behind the loads, so that nothing stands between them and the wait
         if (!__all_sync(0xFFFFFFFFu, ok)) return;
         tc::fence_smem_for_async();
         __syncwarp();
@@ -391,7 +405,7 @@ __device__ __forceinline__ void load_tiled(const Args<T>& g, const void* map_a, 
     }
 }
 
-template <typename T, bool A_K, bool B_K>
+template <typename T, bool A_K, bool B_K, bool LONG>
 __device__ void product_role(const Args<T>& g, uint32_t a_ring, uint32_t b_ring, uint32_t tmem, Control* ctl) {
     using Tr = Traits<T>;
     constexpr int S = Tr::a_slots;
@@ -399,13 +413,13 @@ __device__ void product_role(const Args<T>& g, uint32_t a_ring, uint32_t b_ring,
     constexpr uint32_t part = tc::instruction_descriptor(!std::is_same<T, __half>::value, !A_K, !B_K, kMmaTile / 2);
     constexpr uint32_t a_step = A_K ? 32 : 2048, b_step = B_K ? 32 : 2048;       // bytes from one 16-term step to the next
     Ring<S> ring;
-    Ring<Tr::buffers> buffers;
+    Ring<buffer_count<LONG>()> buffers;
     int issued = 0;
     bool ok = true;
     for (Walk<T> w(g); ok && w.live(); w.next_item()) {
         const uint32_t idesc = g.cols - w.j0() > kMmaTile / 2 ? whole : part;      // columns that do not exist are not multiplied
         for (int c = 0; ok && c < w.chunks; ++c, ring.next()) {
-            const bool fresh = Tr::pieces == 3 || c == 0, last = Tr::pieces == 3 || c + 1 == w.chunks;
+            const bool fresh = LONG ? c % Tr::run == 0 : c == 0, last = (LONG && (c + 1) % Tr::run == 0) || c + 1 == w.chunks;
             if (fresh && buffers.wrapped) ok = tc::mbar_wait(&ctl->acc_empty[buffers.slot], buffers.parity ^ 1, &ctl->gave_up);
             ok = ok && tc::mbar_wait(&ctl->full[ring.slot], ring.parity, &ctl->gave_up);
             if (!ok) break;
@@ -626,16 +640,17 @@ struct Writer {
 };
 
 // The accumulators of one item (float: one per chunk).
-template <typename T, typename O, int ACT, int KIND>
+template <bool LONG, typename T, typename O, int ACT, int KIND>
 __device__ __forceinline__ bool epilogue_item(const Args<T>& g, const Walk<T>& w, const Writer<T, O, ACT, KIND>& out,
-                                              Ring<Traits<T>::buffers>& buffers, uint32_t tmem, Control* ctl) {
+                                              Ring<buffer_count<LONG>()>& buffers, uint32_t tmem, Control* ctl) {
     using Tr = Traits<T>;
     constexpr int CB = Writer<T, O, ACT, KIND>::CB;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int quarter = warp % 4, half = warp / 4;                 // tensor memory lanes and columns of this warp
     const int64_t row0 = w.i0() + quarter * 32, col0 = w.j0() + half * 64;
     auto present = [&](int block) { return row0 < g.rows && col0 + block * CB < g.cols; };
-    const uint32_t mine = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * 64, sums = mine + Tr::buffers * kMmaTile;
+    const uint32_t mine = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * 64;
+    const uint32_t sums = mine + kSumsBlock * kMmaTile;
     auto arrived = [&]() {
         if (!tc::mbar_wait_warp(&ctl->acc_full[buffers.slot], buffers.parity, &ctl->gave_up)) return false;
         tc::fence_after_sync();
@@ -647,8 +662,10 @@ __device__ __forceinline__ bool epilogue_item(const Args<T>& g, const Walk<T>& w
         if (lane == 0) tc::mbar_arrive(&ctl->acc_empty[buffers.slot]);
         buffers.next();
     };
-    if constexpr (Tr::pieces == 3) {
-        for (int part = 0; part + 1 < w.chunks; ++part) {
+    const int parts = LONG ? (w.chunks + Tr::run - 1) / Tr::run : 1;
+    if constexpr (LONG) {
+#pragma unroll 1
+        for (int part = 0; part + 1 < parts; ++part) {
             if (!arrived()) return false;
             const uint32_t from = mine + buffers.slot * kMmaTile;
 #pragma unroll 2
@@ -679,7 +696,7 @@ __device__ __forceinline__ bool epilogue_item(const Args<T>& g, const Walk<T>& w
         float v[CB];
 #pragma unroll
         for (int q = 0; q < CB; q += 16) tc::tmem_load16(from + block * CB + q, *reinterpret_cast<float(*)[16]>(v + q));
-        if (Tr::pieces == 3 && w.chunks > 1) {
+        if (LONG && parts > 1) {
 #pragma unroll
             for (int h = 0; h < CB; h += 16) {
                 float sum[16];
@@ -717,15 +734,15 @@ __device__ __forceinline__ bool epilogue_item(const Args<T>& g, const Walk<T>& w
     return true;
 }
 
-template <typename T, int ACT, int KIND>
+template <bool LONG, typename T, int ACT, int KIND>
 __device__ __forceinline__ void epilogue_role(const Args<T>& g, const void* map_y, const void* map_z, uint32_t staging, uint32_t tmem,
                                               Control* ctl) {
     using O = typename std::conditional<KIND == kParts, float, T>::type;
     const int warp = threadIdx.x / 32;
     const Writer<T, O, ACT, KIND> out(g, map_y, map_z, staging + warp * 4096);
-    Ring<Traits<T>::buffers> buffers;
+    Ring<buffer_count<LONG>()> buffers;
     Walk<T> w(g);
-    for (bool ok = true; ok && w.live(); w.next_item()) ok = epilogue_item<T, O, ACT, KIND>(g, w, out, buffers, tmem, ctl);
+    for (bool ok = true; ok && w.live(); w.next_item()) ok = epilogue_item<LONG, T, O, ACT, KIND>(g, w, out, buffers, tmem, ctl);
     if (threadIdx.x % 32 == 0) tc::stores_done();
 }
 
@@ -838,7 +855,7 @@ __device__ __noinline__ void form_again(const Args<T>& g, const Control* ctl) {
 
 // After a wait that ran out: NaN over all that this block was to write, so that nothing passes for a result.  The
 // epilogue warps do it, once all stores are done: the others have given registers away.  Out of line, so that the
-// roles' registers are not shared out with it in mind (gathered dw of a million rows of 100 x 128 bfloat16 398 us, inline 488).
+// roles' registers are not shared out with it in mind (gathered dw of a million rows of 100 x 128 bfloat16 398 us, inline 488 at the time).
 template <typename T, typename O>
 __device__ __noinline__ void write_nan(const Args<T>& g, O* out) {
     for (Walk<T> w(g); w.live(); w.next_item()) {
@@ -848,13 +865,14 @@ __device__ __noinline__ void write_nan(const Args<T>& g, O* out) {
     }
 }
 
-template <typename T, bool A_K, bool B_K, int ACT, int KIND>
+template <typename T, bool A_K, bool B_K, int ACT, int KIND, bool LONG>
 __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant__ Args<T> g,
                                                           const __grid_constant__ CUtensorMap map_a,
                                                           const __grid_constant__ CUtensorMap map_b,
                                                           const __grid_constant__ CUtensorMap map_y,
                                                           const __grid_constant__ CUtensorMap map_z) {
     using Tr = Traits<T>;
+    using Share = Shares<T, KIND>;
     extern __shared__ char raw[];
     __shared__ Control ctl;
     const uint32_t base = (tc::smem_u32(raw) + 1023) / 1024 * 1024;
@@ -865,7 +883,7 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
             tc::mbar_init(&ctl.full[s], Tr::pieces == 1 && g.tiled ? 1 : kLoaderWarps);
             tc::mbar_init(&ctl.empty[s], 1);
         }
-        for (int s = 0; s < Tr::buffers; ++s) {
+        for (int s = 0; s < buffer_count<LONG>(); ++s) {
             tc::mbar_init(&ctl.acc_full[s], 1);
             tc::mbar_init(&ctl.acc_empty[s], kEpilogueWarps);
         }
@@ -881,25 +899,23 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = ctl.tmem;
-    static_assert(kEpilogueWarps * Tr::epilogue_registers + kLoaderWarps * Tr::loader_registers + 4 * Tr::product_registers <=
-                  (kEpilogueWarps + kLoaderWarps + 4) * kLaunchRegisters, "registers beyond the block's own would be waited for for ever");
     if (warp < kEpilogueWarps) {
-        tc::registers_up<Tr::epilogue_registers>();
-        epilogue_role<T, ACT, KIND>(g, &map_y, &map_z, staging, tmem, &ctl);
+        tc::registers_up<Share::epilogue>();
+        epilogue_role<LONG, T, ACT, KIND>(g, &map_y, &map_z, staging, tmem, &ctl);
     } else if (warp < kEpilogueWarps + kLoaderWarps) {
+        if constexpr (Share::loader < kLaunchRegisters) tc::registers_down<Share::loader>();
+        if constexpr (Tr::pieces == 3) tc::registers_up<Share::loader>();    // as many as it has: without it the compiler spills
         if constexpr (Tr::pieces == 3) {
-            tc::registers_up<Tr::loader_registers>();
             load_split<T, A_K, B_K>(g, a_ring, b_ring, &ctl);
         } else {
-            tc::registers_down<Tr::loader_registers>();
             if (!g.tiled)
                 load_gathered<T, A_K, B_K>(g, a_ring, b_ring, &ctl);
             else if (threadIdx.x == kEpilogueWarps * 32)
                 load_tiled<T, A_K, B_K>(g, &map_a, &map_b, a_ring, b_ring, &ctl);
         }
     } else {
-        tc::registers_down<Tr::product_registers>();
-        if (threadIdx.x == (kEpilogueWarps + kLoaderWarps) * 32) product_role<T, A_K, B_K>(g, a_ring, b_ring, tmem, &ctl);
+        tc::registers_down<Share::product>();
+        if (threadIdx.x == (kEpilogueWarps + kLoaderWarps) * 32) product_role<T, A_K, B_K, LONG>(g, a_ring, b_ring, tmem, &ctl);
         if (warp == kEpilogueWarps + kLoaderWarps + 1) prefetch_role<T, A_K, B_K, KIND>(g, &map_a, &map_b, &ctl);
     }
     __syncwarp();
@@ -971,6 +987,25 @@ bool make_output_map(CUtensorMap* map, O* p, int64_t rows, int64_t cols, int64_t
                   CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <typename T, bool A_K, bool B_K, int ACT, int KIND, bool LONG>
+int launch_kernel(const Args<T>& g, const CUtensorMap& map_a, const CUtensorMap& map_b, const CUtensorMap& map_y, const CUtensorMap& map_z,
+                  unsigned grid, int smem, cudaStream_t stream) {
+    // once per kernel and device
+    static std::atomic<uint64_t> prepared{0};
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return NB200_ERR_CUDA;
+    if (device >= 64 || !(prepared.load(std::memory_order_acquire) >> device & 1)) {
+        cudaFuncAttributes attr;
+        if (cudaFuncSetAttribute(mma_kernel<T, A_K, B_K, ACT, KIND, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+            cudaFuncGetAttributes(&attr, mma_kernel<T, A_K, B_K, ACT, KIND, LONG>) != cudaSuccess)
+            return NB200_ERR_CUDA;
+        if (attr.numRegs != kLaunchRegisters) return NB200_ERR_PRECONDITION;
+        if (device < 64) prepared.fetch_or(uint64_t(1) << device, std::memory_order_release);
+    }
+    mma_kernel<T, A_K, B_K, ACT, KIND, LONG><<<grid, kThreads, smem, stream>>>(g, map_a, map_b, map_y, map_z);
+    return launch_status();
+}
+
 template <typename T, bool A_K, bool B_K, int ACT, int KIND>
 int launch(int64_t rows, int64_t cols, int64_t depth, int64_t splits, int64_t per, const T* a, int64_t as, const T* b, int64_t bs,
                 const Epilogue<T>& ep, int32_t* status, cudaStream_t stream) {
@@ -1009,20 +1044,11 @@ int launch(int64_t rows, int64_t cols, int64_t depth, int64_t splits, int64_t pe
     }
     constexpr int smem = smem_bytes<T>();
     static_assert(smem + sizeof(Control) <= 227 * 1024, "shared memory of the product kernel");
-    // once per kernel and device
-    static std::atomic<uint64_t> prepared{0};
-    int device = 0;
-    if (cudaGetDevice(&device) != cudaSuccess) return NB200_ERR_CUDA;
-    if (device >= 64 || !(prepared.load(std::memory_order_acquire) >> device & 1)) {
-        cudaFuncAttributes attr;
-        if (cudaFuncSetAttribute(mma_kernel<T, A_K, B_K, ACT, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
-            cudaFuncGetAttributes(&attr, mma_kernel<T, A_K, B_K, ACT, KIND>) != cudaSuccess)
-            return NB200_ERR_CUDA;
-        if (attr.numRegs != kLaunchRegisters) return NB200_ERR_PRECONDITION;
-        if (device < 64) prepared.fetch_or(uint64_t(1) << device, std::memory_order_release);
-    }
-    mma_kernel<T, A_K, B_K, ACT, KIND><<<static_cast<unsigned>(grid), kThreads, smem, stream>>>(g, map_a, map_b, map_y, map_z);
-    return launch_status();
+    if (Traits<T>::pieces == 3 || g.chunks > Traits<T>::run)
+        return launch_kernel<T, A_K, B_K, ACT, KIND, true>(g, map_a, map_b, map_y, map_z, static_cast<unsigned>(grid), smem, stream);
+    if constexpr (Traits<T>::pieces == 1)
+        return launch_kernel<T, A_K, B_K, ACT, KIND, false>(g, map_a, map_b, map_y, map_z, static_cast<unsigned>(grid), smem, stream);
+    return NB200_ERR_BAD_ARG;                            // not reached
 }
 
 }  // namespace

@@ -214,3 +214,38 @@ def test_linear_infinities_in_the_backward_pass(m, k, n, dtype):
     both = (dY.sign().amax(0) > 0) & (dY.sign().amin(0) < 0)
     _same_but(_products(Xi, W, dY)[1], clean[1], row=r, value=torch.where(both, float("nan"), dY[0].sign() * inf).to(dtype), what="a column of infinities")
     numml_torch_cpp.check_status()
+
+
+# ---------------------------------------------------------------------------------------------------------
+# very long sums of 16-bit values
+# ---------------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("which", ["y", "dX", "dW"])
+def test_linear_long_sums_do_not_drift(which, dtype):
+    """Sums of 2^18 terms of one sign.  The tensor cores cut off where they add, always in one direction, up to 2^-23 of the
+    sum so far with every eight terms; the 4096 terms that share an accumulator come to 512 / 2 * 2^-23 = 2^-15 (the sum
+    grows evenly), and what is added to nearest after that has no direction.  The mean relative error over N results whose
+    logarithms are spread evenly is then below 2^-15 + 6 sigma / sqrt(N), sigma = half a step."""
+    u, _ = units(dtype)
+    long, (rows, cols) = 1 << 18, ((1152, 1152) if which == "dW" else (640, 128))
+    gen = torch.Generator(device="cuda").manual_seed(3)
+
+    def operand(lines):                                          # [lines, long]: positive, each line at a level of its own
+        level = 2.0 ** torch.rand(lines, 1, generator=gen, device="cuda")
+        return ((torch.rand(lines, long, generator=gen, device="cuda") + 0.5) * level * 2.0 ** -5).to(dtype)
+
+    a, b = operand(rows), operand(cols)
+    if which == "y":
+        got = F.linear(a, b.T.contiguous())
+    elif which == "dX":                                          # dX = dY W^T, sum over the output channels
+        x, w = torch.zeros(rows, cols, dtype=dtype, device="cuda", requires_grad=True), b
+        (got,) = torch.autograd.grad(F.linear(x, w), x, a)
+    else:                                                        # dW = X^T dY, sum over the rows
+        x, w = a.T.contiguous(), torch.zeros(rows, cols, dtype=dtype, device="cuda", requires_grad=True)
+        (got,) = torch.autograd.grad(F.linear(x, w), w, b.T.contiguous())
+    ref = a.double() @ b.double().T
+    error = (got.double() - ref) / ref
+    assert error.abs().max() <= u * 1.01 + 2.0 ** -15
+    assert error.mean().abs() <= 2.0 ** -15 + 6 * u / math.sqrt(got.numel()), error.mean().item()
+    numml_torch_cpp.check_status()
