@@ -4,12 +4,13 @@
 // channels / groups neighbouring channels of a group.  Backward, with dz = dy act'(z) and h = dz gamma:
 //   dx = rstd (h - mean(h) - xhat mean(h xhat)),  dgamma = sum dz xhat,  dbeta = sum dz.
 //
-// Segments may be of any length, so rows are cut into equal chunks, one per block, and not by segment:
-// the work is balanced however ragged the batch is.  A chunk holds pieces of several segments and a
-// segment pieces of several chunks; piece (block b, segment s) has workspace slot b + s, which is unique
-// because b and s never decrease from one piece to the next.  A pass writes per-channel partial results
-// of its pieces, a small kernel joins them per (segment, group) in a fixed order (no atomics: two runs
-// give the same bits), and a second pass over the rows applies them.
+// Segments may be of any length, so rows are cut into equal chunks, one per block, and not by segment: every block
+// has as many rows as the others, however ragged the batch is.  (A chunk's pieces come one after the other, though, at
+// about 0.6 us each: hundreds of segments of a row or two side by side are slow where the kernels of short segments
+// below do not take them.)  A chunk holds pieces of several segments and a segment pieces of several chunks; piece
+// (block b, segment s) has workspace slot b + s, which is unique because b and s never decrease from one piece to the
+// next.  A pass writes per-channel partial results of its pieces, a small kernel joins them per (segment, group) in a
+// fixed order (no atomics: two runs give the same bits), and a second pass over the rows applies them.
 //
 // Variances come from differences: a thread sums (x - k) and (x - k)^2 with k the first value it meets
 // of its channel in the piece, and partial results are joined as (count, mean, sum of squared
@@ -18,6 +19,10 @@
 // Measured on a million rows of 128 floats in 32 groups, silu (537 MB an array; copy 6548 GB/s): stats 104 us = 5.2 TB/s,
 // apply 173 us = 6.2, gradient sums 204 us = 5.3, gradient 265 us = 6.1, joins 6-10 us each: bound by memory.  An array
 // that does not fit on chip is read twice in each direction.
+#include <cooperative_groups.h>
+
+#include <type_traits>
+
 #include "dense_common.cuh"
 
 namespace nb200 {
@@ -32,6 +37,7 @@ struct Shape {
     int64_t segments;
     const int64_t* ptr;           // segments + 1 row pointers, or NULL: segments of `equal` rows
     int64_t equal;
+    int64_t handed;               // 0, or: segments of more rows than this are left to handed_*_kernel
 };
 
 __device__ __forceinline__ int64_t clamp_row(int64_t r, int64_t rows) { return r < 0 ? 0 : (r > rows ? rows : r); }
@@ -57,6 +63,69 @@ __device__ __forceinline__ int64_t find_segment(const Shape& sh, int64_t row, in
     return lo - 1;
 }
 
+// The pieces of a block's chunk of rows, one after the other: piece(s, slot, row, end) for rows of segment s, whose partial
+// results have that place in the workspace, outside(row, end) for rows of no segment.
+struct ChunkPieces {
+    const Shape& sh;
+    template <typename Piece, typename Outside>
+    __device__ __forceinline__ void each(Piece&& piece, Outside&& outside) const {
+        const int64_t limit = min(sh.rows, (blockIdx.x + 1) * sh.chunk);
+        for (int64_t row = blockIdx.x * sh.chunk, end; row < limit; row = end) {
+            const int64_t s = find_segment(sh, row, limit, end);
+            if (s < 0 || s >= sh.segments) outside(row, end);
+            else piece(s, blockIdx.x + s, row, end);
+        }
+    }
+};
+
+// The segments of more than sh.handed rows as an array of their own: they follow one another in it, and each block of the
+// grid has an equal run of its rows.  There are fewer than kMostHanded of them (the host sees to that; of broken row
+// pointers some are left out).
+constexpr int kMostHanded = 64;
+struct HandedPieces {
+    int count;
+    int segment[kMostHanded];
+    int64_t start[kMostHanded + 1];      // where a segment starts in that array
+    int64_t begin[kMostHanded];          // and among all rows
+    int found[kMostHanded];
+
+    __device__ void find(const Shape& sh) {              // this object is in shared memory; all threads of the block
+        if (threadIdx.x == 0) count = 0;
+        __syncthreads();
+        for (int64_t s = threadIdx.x; s < sh.segments; s += kThreads)
+            if (segment_begin(sh, s + 1) - segment_begin(sh, s) > sh.handed) {
+                const int q = atomicAdd(&count, 1);
+                if (q < kMostHanded) found[q] = static_cast<int>(s);
+            }
+        __syncthreads();
+        if (threadIdx.x == 0 && count > kMostHanded) count = kMostHanded;
+        __syncthreads();
+        if (threadIdx.x < count) {                       // in ascending order, whoever came first
+            int rank = 0;
+            for (int q = 0; q < count; ++q) rank += found[q] < found[threadIdx.x];
+            segment[rank] = found[threadIdx.x];
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            start[0] = 0;
+            for (int q = 0; q < count; ++q) {
+                begin[q] = segment_begin(sh, segment[q]);
+                start[q + 1] = start[q] + segment_begin(sh, segment[q] + 1) - begin[q];
+            }
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ int64_t chunk() const { return (start[count] + gridDim.x - 1) / gridDim.x; }
+    template <typename Piece, typename Outside>
+    __device__ __forceinline__ void each(Piece&& piece, Outside&&) const {
+        const int64_t first = blockIdx.x * chunk(), limit = min(first + chunk(), start[count]);
+        for (int q = 0; q < count; ++q) {
+            const int64_t row = max(first, start[q]), end = min(limit, start[q + 1]);
+            if (row < end) piece(int64_t(segment[q]), int64_t(blockIdx.x) + q, row - start[q] + begin[q], end - start[q] + begin[q]);
+        }
+    }
+};
+
 // Join (n, mean, m2) with (nb, mean_b, m2_b).
 template <typename A>
 __device__ __forceinline__ void join(A& n, A& mean, A& m2, A nb, A mean_b, A m2_b) {
@@ -75,17 +144,14 @@ __device__ __forceinline__ void join(A& n, A& mean, A& m2, A nb, A mean_b, A m2_
 }
 
 // ---- forward, first pass: per channel (mean, m2) of every piece ---------------------------------------
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) stats_kernel(Shape sh, const T* __restrict__ x, acc_t<T>* __restrict__ part) {
+template <typename T, int V, typename Pieces>
+__device__ __forceinline__ void form_stats(const Shape& sh, const Pieces& pieces, const T* __restrict__ x, acc_t<T>* __restrict__ part) {
     using A = acc_t<T>;
     __shared__ A sm_mean[kThreads * V], sm_m2[kThreads * V], sm_n[kThreads];
     const int lane = threadIdx.x % sh.lanes, row_lane = threadIdx.x / sh.lanes, row_lanes = kThreads / sh.lanes;
     const int c = (blockIdx.y * sh.lanes + lane) * V;
     const bool live = row_lane < row_lanes && c < sh.channels;
-    const int64_t limit = min(sh.rows, (blockIdx.x + 1) * sh.chunk);
-    for (int64_t row = blockIdx.x * sh.chunk, end; row < limit; row = end) {
-        const int64_t s = find_segment(sh, row, limit, end);
-        if (s < 0 || s >= sh.segments) continue;
+    pieces.each([&](int64_t, int64_t slot, int64_t row, int64_t end) {
         A k[V] = {}, sum[V] = {}, sq[V] = {}, n = 0;
         if (live) {
             int64_t r = row + row_lane;
@@ -135,14 +201,18 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(Shape sh, const T* __re
             __syncthreads();
         }
         if (live && row_lane == 0) {
-            A* out = part + (blockIdx.x + s) * 2 * sh.channels + c;
+            A* out = part + slot * 2 * sh.channels + c;
 #pragma unroll
             for (int q = 0; q < V; ++q) {
                 out[q] = mean[q];
                 out[sh.channels + q] = m2[q];
             }
         }
-    }
+    }, [](int64_t, int64_t) {});
+}
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) stats_kernel(Shape sh, const T* __restrict__ x, acc_t<T>* __restrict__ part) {
+    form_stats<T, V>(sh, ChunkPieces{sh}, x, part);
 }
 
 // Rows of segment s that lie in chunk b.
@@ -169,19 +239,22 @@ __device__ __forceinline__ double team_sum(double v, double* sm) {
 
 constexpr int join_threads(int team) { return team < kThreads ? kThreads : team; }
 
+// A segment's pieces: rows begin .. end of the array that chunks of `chunk` rows cut up, the first piece in slot `slot`.
+struct Span {
+    int64_t begin, end, chunk;
+    __device__ __forceinline__ int64_t first() const { return begin / chunk; }
+    __device__ __forceinline__ int64_t pieces() const { return end > begin ? (end - 1) / chunk - first() + 1 : 0; }
+};
+__device__ __forceinline__ Span segment_span(const Shape& sh, int64_t s) {
+    const int64_t begin = segment_begin(sh, s);
+    return {begin, max(begin, segment_begin(sh, s + 1)), sh.chunk};
+}
+
 template <typename A, int TEAM>
-__global__ void __launch_bounds__(join_threads(TEAM)) stats_join_kernel(Shape sh, const A* __restrict__ part, double eps,
-                                                              A* __restrict__ mean_out, A* __restrict__ rstd_out) {
-    __shared__ double sm[join_threads(TEAM) / 32];
-    const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM;
-    const int64_t item = blockIdx.x * int64_t(join_threads(TEAM) / TEAM) + team;
-    const bool live = item < sh.segments * sh.groups;
-    const int64_t s = live ? item / sh.groups : 0;
-    const int g = static_cast<int>(live ? item % sh.groups : 0), width = sh.channels / sh.groups;
-    const int64_t begin = segment_begin(sh, s), end = max(begin, segment_begin(sh, s + 1));
-    const int64_t first = begin / sh.chunk, last = end > begin ? (end - 1) / sh.chunk : first - 1;
-    const int64_t pieces = live ? last - first + 1 : 0;
-    const A* base = part + (first + s) * 2 * sh.channels + g * width;
+__device__ __forceinline__ void join_stats(const Span& span, bool live, const A* base, int channels, int width, double eps,
+                                           double* sm, A* mean_out, A* rstd_out) {
+    const int t = threadIdx.x % TEAM;
+    const int64_t first = span.first(), pieces = live ? span.pieces() : 0;
     // the team's threads go along the channels first; what does not divide is idle
     const int per = width < TEAM ? width : TEAM, lanes = TEAM / per, lane = t / per;
     double sum = 0;
@@ -189,23 +262,36 @@ __global__ void __launch_bounds__(join_threads(TEAM)) stats_join_kernel(Shape sh
         if (lane < lanes)
 #pragma unroll 4
             for (int64_t b = lane; b < pieces; b += lanes)
-                sum += static_cast<double>(piece_rows(begin, end, first + b, sh.chunk)) * static_cast<double>(base[b * 2 * sh.channels + c]);
-    const double n = static_cast<double>(end - begin) * width;
+                sum += static_cast<double>(piece_rows(span.begin, span.end, first + b, span.chunk)) * static_cast<double>(base[b * 2 * channels + c]);
+    const double n = static_cast<double>(span.end - span.begin) * width;
     const double mean = team_sum<TEAM>(sum, sm) / (n > 0 ? n : 1.0);
     double m2 = 0;
     for (int c = t % per; c < width; c += per)
         if (lane < lanes)
 #pragma unroll 4
             for (int64_t b = lane; b < pieces; b += lanes) {
-                const A* p = base + b * 2 * sh.channels + c;
+                const A* p = base + b * 2 * channels + c;
                 const double d = static_cast<double>(p[0]) - mean;
-                m2 += static_cast<double>(p[sh.channels]) + static_cast<double>(piece_rows(begin, end, first + b, sh.chunk)) * d * d;
+                m2 += static_cast<double>(p[channels]) + static_cast<double>(piece_rows(span.begin, span.end, first + b, span.chunk)) * d * d;
             }
     m2 = team_sum<TEAM>(m2, sm);
     if (live && t == 0) {
-        mean_out[item] = static_cast<A>(n > 0 ? mean : 0.0);
-        rstd_out[item] = n > 0 ? static_cast<A>(1.0 / sqrt(m2 / n + eps)) : A(0);
+        *mean_out = static_cast<A>(n > 0 ? mean : 0.0);
+        *rstd_out = n > 0 ? static_cast<A>(1.0 / sqrt(m2 / n + eps)) : A(0);
     }
+}
+
+template <typename A, int TEAM>
+__global__ void __launch_bounds__(join_threads(TEAM)) stats_join_kernel(Shape sh, const A* __restrict__ part, double eps,
+                                                              A* __restrict__ mean_out, A* __restrict__ rstd_out) {
+    __shared__ double sm[join_threads(TEAM) / 32];
+    const int64_t item = blockIdx.x * int64_t(join_threads(TEAM) / TEAM) + threadIdx.x / TEAM;
+    const bool live = item < sh.segments * sh.groups;
+    const int64_t s = live ? item / sh.groups : 0;
+    const int g = static_cast<int>(live ? item % sh.groups : 0), width = sh.channels / sh.groups;
+    const Span span = segment_span(sh, s);
+    join_stats<A, TEAM>(span, live, part + (span.first() + s) * 2 * sh.channels + g * width, sh.channels, width, eps, sm, mean_out + item,
+                        rstd_out + item);
 }
 
 // ---- what a thread knows of its V channels ------------------------------------------------------------
@@ -224,24 +310,17 @@ struct ChannelParams {
     }
 };
 
-template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads) apply_kernel(Shape sh, const T* __restrict__ x, const T* __restrict__ w,
-                                                         const T* __restrict__ bias, const acc_t<T>* __restrict__ mean,
-                                                         const acc_t<T>* __restrict__ rstd, T* __restrict__ y) {
+// The statistics may be this launch's own results: no __restrict__.
+template <typename T, int V, int ACT, typename Pieces>
+__device__ __forceinline__ void apply_rows(const Shape& sh, const Pieces& pieces, const T* __restrict__ x, const T* __restrict__ w,
+                                           const T* __restrict__ bias, const acc_t<T>* mean, const acc_t<T>* rstd, T* __restrict__ y) {
     using A = acc_t<T>;
     const int lane = threadIdx.x % sh.lanes, row_lane = threadIdx.x / sh.lanes, row_lanes = kThreads / sh.lanes;
     const int c = (blockIdx.y * sh.lanes + lane) * V;
     if (row_lane >= row_lanes || c >= sh.channels) return;
     ChannelParams<T, V> cp;
     cp.load(sh, c, w, bias);
-    const int64_t limit = min(sh.rows, (blockIdx.x + 1) * sh.chunk);
-    for (int64_t row = blockIdx.x * sh.chunk, end; row < limit; row = end) {
-        const int64_t s = find_segment(sh, row, limit, end);
-        if (s < 0 || s >= sh.segments) {
-            const A zero[V] = {};
-            for (int64_t r = row + row_lane; r < end; r += row_lanes) store_acc<T, V>(y + r * sh.channels + c, zero);
-            continue;
-        }
+    pieces.each([&](int64_t s, int64_t, int64_t row, int64_t end) {
         A m[V], a[V];
 #pragma unroll
         for (int q = 0; q < V; ++q) {
@@ -257,15 +336,48 @@ __global__ void __launch_bounds__(kThreads) apply_kernel(Shape sh, const T* __re
             activate_all<ACT>(v);
             store_acc<T, V>(y + r * sh.channels + c, v);
         }
+    }, [&](int64_t row, int64_t end) {
+        const A zero[V] = {};
+        for (int64_t r = row + row_lane; r < end; r += row_lanes) store_acc<T, V>(y + r * sh.channels + c, zero);
+    });
+}
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads) apply_kernel(Shape sh, const T* __restrict__ x, const T* __restrict__ w,
+                                                         const T* __restrict__ bias, const acc_t<T>* __restrict__ mean,
+                                                         const acc_t<T>* __restrict__ rstd, T* __restrict__ y) {
+    apply_rows<T, V, ACT>(sh, ChunkPieces{sh}, x, w, bias, mean, rstd, y);
+}
+
+// Both passes over the segments that short_forward_kernel has handed over, in one cooperative launch; it finds out for
+// itself whether there are any, and is done when there are none.
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads, 2) handed_forward_kernel(Shape sh, const T* __restrict__ x, const T* __restrict__ w,
+                                                                     const T* __restrict__ bias, double eps, acc_t<T>* mean, acc_t<T>* rstd,
+                                                                     acc_t<T>* part, T* __restrict__ y) {
+    using A = acc_t<T>;
+    __shared__ HandedPieces pieces;
+    __shared__ double sm[kThreads / 32];
+    pieces.find(sh);
+    if (pieces.count == 0) return;                       // the same for all blocks
+    form_stats<T, V>(sh, pieces, x, part);
+    cooperative_groups::this_grid().sync();
+    const int width = sh.channels / sh.groups, n = pieces.count * sh.groups;
+    for (int item = blockIdx.y * gridDim.x + blockIdx.x; item < n; item += gridDim.x * gridDim.y) {
+        const int q = item / sh.groups, g = item % sh.groups;
+        const Span span{pieces.start[q], pieces.start[q + 1], pieces.chunk()};
+        const int64_t to = int64_t(pieces.segment[q]) * sh.groups + g;
+        join_stats<A, kThreads>(span, true, part + (span.first() + q) * 2 * sh.channels + g * width, sh.channels, width, eps, sm, mean + to,
+                                rstd + to);
     }
+    cooperative_groups::this_grid().sync();
+    apply_rows<T, V, ACT>(sh, pieces, x, w, bias, mean, rstd, y);
 }
 
 // ---- backward, first pass: per channel (sum dz, sum dz xhat) of every piece and of every block ---------
-template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads) grad_sums_kernel(Shape sh, const T* __restrict__ x, const T* __restrict__ dy,
-                                                             const T* __restrict__ w, const T* __restrict__ bias,
-                                                             const acc_t<T>* __restrict__ mean, const acc_t<T>* __restrict__ rstd,
-                                                             acc_t<T>* __restrict__ part, acc_t<T>* __restrict__ block_sums) {
+template <typename T, int V, int ACT, typename Pieces>
+__device__ __forceinline__ void form_grad_sums(const Shape& sh, const Pieces& pieces, const T* __restrict__ x, const T* __restrict__ dy,
+                                               const T* __restrict__ w, const T* __restrict__ bias, const acc_t<T>* __restrict__ mean,
+                                               const acc_t<T>* __restrict__ rstd, acc_t<T>* part, acc_t<T>* block_sums) {
     using A = acc_t<T>;
     __shared__ A sm[2][kThreads * V];
     const int lane = threadIdx.x % sh.lanes, row_lane = threadIdx.x / sh.lanes, row_lanes = kThreads / sh.lanes;
@@ -274,10 +386,7 @@ __global__ void __launch_bounds__(kThreads) grad_sums_kernel(Shape sh, const T* 
     ChannelParams<T, V> cp;
     if (live) cp.load(sh, c, w, bias);
     A total1[V] = {}, total2[V] = {};
-    const int64_t limit = min(sh.rows, (blockIdx.x + 1) * sh.chunk);
-    for (int64_t row = blockIdx.x * sh.chunk, end; row < limit; row = end) {
-        const int64_t s = find_segment(sh, row, limit, end);
-        if (s < 0 || s >= sh.segments) continue;
+    pieces.each([&](int64_t s, int64_t slot, int64_t row, int64_t end) {
         A s1[V] = {}, s2[V] = {};
         if (live) {
             A m[V], rs[V];
@@ -321,7 +430,7 @@ __global__ void __launch_bounds__(kThreads) grad_sums_kernel(Shape sh, const T* 
             __syncthreads();
         }
         if (live && row_lane == 0) {
-            A* out = part + (blockIdx.x + s) * 2 * sh.channels + c;
+            A* out = part + slot * 2 * sh.channels + c;
 #pragma unroll
             for (int q = 0; q < V; ++q) {
                 out[q] = s1[q];
@@ -330,7 +439,7 @@ __global__ void __launch_bounds__(kThreads) grad_sums_kernel(Shape sh, const T* 
                 total2[q] += s2[q];
             }
         }
-    }
+    }, [](int64_t, int64_t) {});
     if (live && row_lane == 0) {
         A* out = block_sums + blockIdx.x * int64_t(2) * sh.channels + c;
 #pragma unroll
@@ -341,20 +450,20 @@ __global__ void __launch_bounds__(kThreads) grad_sums_kernel(Shape sh, const T* 
     }
 }
 
-// mean(h) and mean(h xhat) of every (segment, group), from the per-channel sums of its pieces.
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads) grad_sums_kernel(Shape sh, const T* __restrict__ x, const T* __restrict__ dy,
+                                                             const T* __restrict__ w, const T* __restrict__ bias,
+                                                             const acc_t<T>* __restrict__ mean, const acc_t<T>* __restrict__ rstd,
+                                                             acc_t<T>* __restrict__ part, acc_t<T>* __restrict__ block_sums) {
+    form_grad_sums<T, V, ACT>(sh, ChunkPieces{sh}, x, dy, w, bias, mean, rstd, part, block_sums);
+}
+
+// mean(h) and mean(h xhat) of a (segment, group), from the per-channel sums of its pieces.
 template <typename T, int TEAM>
-__global__ void __launch_bounds__(join_threads(TEAM)) grad_join_kernel(Shape sh, const acc_t<T>* __restrict__ part, const T* __restrict__ w,
-                                                             acc_t<T>* __restrict__ coef) {
-    __shared__ double sm[join_threads(TEAM) / 32];
-    const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM;
-    const int64_t item = blockIdx.x * int64_t(join_threads(TEAM) / TEAM) + team;
-    const bool live = item < sh.segments * sh.groups;
-    const int64_t s = live ? item / sh.groups : 0;
-    const int g = static_cast<int>(live ? item % sh.groups : 0), width = sh.channels / sh.groups;
-    const int64_t begin = segment_begin(sh, s), end = max(begin, segment_begin(sh, s + 1));
-    const int64_t first = begin / sh.chunk, last = end > begin ? (end - 1) / sh.chunk : first - 1;
-    const int64_t pieces = live ? last - first + 1 : 0;
-    const acc_t<T>* base = part + (first + s) * 2 * sh.channels + g * width;
+__device__ __forceinline__ void join_grads(const Span& span, bool live, const acc_t<T>* base, int channels, int width,
+                                           const T* __restrict__ w, double* sm, acc_t<T>* coef) {
+    const int t = threadIdx.x % TEAM;
+    const int64_t pieces = live ? span.pieces() : 0;
     const int per = width < TEAM ? width : TEAM, lanes = TEAM / per, lane = t / per;
     double a = 0, b = 0;
     for (int c = t % per; c < width; c += per) {
@@ -362,21 +471,34 @@ __global__ void __launch_bounds__(join_threads(TEAM)) grad_join_kernel(Shape sh,
         if (lane < lanes)
 #pragma unroll 4
             for (int64_t q = lane; q < pieces; q += lanes) {
-                const acc_t<T>* p = base + q * 2 * sh.channels + c;
+                const acc_t<T>* p = base + q * 2 * channels + c;
                 ca += static_cast<double>(p[0]);
-                cb += static_cast<double>(p[sh.channels]);
+                cb += static_cast<double>(p[channels]);
             }
-        const double gamma = w ? static_cast<double>(to_acc(w[g * width + c])) : 1.0;
+        const double gamma = w ? static_cast<double>(to_acc(w[c])) : 1.0;
         a += gamma * ca;
         b += gamma * cb;
     }
     a = team_sum<TEAM>(a, sm);
     b = team_sum<TEAM>(b, sm);
     if (live && t == 0) {
-        const double n = static_cast<double>(end - begin) * width;
-        coef[2 * item] = static_cast<acc_t<T>>(n > 0 ? a / n : 0.0);
-        coef[2 * item + 1] = static_cast<acc_t<T>>(n > 0 ? b / n : 0.0);
+        const double n = static_cast<double>(span.end - span.begin) * width;
+        coef[0] = static_cast<acc_t<T>>(n > 0 ? a / n : 0.0);
+        coef[1] = static_cast<acc_t<T>>(n > 0 ? b / n : 0.0);
     }
+}
+
+template <typename T, int TEAM>
+__global__ void __launch_bounds__(join_threads(TEAM)) grad_join_kernel(Shape sh, const acc_t<T>* __restrict__ part, const T* __restrict__ w,
+                                                             acc_t<T>* __restrict__ coef) {
+    __shared__ double sm[join_threads(TEAM) / 32];
+    const int64_t item = blockIdx.x * int64_t(join_threads(TEAM) / TEAM) + threadIdx.x / TEAM;
+    const bool live = item < sh.segments * sh.groups;
+    const int64_t s = live ? item / sh.groups : 0;
+    const int g = static_cast<int>(live ? item % sh.groups : 0), width = sh.channels / sh.groups;
+    const Span span = segment_span(sh, s);
+    join_grads<T, TEAM>(span, live, part + (span.first() + s) * 2 * sh.channels + g * width, sh.channels, width, w ? w + g * width : nullptr, sm,
+                        coef + 2 * item);
 }
 
 // dbeta and dgamma: columns of sums [parts][2][channels] added up; 32 columns x 32 lanes of a block, in an order
@@ -403,25 +525,17 @@ __global__ void __launch_bounds__(1024) column_sums_kernel(int64_t parts, int ch
     }
 }
 
-template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads) grad_apply_kernel(Shape sh, const T* __restrict__ x, const T* __restrict__ dy,
-                                                              const T* __restrict__ w, const T* __restrict__ bias,
-                                                              const acc_t<T>* __restrict__ mean, const acc_t<T>* __restrict__ rstd,
-                                                              const acc_t<T>* __restrict__ coef, T* __restrict__ dx) {
+template <typename T, int V, int ACT, typename Pieces>
+__device__ __forceinline__ void apply_grads(const Shape& sh, const Pieces& pieces, const T* __restrict__ x, const T* __restrict__ dy,
+                                            const T* __restrict__ w, const T* __restrict__ bias, const acc_t<T>* __restrict__ mean,
+                                            const acc_t<T>* __restrict__ rstd, const acc_t<T>* coef, T* __restrict__ dx) {
     using A = acc_t<T>;
     const int lane = threadIdx.x % sh.lanes, row_lane = threadIdx.x / sh.lanes, row_lanes = kThreads / sh.lanes;
     const int c = (blockIdx.y * sh.lanes + lane) * V;
     if (row_lane >= row_lanes || c >= sh.channels) return;
     ChannelParams<T, V> cp;
     cp.load(sh, c, w, bias);
-    const int64_t limit = min(sh.rows, (blockIdx.x + 1) * sh.chunk);
-    for (int64_t row = blockIdx.x * sh.chunk, end; row < limit; row = end) {
-        const int64_t s = find_segment(sh, row, limit, end);
-        if (s < 0 || s >= sh.segments) {
-            const A zero[V] = {};
-            for (int64_t r = row + row_lane; r < end; r += row_lanes) store_acc<T, V>(dx + r * sh.channels + c, zero);
-            continue;
-        }
+    pieces.each([&](int64_t s, int64_t, int64_t row, int64_t end) {
         A m[V], rs[V], c1[V], c2[V];
 #pragma unroll
         for (int q = 0; q < V; ++q) {
@@ -448,7 +562,44 @@ __global__ void __launch_bounds__(kThreads) grad_apply_kernel(Shape sh, const T*
             for (int q = 0; q < V; ++q) v[q] = rs[q] * (g[q] * slope[q] * cp.gamma[q] - c1[q] - v[q] * c2[q]);
             store_acc<T, V>(dx + r * sh.channels + c, v);
         }
+    }, [&](int64_t row, int64_t end) {
+        const A zero[V] = {};
+        for (int64_t r = row + row_lane; r < end; r += row_lanes) store_acc<T, V>(dx + r * sh.channels + c, zero);
+    });
+}
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads) grad_apply_kernel(Shape sh, const T* __restrict__ x, const T* __restrict__ dy,
+                                                              const T* __restrict__ w, const T* __restrict__ bias,
+                                                              const acc_t<T>* __restrict__ mean, const acc_t<T>* __restrict__ rstd,
+                                                              const acc_t<T>* __restrict__ coef, T* __restrict__ dx) {
+    apply_grads<T, V, ACT>(sh, ChunkPieces{sh}, x, dy, w, bias, mean, rstd, coef, dx);
+}
+
+// The same for the segments that short_backward_kernel has handed over.  Without any, its lines of sums are zeros.
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads, 2) handed_backward_kernel(Shape sh, const T* __restrict__ x, const T* __restrict__ dy,
+                                                                      const T* __restrict__ w, const T* __restrict__ bias,
+                                                                      const acc_t<T>* __restrict__ mean, const acc_t<T>* __restrict__ rstd,
+                                                                      acc_t<T>* part, acc_t<T>* block_sums, acc_t<T>* coef, T* __restrict__ dx) {
+    __shared__ HandedPieces pieces;
+    __shared__ double sm[kThreads / 32];
+    pieces.find(sh);
+    if (pieces.count == 0) {
+        for (int c = threadIdx.x; blockIdx.y == 0 && c < 2 * sh.channels; c += kThreads) block_sums[blockIdx.x * int64_t(2) * sh.channels + c] = 0;
+        return;
     }
+    form_grad_sums<T, V, ACT>(sh, pieces, x, dy, w, bias, mean, rstd, part, block_sums);
+    if (!dx) return;
+    cooperative_groups::this_grid().sync();
+    const int width = sh.channels / sh.groups, n = pieces.count * sh.groups;
+    for (int item = blockIdx.y * gridDim.x + blockIdx.x; item < n; item += gridDim.x * gridDim.y) {
+        const int q = item / sh.groups, g = item % sh.groups;
+        const Span span{pieces.start[q], pieces.start[q + 1], pieces.chunk()};
+        join_grads<T, kThreads>(span, true, part + (span.first() + q) * 2 * sh.channels + g * width, sh.channels, width,
+                                w ? w + g * width : nullptr, sm, coef + 2 * (int64_t(pieces.segment[q]) * sh.groups + g));
+    }
+    cooperative_groups::this_grid().sync();
+    apply_grads<T, V, ACT>(sh, pieces, x, dy, w, bias, mean, rstd, coef, dx);
 }
 
 // ---- short segments: one block per (segment, slab of whole groups), one launch per direction -------------------
@@ -466,6 +617,7 @@ struct Divisor {
 struct Slab {
     int channels, lanes;          // channels of a slab (whole groups), vectors of its row
     int pad_blocks;               // blocks that write the rows outside every segment
+    int64_t handed;               // see Shape
     int width, groups;            // channels of a group, groups of a slab
     Divisor by_lanes, by_width;
     // sums over a group: by one vector per column (width / V columns) in the forward pass, per channel in the backward
@@ -531,6 +683,7 @@ __global__ void __launch_bounds__(kShort, 4) short_forward_kernel(Shape sh, Slab
     }
     const int64_t s = blockIdx.x, begin = segment_begin(sh, s), end = max(begin, segment_begin(sh, s + 1));
     const int width = slab.width, groups = slab.groups, first = blockIdx.y * slab.channels, g0 = blockIdx.y * groups;
+    if (sh.handed != 0 && end - begin > sh.handed) return;
     if (end == begin) {
         for (int g = threadIdx.x; g < groups; g += kShort) mean[s * sh.groups + g0 + g] = rstd[s * sh.groups + g0 + g] = A(0);
         return;
@@ -637,6 +790,11 @@ __global__ void __launch_bounds__(kShort, sizeof(T) == 8 ? 2 : 4) short_backward
     }
     const int64_t s = blockIdx.x, begin = segment_begin(sh, s), end = max(begin, segment_begin(sh, s + 1));
     const int width = slab.width, first = blockIdx.y * slab.channels, mine = slab.channels, g0 = blockIdx.y * slab.groups;
+    if (sh.handed != 0 && end - begin > sh.handed) {     // its share of dbeta and dgamma is in another line
+        if (threadIdx.x < mine)
+            channel_sums[s * 2 * sh.channels + first + threadIdx.x] = channel_sums[s * 2 * sh.channels + sh.channels + first + threadIdx.x] = A(0);
+        return;
+    }
     const int row_lane = slab.by_lanes.div(threadIdx.x), lane = threadIdx.x - row_lane * slab.lanes, row_lanes = slab.by_lanes.div(kShort);
     const int c = lane * V;
     const int used = static_cast<int>(min(int64_t(row_lanes), end - begin));
@@ -733,14 +891,21 @@ int64_t block_count(int64_t rows) {
 }
 
 // Whether the one-block-per-segment kernels run, and with which slabs of channels.  They need segments that stay in
-// a block's L1 on average (a slab of one up to 128 KB) and an array in which even one segment that has all rows is
-// read by a single block in about 0.1 ms (slabs up to 8 MB); beyond that the row chunks, which are balanced however
-// long a segment is, take over.  Slabs are made narrower (whole groups) while there are fewer than eight blocks for
+// a block's L1 on average (a slab of one up to 128 KB) and an array of at most 8 MB a slab; beyond that the row chunks
+// take over.  A single block reads about 20 GB/s, so a long segment among short ones would be waited for: in an
+// array above 512 KB a slab, segments above 128 KB a slab (fewer than 64 of them) are handed over to one more launch,
+// which finds none in most batches.  Measured, forward / backward of 61,441 rows x 128 bfloat16 in 512 graphs, one of
+// which has all rows but 511: 47 / 76 us, with that graph in one block 581 / 1166, in row chunks 397 / 397; the launch
+// costs equal graphs 4 us (23 -> 28 forward).  At 512 KB (8192 rows in 64 graphs) the long one in one block
+// takes 48 / 92 us.
+// Slabs are made narrower (whole groups) while there are fewer than eight blocks for
 // every SM, down to rows of 64 bytes, or fewer than two, down to 32.  Measured on 512 graphs of 1 to 1076 rows, mean
 // 118, x 128 bfloat16 channels with gelu, forward / backward: slabs of 128 channels 46 / 100 us, 64: 32 / 65, 32: 31 /
-// 57, with four channels to a thread 31 / 51 (the longest graph's arithmetic on one SM is what is left; clusters of 2 to
-// 8 blocks per graph, which split it, were no faster: 34-41 / 67-72); the row chunks 82 / 117 us in six launches.
-bool short_segments(int64_t rows, int64_t channels, int64_t groups, int64_t segments, size_t size, int V, Slab* slab) {
+// 57, with four channels to a thread 31 / 51 (clusters of 2 to 8 blocks per graph were no faster: 34-41 / 67-72); the row
+// chunks 82 / 117 us in six launches.
+constexpr int64_t kAlone = 512 * 1024, kInBlock = 128 * 1024;
+constexpr int64_t kMostSegments = 16384;             // of a batch that may hand some over: every block of that launch looks through them
+bool short_segments(int64_t rows, int64_t channels, int64_t groups, int64_t segments, bool ragged, size_t size, int V, Slab* slab) {
     if (segments < 1 || segments > 65535 * 16) return false;
     const int64_t width = channels / groups;
     auto divisor = [&](int64_t most) {                                 // the largest divisor of groups up to it whose rows are whole vectors
@@ -760,7 +925,9 @@ bool short_segments(int64_t rows, int64_t channels, int64_t groups, int64_t segm
         in_slab = d;
     }
     const int64_t line = in_slab * width * int64_t(size);
-    if (rows / segments * line > 128 * 1024 || rows * line > 8 * 1024 * 1024) return false;
+    if (rows / segments * line > kInBlock || rows * line > 8 * 1024 * 1024) return false;
+    slab->handed = ragged && rows * line > kAlone ? kInBlock / line : 0;
+    if (slab->handed != 0 && (segments > kMostSegments || ceil_div(channels, kThreads) > 2 * kSMs)) return false;
     if (groups / in_slab > 65535) return false;
     slab->channels = static_cast<int>(in_slab * width);
     slab->lanes = static_cast<int>(in_slab * width / V);
@@ -775,7 +942,10 @@ bool short_segments(int64_t rows, int64_t channels, int64_t groups, int64_t segm
     return true;
 }
 
-// Partial results of the pieces, of the blocks, and the two coefficients per (segment, group).
+// Lines of sums for segments beside those for blocks: a batch that may hand segments over needs both.
+int64_t line_sums(int64_t segments) { return segments <= kMostSegments ? segments : 0; }
+
+// Partial results of the pieces.
 size_t part_elements(int64_t rows, int channels, int64_t segments) { return size_t(block_count(rows) + segments) * 2 * channels; }
 
 bool bad_shape(int64_t rows, int64_t channels, int64_t groups, int64_t segments, const int64_t* ptr) {
@@ -801,25 +971,15 @@ Launch make_launch(int64_t rows, int64_t channels, int64_t groups, int64_t segme
     const int64_t blocks = block_count(rows), chunk = ceil_div(rows, blocks);
     const int lanes = vectors < kThreads ? vectors : kThreads;
     l.sh = {rows, chunk, static_cast<int>(channels), static_cast<int>(groups), lanes, segments, ptr,
-            segments > 0 ? rows / segments : rows};
+            segments > 0 ? rows / segments : rows, 0};
     l.grid = dim3(static_cast<unsigned>(ceil_div(rows, chunk)), static_cast<unsigned>(ceil_div(vectors, lanes)));
     return l;
 }
 
 template <typename T, int V>
-int forward(const Launch& l, const T* x, const T* w, const T* b, double eps, int act, T* y, acc_t<T>* mean, acc_t<T>* rstd,
-            acc_t<T>* part, cudaStream_t stream) {
+int forward_chunks(const Launch& l, const T* x, const T* w, const T* b, double eps, int act, T* y, acc_t<T>* mean, acc_t<T>* rstd,
+                   acc_t<T>* part, cudaStream_t stream) {
     using A = acc_t<T>;
-    Slab slab;
-    if (short_segments(l.sh.rows, l.sh.channels, l.sh.groups, l.sh.segments, sizeof(T), V, &slab)) {
-        slab.pad_blocks = l.sh.ptr ? kSMs / 4 : 0;
-        const dim3 grid(static_cast<unsigned>(l.sh.segments + slab.pad_blocks), static_cast<unsigned>(l.sh.channels / slab.channels));
-        if (l.sh.channels / l.sh.groups % V == 0)
-            return NB200_DISPATCH_ACT(act, (short_forward_kernel<T, V, ACT, true><<<grid, kShort, 0, stream>>>(l.sh, slab, x, w, b, eps, mean,
-                                                                                                            rstd, y), launch_status()));
-        return NB200_DISPATCH_ACT(act, (short_forward_kernel<T, V, ACT, false><<<grid, kShort, 0, stream>>>(l.sh, slab, x, w, b, eps, mean,
-                                                                                                         rstd, y), launch_status()));
-    }
     stats_kernel<T, V><<<l.grid, kThreads, 0, stream>>>(l.sh, x, part);
     const int64_t items = l.sh.segments * l.sh.groups;
     if (items > 0) {
@@ -828,47 +988,118 @@ int forward(const Launch& l, const T* x, const T* w, const T* b, double eps, int
         else
             stats_join_kernel<A, 1024><<<static_cast<unsigned>(items), 1024, 0, stream>>>(l.sh, part, eps, mean, rstd);
     }
-    return NB200_DISPATCH_ACT(act, (apply_kernel<T, V, ACT><<<l.grid, kThreads, 0, stream>>>(l.sh, x, w, b, mean, rstd, y), launch_status()));
+    return NB200_DISPATCH_ACT(act, (apply_kernel<T, V, ACT><<<l.grid, kThreads, 0, stream>>>(l.sh, x, w, b, mean, rstd, y),
+                                    launch_status()));
 }
+
+// Blocks that are resident together, two to an SM; not more in a row than the row chunks' workspace is made for.
+dim3 handed_grid(const Launch& l) {
+    const unsigned row = 2 * kSMs / l.grid.y;
+    return dim3(row < l.grid.x ? row : l.grid.x, l.grid.y);
+}
+template <typename... Params, typename... Args>
+int launch_handed(void (*kernel)(Params...), dim3 grid, cudaStream_t stream, const Args&... args) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = dim3(kThreads);
+    config.stream = stream;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeCooperative;
+    attribute[0].val.cooperative = 1;
+    config.attrs = attribute;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...) == cudaSuccess ? launch_status() : NB200_ERR_CUDA;
+}
+
+template <typename T, int V>
+int forward(Launch l, const T* x, const T* w, const T* b, double eps, int act, T* y, acc_t<T>* mean, acc_t<T>* rstd, acc_t<T>* part,
+            cudaStream_t stream) {
+    Slab slab;
+    if (!short_segments(l.sh.rows, l.sh.channels, l.sh.groups, l.sh.segments, l.sh.ptr != nullptr, sizeof(T), V, &slab))
+        return forward_chunks<T, V>(l, x, w, b, eps, act, y, mean, rstd, part, stream);
+    slab.pad_blocks = l.sh.ptr ? kSMs / 4 : 0;
+    l.sh.handed = slab.handed;
+    const dim3 grid(static_cast<unsigned>(l.sh.segments + slab.pad_blocks), static_cast<unsigned>(l.sh.channels / slab.channels));
+    const int rc = l.sh.channels / l.sh.groups % V == 0
+                       ? NB200_DISPATCH_ACT(act, (short_forward_kernel<T, V, ACT, true><<<grid, kShort, 0, stream>>>(l.sh, slab, x, w, b, eps, mean,
+                                                                                                                   rstd, y), launch_status()))
+                       : NB200_DISPATCH_ACT(act, (short_forward_kernel<T, V, ACT, false><<<grid, kShort, 0, stream>>>(l.sh, slab, x, w, b, eps, mean,
+                                                                                                                    rstd, y), launch_status()));
+    if (rc != NB200_OK || slab.handed == 0) return rc;
+    return NB200_DISPATCH_ACT(act, launch_handed(handed_forward_kernel<T, V, ACT>, handed_grid(l), stream, l.sh, x, w, b, eps, mean, rstd, part, y));
+}
+
+// Workspace of the backward pass: results of the pieces; sums of dbeta and dgamma, one line of 2 x channels per segment (short
+// segments only), then one per block; the two coefficients per (segment, group).
+template <typename A>
+struct BackwardWork {
+    A *part, *segment_sums, *block_sums, *coef;
+};
 
 template <typename T, int V>
 int backward_short(const Launch& l, Slab slab, const T* dy, const T* x, const T* w, const T* b, const acc_t<T>* mean, const acc_t<T>* rstd,
-                   int act, T* dx, T* dw, T* db, acc_t<T>* part, cudaStream_t stream) {
+                   int act, T* dx, acc_t<T>* segment_sums, cudaStream_t stream) {
     slab.pad_blocks = l.sh.ptr && dx ? kSMs / 4 : 0;
     const dim3 grid(static_cast<unsigned>(l.sh.segments + slab.pad_blocks), static_cast<unsigned>(l.sh.channels / slab.channels));
-    const int rc = l.sh.channels / l.sh.groups % V == 0
-                       ? NB200_DISPATCH_ACT(act, (short_backward_kernel<T, V, ACT, true><<<grid, kShort, 0, stream>>>(
-                                                      l.sh, slab, x, dy, w, b, mean, rstd, part, dx), launch_status()))
-                       : NB200_DISPATCH_ACT(act, (short_backward_kernel<T, V, ACT, false><<<grid, kShort, 0, stream>>>(
-                                                      l.sh, slab, x, dy, w, b, mean, rstd, part, dx), launch_status()));
-    if (rc != NB200_OK || !(dw || db)) return rc;
-    column_sums_kernel<T><<<static_cast<unsigned>(ceil_div(2 * l.sh.channels, 32)), 1024, 0, stream>>>(l.sh.segments, l.sh.channels, part, db,
-                                                                                                     dw);
-    return launch_status();
+    return l.sh.channels / l.sh.groups % V == 0
+               ? NB200_DISPATCH_ACT(act, (short_backward_kernel<T, V, ACT, true><<<grid, kShort, 0, stream>>>(
+                                              l.sh, slab, x, dy, w, b, mean, rstd, segment_sums, dx), launch_status()))
+               : NB200_DISPATCH_ACT(act, (short_backward_kernel<T, V, ACT, false><<<grid, kShort, 0, stream>>>(
+                                              l.sh, slab, x, dy, w, b, mean, rstd, segment_sums, dx), launch_status()));
 }
 
+// Up to dx; dbeta and dgamma are left as one line of sums per block.
 template <typename T, int V>
 int backward_chunks(const Launch& l, const T* dy, const T* x, const T* w, const T* b, const acc_t<T>* mean, const acc_t<T>* rstd, int act,
-             T* dx, T* dw, T* db, acc_t<T>* part, cudaStream_t stream) {
-    using A = acc_t<T>;
-    A* block_sums = part + part_elements(l.sh.rows, l.sh.channels, l.sh.segments);
-    A* coef = block_sums + size_t(block_count(l.sh.rows)) * 2 * l.sh.channels;
-    int rc = NB200_DISPATCH_ACT(act, (grad_sums_kernel<T, V, ACT><<<l.grid, kThreads, 0, stream>>>(l.sh, x, dy, w, b, mean, rstd, part,
-                                                                                                 block_sums), launch_status()));
-    if (rc != NB200_OK) return rc;
-    if (dw || db)
-        column_sums_kernel<T><<<static_cast<unsigned>(ceil_div(2 * l.sh.channels, 32)), 1024, 0, stream>>>(
-            l.grid.x, l.sh.channels, block_sums, db, dw);
-    if (!dx) return launch_status();
+                    T* dx, const BackwardWork<acc_t<T>>& work, cudaStream_t stream) {
+    const int rc = NB200_DISPATCH_ACT(act, (grad_sums_kernel<T, V, ACT><<<l.grid, kThreads, 0, stream>>>(
+                                                l.sh, x, dy, w, b, mean, rstd, work.part, work.block_sums), launch_status()));
+    if (rc != NB200_OK || !dx) return rc;
     const int64_t items = l.sh.segments * l.sh.groups;
     if (items > 0) {
         if (items > kSMs * 8)
-            grad_join_kernel<T, 32><<<static_cast<unsigned>(ceil_div(items, kThreads / 32)), kThreads, 0, stream>>>(l.sh, part, w, coef);
+            grad_join_kernel<T, 32><<<static_cast<unsigned>(ceil_div(items, kThreads / 32)), kThreads, 0, stream>>>(l.sh, work.part, w, work.coef);
         else
-            grad_join_kernel<T, 1024><<<static_cast<unsigned>(items), 1024, 0, stream>>>(l.sh, part, w, coef);
+            grad_join_kernel<T, 1024><<<static_cast<unsigned>(items), 1024, 0, stream>>>(l.sh, work.part, w, work.coef);
     }
-    return NB200_DISPATCH_ACT(act, (grad_apply_kernel<T, V, ACT><<<l.grid, kThreads, 0, stream>>>(l.sh, x, dy, w, b, mean, rstd, coef, dx),
-                                    launch_status()));
+    return NB200_DISPATCH_ACT(act, (grad_apply_kernel<T, V, ACT><<<l.grid, kThreads, 0, stream>>>(l.sh, x, dy, w, b, mean, rstd, work.coef,
+                                                                                                        dx), launch_status()));
+}
+
+// W: channels of a thread in the row chunks, V: in the blocks of short segments.
+template <typename T, int V, int W>
+int backward(int64_t rows, int64_t channels, int64_t groups, int64_t segments, const int64_t* ptr, const T* dy, const T* x, const T* w,
+             const T* b, const acc_t<T>* mean, const acc_t<T>* rstd, int act, T* dx, T* dw, T* db, acc_t<T>* at, cudaStream_t stream) {
+    BackwardWork<acc_t<T>> work;
+    work.part = at;
+    work.segment_sums = work.part + part_elements(rows, static_cast<int>(channels), segments);
+    work.block_sums = work.segment_sums + size_t(line_sums(segments)) * 2 * channels;
+    work.coef = work.block_sums + size_t(block_count(rows)) * 2 * channels;
+    Launch chunks = make_launch<W>(rows, channels, groups, segments, ptr);
+    Slab slab;
+    const acc_t<T>* lines = work.block_sums;
+    int64_t count = chunks.grid.x;
+    int rc;
+    if (short_segments(rows, channels, groups, segments, ptr != nullptr, sizeof(T), V, &slab)) {
+        Launch blocks = make_launch<V>(rows, channels, groups, segments, ptr);
+        blocks.sh.handed = chunks.sh.handed = slab.handed;
+        // with a line per segment and per block the two have to follow one another; else the pieces' place is free
+        acc_t<T>* sums = slab.handed != 0 ? work.segment_sums : work.part;
+        rc = backward_short<T, V>(blocks, slab, dy, x, w, b, mean, rstd, act, dx, sums, stream);
+        lines = sums;
+        count = segments;
+        if (rc == NB200_OK && slab.handed != 0) {
+            const dim3 grid = handed_grid(chunks);
+            rc = NB200_DISPATCH_ACT(act, launch_handed(handed_backward_kernel<T, W, ACT>, grid, stream, chunks.sh, x, dy, w, b, mean, rstd, work.part,
+                                                       work.block_sums, work.coef, dx));
+            count += grid.x;
+        }
+    } else {
+        rc = backward_chunks<T, W>(chunks, dy, x, w, b, mean, rstd, act, dx, work, stream);
+    }
+    if (rc != NB200_OK || !(dw || db)) return rc;
+    column_sums_kernel<T><<<static_cast<unsigned>(ceil_div(2 * channels, 32)), 1024, 0, stream>>>(count, static_cast<int>(channels), lines, db, dw);
+    return launch_status();
 }
 
 }  // namespace
@@ -879,7 +1110,7 @@ using namespace nb200;
 extern "C" size_t nb200_group_norm_workspace_bytes(int64_t rows, int64_t channels, int64_t groups, int64_t segments, int dtype) {
     if (rows < 0 || channels < 1 || groups < 1 || segments < 0) return 0;
     const size_t a = dtype == NB200_F64 ? 8 : 4;
-    return a * (part_elements(rows, static_cast<int>(channels), segments) + size_t(block_count(rows)) * 2 * channels +
+    return a * (part_elements(rows, static_cast<int>(channels), segments) + size_t(line_sums(segments) + block_count(rows)) * 2 * channels +
                 size_t(segments) * groups * 2);
 }
 
@@ -936,18 +1167,13 @@ extern "C" int nb200_group_norm_backward(int64_t rows, int64_t channels, int64_t
         A* part = static_cast<A*>(work);
         T *dxt = static_cast<T*>(dx), *dwt = static_cast<T*>(dweight), *dbt = static_cast<T*>(dbias);
         constexpr int V = few_channels<T>(), W = 16 / sizeof(T);
-        Slab slab;
-        if (channels % V == 0) {
-            if (short_segments(rows, channels, groups, segments, sizeof(T), V, &slab))
-                return backward_short<T, V>(make_launch<V>(rows, channels, groups, segments, ptr), slab, gt, xt, wt, bt, m, rs, activation, dxt,
-                                            dwt, dbt, part, as_stream(stream));
-        } else if (short_segments(rows, channels, groups, segments, sizeof(T), 1, &slab)) {
-            return backward_short<T, 1>(make_launch<1>(rows, channels, groups, segments, ptr), slab, gt, xt, wt, bt, m, rs, activation, dxt,
-                                        dwt, dbt, part, as_stream(stream));
-        }
-        return channels % W == 0 ? backward_chunks<T, W>(make_launch<W>(rows, channels, groups, segments, ptr), gt, xt, wt, bt, m, rs, activation,
-                                                         dxt, dwt, dbt, part, as_stream(stream))
-                                 : backward_chunks<T, 1>(make_launch<1>(rows, channels, groups, segments, ptr), gt, xt, wt, bt, m, rs, activation,
-                                                         dxt, dwt, dbt, part, as_stream(stream));
+        auto run = [&](auto v, auto u) {
+            return backward<T, decltype(v)::value, decltype(u)::value>(rows, channels, groups, segments, ptr, gt, xt, wt, bt, m, rs, activation, dxt,
+                                                                       dwt, dbt, part, as_stream(stream));
+        };
+        using One = std::integral_constant<int, 1>;
+        if (channels % W == 0) return run(std::integral_constant<int, V>(), std::integral_constant<int, W>());
+        if (channels % V == 0) return run(std::integral_constant<int, V>(), One());
+        return run(One(), One());
     }()));
 }

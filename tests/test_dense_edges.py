@@ -9,7 +9,7 @@ import torch
 import numml_b200.functional as F
 import numml_b200.nn as nn
 from numml_b200 import numml_torch_cpp
-from test_dense_ops import CURVE, act64, check, normal, tiny, units
+from test_dense_ops import CURVE, TYPES, act64, check, normal, run_group_norm, tiny, units
 
 gpu = pytest.mark.gpu
 
@@ -249,3 +249,100 @@ def test_linear_long_sums_do_not_drift(which, dtype):
     assert error.abs().max() <= u * 1.01 + 2.0 ** -15
     assert error.mean().abs() <= 2.0 ** -15 + 6 * u / math.sqrt(got.numel()), error.mean().item()
     numml_torch_cpp.check_status()
+
+
+# ---------------------------------------------------------------------------------------------------------
+# long graphs among short ones
+# ---------------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("C,groups,act", [(64, 8, "gelu"), (33, 3, None), (36, 2, "silu")])
+def test_group_norm_long_graphs_among_short_ones(C, groups, act, dtype):
+    """Long graphs at the start, in the middle, side by side and at the end of a batch of short and empty ones, with rows
+    before the first and behind the last."""
+    gen = torch.Generator().manual_seed(1)
+    short = lambda n: torch.randint(0, 9, (n,), generator=gen).tolist()
+    sizes = [9001] + short(150) + [0, 12007, 4999, 8000, 0] + short(200) + [7003, 1, 0]
+    ptr = [5]
+    for s in sizes:
+        ptr.append(ptr[-1] + s)
+    run_group_norm(normal((ptr[-1] + 70, C), 9, dtype, 1.0, 2.0), groups, dtype, act, ptr=ptr, seed=5)
+    run_group_norm(normal((ptr[-1], C), 8, dtype, 1.0, 2.0), groups, dtype, act, affine=False, ptr=ptr, seed=6)
+
+
+@gpu
+def test_group_norm_broken_row_pointers_of_a_long_batch_touch_nothing_else():
+    rows, C = 50000, 64
+    ptr = torch.randint(-60000, 120000, (300,), generator=torch.Generator().manual_seed(2)).cuda()
+    store = torch.full((rows + 200, C), 7.0, device="cuda")
+    x = store[100:rows + 100].normal_().requires_grad_(True)
+    y = F.group_norm(x, 8, ptr=ptr)
+    torch.autograd.grad(y, x, torch.ones_like(y))
+    torch.cuda.synchronize()
+    assert (store[:100] == 7).all() and (store[rows + 100:] == 7).all()
+    good = torch.tensor([0, 30000, 30010, rows], device="cuda")
+    assert torch.isfinite(F.group_norm(x, 8, ptr=good)).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_group_norm_one_long_graph_is_not_left_to_one_block(dtype):
+    """One graph of most of a batch's rows beside 511 of one row: a training step of it takes no more than a few times
+    that of equal graphs (a block that had the long one to itself took 20 to 30 times as long)."""
+    rows, graphs = 61440, 512
+    X, dY = normal((rows, 128), 1, dtype).cuda().requires_grad_(True), normal((rows, 128), 2, dtype).cuda()
+    equal = torch.arange(graphs + 1, device="cuda") * (rows // graphs)
+    skewed = torch.arange(graphs + 1, device="cuda")
+    skewed[-1] = rows
+
+    def time(ptr):
+        best = math.inf
+        for _ in range(6):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            torch.cuda.synchronize()
+            a.record()
+            for _ in range(5):
+                torch.autograd.grad(F.group_norm(X, 16, activation="gelu", ptr=ptr), X, dY)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    assert time(skewed) < 8 * time(equal)
+
+
+@gpu
+def test_group_norm_long_batch_captured_and_on_two_streams():
+    """The pass over long graphs under capture (two graphs, replayed in turn with other row pointers) and on two streams."""
+    rows, C = 30000, 64
+    X, dY = normal((rows, C), 1, torch.float32).cuda(), normal((rows, C), 2, torch.float32).cuda()
+    w = normal((C,), 3, torch.float32, 0.3, 1.0).cuda()
+    ptrs = [torch.tensor(p, device="cuda") for p in ([0, 20000, 20001, 29000, 30000], [0, 10, 20, 30, 30000], [0, 7500, 15000, 22500, 30000])]
+    ptrs.append(torch.arange(5, device="cuda") * 600)                     # none that is long
+
+    def step(ptr):
+        x, wl = X.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        y = F.group_norm(x, 8, wl, activation="silu", ptr=ptr)
+        return [y.detach(), *torch.autograd.grad(y, (x, wl), dY)]
+
+    want = [[t.clone() for t in step(p)] for p in ptrs]
+    graphs = []
+    for _ in range(2):
+        ptr = ptrs[0].clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(ptr)
+        graphs.append((g, ptr, out))
+    for q in (1, 0, 3, 2, 1):
+        g, ptr, out = graphs[q % 2]
+        ptr.copy_(ptrs[q])
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want[q])), q
+    streams, got = [torch.cuda.Stream() for _ in range(2)], {}
+    torch.cuda.synchronize()
+    for q in (0, 1, 2, 3, 0, 1):
+        with torch.cuda.stream(streams[q % 2]):
+            got[q] = step(ptrs[q])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for q in got for a, b in zip(got[q], want[q]))
