@@ -137,7 +137,7 @@ class Dropout(torch.nn.Module):
     ``seed`` (drawn from torch's generator when None) and a counter of the calls made so far name the mask.
     They live on the host, where a captured CUDA graph would freeze them, so a call under capture raises
     unless the layer was made with ``capturable=True``: then they are a buffer on the device that every
-    call advances, and a replayed graph takes new masks.
+    call advances, and a replayed graph takes new masks.  ``state_dict`` holds both, in either form.
 
     A forward pass that is run again inside the backward pass (``torch.utils.checkpoint``) has to see the mask of
     the first run, and the layer cannot tell which call that was.  Take ``call = layer.next_call()`` in front of the
@@ -149,13 +149,35 @@ class Dropout(torch.nn.Module):
             raise RuntimeError(f"dropout probability must be in [0, 1], got {p}")
         self.p = p
         self.seed = int(torch.randint(0, 1 << 62, (1,))) if seed is None else int(seed)
+        if not 0 <= self.seed < 1 << 64:
+            raise RuntimeError(f"seed must be in [0, 2**64), got {self.seed}")
         self.calls = 0
         if capturable:
-            # the words are int64: a seed of 2**63 and above is stored as the negative number of the same bits
-            word = self.seed - (1 << 64) if self.seed >= 1 << 63 else self.seed
-            self.register_buffer("state", torch.tensor([word, 0], dtype=torch.int64), persistent=False)
+            self.register_buffer("state", self._words(), persistent=False)
         else:
             self.state = None
+
+    def _words(self):
+        """[seed, calls] as int64: a seed of 2**63 and above is the negative number of the same bits."""
+        return torch.tensor([self.seed - (1 << 64) if self.seed >= 1 << 63 else self.seed, self.calls], dtype=torch.int64)
+
+    # seed and counter go into state_dict, so that a run that is resumed takes the masks that would have come next
+    def get_extra_state(self):
+        return self._words() if self.state is None else self.state.detach().cpu().clone()
+
+    def set_extra_state(self, words):
+        seed, calls = (int(v) for v in words)
+        self.seed = seed % (1 << 64)
+        if self.state is None:
+            self.calls = calls
+        else:
+            self.state.copy_(words)                    # in place: a captured graph reads it there
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        key = prefix + "_extra_state"
+        if key in missing_keys:                        # saved before there was one: seed and counter stay
+            missing_keys.remove(key)
 
     def _refuse_capture(self):
         if self.state is None and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():

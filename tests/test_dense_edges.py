@@ -107,6 +107,37 @@ def test_dropout_recomputed_on_the_host(use_reentrant, capturable, monkeypatch):
     assert torch.equal(drop(None, X) != 0, want)
 
 
+@pytest.mark.parametrize("seed", [11, 2 ** 64 - 3, None])
+@pytest.mark.parametrize("first", [False, True])
+@pytest.mark.parametrize("second", [False, True])
+def test_dropout_resumed_from_a_state_dict(first, second, seed, monkeypatch, tmp_path):
+    """A layer that is loaded goes on with the masks that the saved one would have taken next, whichever form either has."""
+    offsets = []
+    monkeypatch.setattr(nn.F, "dropout", lambda X, p, seed, offset=0, residual=None: offsets.append(
+        [int(seed[0]) % 2 ** 64, int(seed[1])] if isinstance(seed, torch.Tensor) else [seed, offset]) or X)
+    net = nn.Sequential(nn.Dropout(0.5, seed=seed, capturable=first), nn.SeqWrapper(torch.nn.Linear(2, 2)))
+    X = torch.ones(3, 2)
+    for _ in range(3):
+        net.modlist[0](None, X)
+    torch.save(net.state_dict(), tmp_path / "net.pt")
+    other = nn.Sequential(nn.Dropout(0.5, seed=5, capturable=second), nn.SeqWrapper(torch.nn.Linear(2, 2)))
+    place = other.modlist[0].state.data_ptr() if second else None
+    other.load_state_dict(torch.load(tmp_path / "net.pt", weights_only=True))
+    net.modlist[0](None, X), other.modlist[0](None, X), other.modlist[0](None, X)
+    assert offsets[3] == offsets[4] == [net.modlist[0].seed, 3] and offsets[5] == [net.modlist[0].seed, 4]
+    assert not second or other.modlist[0].state.data_ptr() == place
+    old = {k: v for k, v in net.state_dict().items() if "_extra_state" not in k}
+    other.load_state_dict(old)                                   # strict: saved before there was such a state
+    other.modlist[0](None, X)
+    assert offsets[-1] == [net.modlist[0].seed, 5]
+
+
+def test_dropout_seed_out_of_range():
+    for seed in (-1, 2 ** 64):
+        with pytest.raises(RuntimeError, match="seed"):
+            nn.Dropout(0.5, seed=seed)
+
+
 @gpu
 @pytest.mark.parametrize("use_reentrant", [False, True])
 @pytest.mark.parametrize("capturable", [False, True])
