@@ -432,7 +432,6 @@ int backward(int64_t m, int64_t k, int64_t n, const T* dy, int64_t ldd, const T*
         rc = product<T, false, false, NB200_ACT_NONE>(k, n, m, split, x, ldx, g, ldg, {nullptr, nullptr, 0, nullptr, nullptr, partial}, status,
                                                       stream);
         if (rc != NB200_OK) return rc;
-        if (rc != NB200_OK) return rc;
         join_dw = Join<T>{k * n, static_cast<int>(split.parts), partial, dw};
     }
     return join_parts<T>(join_dw, join_db, stream);
