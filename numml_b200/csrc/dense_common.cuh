@@ -47,6 +47,14 @@ __device__ __forceinline__ void store_acc(T* p, const acc_t<T> (&in)[V]) {
 __device__ __forceinline__ float tanh_acc(float v) { return tanhf(v); }
 __device__ __forceinline__ double tanh_acc(double v) { return tanh(v); }
 
+__device__ __forceinline__ float abs_acc(float v) { return fabsf(v); }
+__device__ __forceinline__ double abs_acc(double v) { return fabs(v); }
+// In 32 bits the short forms, good to a few units in the last place (the exponential to 2 + 1.2 |v|).
+__device__ __forceinline__ float exp_acc(float v) { return __expf(v); }
+__device__ __forceinline__ double exp_acc(double v) { return exp(v); }
+__device__ __forceinline__ float reciprocal(float v) { return __fdividef(1.f, v); }
+__device__ __forceinline__ double reciprocal(double v) { return 1.0 / v; }
+
 // 1 / (1 + exp(-z)).  In 32 bits with the short exponential and division, whose errors of a few units relative to
 // exp(-z) are multiplied by exp(-z) / (1 + exp(-z)): they fade where they grow.  exp(-z) = infinity gives 0.
 __device__ __forceinline__ float logistic(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
@@ -96,9 +104,9 @@ __device__ __forceinline__ A activate_slope(A z) {
         const A cdf = normal_cdf(z, e);
         return cdf + z * A(kInvRoot2Pi) * e;
     }
-    if constexpr (ACT == NB200_ACT_TANH) {                        // 1 - tanh^2 = 4 s (1 - s) with s = logistic(2 z)
-        const A s = logistic(A(2) * z);
-        return A(4) * s * (A(1) - s);
+    if constexpr (ACT == NB200_ACT_TANH) {                        // 1 - tanh^2 = 4 e / (1 + e)^2 with e = exp(-2 |z|): nothing cancels
+        const A e = exp_acc(A(-2) * abs_acc(z)), r = reciprocal(A(1) + e);
+        return A(4) * e * r * r;
     }
     return A(1);
 }

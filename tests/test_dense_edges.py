@@ -377,3 +377,26 @@ def test_group_norm_long_batch_captured_and_on_two_streams():
             got[q] = step(ptrs[q])
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for q in got for a, b in zip(got[q], want[q]))
+
+
+# ---------------------------------------------------------------------------------------------------------
+# the slope of tanh
+# ---------------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("m", [40, 3000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64], ids=str)
+def test_slope_of_tanh_to_the_last_places(dtype, m):
+    """The slope relative to itself, for z of both signs: 4 e / (1 + e)^2, e = exp(-2 |z|).  The exponential is good to
+    2 + 1.173 * 2 |z| units in the last place (the short one of 32 bits; the other to one), twice ua each; two
+    divisions and four products come to 16 ua more."""
+    _, ua = units(dtype)
+    z = torch.linspace(-40, 40, m, dtype=torch.float64).to(dtype)
+    one = torch.ones(1, 1, dtype=dtype)
+    x = z[:, None].cuda().requires_grad_(True)
+    (got,) = torch.autograd.grad(F.linear(x, one.cuda(), None, "tanh"), x, torch.ones(m, 1, dtype=dtype, device="cuda"))
+    e = torch.exp(-2 * z.double().abs())
+    ref = 4 * e / (1 + e) ** 2
+    bound = ref * ua * (16 + 2 * (2 + 2.35 * z.double().abs())) + (ref * 2.0 ** -50 if dtype == torch.float64 else 0)
+    check(got[:, 0], ref, bound + 2.0 ** -125, "slope")
+    y = F.group_norm(torch.stack([z, -z], 1).cuda().requires_grad_(True), 2, activation="tanh")     # the same slope there
+    assert torch.isfinite(torch.autograd.grad(y.sum(), y.grad_fn.next_functions[0][0].variable)[0]).all()
