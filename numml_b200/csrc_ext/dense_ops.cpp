@@ -124,8 +124,10 @@ struct Needs {
     bool operator()(bool present) { return present && ctx->needs_input_grad(next++); }
 };
 
-// A backward pass under capture may not hand a gradient to a leaf that a live eager graph holds on another stream: the
+// A backward pass under capture may not hand a gradient to a leaf that a live eager graph holds on the default stream: the
 // engine would make that stream wait for the capture, which invalidates it or ends the process.  Raised here instead.
+// (Another stream that waits becomes part of the capture, and the engine joins it again: warming up on a side stream and
+// keeping the results is fine.)
 void refuse_foreign_accumulation() {
     const auto current = at::cuda::getCurrentCUDAStream();
     cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
@@ -140,9 +142,9 @@ void refuse_foreign_accumulation() {
             if (it == info->end() || !it->second.should_execute()) continue;
         }
         const auto stream = edge.function->stream();
-        TORCH_CHECK(!stream.has_value() || *stream == current.unwrap(),
-                    "a backward pass is being captured into a CUDA graph while an eager graph of the same leaf is alive on another "
-                    "stream; drop the eager results first, or make the leaf inside the capture");
+        TORCH_CHECK(!stream.has_value() || *stream == current.unwrap() || at::cuda::CUDAStream(*stream).stream() != nullptr,
+                    "a backward pass is being captured into a CUDA graph while an eager graph of the same leaf is alive on the default "
+                    "stream; drop the eager results first, run them on another stream, or make the leaf inside the capture");
     }
 }
 

@@ -400,3 +400,38 @@ def test_slope_of_tanh_to_the_last_places(dtype, m):
     check(got[:, 0], ref, bound + 2.0 ** -125, "slope")
     y = F.group_norm(torch.stack([z, -z], 1).cuda().requires_grad_(True), 2, activation="tanh")     # the same slope there
     assert torch.isfinite(torch.autograd.grad(y.sum(), y.grad_fn.next_functions[0][0].variable)[0]).all()
+
+
+# ---------------------------------------------------------------------------------------------------------
+# captures
+# ---------------------------------------------------------------------------------------------------------
+@gpu
+def test_capture_after_a_warm_up_whose_results_live():
+    """The usual way to capture a training step: warm-up on a side stream, whose last results are still there when the
+    step is captured."""
+    net = nn.Sequential(nn.Linear(32, 48, activation="gelu"), nn.GroupNorm(4, 48, activation="silu"),
+                        nn.Dropout(0.5, seed=3, capturable=True), nn.Linear(48, 24)).cuda()
+    X = normal((700, 32), 1, torch.float32).cuda().requires_grad_(True)
+    leaves = [X, *net.parameters()]
+
+    def step():
+        for t in leaves:
+            t.grad = None
+        net.modlist[2].state[1].zero_()
+        y = net(None, X).square().sum()
+        y.backward()
+        return y
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            alive = step()
+    torch.cuda.current_stream().wait_stream(side)
+    want = [t.grad.clone() for t in leaves]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = step()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, alive) and all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
