@@ -50,12 +50,14 @@ struct Matrix {
     int64_t ld;
 };
 // A [rows, cols] matrix over t's memory (a copy only where rows are not evenly strided runs) and its row stride.
-Matrix rows_of(const Tensor& t, int64_t cols) {
+// Lazily negated values (the imaginary part of a conjugate) are negated first, here and below.
+Matrix rows_of(const Tensor& given, int64_t cols) {
+    const Tensor t = given.resolve_neg();
     if (t.dim() == 2 && (cols <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= cols)) return {t, t.size(0) > 1 ? t.stride(0) : cols};
     return {t.contiguous(), cols};
 }
 Tensor aligned(const Tensor& t) {
-    Tensor c = t.contiguous();
+    Tensor c = t.resolve_neg().contiguous();
     return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
 }
 int64_t row_count(const Tensor& X) {
@@ -64,7 +66,7 @@ int64_t row_count(const Tensor& X) {
     return n;
 }
 Tensor or_empty(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
-Tensor contiguous_or_empty(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+Tensor contiguous_or_empty(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
 // Tangents of forward-mode differentiation are refused: no operator passes them on, and a result without one reads as zero.
 void refuse_tangents(std::initializer_list<std::reference_wrapper<const Tensor>> operands) {
     if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;

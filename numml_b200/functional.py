@@ -54,7 +54,9 @@ def _check_operands(X, **others):
 
 
 def _rows(t, cols):
-    """A [rows, cols] matrix over t's memory (a copy only where rows are not evenly strided runs) and its row stride."""
+    """A [rows, cols] matrix over t's memory (a copy only where rows are not evenly strided runs) and its row stride.
+    Lazily negated values (the imaginary part of a conjugate) are negated first, here and below."""
+    t = t.resolve_neg()
     if t.ndim == 2 and (cols <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= cols):
         return t, (t.stride(0) if t.shape[0] > 1 else cols)
     return t.contiguous().view(-1, cols) if cols > 0 else t.reshape(math.prod(t.shape[:-1]), 0), cols
@@ -62,8 +64,13 @@ def _rows(t, cols):
 
 def _aligned(t):
     """Contiguous and on a 16-byte boundary, as the vector loads need it."""
-    t = t.contiguous()
+    t = t.resolve_neg().contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _vector(t):
+    """Contiguous, or None."""
+    return t.resolve_neg().contiguous() if t is not None else None
 
 
 def _shim(*operands):
@@ -104,7 +111,7 @@ def _linear_forward(X, weights, bias, residual, act, keep_z):
     x, ldx = _rows(X, K)
     w, ldw = _rows(weights, N)
     r, ldr = _rows(residual, N) if residual is not None else (None, 0)
-    b = bias.contiguous() if bias is not None else None
+    b = _vector(bias)
     M = x.shape[0]
     with _on(X.device):
         y = torch.empty(X.shape[:-1] + (N,), dtype=X.dtype, device=X.device)
@@ -192,8 +199,8 @@ def _segments(X, ptr):
 
 def _group_norm_forward(X, groups, weight, bias, eps, act, ptr):
     x = _aligned(X)
-    w = weight.contiguous() if weight is not None else None
-    b = bias.contiguous() if bias is not None else None
+    w = _vector(weight)
+    b = _vector(bias)
     p = ptr.contiguous() if ptr is not None else None
     C = X.shape[-1]
     rows, segments = _segments(X, ptr)
@@ -210,8 +217,8 @@ def _group_norm_forward(X, groups, weight, bias, eps, act, ptr):
 
 def _group_norm_backward(dY, X, groups, weight, bias, act, ptr, stats, want_x, want_w, want_b):
     x, g = _aligned(X), _aligned(dY)
-    w = weight.contiguous() if weight is not None else None
-    b = bias.contiguous() if bias is not None else None
+    w = _vector(weight)
+    b = _vector(bias)
     p = ptr.contiguous() if ptr is not None else None
     C = X.shape[-1]
     rows, segments = _segments(X, ptr)

@@ -435,3 +435,29 @@ def test_capture_after_a_warm_up_whose_results_live():
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(y, alive) and all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
+
+
+# ---------------------------------------------------------------------------------------------------------
+# lazily negated operands
+# ---------------------------------------------------------------------------------------------------------
+@gpu
+def test_lazily_negated_operands():
+    """Operands whose memory holds the negated values (torch keeps the imaginary part of a conjugate so)."""
+    lazy = lambda t: torch._neg_view(-t)
+    X, W, v, R, dY = (normal(s, q, torch.float32).cuda() for q, s in enumerate(((300, 16), (16, 16), (16,), (300, 16), (300, 16))))
+    column = torch.view_as_complex(torch.stack((R[:, :1], X[:, :1]), -1)).conj().imag                 # one channel: any stride will do
+    assert lazy(X).is_neg() and column.is_neg()
+
+    def run(X, W, v, R, dY, column):
+        leaves = [t.detach().requires_grad_(True) for t in (X, W, v, R)]
+        x, w, b, r = leaves
+        out = []
+        for y in (F.linear(x, w, b, "silu", r), F.group_norm(x, 4, b, v, activation="gelu"), F.dropout(x, 0.3, 5, residual=r)):
+            out += [y, *torch.autograd.grad(y, leaves, dY, allow_unused=True)]
+        with torch.no_grad():
+            out += [F.linear(column, w[:1]), F.linear(x[:3], w), F.group_norm(column, 1), F.dropout(column, 0.3, 5)]
+        return [t for t in out if t is not None]
+
+    plain = run(X, W, v, R, dY, -X[:, :1])
+    for got, want in zip(run(*(lazy(t) for t in (X, W, v, R, dY)), column), plain):
+        assert torch.equal(got, want)
