@@ -79,9 +79,11 @@ struct ChunkPieces {
 };
 
 // The segments of more than sh.handed rows as an array of their own: they follow one another in it, and each block of the
-// grid has an equal run of its rows.  There are fewer than kMostHanded of them (the host sees to that; of broken row
-// pointers some are left out).
-constexpr int kMostHanded = 64;
+// grid has an equal run of its rows.  There are at most kMostHanded (the host sees to that; of broken row pointers some are
+// left out).  Among few segments a block looks at all of them (512: 2.3 us a launch that finds none); among more it
+// searches: each long segment holds a row whose number is a multiple of sh.handed, so there are rows / sh.handed searches
+// (3.8 us), however many segments there are.
+constexpr int kMostHanded = 72, kFewSegments = 2048;
 struct HandedPieces {
     int count;
     int segment[kMostHanded];
@@ -92,17 +94,29 @@ struct HandedPieces {
     __device__ void find(const Shape& sh) {              // this object is in shared memory; all threads of the block
         if (threadIdx.x == 0) count = 0;
         __syncthreads();
-        for (int64_t s = threadIdx.x; s < sh.segments; s += kThreads)
-            if (segment_begin(sh, s + 1) - segment_begin(sh, s) > sh.handed) {
-                const int q = atomicAdd(&count, 1);
-                if (q < kMostHanded) found[q] = static_cast<int>(s);
+        auto add = [&](int64_t s) {
+            const int q = atomicAdd(&count, 1);
+            if (q < kMostHanded) found[q] = static_cast<int>(s);
+        };
+        const int64_t row = threadIdx.x * sh.handed;
+        if (sh.segments <= kFewSegments) {
+            for (int64_t s = threadIdx.x; s < sh.segments; s += kThreads)
+                if (segment_begin(sh, s + 1) - segment_begin(sh, s) > sh.handed) add(s);
+        } else if (threadIdx.x < kMostHanded && row < sh.rows) {
+            int64_t end;
+            const int64_t s = find_segment(sh, row, sh.rows, end);
+            if (s >= 0 && s < sh.segments) {
+                const int64_t first = segment_begin(sh, s);          // a segment that holds an earlier such row has been found there
+                if (segment_begin(sh, s + 1) - first > sh.handed && (row == 0 || first > row - sh.handed)) add(s);
             }
+        }
         __syncthreads();
-        if (threadIdx.x == 0 && count > kMostHanded) count = kMostHanded;
+        if (threadIdx.x == 0) count = min(count, kMostHanded);
         __syncthreads();
         if (threadIdx.x < count) {                       // in ascending order, whoever came first
             int rank = 0;
-            for (int q = 0; q < count; ++q) rank += found[q] < found[threadIdx.x];
+            for (int q = 0; q < count; ++q)
+                rank += found[q] < found[threadIdx.x] || (found[q] == found[threadIdx.x] && q < threadIdx.x);
             segment[rank] = found[threadIdx.x];
         }
         __syncthreads();
@@ -110,7 +124,7 @@ struct HandedPieces {
             start[0] = 0;
             for (int q = 0; q < count; ++q) {
                 begin[q] = segment_begin(sh, segment[q]);
-                start[q + 1] = start[q] + segment_begin(sh, segment[q] + 1) - begin[q];
+                start[q + 1] = start[q] + max(int64_t(0), segment_begin(sh, segment[q] + 1) - begin[q]);
             }
         }
         __syncthreads();
@@ -893,7 +907,7 @@ int64_t block_count(int64_t rows) {
 // Whether the one-block-per-segment kernels run, and with which slabs of channels.  They need segments that stay in
 // a block's L1 on average (a slab of one up to 128 KB) and an array of at most 8 MB a slab; beyond that the row chunks
 // take over.  A single block reads about 20 GB/s, so a long segment among short ones would be waited for: in an
-// array above 512 KB a slab, segments above 128 KB a slab (fewer than 64 of them) are handed over to one more launch,
+// array above 512 KB a slab, segments above 128 KB a slab are handed over to one more launch,
 // which finds none in most batches.  Measured, forward / backward of 61,441 rows x 128 bfloat16 in 512 graphs, one of
 // which has all rows but 511: 47 / 76 us, with that graph in one block 581 / 1166, in row chunks 397 / 397; the launch
 // costs equal graphs 4 us (23 -> 28 forward).  At 512 KB (8192 rows in 64 graphs) the long one in one block
@@ -904,7 +918,6 @@ int64_t block_count(int64_t rows) {
 // 57, with four channels to a thread 31 / 51 (clusters of 2 to 8 blocks per graph were no faster: 34-41 / 67-72); the row
 // chunks 82 / 117 us in six launches.
 constexpr int64_t kAlone = 512 * 1024, kInBlock = 128 * 1024;
-constexpr int64_t kMostSegments = 16384;             // of a batch that may hand some over: every block of that launch looks through them
 bool short_segments(int64_t rows, int64_t channels, int64_t groups, int64_t segments, bool ragged, size_t size, int V, Slab* slab) {
     if (segments < 1 || segments > 65535 * 16) return false;
     const int64_t width = channels / groups;
@@ -927,7 +940,7 @@ bool short_segments(int64_t rows, int64_t channels, int64_t groups, int64_t segm
     const int64_t line = in_slab * width * int64_t(size);
     if (rows / segments * line > kInBlock || rows * line > 8 * 1024 * 1024) return false;
     slab->handed = ragged && rows * line > kAlone ? kInBlock / line : 0;
-    if (slab->handed != 0 && (segments > kMostSegments || ceil_div(channels, kThreads) > 2 * kSMs)) return false;
+    if (slab->handed != 0 && (ceil_div(rows, slab->handed) > kMostHanded || ceil_div(channels, kThreads) > 2 * kSMs)) return false;
     if (groups / in_slab > 65535) return false;
     slab->channels = static_cast<int>(in_slab * width);
     slab->lanes = static_cast<int>(in_slab * width / V);
@@ -942,11 +955,11 @@ bool short_segments(int64_t rows, int64_t channels, int64_t groups, int64_t segm
     return true;
 }
 
-// Lines of sums for segments beside those for blocks: a batch that may hand segments over needs both.
-int64_t line_sums(int64_t segments) { return segments <= kMostSegments ? segments : 0; }
-
-// Partial results of the pieces.
-size_t part_elements(int64_t rows, int channels, int64_t segments) { return size_t(block_count(rows) + segments) * 2 * channels; }
+// The workspace: a line of 2 x channels values per block and per segment; one per block, and kMostHanded; two values per
+// (segment, group).  The first holds the pieces' partial results and the second the blocks' sums of dbeta and dgamma, or,
+// in the backward pass over short segments, the first these sums per segment and per block, and the second the pieces.
+size_t first_elements(int64_t rows, int64_t channels, int64_t segments) { return size_t(block_count(rows) + segments) * 2 * channels; }
+size_t second_elements(int64_t rows, int64_t channels) { return size_t(block_count(rows) + kMostHanded) * 2 * channels; }
 
 bool bad_shape(int64_t rows, int64_t channels, int64_t groups, int64_t segments, const int64_t* ptr) {
     return rows < 0 || channels < 1 || channels > (1 << 20) || groups < 1 || channels % groups != 0 || segments < 0 ||
@@ -1029,13 +1042,6 @@ int forward(Launch l, const T* x, const T* w, const T* b, double eps, int act, T
     return NB200_DISPATCH_ACT(act, launch_handed(handed_forward_kernel<T, V, ACT>, handed_grid(l), stream, l.sh, x, w, b, eps, mean, rstd, part, y));
 }
 
-// Workspace of the backward pass: results of the pieces; sums of dbeta and dgamma, one line of 2 x channels per segment (short
-// segments only), then one per block; the two coefficients per (segment, group).
-template <typename A>
-struct BackwardWork {
-    A *part, *segment_sums, *block_sums, *coef;
-};
-
 template <typename T, int V>
 int backward_short(const Launch& l, Slab slab, const T* dy, const T* x, const T* w, const T* b, const acc_t<T>* mean, const acc_t<T>* rstd,
                    int act, T* dx, acc_t<T>* segment_sums, cudaStream_t stream) {
@@ -1051,18 +1057,18 @@ int backward_short(const Launch& l, Slab slab, const T* dy, const T* x, const T*
 // Up to dx; dbeta and dgamma are left as one line of sums per block.
 template <typename T, int V>
 int backward_chunks(const Launch& l, const T* dy, const T* x, const T* w, const T* b, const acc_t<T>* mean, const acc_t<T>* rstd, int act,
-                    T* dx, const BackwardWork<acc_t<T>>& work, cudaStream_t stream) {
+                    T* dx, acc_t<T>* part, acc_t<T>* block_sums, acc_t<T>* coef, cudaStream_t stream) {
     const int rc = NB200_DISPATCH_ACT(act, (grad_sums_kernel<T, V, ACT><<<l.grid, kThreads, 0, stream>>>(
-                                                l.sh, x, dy, w, b, mean, rstd, work.part, work.block_sums), launch_status()));
+                                                l.sh, x, dy, w, b, mean, rstd, part, block_sums), launch_status()));
     if (rc != NB200_OK || !dx) return rc;
     const int64_t items = l.sh.segments * l.sh.groups;
     if (items > 0) {
         if (items > kSMs * 8)
-            grad_join_kernel<T, 32><<<static_cast<unsigned>(ceil_div(items, kThreads / 32)), kThreads, 0, stream>>>(l.sh, work.part, w, work.coef);
+            grad_join_kernel<T, 32><<<static_cast<unsigned>(ceil_div(items, kThreads / 32)), kThreads, 0, stream>>>(l.sh, part, w, coef);
         else
-            grad_join_kernel<T, 1024><<<static_cast<unsigned>(items), 1024, 0, stream>>>(l.sh, work.part, w, work.coef);
+            grad_join_kernel<T, 1024><<<static_cast<unsigned>(items), 1024, 0, stream>>>(l.sh, part, w, coef);
     }
-    return NB200_DISPATCH_ACT(act, (grad_apply_kernel<T, V, ACT><<<l.grid, kThreads, 0, stream>>>(l.sh, x, dy, w, b, mean, rstd, work.coef,
+    return NB200_DISPATCH_ACT(act, (grad_apply_kernel<T, V, ACT><<<l.grid, kThreads, 0, stream>>>(l.sh, x, dy, w, b, mean, rstd, coef,
                                                                                                         dx), launch_status()));
 }
 
@@ -1070,32 +1076,28 @@ int backward_chunks(const Launch& l, const T* dy, const T* x, const T* w, const 
 template <typename T, int V, int W>
 int backward(int64_t rows, int64_t channels, int64_t groups, int64_t segments, const int64_t* ptr, const T* dy, const T* x, const T* w,
              const T* b, const acc_t<T>* mean, const acc_t<T>* rstd, int act, T* dx, T* dw, T* db, acc_t<T>* at, cudaStream_t stream) {
-    BackwardWork<acc_t<T>> work;
-    work.part = at;
-    work.segment_sums = work.part + part_elements(rows, static_cast<int>(channels), segments);
-    work.block_sums = work.segment_sums + size_t(line_sums(segments)) * 2 * channels;
-    work.coef = work.block_sums + size_t(block_count(rows)) * 2 * channels;
+    acc_t<T>*first = at, *second = first + first_elements(rows, channels, segments), *coef = second + second_elements(rows, channels);
     Launch chunks = make_launch<W>(rows, channels, groups, segments, ptr);
     Slab slab;
-    const acc_t<T>* lines = work.block_sums;
-    int64_t count = chunks.grid.x;
+    const acc_t<T>* lines;
+    int64_t count;
     int rc;
     if (short_segments(rows, channels, groups, segments, ptr != nullptr, sizeof(T), V, &slab)) {
         Launch blocks = make_launch<V>(rows, channels, groups, segments, ptr);
         blocks.sh.handed = chunks.sh.handed = slab.handed;
-        // with a line per segment and per block the two have to follow one another; else the pieces' place is free
-        acc_t<T>* sums = slab.handed != 0 ? work.segment_sums : work.part;
-        rc = backward_short<T, V>(blocks, slab, dy, x, w, b, mean, rstd, act, dx, sums, stream);
-        lines = sums;
+        rc = backward_short<T, V>(blocks, slab, dy, x, w, b, mean, rstd, act, dx, first, stream);
+        lines = first;
         count = segments;
         if (rc == NB200_OK && slab.handed != 0) {
             const dim3 grid = handed_grid(chunks);
-            rc = NB200_DISPATCH_ACT(act, launch_handed(handed_backward_kernel<T, W, ACT>, grid, stream, chunks.sh, x, dy, w, b, mean, rstd, work.part,
-                                                       work.block_sums, work.coef, dx));
+            rc = NB200_DISPATCH_ACT(act, launch_handed(handed_backward_kernel<T, W, ACT>, grid, stream, chunks.sh, x, dy, w, b, mean, rstd, second,
+                                                       first + size_t(segments) * 2 * channels, coef, dx));
             count += grid.x;
         }
     } else {
-        rc = backward_chunks<T, W>(chunks, dy, x, w, b, mean, rstd, act, dx, work, stream);
+        rc = backward_chunks<T, W>(chunks, dy, x, w, b, mean, rstd, act, dx, first, second, coef, stream);
+        lines = second;
+        count = chunks.grid.x;
     }
     if (rc != NB200_OK || !(dw || db)) return rc;
     column_sums_kernel<T><<<static_cast<unsigned>(ceil_div(2 * channels, 32)), 1024, 0, stream>>>(count, static_cast<int>(channels), lines, db, dw);
@@ -1110,8 +1112,7 @@ using namespace nb200;
 extern "C" size_t nb200_group_norm_workspace_bytes(int64_t rows, int64_t channels, int64_t groups, int64_t segments, int dtype) {
     if (rows < 0 || channels < 1 || groups < 1 || segments < 0) return 0;
     const size_t a = dtype == NB200_F64 ? 8 : 4;
-    return a * (part_elements(rows, static_cast<int>(channels), segments) + size_t(line_sums(segments) + block_count(rows)) * 2 * channels +
-                size_t(segments) * groups * 2);
+    return a * (first_elements(rows, channels, segments) + second_elements(rows, channels) + size_t(segments) * groups * 2);
 }
 
 extern "C" int nb200_group_norm_forward(int64_t rows, int64_t channels, int64_t groups, int64_t segments, const int64_t* ptr,

@@ -302,6 +302,15 @@ def test_group_norm_long_graphs_among_short_ones(C, groups, act, dtype):
 
 
 @gpu
+def test_group_norm_long_graphs_among_very_many():
+    """More graphs than rows, most of them empty, and as many long ones as there can be."""
+    ptr = [0]
+    for q in range(13):
+        ptr += [ptr[-1]] * 3000 + [ptr[-1] + 4200 + q] + [ptr[-1] + 4200 + q + 1]
+    run_group_norm(normal((ptr[-1], 32), 9, torch.float32, 1.0, 2.0), 4, torch.float32, "gelu", ptr=ptr, seed=5)
+
+
+@gpu
 def test_group_norm_broken_row_pointers_of_a_long_batch_touch_nothing_else():
     rows, C = 50000, 64
     ptr = torch.randint(-60000, 120000, (300,), generator=torch.Generator().manual_seed(2)).cuda()
