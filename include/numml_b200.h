@@ -601,7 +601,9 @@ NB200_API int nb200_ipc_free(void* ptr);
 /* ---------------------------------------------------------------------------------------------
  * Dense operators of the graph layers.  Node features are channels-last rows; `dtype` is any
  * nb200_dtype; sums, statistics and activations are held in 32 bits (64 for NB200_F64) and results
- * are rounded once.  `activation` is an nb200_activation.
+ * are rounded at the end; what else is rounded stands at the operator.  `activation` is an nb200_activation.  In
+ * 32 bits gelu's erf is good to 1.5e-7 absolute (Abramowitz and Stegun 7.1.26): far out on the negative side, where gelu
+ * is next to nothing, its relative error grows (5e-5 at z = -3, 1.6e-3 at -5).
  * ------------------------------------------------------------------------------------------- */
 typedef enum {
     NB200_ACT_NONE = 0,
@@ -617,10 +619,13 @@ typedef enum {
  *
  * Backward, dz = dy act'(z):  dx = dz w^T [m, k],  dw = x^T dz [k, n],  dbias = column sums of dz [n], each
  * contiguous and each skipped when NULL; the residual's gradient is dy itself.  float factors below 2^-102 may count
- * as up to 2^-125 less than they are (their low-order pieces are below the smallest normal number).  z may be NULL for NB200_ACT_NONE.
- * `status` (device word, may be NULL) receives NB200_ERR_WAIT_BUDGET if a bounded wait of a kernel ever runs out.
- * No alignment is required of any array but `work` (16 bytes); aligned rows are read faster.  Results do not depend on the run: sums are cut at
- * places that depend on the sizes alone and joined in order. */
+ * as up to 2^-125 less than they are (their low-order pieces are below the smallest normal number).  z may be NULL for
+ * NB200_ACT_NONE.  With 16-bit types and an activation, z is rounded to the type between the passes (a finite one stays
+ * finite) and dz before its products: the backward pass is that of a layer which keeps 16-bit intermediate results.
+ * `status` (device word, may be NULL) receives NB200_ERR_WAIT_BUDGET if a bounded wait of a kernel ever runs out, and the
+ * outputs of the blocks concerned hold NaN.  No alignment is required of any array but `work` (16 bytes); aligned rows
+ * are read faster.  Results do not depend on the run: sums are cut at places that depend on the sizes alone and joined
+ * in order. */
 NB200_API int nb200_linear_forward(int64_t m, int64_t k, int64_t n, const void* x, int64_t ldx, const void* w, int64_t ldw,
                                    const void* bias, const void* residual, int64_t ldr, int activation, void* z, void* y,
                                    int32_t* status, int dtype, nb200_stream stream);

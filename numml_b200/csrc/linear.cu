@@ -269,7 +269,8 @@ __global__ void __launch_bounds__(kThreads) join_parts_kernel(Join<T> first, Joi
     }
 }
 
-// dz = dy act'(z) (not stored when dz is NULL: then dy is dz) and the column sums of dz over a band of rows.
+// dz = dy act'(z) (not stored when dz is NULL: then dy is dz) and the column sums of dz over a band of rows.  dz is
+// rounded to the type of the layer, which the products of 16-bit types need as their operand; its sums are of the unrounded.
 // A thread owns V neighbouring columns of every row_lanes-th row; blockIdx.y selects the columns.  Moves
 // 3 values per element (1 without an activation) and is bound by that: a million rows of 128 floats with silu 257 us =
 // 6.3 TB/s, 0.96 of the copy rate; 131,072 x 512 bfloat16 93 us = 4.3 TB/s, where the slopes' instructions show.

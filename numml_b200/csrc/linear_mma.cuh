@@ -23,7 +23,9 @@ template <> __device__ __forceinline__ float largest_finite<__half>() { return 6
 // Whether the slope of an activation is a number times z: at an infinity it is then 0 * infinity.
 template <int ACT> constexpr bool slope_has_z() { return ACT == NB200_ACT_SILU || ACT == NB200_ACT_GELU; }
 
-// z as the backward pass will read it, one rounding of the 32-bit value that the activation was applied to.  A finite z
+// z as the backward pass will read it: rounded to the type of the layer, a choice that halves what 16-bit layers write and
+// read for it (the slope is then off by up to 0.8 |z| half-steps; measured, dx and dw of a layer of 512 x 512 bfloat16 2.4e-3
+// from 64 bits, 1.7e-3 with a 32-bit z and dz).  A finite z
 // stays finite in 16 bits: beyond their range the slopes are constant, so the largest number stands for it, where an
 // infinity would make a NaN.  For relu only the sign counts, and rounding keeps it, except that a positive z below half
 // the smallest fp16 number would become zero.

@@ -7,7 +7,10 @@
 They complete what a layer of :mod:`numml_b200.nn` does around its sparse product.  Node features are
 channels-last, ``[nodes, channels]``; a batch of graphs is a concatenation of their rows with a pointer
 array.  Values are float32, float64, bfloat16 or float16 (one type per call); sums, statistics and
-activations are held in 32 bits (64 for float64) and every result is rounded once.  All tensors are on
+activations are held in 32 bits (64 for float64) and results are rounded at the end.  One more rounding is
+made on purpose: :func:`linear` in a 16-bit type keeps its pre-activation, and takes the gradient behind the
+activation's slope to its products, in that type, as a layer of 16-bit operators does (32-bit ones would be twice
+the bytes, and twice the products).  All tensors are on
 one CUDA device (there is no CPU path); calls run on that device's current stream.  Results do not
 depend on the run: no operator adds with atomics.  Gradients of gradients and forward-mode tangents are refused.
 
@@ -163,7 +166,8 @@ def linear(X, weights, bias=None, activation=None, residual=None):
     """``act(X @ weights + bias) + residual`` in one pass.
 
     X: [..., K]; weights: [K, N]; bias: [N] or None; residual: [..., N] or None (no broadcasting);
-    activation: None / 'none', 'relu', 'silu', 'gelu' (the erf form) or 'tanh'.  X, weights and residual
+    activation: None / 'none', 'relu', 'silu', 'gelu' (the erf form; in 32 bits with an erf that is good to 1.5e-7
+    absolute, so relative to itself gelu(-3) is off by up to 5e-5) or 'tanh'.  X, weights and residual
     may be 2-D views with any row stride.  float32 products are as exact as float32 multiply-adds, for factors
     from 2^-102 (2e-31) upwards; of smaller ones up to 2^-125 may be lost."""
     act = _activation_code(activation)
