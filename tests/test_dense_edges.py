@@ -9,7 +9,7 @@ import torch
 import numml_b200.functional as F
 import numml_b200.nn as nn
 from numml_b200 import numml_torch_cpp
-from test_dense_ops import CURVE, TYPES, act64, check, normal, run_group_norm, tiny, units
+from test_dense_ops import CURVE, TYPES, act64, check, normal, run_group_norm, run_linear, tiny, units
 
 gpu = pytest.mark.gpu
 
@@ -470,3 +470,49 @@ def test_lazily_negated_operands():
     plain = run(X, W, v, R, dY, -X[:, :1])
     for got, want in zip(run(*(lazy(t) for t in (X, W, v, R, dY)), column), plain):
         assert torch.equal(got, want)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("m,k,n", [(640, 4097, 72), (1300, 5000, 136), (700, 9001, 41)])
+def test_linear_long_sums_with_everything(m, k, n, dtype):
+    """Sums in several runs, with bias, activation, residual and the backward pass, tiled and gathered; dX's over few."""
+    run_linear(m, k, n, dtype, "gelu", True, True, seed=m)
+    run_linear(k, 48, n, dtype, "silu", True, False, seed=n)
+
+
+@gpu
+@pytest.mark.parametrize("act", [None, "relu", "silu", "gelu", "tanh"])
+@pytest.mark.parametrize("m,k,n", [(600, 130, 72), (900, 70, 41), (3, 130, 72)])
+def test_linear_infinities_through_the_epilogue(m, k, n, act):
+    """Float sums that are not finite get bias, activation and residual like the others, with and without z kept, and
+    the values around them do not notice."""
+    X, W = normal((m, k), 1, torch.float32), normal((k, n), 2, torch.float32, 0.2)
+    b, R, dY = normal((n,), 3, torch.float32), normal((m, n), 4, torch.float32), normal((m, n), 5, torch.float32)
+    clean = F.linear(X.cuda(), W.cuda(), b.cuda(), act, R.cuda()).cpu()
+    X[m - 2, 7], X[0, 3], X[m - 1, 5] = float("inf"), float("nan"), -float("inf")
+    W[9, n - 1] = float("inf")                                   # a column, of either sign
+    z = X.double() @ W.double() + b.double()
+    odd = ~torch.isfinite(z)
+    a, _ = act64(z, act)
+    if act == "relu":                                            # there the formula is -infinity * 0
+        a = torch.relu(z)
+    want = (a + R.double()).float()
+    with torch.no_grad():
+        quiet = F.linear(X.cuda(), W.cuda(), b.cuda(), act, R.cuda()).cpu()
+    x, w, r = X.cuda().requires_grad_(True), W.cuda().requires_grad_(True), R.cuda().requires_grad_(True)
+    y = F.linear(x, w, b.cuda(), act, r)
+    grads = torch.autograd.grad(y, (x, w, r), dY.cuda())
+    assert torch.equal(quiet.nan_to_num(1.5), y.detach().cpu().nan_to_num(1.5)) and torch.equal(quiet.isnan(), y.detach().cpu().isnan())
+    assert torch.equal(quiet[~odd], clean[~odd])                 # what is finite is what it was without them
+    got = quiet[odd]
+    assert torch.equal(got.isnan(), want[odd].isnan())
+    assert torch.equal(got.isinf(), want[odd].isinf()) and torch.equal(got[got.isinf()], want[odd][got.isinf()])
+    fine = torch.isfinite(got)
+    assert ((got[fine] - want[odd][fine]).abs() <= 4 * 2.0 ** -24 * (1 + want[odd][fine].abs())).all()
+    assert torch.equal(grads[2].cpu(), dY)
+    rows = torch.ones(m, dtype=torch.bool)
+    rows[[m - 2, 0, m - 1]] = False
+    if act in ("relu", "tanh"):                                  # slopes of 0 and 1 there: dX of the other rows stays finite
+        assert torch.isfinite(grads[0].cpu()[rows][:, :9]).all()
+    numml_torch_cpp.check_status()
