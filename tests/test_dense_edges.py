@@ -302,6 +302,21 @@ def test_group_norm_long_graphs_among_short_ones(C, groups, act, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_group_norm_long_graphs_of_many_channels(dtype):
+    """Rows that several blocks side by side cover; a NaN stays in its long graph and group."""
+    ptr = [0, 3, 2700, 2700, 2710, 4801, 4850]
+    X = normal((4860, 2048), 3, dtype)
+    run_group_norm(X, 32, dtype, "silu", ptr=ptr, seed=5)
+    clean = F.group_norm(X.cuda(), 32, ptr=torch.tensor(ptr, device="cuda"))
+    X[1000, 100] = float("nan")
+    got = F.group_norm(X.cuda(), 32, ptr=torch.tensor(ptr, device="cuda"))
+    assert got[3:2700, 64:128].isnan().all()
+    got[3:2700, 64:128] = clean[3:2700, 64:128]
+    assert torch.equal(got, clean)
+
+
+@gpu
 def test_group_norm_long_graphs_among_very_many():
     """More graphs than rows, most of them empty, and as many long ones as there can be."""
     ptr = [0]
