@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kThreads) apply_kernel(Shape sh, const T* __re
 }
 
 // Both passes over the segments that short_forward_kernel has handed over, in one cooperative launch; it finds out for
-// itself whether there are any, and is done when there are none.
+// itself whether there are any, and is done when there are none.  sh.ptr is what that kernel has kept of the row pointers.
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(kThreads, 2) handed_forward_kernel(Shape sh, const T* __restrict__ x, const T* __restrict__ w,
                                                                      const T* __restrict__ bias, double eps, acc_t<T>* mean, acc_t<T>* rstd,
@@ -681,12 +681,21 @@ __device__ __forceinline__ void zero_outside(const Shape& sh, int64_t first, int
     }
 }
 
+// What a block of the short segments has read of the row pointers, for the launch that takes the long ones: its blocks wait
+// for one another at grid barriers, so they must not disagree about the segments, whatever happens to the row pointers
+// meanwhile.
+__device__ __forceinline__ void keep_pointers(const Shape& sh, int64_t* kept, int64_t s, int64_t begin) {
+    if (kept == nullptr || blockIdx.y != 0 || threadIdx.x != 0) return;
+    kept[s] = begin;
+    if (s == sh.segments - 1) kept[sh.segments] = segment_begin(sh, sh.segments);
+}
+
 // ONE: a vector of channels belongs to one group (V divides channels / groups), so that a thread has one mean and one
 // sum instead of V.
 template <typename T, int V, int ACT, bool ONE>
 __global__ void __launch_bounds__(kShort, 4) short_forward_kernel(Shape sh, Slab slab, const T* __restrict__ x, const T* __restrict__ w,
                                                                const T* __restrict__ bias, double eps, acc_t<T>* __restrict__ mean,
-                                                               acc_t<T>* __restrict__ rstd, T* __restrict__ y) {
+                                                               acc_t<T>* __restrict__ rstd, T* __restrict__ y, int64_t* __restrict__ kept) {
     using A = acc_t<T>;
     constexpr int G = ONE ? 1 : V;                                     // groups that a thread may touch
     __shared__ A sm[kShort * G], scale[kSlabGroups];
@@ -697,6 +706,7 @@ __global__ void __launch_bounds__(kShort, 4) short_forward_kernel(Shape sh, Slab
     }
     const int64_t s = blockIdx.x, begin = segment_begin(sh, s), end = max(begin, segment_begin(sh, s + 1));
     const int width = slab.width, groups = slab.groups, first = blockIdx.y * slab.channels, g0 = blockIdx.y * groups;
+    keep_pointers(sh, kept, s, begin);
     if (sh.handed != 0 && end - begin > sh.handed) return;
     if (end == begin) {
         for (int g = threadIdx.x; g < groups; g += kShort) mean[s * sh.groups + g0 + g] = rstd[s * sh.groups + g0 + g] = A(0);
@@ -792,7 +802,8 @@ template <typename T, int V, int ACT, bool ONE>
 __global__ void __launch_bounds__(kShort, sizeof(T) == 8 ? 2 : 4) short_backward_kernel(Shape sh, Slab slab, const T* __restrict__ x, const T* __restrict__ dy,
                                                                 const T* __restrict__ w, const T* __restrict__ bias,
                                                                 const acc_t<T>* __restrict__ mean, const acc_t<T>* __restrict__ rstd,
-                                                                acc_t<T>* __restrict__ channel_sums, T* __restrict__ dx) {
+                                                                acc_t<T>* __restrict__ channel_sums, T* __restrict__ dx,
+                                                                int64_t* __restrict__ kept) {
     using A = acc_t<T>;
     constexpr int G = ONE ? 1 : V;
     __shared__ A sm[kShort * V];
@@ -804,6 +815,7 @@ __global__ void __launch_bounds__(kShort, sizeof(T) == 8 ? 2 : 4) short_backward
     }
     const int64_t s = blockIdx.x, begin = segment_begin(sh, s), end = max(begin, segment_begin(sh, s + 1));
     const int width = slab.width, first = blockIdx.y * slab.channels, mine = slab.channels, g0 = blockIdx.y * slab.groups;
+    keep_pointers(sh, kept, s, begin);
     if (sh.handed != 0 && end - begin > sh.handed) {     // its share of dbeta and dgamma is in another line
         if (threadIdx.x < mine)
             channel_sums[s * 2 * sh.channels + first + threadIdx.x] = channel_sums[s * 2 * sh.channels + sh.channels + first + threadIdx.x] = A(0);
@@ -916,7 +928,9 @@ int64_t block_count(int64_t rows) {
 // every SM, down to rows of 64 bytes, or fewer than two, down to 32.  Measured on 512 graphs of 1 to 1076 rows, mean
 // 118, x 128 bfloat16 channels with gelu, forward / backward: slabs of 128 channels 46 / 100 us, 64: 32 / 65, 32: 31 /
 // 57, with four channels to a thread 31 / 51 (clusters of 2 to 8 blocks per graph were no faster: 34-41 / 67-72); the row
-// chunks 82 / 117 us in six launches.
+// chunks 82 / 117 us in six launches.  On other batches (2048 to 131,072 rows in 16 to 4096 graphs, equal and cut at random;
+// 32 floats, 128 floats, 256 halves, 512 doubles) the row chunks take 1.0 to 5 times as long, but for 256 halves in graphs of
+// 32 rows (0.7 forward, 1.04 backward) and 512 doubles at the limit (0.9).
 constexpr int64_t kAlone = 512 * 1024, kInBlock = 128 * 1024;
 bool short_segments(int64_t rows, int64_t channels, int64_t groups, int64_t segments, bool ragged, size_t size, int V, Slab* slab) {
     if (segments < 1 || segments > 65535 * 16) return false;
@@ -956,10 +970,17 @@ bool short_segments(int64_t rows, int64_t channels, int64_t groups, int64_t segm
 }
 
 // The workspace: a line of 2 x channels values per block and per segment; one per block, and kMostHanded; two values per
-// (segment, group).  The first holds the pieces' partial results and the second the blocks' sums of dbeta and dgamma, or,
+// (segment, group); row pointers.  The first holds the pieces' partial results and the second the blocks' sums of dbeta and dgamma, or,
 // in the backward pass over short segments, the first these sums per segment and per block, and the second the pieces.
 size_t first_elements(int64_t rows, int64_t channels, int64_t segments) { return size_t(block_count(rows) + segments) * 2 * channels; }
 size_t second_elements(int64_t rows, int64_t channels) { return size_t(block_count(rows) + kMostHanded) * 2 * channels; }
+size_t elements(int64_t rows, int64_t channels, int64_t groups, int64_t segments) {
+    return first_elements(rows, channels, segments) + second_elements(rows, channels) + size_t(segments) * groups * 2;
+}
+template <typename A>
+int64_t* kept_pointers(int64_t rows, int64_t channels, int64_t groups, int64_t segments, A* work) {
+    return reinterpret_cast<int64_t*>(work + elements(rows, channels, groups, segments));      // an even number of values: 8-byte aligned
+}
 
 bool bad_shape(int64_t rows, int64_t channels, int64_t groups, int64_t segments, const int64_t* ptr) {
     return rows < 0 || channels < 1 || channels > (1 << 20) || groups < 1 || channels % groups != 0 || segments < 0 ||
@@ -1032,26 +1053,28 @@ int forward(Launch l, const T* x, const T* w, const T* b, double eps, int act, T
         return forward_chunks<T, V>(l, x, w, b, eps, act, y, mean, rstd, part, stream);
     slab.pad_blocks = l.sh.ptr ? kSMs / 4 : 0;
     l.sh.handed = slab.handed;
+    int64_t* kept = slab.handed != 0 ? kept_pointers(l.sh.rows, l.sh.channels, l.sh.groups, l.sh.segments, part) : nullptr;
     const dim3 grid(static_cast<unsigned>(l.sh.segments + slab.pad_blocks), static_cast<unsigned>(l.sh.channels / slab.channels));
     const int rc = l.sh.channels / l.sh.groups % V == 0
                        ? NB200_DISPATCH_ACT(act, (short_forward_kernel<T, V, ACT, true><<<grid, kShort, 0, stream>>>(l.sh, slab, x, w, b, eps, mean,
-                                                                                                                   rstd, y), launch_status()))
+                                                                                                                   rstd, y, kept), launch_status()))
                        : NB200_DISPATCH_ACT(act, (short_forward_kernel<T, V, ACT, false><<<grid, kShort, 0, stream>>>(l.sh, slab, x, w, b, eps, mean,
-                                                                                                                    rstd, y), launch_status()));
+                                                                                                                    rstd, y, kept), launch_status()));
     if (rc != NB200_OK || slab.handed == 0) return rc;
+    l.sh.ptr = kept;
     return NB200_DISPATCH_ACT(act, launch_handed(handed_forward_kernel<T, V, ACT>, handed_grid(l), stream, l.sh, x, w, b, eps, mean, rstd, part, y));
 }
 
 template <typename T, int V>
 int backward_short(const Launch& l, Slab slab, const T* dy, const T* x, const T* w, const T* b, const acc_t<T>* mean, const acc_t<T>* rstd,
-                   int act, T* dx, acc_t<T>* segment_sums, cudaStream_t stream) {
+                   int act, T* dx, acc_t<T>* segment_sums, int64_t* kept, cudaStream_t stream) {
     slab.pad_blocks = l.sh.ptr && dx ? kSMs / 4 : 0;
     const dim3 grid(static_cast<unsigned>(l.sh.segments + slab.pad_blocks), static_cast<unsigned>(l.sh.channels / slab.channels));
     return l.sh.channels / l.sh.groups % V == 0
                ? NB200_DISPATCH_ACT(act, (short_backward_kernel<T, V, ACT, true><<<grid, kShort, 0, stream>>>(
-                                              l.sh, slab, x, dy, w, b, mean, rstd, segment_sums, dx), launch_status()))
+                                              l.sh, slab, x, dy, w, b, mean, rstd, segment_sums, dx, kept), launch_status()))
                : NB200_DISPATCH_ACT(act, (short_backward_kernel<T, V, ACT, false><<<grid, kShort, 0, stream>>>(
-                                              l.sh, slab, x, dy, w, b, mean, rstd, segment_sums, dx), launch_status()));
+                                              l.sh, slab, x, dy, w, b, mean, rstd, segment_sums, dx, kept), launch_status()));
 }
 
 // Up to dx; dbeta and dgamma are left as one line of sums per block.
@@ -1085,11 +1108,13 @@ int backward(int64_t rows, int64_t channels, int64_t groups, int64_t segments, c
     if (short_segments(rows, channels, groups, segments, ptr != nullptr, sizeof(T), V, &slab)) {
         Launch blocks = make_launch<V>(rows, channels, groups, segments, ptr);
         blocks.sh.handed = chunks.sh.handed = slab.handed;
-        rc = backward_short<T, V>(blocks, slab, dy, x, w, b, mean, rstd, act, dx, first, stream);
+        int64_t* kept = slab.handed != 0 ? kept_pointers(rows, channels, groups, segments, at) : nullptr;
+        rc = backward_short<T, V>(blocks, slab, dy, x, w, b, mean, rstd, act, dx, first, kept, stream);
         lines = first;
         count = segments;
         if (rc == NB200_OK && slab.handed != 0) {
             const dim3 grid = handed_grid(chunks);
+            chunks.sh.ptr = kept;
             rc = NB200_DISPATCH_ACT(act, launch_handed(handed_backward_kernel<T, W, ACT>, grid, stream, chunks.sh, x, dy, w, b, mean, rstd, second,
                                                        first + size_t(segments) * 2 * channels, coef, dx));
             count += grid.x;
@@ -1112,7 +1137,7 @@ using namespace nb200;
 extern "C" size_t nb200_group_norm_workspace_bytes(int64_t rows, int64_t channels, int64_t groups, int64_t segments, int dtype) {
     if (rows < 0 || channels < 1 || groups < 1 || segments < 0) return 0;
     const size_t a = dtype == NB200_F64 ? 8 : 4;
-    return a * (first_elements(rows, channels, segments) + second_elements(rows, channels) + size_t(segments) * groups * 2);
+    return a * elements(rows, channels, groups, segments) + sizeof(int64_t) * (size_t(segments) + 1);
 }
 
 extern "C" int nb200_group_norm_forward(int64_t rows, int64_t channels, int64_t groups, int64_t segments, const int64_t* ptr,
