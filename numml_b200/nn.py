@@ -199,7 +199,7 @@ class Dropout(torch.nn.Module):
         if not self.training:
             return X
         if call is None:
-            if torch._C._current_graph_task_id() != -1:
+            if 0.0 < self.p < 1.0 and torch._C._current_graph_task_id() != -1:       # else every mask is the same
                 raise RuntimeError("Dropout is being run inside a backward pass, as a recomputed forward pass is, where another mask "
                                    "would belong to the gradients than to the output; take call = layer.next_call() in front of "
                                    "the recomputed region and give it to the layer: layer(A, X, call)")
